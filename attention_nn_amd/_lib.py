@@ -40,10 +40,31 @@ class AnnSampling(ctypes.Structure):
                 ("seed", ctypes.c_uint64), ("step", ctypes.c_uint64)]
 
 
+class AnnQkRows(ctypes.Structure):
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("q", "k", "v", "gq", "gk", "q_out", "k_out")]
+                + [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride",
+                                                     "gq_stride", "gk_stride")]
+                + [(k, ctypes.c_void_p) for k in ("cs", "sn", "pos")]
+                + [(k, ctypes.c_int32) for k in ("pos_each", "pos0", "table_rows", "B", "T", "Hq",
+                                                 "Hk", "D", "dtype")]
+                + [("eps", ctypes.c_float)])
+
+
+class AnnPaged(ctypes.Structure):
+    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+                + [(k, ctypes.c_int64) for k in ("k_page", "k_head", "k_slot", "v_page", "v_head",
+                                                 "v_slot")]
+                + [("table", ctypes.c_void_p), ("table_row", ctypes.c_int64),
+                   ("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p)]
+                + [(k, ctypes.c_int32) for k in ("pages", "page_size", "heads", "head_dim", "seqs",
+                                                 "cols", "rows")])
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_L = ctypes.c_int64
 
 # name -> (restype, argtypes); every symbol include/attnnn.h declares.
 SIGNATURES = {
@@ -76,6 +97,17 @@ SIGNATURES = {
     "ann_op_normuon_update": (ctypes.c_int, [_P, _P, _I, _I, _I, _F, _P, _F, _F, _P, _P, _SZ, _P]),
     "ann_op_normuon_noalloc_max_bytes": (ctypes.c_size_t, []),
     "ann_op_normuon_noalloc": (ctypes.c_int, [_P, _P, _I, _I, _I, _F, _P, _P]),
+    "ann_op_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(AnnQkRows), _P]),
+    "ann_op_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(AnnQkRows), _P]),
+    "ann_op_paged_append": (ctypes.c_int, [ctypes.POINTER(AnnPaged), ctypes.POINTER(AnnQkRows), _P]),
+    "ann_op_paged_attention_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I]),
+    "ann_op_paged_attention": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _L, _I, _F, _I, _P,
+                                              _P, _P, _SZ, _P]),
+    "ann_op_paged_weight_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I]),
+    "ann_op_paged_weight": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _L, _I, _P, _F, _I, _P,
+                                           _L, _P, _L, _P, _SZ, _P]),
+    "ann_op_paged_evict": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _I, _P, _L, _I, _I, _P,
+                                          _P, _P, _L, _P]),
     "ann_profile_enable": (ctypes.c_int, [_P, _I, _I]),
     "ann_profile_read": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(_I)]),
     "ann_check_device": (ctypes.c_int, [_P, _P]),
@@ -118,6 +150,17 @@ def check(rc):
             raise AnnArgError(rc, msg)
         raise AnnError(rc, msg)
     return rc
+
+
+def launch(device, fn, *args):
+    """Call an entry point whose last argument is the stream: the current one of
+    ``device``, which is made the current device for the call where it is not."""
+    import torch
+    from ._stream import current_stream
+    if device.index == torch.cuda.current_device():
+        return check(fn(*args, current_stream()))
+    with torch.cuda.device(device):
+        return check(fn(*args, current_stream()))
 
 
 def make_config(cfg, max_batch, max_ctx, max_tokens, v_sample=50257):

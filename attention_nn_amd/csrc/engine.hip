@@ -1122,6 +1122,212 @@ int ann_op_rms_norm(const void* x, void* y, int32_t rows, int32_t dim, float eps
   return ANN_OK;
 }
 
+// ---- queries and keys, paged cache --------------------------------------------
+
+namespace {
+
+int qk_rows(const ann_qk_rows* r, bool bwd, QkRows* a) {
+  if (!r) return fail(ANN_E_ARG, "rows are null");
+  if (r->B < 0 || r->T < 0 || r->Hq < 0 || r->Hk < 0 || r->D <= 0 || r->D % 4 ||
+      r->Hq + (long long)r->Hk > 65535)
+    return fail(ANN_E_ARG, "bad shape B=%d T=%d Hq=%d Hk=%d D=%d", r->B, r->T, r->Hq, r->Hk, r->D);
+  if (r->dtype != ANN_DTYPE_F32 && r->dtype != ANN_DTYPE_BF16) return fail(ANN_E_ARG, "bad dtype");
+  if (!(r->eps > 0.f)) return fail(ANN_E_ARG, "eps must be positive");
+  const bool some = r->B > 0 && r->T > 0;
+  if (some && ((r->Hq && (!r->q || !r->q_out)) || !r->cs || !r->sn ||
+               (bwd && ((r->Hq && !r->gq) || (r->Hk && !r->gk)))))
+    return fail(ANN_E_ARG, "null argument");
+  if (some && r->table_rows < 1) return fail(ANN_E_ARG, "the RoPE tables are empty");
+  a->q = r->q;
+  a->k = r->k;
+  a->gq = r->gq;
+  a->gk = r->gk;
+  a->qo = r->q_out;
+  a->ko = r->k_out;
+  for (int i = 0; i < 3; ++i) {
+    a->qs[i] = r->q_stride[i];
+    a->ks[i] = r->k_stride[i];
+    a->gqs[i] = r->gq_stride[i];
+    a->gks[i] = r->gk_stride[i];
+  }
+  a->cs = r->cs;
+  a->sn = r->sn;
+  a->pos = r->pos;
+  a->pos_each = r->pos_each;
+  a->pos0 = r->pos0;
+  a->table_rows = r->table_rows;
+  a->B = r->B;
+  a->T = r->T;
+  a->Hq = r->Hq;
+  a->Hk = r->Hk;
+  a->D = r->D;
+  a->eps = r->eps;
+  return ANN_OK;
+}
+
+int op_qk_norm_rope(const ann_qk_rows* r, bool bwd, void* stream) {
+  QkRows a{};
+  const int rc = qk_rows(r, bwd, &a);
+  if (rc) return rc;
+  if (r->B == 0 || r->T == 0) return ANN_OK;
+  if (r->Hk && (!r->k || !r->k_out)) return fail(ANN_E_ARG, "null argument");
+  if (!r->pos && (r->pos0 < 0 || (long long)r->pos0 + r->T > r->table_rows))
+    return fail(ANN_E_ARG, "positions %d .. %lld outside the tables' %d rows", r->pos0,
+                (long long)r->pos0 + r->T - 1, r->table_rows);
+  HIPCHK(qk_norm_rope(a, bwd, r->dtype, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+// Checks of a cache and of what a call reads of it: its keys and values, its new tokens.
+int paged_args(const ann_paged* c, bool kv, bool tokens, PagedArgs* a) {
+  if (!c) return fail(ANN_E_ARG, "cache is null");
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(ANN_E_ARG, "head_dim %d unsupported (64 or 128)", c->head_dim);
+  if (c->heads < 1 || c->heads > 65535 || c->pages < 1 || c->seqs < 0 || c->seqs > 65535 ||
+      c->cols < 0 || c->rows < 0)
+    return fail(ANN_E_ARG, "bad shape pages=%d heads=%d seqs=%d cols=%d rows=%d (seqs and heads up to 65535)",
+                c->pages, c->heads, c->seqs, c->cols, c->rows);
+  int sh = 4;
+  while (sh < 10 && (1 << sh) != c->page_size) ++sh;
+  if ((1 << sh) != c->page_size)
+    return fail(ANN_E_ARG, "page_size %d must be a power of two from 16 to 1024", c->page_size);
+  if (((long long)c->cols << sh) > (1LL << 30))
+    return fail(ANN_E_ARG, "a table row of %d pages of %d passes 2^30 entries", c->cols, c->page_size);
+  if (!c->k || !c->lens || (c->cols && !c->table) || (kv && !c->v) || (tokens && !c->starts))
+    return fail(ANN_E_ARG, "null argument");
+  if (((uintptr_t)c->k | (kv ? (uintptr_t)c->v : 0)) & 15 ||
+      (c->k_page | c->k_head | c->k_slot) & 7 || (kv && ((c->v_page | c->v_head | c->v_slot) & 7)))
+    return fail(ANN_E_ARG, "cache rows must be 16-byte aligned");
+  *a = PagedArgs{(uint16_t*)c->k, (uint16_t*)c->v, c->k_page, c->k_head, c->k_slot, c->v_page,
+                 c->v_head, c->v_slot, c->table, c->table_row, c->starts, c->lens, c->pages, sh,
+                 c->heads, c->seqs, c->cols, c->rows};
+  return ANN_OK;
+}
+
+int paged_query(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head, int heads,
+                float scale, int window) {
+  if (window < 0) return fail(ANN_E_ARG, "window=%d must be positive, or 0 for none", window);
+  if (heads < 1 || heads > 65535 || heads % c->heads)
+    return fail(ANN_E_ARG, "%d query heads over %d cache heads", heads, c->heads);
+  if (c->rows && !q) return fail(ANN_E_ARG, "null argument");
+  if (((uintptr_t)q & 15) || ((q_row | q_head) & 7))
+    return fail(ANN_E_ARG, "query rows must be 16-byte aligned");
+  if (!(scale == scale) || scale - scale != 0.f) return fail(ANN_E_ARG, "scale must be finite");
+  return ANN_OK;
+}
+
+int paged_ws(const void* ws, size_t have, size_t need) {
+  if (have < need) return fail(ANN_E_CAPACITY, "workspace %zu < %zu bytes", have, need);
+  if (need && (!ws || ((uintptr_t)ws & 15)))
+    return fail(ANN_E_ARG, "the workspace is null or not 16-byte aligned");
+  return ANN_OK;
+}
+
+}  // namespace
+
+int ann_op_qk_norm_rope(const ann_qk_rows* r, void* stream) {
+  return op_qk_norm_rope(r, false, stream);
+}
+
+int ann_op_qk_norm_rope_bwd(const ann_qk_rows* r, void* stream) {
+  return op_qk_norm_rope(r, true, stream);
+}
+
+int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream) {
+  PagedArgs p;
+  QkRows a{};
+  int rc = paged_args(c, true, true, &p);
+  if (rc) return rc;
+  if (r && (r->dtype != ANN_DTYPE_BF16 || r->D != c->head_dim || r->Hk != c->heads || r->Hq < 1 ||
+            r->B != 1 || r->T != c->rows))
+    return fail(ANN_E_ARG, "the rows are not the cache's: bf16, B 1, T %d, %d key heads of %d",
+                c->rows, c->heads, c->head_dim);
+  rc = qk_rows(r, false, &a);
+  if (rc) return rc;
+  if (c->rows == 0) return ANN_OK;
+  if (!r->k || !r->v) return fail(ANN_E_ARG, "null argument");
+  if (r->pos && r->pos_each != 1) return fail(ANN_E_ARG, "positions must be one for each row");
+  if (((uintptr_t)r->q | (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->q_out |
+       (uintptr_t)r->cs | (uintptr_t)r->sn) & 15 ||
+      (r->q_stride[1] | r->q_stride[2] | r->k_stride[1] | r->k_stride[2] | r->v_stride[1] |
+       r->v_stride[2]) & 7)
+    return fail(ANN_E_ARG, "query, key, value and table rows must be 16-byte aligned");
+  HIPCHK(paged_append(p, a, (const bf16_t*)r->v, r->v_stride[1], r->v_stride[2],
+                      (hipStream_t)stream));
+  return ANN_OK;
+}
+
+size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads) {
+  PagedArgs p;
+  if (paged_args(c, true, true, &p) || heads < 1 || heads % c->heads) return 0;
+  return paged_attention_ws_bytes(p, heads, c->head_dim);
+}
+
+int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
+                           int32_t heads, float scale, int32_t window, void* out, float* lse,
+                           void* ws, size_t ws_bytes, void* stream) {
+  PagedArgs p;
+  int rc = paged_args(c, true, true, &p);
+  if (rc) return rc;
+  rc = paged_query(c, q, q_row, q_head, heads, scale, window);
+  if (rc) return rc;
+  if (c->rows == 0) return ANN_OK;
+  if (!out) return fail(ANN_E_ARG, "out is null");
+  if ((uintptr_t)out & 15) return fail(ANN_E_ARG, "out must be 16-byte aligned");
+  rc = paged_ws(ws, ws_bytes, paged_attention_ws_bytes(p, heads, c->head_dim));
+  if (rc) return rc;
+  HIPCHK(paged_attention(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, scale, window,
+                         (bf16_t*)out, lse, ws, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+size_t ann_op_paged_weight_ws_bytes(const ann_paged* c, int32_t heads) {
+  PagedArgs p;
+  if (paged_args(c, false, true, &p) || heads < 1 || heads % c->heads) return 0;
+  return paged_weight_ws_bytes(p, heads, c->head_dim);
+}
+
+int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
+                        int32_t heads, const float* lse, float scale, int32_t window,
+                        const float* weight, int64_t w_row, float* weight_out, int64_t out_row,
+                        void* ws, size_t ws_bytes, void* stream) {
+  PagedArgs p;
+  int rc = paged_args(c, false, true, &p);
+  if (rc) return rc;
+  rc = paged_query(c, q, q_row, q_head, heads, scale, window);
+  if (rc) return rc;
+  if (c->seqs == 0 || c->cols == 0) return ANN_OK;
+  if ((c->rows && !lse) || !weight || !weight_out) return fail(ANN_E_ARG, "null argument");
+  if (weight == weight_out && w_row != out_row)
+    return fail(ANN_E_ARG, "weight in place with another row stride");
+  rc = paged_ws(ws, ws_bytes, paged_weight_ws_bytes(p, heads, c->head_dim));
+  if (rc) return rc;
+  HIPCHK(paged_weight(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, lse, scale, window,
+                      weight, w_row, weight_out, out_row, ws, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out_row,
+                       int32_t out_cols, const float* weight, int64_t w_row, int32_t keep,
+                       int32_t recent, int32_t* index, int32_t* new_lens, float* weight_out,
+                       int64_t wo_row, void* stream) {
+  PagedArgs p;
+  int rc = paged_args(c, true, false, &p);
+  if (rc) return rc;
+  if (keep < 1 || recent < 0 || recent > keep)
+    return fail(ANN_E_ARG, "keep=%d must be at least 1 and recent=%d lie in [0, keep]", keep, recent);
+  if (out_cols < 0 || ((long long)out_cols << p.sh) < keep)
+    return fail(ANN_E_CAPACITY, "%d pages of %d do not hold %d entries", out_cols, c->page_size, keep);
+  if (c->seqs == 0) return ANN_OK;
+  if (!out_table || !index || !new_lens || (c->cols && (!weight || !weight_out)))
+    return fail(ANN_E_ARG, "null argument");
+  if (weight == weight_out && w_row != wo_row)
+    return fail(ANN_E_ARG, "weight in place with another row stride");
+  HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,
+                     index, new_lens, weight_out, wo_row, (hipStream_t)stream));
+  return ANN_OK;
+}
+
 // ---- optimizer step (muon.py, metal_kernels.py:236-328) -------------------------
 
 int ann_op_adam_step(const float* p, const float* g, const float* m, const float* v, size_t n,

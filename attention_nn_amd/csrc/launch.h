@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "common.h"
+#include "paged.h"
 #include "per_device.h"
 
 namespace ann {
@@ -391,5 +392,45 @@ hipError_t op_relu2(const void* x, void* y, size_t n, int dtype, hipStream_t st)
 hipError_t op_rope(const void* x, void* y, const float* cs, const float* sn, int B, int T, int H,
                    int D, int pos0, int inverse, int dtype, hipStream_t st);
 hipError_t op_rms(const void* x, void* y, int rows, int dim, float eps, int dtype, hipStream_t st);
+
+// Rows of queries and keys (qk_rope.hip): x (B, T, H, D) by element strides of
+// batch, token and head; outputs contiguous.  Token (b, t) is turned by its
+// position pos0 + t, pos[b] + t or (pos_each) pos[b T + t].
+struct QkRows {
+  const void* q;
+  const void* k;
+  const void* gq;   // gradients (backward only)
+  const void* gk;
+  void* qo;
+  void* ko;
+  long long qs[3], ks[3], gqs[3], gks[3];
+  const float* cs;  // (table_rows, D / 4)
+  const float* sn;
+  const int32_t* pos;
+  int pos_each, pos0, table_rows;
+  int B, T, Hq, Hk, D;
+  float eps;
+};
+hipError_t qk_norm_rope(const QkRows& a, bool bwd, int dtype, hipStream_t st);
+// The same of c.rows new tokens (a.T of one batch), keys and values (row
+// strides vt, vh) into the cache.  a.pos: each token's position, or null: its
+// entry.  bf16, D 64 or 128, 16-byte aligned rows.
+hipError_t paged_append(const PagedArgs& c, const QkRows& a, const bf16_t* v, long long vt,
+                        long long vh, hipStream_t st);
+// Attention of c.rows new tokens over the cache (paged_attn.hip); window <= 0:
+// none.  lse: (rows, heads) or null.
+size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh);
+hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
+                           int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
+                           void* ws, hipStream_t st);
+// out[s][j] = w[s][j] + the weight entry j receives (j < len), else w[s][j].
+size_t paged_weight_ws_bytes(const PagedArgs& c, int heads, int Dh);
+hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads,
+                        int Dh, const float* lse, float scale, int window, const float* w,
+                        long long wrow, float* out, long long orow, void* ws, hipStream_t st);
+hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, long long out_row,
+                       int out_cols, const float* w, long long wrow, int keep, int recent,
+                       int32_t* index, int32_t* new_lens, float* out, long long orow,
+                       hipStream_t st);
 
 }  // namespace ann

@@ -1,0 +1,84 @@
+// Addresses in a paged key/value cache (internal; plain C++ on the host too).
+//
+// A cache is two tensors of pages; entry e of sequence s is slot e % page of
+// page table[s][e / page].  New tokens of all sequences lie behind one another,
+// sequence s in rows starts[s] .. starts[s + 1] - 1; lens[s] counts its entries
+// with these, so its token i of n is entry lens[s] - n + i.  Tables, starts and
+// lengths live on the device where the host cannot look at them: every value
+// read from them is brought into range here before it forms an address, so
+// that a wrong one gives a wrong result and never an access out of bounds.
+#pragma once
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define ANN_HD __host__ __device__ __forceinline__
+#else
+#define ANN_HD inline
+#endif
+
+namespace ann {
+
+struct PagedArgs {
+  uint16_t* k;              // bf16 (pages, heads, page, head_dim) by the strides below
+  uint16_t* v;
+  long long kp, kh, ks;     // elements from page to page, head to head, slot to slot
+  long long vp, vh, vs;
+  const int32_t* table;     // (seqs, cols), row stride trow
+  long long trow;
+  const int32_t* starts;    // seqs + 1
+  const int32_t* lens;      // seqs
+  int pages, sh, heads, seqs, cols, rows;   // sh: log2 of the page size; rows: of new tokens
+};
+
+// Entries of a sequence: a length below zero is none, one past the table's
+// last page ends there.
+ANN_HD int pg_len(int len, int cols, int sh) {
+  const long long cap = (long long)cols << sh;
+  return len < 0 ? 0 : len > cap ? (int)cap : len;
+}
+
+struct PgRange {
+  int first, n;   // row of the first new token, how many
+};
+// Rows of a sequence's new tokens from starts[s] and starts[s + 1].
+ANN_HD PgRange pg_range(int a, int b, int rows) {
+  if (a < 0) a = 0;
+  if (a > rows) a = rows;
+  if (b < a) b = a;
+  if (b > rows) b = rows;
+  return {a, b - a};
+}
+
+// A page to read from: an id that is no page reads page 0.
+ANN_HD int pg_read(int id, int pages) { return (unsigned)id < (unsigned)pages ? id : 0; }
+// Whether a page may be written.
+ANN_HD bool pg_writable(int id, int pages) { return (unsigned)id < (unsigned)pages; }
+
+// Offset of entry e's slot within its page.
+ANN_HD long long pg_slot(int e, int sh, long long slot) {
+  return (long long)(e & ((1 << sh) - 1)) * slot;
+}
+
+#if defined(__HIPCC__)
+// The sequence whose new tokens row n belongs to, by a whole wave: the last s
+// with starts[s] <= n, found among 64 of them at a time (two loads in a row up
+// to 4096 sequences); -1 where there is none.  The caller checks the row
+// against that sequence's range, so starts that do not rise find no entry.
+__device__ __forceinline__ int pg_sequence(const int32_t* __restrict__ starts, int seqs, int n) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, span = seqs;
+  while (span > 64) {
+    const int step = (span + 63) / 64;
+    const int i = lane * step;
+    const unsigned long long le = __ballot(i < span && starts[lo + i] <= n);
+    if (!le) return -1;
+    const int at = (63 - __builtin_clzll(le)) * step;
+    lo += at;
+    span = span - at < step ? span - at : step;
+  }
+  const unsigned long long le = __ballot(lane < span && starts[lo + lane] <= n);
+  return le ? lo + 63 - __builtin_clzll(le) : -1;
+}
+#endif
+
+}  // namespace ann

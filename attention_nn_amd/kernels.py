@@ -4,6 +4,8 @@
     rope_ht(x, cs, sn, pos0=0)      metal_kernels.py:87-134
     make_rope_tables(T, D, base)    metal_kernels.py:144-150
     rms(x)                          model.py:48-49
+    qk_norm_rope(q, k, cs, sn)      rms and rope_ht of q and k in one pass
+                                    (model.py:244-247); qk_norm_rope_bwd is its gradient
 
 Inputs are torch tensors on the GPU (fp32 or bf16); outputs keep the input
 dtype, computed in fp32 inside the HIP kernels.  ``rope_ht`` takes the
@@ -72,3 +74,78 @@ def rms(x, eps=1e-6):
     _lib.check(_lib.lib().ann_op_rms_norm(_p(x), _p(y), x.numel() // dim, dim, float(eps),
                                           _dt(x), current_stream()))
     return y
+
+
+def _qk_struct(q, k, cs, sn, pos, eps, grads=()):
+    """AnnQkRows of (B, T, H, D) rows, and what has to outlive the call."""
+    rows = []
+    for x in (q, k, *grads):
+        if not (isinstance(x, torch.Tensor) and x.is_cuda):
+            raise ValueError("expected a GPU tensor")
+        if x.dim() != 4:
+            raise ValueError("rows must be (B, T, H, D)")
+        rows.append(x if x.stride(3) == 1 else x.contiguous())
+    q, k = rows[:2]
+    B, T, Hq, D = q.shape
+    Hk = k.shape[2]
+    if k.shape[:2] != (B, T) or k.shape[3] != D:
+        raise ValueError(f"k {tuple(k.shape)} must be (B, T, Hk, D) of q {tuple(q.shape)}")
+    for x, like in zip(rows[2:], (q, k)):
+        if x.shape != like.shape:
+            raise ValueError(f"gradient {tuple(x.shape)} must match {tuple(like.shape)}")
+    dt = _dt(q)
+    cs, sn = _gpu(cs).float(), _gpu(sn).float()
+    if D % 4 or cs.dim() != 2 or cs.shape[1] != D // 4 or sn.shape != cs.shape:
+        raise ValueError("D must be a multiple of 4 and the tables (rows, D/4)")
+    a = _lib.AnnQkRows()
+    if isinstance(pos, torch.Tensor):
+        if pos.dtype != torch.int32 or tuple(pos.shape) not in ((B,), (B, T)):
+            raise ValueError("pos must be a number or int32 of shape (B,) or (B, T)")
+        pos = _gpu(pos)
+        a.pos, a.pos_each = pos.data_ptr(), int(pos.dim() == 2)
+        rows.append(pos)
+    else:
+        a.pos0 = pos
+        if B and T and (pos < 0 or pos + T > cs.shape[0]):
+            raise ValueError("tables must be (>= pos + T, D/4)")
+    for x in rows[1:] + [cs, sn]:
+        if x.device != q.device:
+            raise ValueError(f"tensors on {q.device} and {x.device}")
+    for x in rows[1:2 + len(grads)]:
+        if x.dtype != q.dtype:
+            raise TypeError(f"dtypes {q.dtype} and {x.dtype} differ")
+    a.q, a.k = q.data_ptr(), k.data_ptr()
+    a.q_stride[:], a.k_stride[:] = q.stride()[:3], k.stride()[:3]
+    if grads:
+        a.gq, a.gk = rows[2].data_ptr(), rows[3].data_ptr()
+        a.gq_stride[:], a.gk_stride[:] = rows[2].stride()[:3], rows[3].stride()[:3]
+    a.cs, a.sn, a.table_rows = cs.data_ptr(), sn.data_ptr(), cs.shape[0]
+    a.B, a.T, a.Hq, a.Hk, a.D, a.dtype, a.eps = B, T, Hq, Hk, D, dt, eps
+    qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    ko = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
+    a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
+    return a, (rows, cs, sn), qo, ko
+
+
+def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
+    """Queries (B, T, Hq, D) and keys (B, T, Hk, D) as the attention takes them:
+    each head's row over sqrt(mean(x^2) + eps), its first half rotated as
+    ``rope_ht`` does.  -> (q, k), contiguous, in the input dtype.
+
+    One pass, rounded once: a bf16 result is within one rounding of the exact
+    one, where ``rope_ht(rms(x))`` rounds twice.  The inputs may be views with
+    any strides over batch, token and head (of a fused projection, say).
+    ``pos`` is the position of token 0, or an int32 GPU tensor: (B,) one start
+    for each batch row, (B, T) one position for each token (a value outside the
+    tables takes their nearest row)."""
+    a, keep, qo, ko = _qk_struct(q, k, cs, sn, pos, eps)
+    _lib.launch(qo.device, _lib.lib().ann_op_qk_norm_rope, a)
+    return qo, ko
+
+
+def qk_norm_rope_bwd(gq, gk, q, k, cs, sn, pos=0, eps=1e-6):
+    """Gradients of ``qk_norm_rope``'s inputs from those of its outputs -> (dq, dk).
+    ``q`` and ``k`` are its inputs."""
+    a, keep, qo, ko = _qk_struct(q, k, cs, sn, pos, eps, (gq, gk))
+    _lib.launch(qo.device, _lib.lib().ann_op_qk_norm_rope_bwd, a)
+    return qo, ko

@@ -33,6 +33,11 @@
  *   ann_op_muon_apply                         <- muon_apply (metal_kernels.py:306-329)
  *   ann_op_polar_express(_ws_bytes)           <- polar_express (muon.py:28-44)
  *   ann_op_normuon(_ws_bytes)                 <- normuon_rescale (muon.py:47-63)
+ *   ann_op_qk_norm_rope(_bwd)                 <- rms and rope_ht of q and k, and their
+ *                                                gradient (model.py:244-247)
+ *   ann_op_paged_*                               no counterpart: attention over a cache
+ *                                                (model.py:248-254) that sequences of
+ *                                                any lengths share
  */
 #ifndef ATTNNN_H
 #define ATTNNN_H
@@ -242,6 +247,104 @@ int ann_op_normuon_update(const void* v, float* second_mom, int32_t batch, int32
 size_t ann_op_normuon_noalloc_max_bytes(void);
 int ann_op_normuon_noalloc(const void* v, float* second_mom, int32_t batch, int32_t M, int32_t N,
                            float beta2, float* out, void* stream);
+
+/* ---- queries and keys ------------------------------------------------------
+ * Each head's row normalised and its first half turned by the token's position
+ * in one pass (model.py:244-247): n = x / sqrt(mean(x^2) + eps), pairs p < D/4
+ * as in ann_op_rope_ht.  fp32 inside, rounded once to dtype. */
+typedef struct ann_qk_rows {
+  const void* q;         /* (B, T, Hq, D) in dtype, last dimension contiguous */
+  const void* k;         /* (B, T, Hk, D); Hk may be 0 */
+  const void* v;         /* ann_op_paged_append only: (B, T, Hk, D) */
+  const void* gq;        /* ann_op_qk_norm_rope_bwd only: gradients of the outputs */
+  const void* gk;
+  void* q_out;           /* (B, T, Hq, D) contiguous */
+  void* k_out;           /* (B, T, Hk, D) contiguous */
+  int64_t q_stride[3];   /* elements from batch to batch, token to token, head to head */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t gq_stride[3];
+  int64_t gk_stride[3];
+  const float* cs;       /* RoPE tables (table_rows, D/4) */
+  const float* sn;
+  const int32_t* pos;    /* null: token t is at pos0 + t */
+  int32_t pos_each;      /* pos: 0 (B,), token t at pos[b] + t; 1 (B, T) */
+  int32_t pos0;
+  int32_t table_rows;    /* a device position outside the table takes its nearest row */
+  int32_t B, T, Hq, Hk, D;
+  int32_t dtype;
+  float eps;
+} ann_qk_rows;
+int ann_op_qk_norm_rope(const ann_qk_rows* r, void* stream);
+/* The gradients of q and k from those of the outputs, to q_out and k_out. */
+int ann_op_qk_norm_rope_bwd(const ann_qk_rows* r, void* stream);
+
+/* ---- paged key/value cache -----------------------------------------------
+ * Sequences of any lengths share a pool of pages.  Entry e of sequence s is
+ * slot e % page_size of page table[s][e / page_size].  The new tokens of a call
+ * lie behind one another, those of sequence s in rows starts[s] ..
+ * starts[s + 1] - 1 (starts never falls; rows from starts[seqs] on belong to no
+ * sequence and are left as they were); lens[s] counts its entries with these,
+ * so the last new token is entry lens[s] - 1.  table, starts and lens are
+ * device arrays: ids that are no page are never written to and read page 0,
+ * lengths outside the table end at it.  Rows of queries, keys, values and
+ * cache slots are 16-byte aligned (strides multiples of 8).  A head of the
+ * cache serves heads / cache heads query heads behind one another. */
+typedef struct ann_paged {
+  void* k;               /* bf16, (pages, heads, page_size, head_dim) by the strides */
+  void* v;
+  int64_t k_page, k_head, k_slot;   /* elements */
+  int64_t v_page, v_head, v_slot;
+  const int32_t* table;  /* (seqs, cols), rows table_row elements apart */
+  int64_t table_row;
+  const int32_t* starts; /* seqs + 1 */
+  const int32_t* lens;   /* seqs */
+  int32_t pages, page_size;   /* page_size a power of two, 16 .. 1024 */
+  int32_t heads, head_dim;    /* head_dim 64 or 128 */
+  int32_t seqs, cols;         /* cols * page_size <= 2^30 */
+  int32_t rows;               /* rows of new tokens */
+} ann_paged;
+
+/* Queries and keys of c->rows new tokens (r: bf16, B 1, T rows) normalised and
+ * turned as above, queries to q_out, keys and values to their entries.  A
+ * token's position is its entry, or pos[row] (pos_each 1). */
+int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream);
+
+/* A new token at entry e sees the entries j <= e and, with window > 0, e - j <
+ * window: out = softmax(scale q.k_j) v_j (rows, heads, head_dim) bf16, lse
+ * (rows, heads) fp32 the natural log of the softmax sum, or null.  A token that
+ * sees nothing gets 0 and -infinity.  q (rows, heads, head_dim) bf16 by
+ * strides; ws: ann_op_paged_attention_ws_bytes bytes (16-byte aligned). */
+size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads);
+int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
+                           int32_t heads, float scale, int32_t window, void* out, float* lse,
+                           void* ws, size_t ws_bytes, void* stream);
+
+/* weight_out[s][j] = weight[s][j] + sum over sequence s's new tokens that see
+ * entry j and over heads of exp(scale q.k_j - lse), lse as
+ * ann_op_paged_attention gives it; entries behind the sequence keep their
+ * weight.  weight and weight_out (seqs, cols * page_size) fp32, rows w_row and
+ * out_row elements apart; they may be the same.  c->v is not read.  The sums'
+ * order does not depend on what else runs: results are reproducible. */
+size_t ann_op_paged_weight_ws_bytes(const ann_paged* c, int32_t heads);
+int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
+                        int32_t heads, const float* lse, float scale, int32_t window,
+                        const float* weight, int64_t w_row, float* weight_out, int64_t out_row,
+                        void* ws, size_t ws_bytes, void* stream);
+
+/* Eviction by weight: a sequence of more than `keep` entries keeps its last
+ * `recent` and, of the others, those of the largest weight (of equal ones the
+ * lower entry; NaN below every number), min(len, keep) in all, moved in order
+ * to entries 0 .. of the pages in out_table (seqs, out_cols; rows out_row
+ * elements apart).  out_table is the table itself (in place) or names pages
+ * that the table does not.  index (seqs, keep): the entry each came from, -1
+ * behind them; new_lens (seqs); weight_out (seqs, cols * page_size): their
+ * weights, 0 behind them; it may be weight, and new_lens may be c->lens.
+ * c->starts is not read. */
+int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out_row,
+                       int32_t out_cols, const float* weight, int64_t w_row, int32_t keep,
+                       int32_t recent, int32_t* index, int32_t* new_lens, float* weight_out,
+                       int64_t wo_row, void* stream);
 
 /* Device status of the decode steps (no reference counterpart).  The
  * cross-work-group waits of the persistent batch-1 step and of the decode
