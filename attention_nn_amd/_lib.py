@@ -100,7 +100,7 @@ SIGNATURES = {
     "ann_op_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(AnnQkRows), _P]),
     "ann_op_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(AnnQkRows), _P]),
     "ann_op_paged_append": (ctypes.c_int, [ctypes.POINTER(AnnPaged), ctypes.POINTER(AnnQkRows), _P]),
-    "ann_op_paged_attention_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I]),
+    "ann_op_paged_attention_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I, _I]),
     "ann_op_paged_attention": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _L, _I, _F, _I, _P,
                                               _P, _P, _SZ, _P]),
     "ann_op_paged_weight_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I]),

@@ -1257,10 +1257,10 @@ int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream) 
   return ANN_OK;
 }
 
-size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads) {
+size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads, int32_t window) {
   PagedArgs p;
   if (paged_args(c, true, true, &p) || heads < 1 || heads % c->heads) return 0;
-  return paged_attention_ws_bytes(p, heads, c->head_dim);
+  return paged_attention_ws_bytes(p, heads, c->head_dim, window);
 }
 
 int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
@@ -1274,7 +1274,7 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
   if (c->rows == 0) return ANN_OK;
   if (!out) return fail(ANN_E_ARG, "out is null");
   if ((uintptr_t)out & 15) return fail(ANN_E_ARG, "out must be 16-byte aligned");
-  rc = paged_ws(ws, ws_bytes, paged_attention_ws_bytes(p, heads, c->head_dim));
+  rc = paged_ws(ws, ws_bytes, paged_attention_ws_bytes(p, heads, c->head_dim, window));
   if (rc) return rc;
   HIPCHK(paged_attention(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, scale, window,
                          (bf16_t*)out, lse, ws, (hipStream_t)stream));

@@ -419,7 +419,7 @@ hipError_t paged_append(const PagedArgs& c, const QkRows& a, const bf16_t* v, lo
                         long long vh, hipStream_t st);
 // Attention of c.rows new tokens over the cache (paged_attn.hip); window <= 0:
 // none.  lse: (rows, heads) or null.
-size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh);
+size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh, int window);
 hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
                            int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
                            void* ws, hipStream_t st);

@@ -79,6 +79,38 @@ __device__ __forceinline__ int pg_sequence(const int32_t* __restrict__ starts, i
   const unsigned long long le = __ballot(lane < span && starts[lo + lane] <= n);
   return le ? lo + 63 - __builtin_clzll(le) : -1;
 }
+
+// The tile-th tile of br rows of the sequences with more than `few` rows (g rows
+// for each new token), by a whole wave: its sequence and first row, or false where
+// there are fewer tiles.
+__device__ __forceinline__ bool pg_tile(const int32_t* __restrict__ starts, int seqs, int rows,
+                                        int g, int few, int br, int tile, int& seq, int& row0) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < seqs; s0 += 64) {
+    const int s = s0 + lane;
+    int n = 0;
+    if (s < seqs) {
+      const int r = pg_range(starts[s], starts[s + 1], rows).n * g;
+      n = r > few ? (r + br - 1) / br : 0;
+    }
+    int sum = n;   // of this lane's sequence and those before it
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    const unsigned long long past = __ballot(before + sum > tile);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      seq = s0 + at;
+      row0 = (tile - before - __shfl(sum - n, at, 64)) * br;
+      return true;
+    }
+    before += __shfl(sum, 63, 64);
+  }
+  return false;
+}
 #endif
 
 }  // namespace ann

@@ -172,7 +172,7 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
             raise ValueError(f"out must be contiguous {tuple(q.shape)}")
     lse = torch.empty((N, H), dtype=_F32, device=device) if want_lse else None
     L = _lib.lib()
-    nws = L.ann_op_paged_attention_ws_bytes(c, H)
+    nws = L.ann_op_paged_attention_ws_bytes(c, H, window)
     ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
     st = q.stride()
     _lib.launch(device, L.ann_op_paged_attention, c, q.data_ptr(), st[0], st[1], H, scale,
