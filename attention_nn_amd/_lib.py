@@ -6,6 +6,7 @@ point raises -- there is no CPU fallback on the product path.
 
 import ctypes
 import os
+import struct
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libattnnn.so")
 
@@ -49,6 +50,15 @@ class AnnQkRows(ctypes.Structure):
                                                  "Hk", "D", "dtype")]
                 + [("eps", ctypes.c_float)])
 
+    # every field in order, for from_values
+    _pack = struct.Struct("7Q15q3Q9if").pack
+
+    @classmethod
+    def from_values(cls, *values):
+        """All fields at once, arrays as their elements (a tenth of the time of
+        setting them one by one)."""
+        return cls.from_buffer_copy(cls._pack(*values))
+
 
 class AnnPaged(ctypes.Structure):
     _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
@@ -58,6 +68,12 @@ class AnnPaged(ctypes.Structure):
                    ("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p)]
                 + [(k, ctypes.c_int32) for k in ("pages", "page_size", "heads", "head_dim", "seqs",
                                                  "cols", "rows")])
+
+    _pack = struct.Struct("2Q6qQq2Q7i4x").pack
+
+    @classmethod
+    def from_values(cls, *values):
+        return cls.from_buffer_copy(cls._pack(*values))
 
 
 _P = ctypes.c_void_p
@@ -150,17 +166,6 @@ def check(rc):
             raise AnnArgError(rc, msg)
         raise AnnError(rc, msg)
     return rc
-
-
-def launch(device, fn, *args):
-    """Call an entry point whose last argument is the stream: the current one of
-    ``device``, which is made the current device for the call where it is not."""
-    import torch
-    from ._stream import current_stream
-    if device.index == torch.cuda.current_device():
-        return check(fn(*args, current_stream()))
-    with torch.cuda.device(device):
-        return check(fn(*args, current_stream()))
 
 
 def make_config(cfg, max_batch, max_ctx, max_tokens, v_sample=50257):

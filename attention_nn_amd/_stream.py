@@ -16,3 +16,15 @@ def current_stream():
     if _raw is None:
         return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     return ctypes.c_void_p(_raw(torch.cuda.current_device()))
+
+
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def on_device(index, fn, *args):
+    """``fn(*args, stream)`` with the current stream of GPU ``index``, which is made
+    the current device for the call where it is not."""
+    if index != _device():
+        with torch.cuda.device(index):
+            return fn(*args, current_stream())
+    return fn(*args, _raw(index) if _raw is not None else current_stream())

@@ -1183,9 +1183,9 @@ int paged_args(const ann_paged* c, bool kv, bool tokens, PagedArgs* a) {
   if (!c) return fail(ANN_E_ARG, "cache is null");
   if (c->head_dim != 64 && c->head_dim != 128)
     return fail(ANN_E_ARG, "head_dim %d unsupported (64 or 128)", c->head_dim);
-  if (c->heads < 1 || c->heads > 65535 || c->pages < 1 || c->seqs < 0 || c->seqs > 65535 ||
+  if (c->heads < 1 || c->heads > 32767 || c->pages < 1 || c->seqs < 0 || c->seqs > 65535 ||
       c->cols < 0 || c->rows < 0)
-    return fail(ANN_E_ARG, "bad shape pages=%d heads=%d seqs=%d cols=%d rows=%d (seqs and heads up to 65535)",
+    return fail(ANN_E_ARG, "bad shape pages=%d heads=%d seqs=%d cols=%d rows=%d (seqs up to 65535, heads to 32767)",
                 c->pages, c->heads, c->seqs, c->cols, c->rows);
   int sh = 4;
   while (sh < 10 && (1 << sh) != c->page_size) ++sh;

@@ -830,51 +830,113 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 
 // ---- weight of the entries -------------------------------------------------------
 //
-// A work-group takes 64 entries of a sequence, a lane for each entry, and its
-// four waves every fourth (token, head): a lane's sum runs in row order and the
-// four are added in wave order, so the result does not depend on the grid.
+// A work-group takes 64 entries of a sequence and all rows (token, head) that see
+// any of them; a wave takes 64 rows of one cache head at a time, its keys in
+// registers.  S = K Q^T, entries x rows, 16 x 16 a product: a lane adds the weights
+// of its row's column for its four entries of each block, and only at the end are
+// the 16 columns and the eight waves added, in a fixed order, so a sum does not
+// depend on what else is in the call.
 template <int DH>
-__global__ __launch_bounds__(256) void k_paged_weight(PagedArgs c, const bf16_t* __restrict__ q,
+__global__ __launch_bounds__(512) void k_paged_weight(PagedArgs c, const bf16_t* __restrict__ q,
                                                       long long qt, long long qh, int heads,
-                                                      const float* __restrict__ lse, float scale,
-                                                      int window, const float* __restrict__ w,
-                                                      long long wrow, float* __restrict__ out,
-                                                      long long orow, int cap) {
-  __shared__ float part[4][64];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int s = blockIdx.y, j = blockIdx.x * 64 + lane;
+                                                      const float* __restrict__ lse, float sl2,
+                                                      int neg, int window, const float* w,
+                                                      long long wrow, float* out, long long orow,
+                                                      int cap) {
+  constexpr int NKS = DH / 32, RC = 64;
+  __shared__ float part[8][64];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = blockIdx.y, j0 = blockIdx.x * 64;
   const int len = pg_len(c.lens[s], c.cols, c.sh);
   const PgRange r = pg_range(c.starts[s], c.starts[s + 1], c.rows);
-  float sum = 0.f;
-  if (blockIdx.x * 64 < len) {
-    const int jr = min(j, len - 1);
-    const int id = pg_read(c.table[s * c.trow + (jr >> c.sh)], c.pages);
-    const bf16_t* kr = c.k + id * c.kp + pg_slot(jr, c.sh, c.ks);
-    const int G = heads / c.heads, rows = r.n * heads;
-    for (int x = wv; x < rows; x += 4) {
-      const int i = x / heads, h = x % heads, n = r.first + i, e = len - r.n + i;
-      const bf16_t* qr = q + n * qt + h * qh;
-      const bf16_t* kk = kr + (h / G) * c.kh;
-      float a = 0.f;
-      for (int d = 0; d < DH; d += 8) {
-        float f[8], g[8];
-        unpack8(*(const uint4*)(kk + d), f);
-        unpack8(*(const uint4*)(qr + d), g);
+  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + 63, len - 1);
+  // tokens t0 .. t1 - 1 see one of the entries j0 .. jl
+  const int t0 = max(0, j0 - e0), t1 = jl - e0 < r.n - window ? jl - e0 + window : r.n;
+  float acc[4][4];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) a += f[t] * g[t];
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
+  if (j0 < len && t1 > t0) {
+    const int lo = t0 * G, hi = t1 * G, chunks = (hi - lo + RC - 1) / RC;
+    const int32_t* table = c.table + s * c.trow;
+    for (int u = wv; u < c.heads * chunks; u += 8) {
+      const int kvh = u / chunks, c0 = lo + u % chunks * RC, c1 = min(c0 + RC, hi);
+      bf16x8_t kf[4][NKS];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int k0 = min(j0 + 16 * b, jl & ~15);
+        const int id = pg_read(table[k0 >> c.sh], c.pages);
+        const bf16_t* kr = c.k + id * c.kp + kvh * c.kh + pg_slot(k0, c.sh, c.ks) +
+                           min(r16, jl - k0) * c.ks + g4 * 8;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) kf[b][ks] = *(const bf16x8_t*)(kr + ks * 32);
       }
-      if (j <= e && e - j < window)
-        sum += __builtin_amdgcn_exp2f((a * scale - lse[(long long)n * heads + h]) * PA_LOG2E);
+      auto load = [&](int row0, bf16x8_t* qf, float& l2, int& e) {
+        const int row = min(row0 + r16, hi - 1), t = row / G;
+        const int h = kvh * G + row % G;
+        const bf16_t* qr = q + (r.first + t) * qt + h * qh + g4 * 8;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_query(qr + ks * 32, neg);
+        l2 = lse[(long long)(r.first + t) * heads + h] * PA_LOG2E;
+        e = row0 + r16 < c1 ? e0 + t : -1;   // a row past the chunk sees nothing
+      };
+      bf16x8_t qf[NKS];
+      float l2;
+      int e;
+      load(c0, qf, l2, e);
+      for (int row0 = c0; row0 < c1; row0 += 16) {
+        floatx4_t sc[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) sc[b] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], sc[b], 0, 0, 0);
+        const float base = l2;
+        const int at = e;
+        if (row0 + 16 < c1) load(row0 + 16, qf, l2, e);
+        // entry jl is the last that any row here sees or the tile holds
+        const bool full = row0 + 16 <= c1 && e0 + row0 / G >= j0 + 63 &&
+                          e0 + (row0 + 15) / G - j0 < window;
+        if (full) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[b][i] += __builtin_amdgcn_exp2f(sc[b][i] * sl2 - base);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = j0 + 16 * b + 4 * g4 + i;
+              acc[b][i] += j <= at && at - j < window ? __builtin_amdgcn_exp2f(sc[b][i] * sl2 - base) : 0.f;
+            }
+        }
+      }
     }
   }
-  part[wv][lane] = sum;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = group_sum<16>(acc[b][i]);
+      if (r16 == 0) part[wv][16 * b + 4 * g4 + i] = v;
+    }
   __syncthreads();
-  if (wv || j >= cap) return;
+  const int j = j0 + tid;
+  if (tid >= 64 || j >= cap) return;
   const float was = w[s * wrow + j];
-  if (j < len)
-    out[s * orow + j] = was + (((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane]);
-  else if (out != w)
+  if (j < len) {
+    float v = part[0][tid];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += part[k][tid];
+    out[s * orow + j] = was + v;
+  } else if (out != w) {
     out[s * orow + j] = was;
+  }
 }
 
 size_t paged_weight_ws_bytes(const PagedArgs&, int, int) { return 0; }
@@ -886,10 +948,10 @@ hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long 
   if (c.seqs == 0 || cap == 0) return hipSuccess;
   (void)ws;
   const int win = window > 0 ? window : 0x7fffffff;
-  const dim3 grid((unsigned)((cap + 63) / 64), (unsigned)c.seqs), block(256);
-#define ANN_PW(D)                                                                              \
-  hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads, lse, scale, win, \
-                     w, wrow, out, orow, cap)
+  const dim3 grid((unsigned)((cap + 63) / 64), (unsigned)c.seqs), block(512);
+#define ANN_PW(D)                                                                               \
+  hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads, lse,           \
+                     fabsf(scale) * PA_LOG2E, (int)(scale < 0.f), win, w, wrow, out, orow, cap)
   if (Dh == 64) ANN_PW(64);
   else if (Dh == 128) ANN_PW(128);
   else return hipErrorInvalidValue;

@@ -17,17 +17,50 @@ __device__ __forceinline__ uint32_t ev_key(float f) {
 
 // One work-group for each sequence.  The smallest weight that stays is found a
 // byte at a time, from the top: a count of the words by their next byte among
-// those that agree with the bytes found so far.  Then one walk in entry order
-// writes down what stays.
-constexpr int EV_T = 1024;
-__global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__ lens, int cols,
-                                                     int sh, const float* w, long long wrow,
-                                                     int keep, int recent, int32_t* __restrict__ index,
-                                                     int32_t* __restrict__ new_lens, float* out,
-                                                     long long orow, int cap) {
+// those that agree with the bytes found so far.  Then what stays is written down
+// in entry order, its places from the counts of each wave's ballots.  Up to SEG
+// entries lie in registers throughout; longer sequences are read again, SEG at a
+// time, for each of the five walks.
+constexpr int EV_T = 1024, EV_W = EV_T / 64;
+
+// Exclusive prefix sums of the n <= 256 counts in cnt, and their total, by the
+// first wave.
+__device__ __forceinline__ void ev_scan(int* cnt, int n, int* total) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < 64) {
+    int v[4], own = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = 4 * lane + k < n ? cnt[4 * lane + k] : 0;
+      own += v[k];
+    }
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += x;
+    }
+    int at = sum - own;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (4 * lane + k < n) cnt[4 * lane + k] = at;
+      at += v[k];
+    }
+    if (lane == 63) *total = sum;
+  }
+}
+
+template <int NPT>
+__global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int cols, int sh,
+                                                     const float* w, long long wrow, int keep,
+                                                     int recent, int32_t* __restrict__ index,
+                                                     int32_t* new_lens, float* out, long long orow,
+                                                     int cap) {
+  constexpr int SEG = EV_T * NPT;
+  static_assert(NPT * EV_W <= 256, "counts of a segment");
   __shared__ unsigned hist[256];
   __shared__ unsigned s_prefix, s_want;
-  __shared__ int s_sum[EV_T / 64][2];
+  __shared__ int s_cnt[256], s_total;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int len = pg_len(lens[s], cols, sh);
   const float* ws = w + s * wrow;
@@ -37,8 +70,18 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__
   const int last = min(recent, left);   // entries that stay whatever they weigh
   const int old = len - last;           // those that are ranked
   const int want = left - last;         // and how many of them stay
+  const int segs = (old + SEG - 1) / SEG;
+  float x[NPT];                         // entry seg * SEG + k * EV_T + tid
+  auto load = [&](int seg) {
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) {
+      const int i = seg * SEG + k * EV_T + tid;
+      x[k] = i < old ? ws[i] : 0.f;
+    }
+  };
+  if (segs == 1) load(0);
   uint32_t edge = 0;                    // smallest word that stays
-  unsigned ties = 0;                    // how many of the words equal to it do
+  int ties = 0;                         // how many of the words equal to it do
   if (want < old && want > 0) {
     if (tid == 0) {
       s_prefix = 0;
@@ -48,14 +91,18 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
       const uint32_t prefix = s_prefix, mask = byte == 3 ? 0u : ~0u << (8 * byte + 8);
-      for (int i = tid; i < old; i += EV_T) {
-        const uint32_t u = ev_key(ws[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> (8 * byte)) & 255], 1u);
+      for (int seg = 0; seg < segs; ++seg) {
+        if (segs > 1) load(seg);
+#pragma unroll
+        for (int k = 0; k < NPT; ++k) {
+          const uint32_t u = ev_key(x[k]);
+          if (seg * SEG + k * EV_T + tid < old && (u & mask) == prefix)
+            atomicAdd(&hist[(u >> (8 * byte)) & 255], 1u);
+        }
       }
       __syncthreads();
       if (wv == 0) {   // the byte at which the words above it no longer fill `want`
-        unsigned need = s_want, above = 0;
-        int b = 255;
+        const unsigned need = s_want;
         // lane l holds bytes 4 l .. 4 l + 3
         const unsigned own = hist[4 * lane] + hist[4 * lane + 1] + hist[4 * lane + 2] + hist[4 * lane + 3];
         unsigned suffix = own;   // words of this lane's bytes and those above
@@ -64,11 +111,12 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__
           const unsigned v = __shfl_down(suffix, o, 64);
           if (lane + o < 64) suffix += v;
         }
-        const unsigned long long ok = __ballot(suffix >= need);
-        const int at = 63 - __builtin_clzll(ok);   // highest lane that reaches it
-        above = __shfl(suffix - own, at, 64);
+        // highest lane that reaches it
+        const int at = 63 - __builtin_clzll(__ballot(suffix >= need));
         if (lane == at) {
-          for (b = 4 * lane + 3; above + hist[b] < need; --b) above += hist[b];
+          unsigned above = suffix - own;
+          int b = 4 * lane + 3;
+          for (; above + hist[b] < need; --b) above += hist[b];
           s_prefix = prefix | ((uint32_t)b << (8 * byte));
           s_want = need - above;
         }
@@ -76,54 +124,64 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__
       __syncthreads();
     }
     edge = s_prefix;
-    ties = s_want;
+    ties = (int)s_want;
   }
   const bool all = want >= old;   // nothing is ranked out
   __syncthreads();
   if (tid == 0) new_lens[s] = left;   // may be lens[s]: every thread has read it
-  // entry order: ranks among the equal words and among what stays, by ballots
+  const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
   int done = 0, tied = 0;
-  for (int i0 = 0; i0 < old && want > 0; i0 += EV_T) {
-    const int i = i0 + tid;
-    const float x = i < old ? ws[i] : 0.f;
-    const uint32_t u = ev_key(x);
-    const bool eq = i < old && !all && u == edge;
-    const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
-    const unsigned long long be = __ballot(eq);
-    if (lane == 0) s_sum[wv][0] = __popcll(be);
+  for (int seg = 0; seg < segs && want > 0; ++seg) {
+    if (segs > 1) load(seg);
+    const int waves = min(NPT, (old - seg * SEG + EV_T - 1) / EV_T) * EV_W;   // counts in use
+    unsigned long long be[NPT];
+    if (!all) {   // ranks among the words equal to the edge
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) {
+        be[k] = __ballot(seg * SEG + k * EV_T + tid < old && ev_key(x[k]) == edge);
+        if (lane == 0) s_cnt[k * EV_W + wv] = __popcll(be[k]);
+      }
+      __syncthreads();
+      ev_scan(s_cnt, waves, &s_total);
+      __syncthreads();
+    }
+    unsigned stays = 0;
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) {
+      const int i = seg * SEG + k * EV_T + tid;
+      const uint32_t u = ev_key(x[k]);
+      const bool in = i < old && (all || u > edge ||
+                                  (u == edge && tied + s_cnt[k * EV_W + wv] + __popcll(be[k] & below) < ties));
+      stays |= (unsigned)in << k;
+    }
+    if (!all) tied += s_total;
     __syncthreads();
-    int t = tied, total = tied;
-    for (int k = 0; k < EV_T / 64; ++k) {
-      if (k < wv) t += s_sum[k][0];
-      total += s_sum[k][0];
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) {
+      be[k] = __ballot((stays >> k) & 1);
+      if (lane == 0) s_cnt[k * EV_W + wv] = __popcll(be[k]);
     }
-    tied = total;
-    const bool stays = i < old && (all || u > edge || (eq && t + __popcll(be & below) < (int)ties));
-    const unsigned long long bs = __ballot(stays);
-    if (lane == 0) s_sum[wv][1] = __popcll(bs);
     __syncthreads();
-    int p = done;
-    total = done;
-    for (int k = 0; k < EV_T / 64; ++k) {
-      if (k < wv) p += s_sum[k][1];
-      total += s_sum[k][1];
-    }
-    done = total;
-    p += __popcll(bs & below);
-    if (stays) {   // p <= i: entries not read yet are never written
-      ix[p] = i;
-      os[p] = x;
-    }
+    ev_scan(s_cnt, waves, &s_total);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+      if ((stays >> k) & 1) {   // its place p <= its entry: entries of later walks are never written
+        const int p = done + s_cnt[k * EV_W + wv] + __popcll(be[k] & below);
+        ix[p] = seg * SEG + k * EV_T + tid;
+        os[p] = x[k];
+      }
+    done += s_total;
     __syncthreads();
   }
-  // the last entries, in place order too
+  // the last entries, in order too: out may be w
   for (int i0 = 0; i0 < last; i0 += EV_T) {
     const int i = i0 + tid;
-    const float x = i < last ? ws[old + i] : 0.f;
+    const float v = i < last ? ws[old + i] : 0.f;
     __syncthreads();
     if (i < last) {
       ix[want + i] = old + i;
-      os[want + i] = x;
+      os[want + i] = v;
     }
     __syncthreads();
   }
@@ -131,45 +189,79 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* __restrict__
   for (int i = left + tid; i < cap; i += EV_T) os[i] = 0.f;
 }
 
-// The rows that stay, moved.  A work-group takes 128 bytes of one head's keys
-// or values of a sequence and walks the entries in order, 256 at a time: read,
-// wait for all, write.  Entry i comes from index[i] >= i, and the ones read
-// later lie above all that are written before, so the pages may be the same.
-constexpr int EM_ROWS = 256;
-template <int DH>
-__global__ __launch_bounds__(256) void k_evict_move(PagedArgs c, const int32_t* __restrict__ out_table,
-                                                    long long orow, int out_cols,
-                                                    const int32_t* __restrict__ index,
-                                                    const int32_t* __restrict__ new_lens, int keep) {
-  constexpr int PARTS = DH / 64;
-  const int s = blockIdx.y, tid = threadIdx.x;
-  const int part = blockIdx.x % PARTS, h = (blockIdx.x / PARTS) % c.heads;
-  const bool isv = blockIdx.x / PARTS >= c.heads;
-  const long long page = isv ? c.vp : c.kp, slot = isv ? c.vs : c.ks;
-  bf16_t* base = (isv ? c.v + h * c.vh : c.k + h * c.kh) + part * 64 + (tid & 7) * 8;
+// The rows that stay, moved: keys or values of one head, 8 NT / W entries at a
+// time (W lanes of 16 bytes a row).  Into other pages each work-group takes one
+// such tile.  Into the same pages (their ids agree in some place) a sequence's
+// first work-group takes all of them, in order: read, wait for all, write.  Entry i
+// comes from index[i] >= i, and the ones read later lie above all that are written
+// before.
+template <int DH, int NT>
+__global__ __launch_bounds__(NT) void k_evict_move(PagedArgs c, const int32_t* __restrict__ out_table,
+                                                   long long orow, int out_cols,
+                                                   const int32_t* __restrict__ index,
+                                                   const int32_t* __restrict__ new_lens, int keep) {
+  constexpr int W = DH / 8, RP = NT / W, ROWS = 8 * RP;   // rows a load, rows a tile
+  __shared__ long long s_from[2][ROWS], s_to[2][ROWS];
+  const int s = blockIdx.z, tid = threadIdx.x;
   const int left = new_lens[s];
-  for (int i0 = 0; i0 < left; i0 += EM_ROWS) {
-    uint4 w[8];
-    bf16_t* to[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = i0 + u * 32 + (tid >> 3);
-      to[u] = nullptr;
-      if (i < left) {
-        const int e = index[(long long)s * keep + i];
-        const int a = pg_read(c.table[s * c.trow + (e >> c.sh)], c.pages);
-        const int b = out_table[s * orow + (i >> c.sh)];
-        w[u] = *(const uint4*)(base + a * page + pg_slot(e, c.sh, slot));
-        if (pg_writable(b, c.pages)) to[u] = base + b * page + pg_slot(i, c.sh, slot);
+  int i0 = blockIdx.x * ROWS;
+  if (i0 >= left) return;
+  const int h = blockIdx.y % c.heads;
+  const bool isv = (int)blockIdx.y >= c.heads;
+  const long long page = isv ? c.vp : c.kp, slot = isv ? c.vs : c.ks;
+  bf16_t* base = (isv ? c.v + h * c.vh : c.k + h * c.kh) + (tid % W) * 8;
+  const int32_t* from = c.table + s * c.trow;
+  const int32_t* to = out_table + s * orow;
+  bool same = from == to;
+  if (!same) {
+    const int n = min(((left - 1) >> c.sh) + 1, c.cols);
+    int any = 0;
+    for (int i = tid; i < n; i += NT) any |= from[i] == to[i];
+    same = __syncthreads_or(any);
+  }
+  if (same && blockIdx.x) return;
+  const int end = same ? left : min(left, i0 + ROWS);
+  // where rows i .. i + ROWS - 1 come from and go to, -1: nowhere
+  auto places = [&](int i, int b) {
+    for (int k = tid; k < ROWS; k += NT) {
+      long long f = 0, t = -1;
+      if (i + k < end) {
+        const int e = index[(long long)s * keep + i + k];
+        const int id = to[(i + k) >> c.sh];
+        f = pg_read(from[e >> c.sh], c.pages) * page + pg_slot(e, c.sh, slot);
+        if (pg_writable(id, c.pages)) t = id * page + pg_slot(i + k, c.sh, slot);
       }
+      s_from[b][k] = f;
+      s_to[b][k] = t;
     }
+  };
+  places(i0, 0);
+  __syncthreads();
+  for (int b = 0; i0 < end; i0 += ROWS, b ^= 1) {
+    uint4 w[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) w[u] = *(const uint4*)(base + s_from[b][u * RP + tid / W]);
+    if (i0 + ROWS < end) places(i0 + ROWS, b ^ 1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every read of the wave has returned
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (to[u]) *(uint4*)to[u] = w[u];
-    __syncthreads();
+    for (int u = 0; u < 8; ++u) {
+      const long long t = s_to[b][u * RP + tid / W];
+      if (t >= 0) *(uint4*)(base + t) = w[u];
+    }
+    if (i0 + ROWS < end) __syncthreads();   // s_to[b] is read before the next places take it
   }
+}
+
+template <int DH, int NT>
+static void evict_move(const PagedArgs& c, const int32_t* out_table, long long out_row, int out_cols,
+                       const int32_t* index, const int32_t* new_lens, int keep, hipStream_t st) {
+  constexpr int ROWS = 8 * NT / (DH / 8);
+  const bool same = out_table == c.table;
+  const dim3 grid(same ? 1u : (unsigned)((keep + ROWS - 1) / ROWS), (unsigned)(2 * c.heads),
+                  (unsigned)c.seqs);
+  hipLaunchKernelGGL((k_evict_move<DH, NT>), grid, dim3(NT), 0, st, c, out_table, out_row, out_cols,
+                     index, new_lens, keep);
 }
 
 hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, long long out_row,
@@ -177,17 +269,25 @@ hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, lon
                        int32_t* index, int32_t* new_lens, float* out, long long orow,
                        hipStream_t st) {
   if (c.seqs == 0) return hipSuccess;
-  hipLaunchKernelGGL(k_evict_pick, dim3(c.seqs), dim3(EV_T), 0, st, c.lens, c.cols, c.sh, w, wrow,
-                     keep, recent, index, new_lens, out, orow, c.cols << c.sh);
-  hipError_t e = hipGetLastError();
+  if (Dh != 64 && Dh != 128) return hipErrorInvalidValue;
+  const int cap = c.cols << c.sh;
+#define ANN_EP(N)                                                                                \
+  hipLaunchKernelGGL(k_evict_pick<N>, dim3(c.seqs), dim3(EV_T), 0, st, c.lens, c.cols, c.sh, w,  \
+                     wrow, keep, recent, index, new_lens, out, orow, cap)
+  if (cap <= 2 * EV_T) ANN_EP(2);
+  else if (cap <= 8 * EV_T) ANN_EP(8);
+  else ANN_EP(16);
+#undef ANN_EP
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(2 * c.heads * (Dh / 64)), (unsigned)c.seqs), block(256);
-  if (Dh == 64)
-    hipLaunchKernelGGL(k_evict_move<64>, grid, block, 0, st, c, out_table, out_row, out_cols, index, new_lens, keep);
-  else if (Dh == 128)
-    hipLaunchKernelGGL(k_evict_move<128>, grid, block, 0, st, c, out_table, out_row, out_cols, index, new_lens, keep);
-  else
-    return hipErrorInvalidValue;
+  // in place a sequence's tiles follow one another: large work-groups
+#define ANN_EM(D, NT) evict_move<D, NT>(c, out_table, out_row, out_cols, index, new_lens, keep, st)
+  if (out_table == c.table) {
+    if (Dh == 64) ANN_EM(64, 1024); else ANN_EM(128, 1024);
+  } else {
+    if (Dh == 64) ANN_EM(64, 256); else ANN_EM(128, 256);
+  }
+#undef ANN_EM
   return hipGetLastError();
 }
 

@@ -102,11 +102,126 @@ __global__ __launch_bounds__(256) void k_qk_rope_any(QkRows a, long long n) {
   }
 }
 
+// The same for head dims 64 and 128 of 16-byte aligned rows: one wave for each
+// token, whose heads pass four (or so) at a time, W lanes of 16 bytes each, with
+// the token's angles read once.
+template <typename T>
+struct QrWord;
+template <>
+struct QrWord<float> {
+  static constexpr int NV = 4;
+  static __device__ __forceinline__ void load(const float* p, float* f) {
+    const float4 w = *(const float4*)p;
+    f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float* f) {
+    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+  }
+  static __device__ __forceinline__ void angles(const float* p, float* f) {
+    const float2 w = *(const float2*)p;
+    f[0] = w.x; f[1] = w.y;
+  }
+};
+template <>
+struct QrWord<bf16_t> {
+  static constexpr int NV = 8;
+  static __device__ __forceinline__ void load(const bf16_t* p, float* f) { unpack8(*(const uint4*)p, f); }
+  static __device__ __forceinline__ void store(bf16_t* p, const float* f) {
+    *(uint4*)p = make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+  }
+  static __device__ __forceinline__ void angles(const float* p, float* f) {
+    const float4 w = *(const float4*)p;
+    f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+  }
+};
+
+template <typename T, int D, bool BWD>
+__global__ __launch_bounds__(256) void k_qk_rope(QkRows a, int tokens) {
+  using V = QrWord<T>;
+  constexpr int NV = V::NV, W = D / NV, HP = 64 / W, U = BWD ? 2 : 4;
+  const int tok = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (tok >= tokens) return;
+  const int lane = threadIdx.x & 63, l = lane % W;
+  const int b = a.B == 1 ? 0 : tok / a.T, t = tok - b * a.T;
+  const int H = a.Hq + a.Hk;
+  const bool turn = l < W / 2;
+  const long long at = (long long)qk_position(a, b, t) * (D / 4) + (turn ? l : 0) * (NV / 2);
+  float cs[NV / 2], sn[NV / 2];
+  V::angles(a.cs + at, cs);
+  V::angles(a.sn + at, sn);
+  for (int h0 = 0; h0 < H; h0 += HP * U) {
+    float x[U][NV], g[BWD ? U : 1][NV];
+    QkRow<T> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = min(h0 + u * HP + lane / W, H - 1);   // past the last head: that one again
+      r[u] = qk_row<T, BWD>(a, b, t, h);
+      V::load(r[u].x + l * NV, x[u]);
+      if constexpr (BWD) V::load(r[u].g + l * NV, g[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h0 + u * HP >= H) break;
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) ss += x[u][j] * x[u][j];
+      const float rr = rsqrtf(group_sum<W>(ss) / (float)D + a.eps);
+      float y[NV];
+      if constexpr (BWD) {
+        float sg = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j += 2) {
+          const float u0 = g[u][j], u1 = g[u][j + 1];
+          y[j] = turn ? cs[j / 2] * u0 - sn[j / 2] * u1 : u0;
+          y[j + 1] = turn ? cs[j / 2] * u1 + sn[j / 2] * u0 : u1;
+          sg += x[u][j] * y[j] + x[u][j + 1] * y[j + 1];
+        }
+        const float f = rr * rr * (group_sum<W>(sg) / (float)D);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) y[j] = rr * (y[j] - x[u][j] * f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; j += 2) {
+          const float u0 = x[u][j] * rr, u1 = x[u][j + 1] * rr;
+          y[j] = turn ? cs[j / 2] * u0 + sn[j / 2] * u1 : u0;
+          y[j + 1] = turn ? cs[j / 2] * u1 - sn[j / 2] * u0 : u1;
+        }
+      }
+      if (h0 + u * HP + lane / W < H) V::store(r[u].y + l * NV, y);
+    }
+  }
+}
+
+// Whether 16-byte words reach every row of the operands.
+static bool qk_words(const QkRows& a, bool bwd, int size) {
+  const auto fine = [&](const void* p, const long long* s) {
+    const long long m = 16 / size - 1;
+    return (((uintptr_t)p) & 15) == 0 && ((s[0] | s[1] | s[2]) & m) == 0;
+  };
+  return (a.D == 64 || a.D == 128) && fine(a.q, a.qs) && (!a.Hk || fine(a.k, a.ks)) &&
+         (!bwd || (fine(a.gq, a.gqs) && (!a.Hk || fine(a.gk, a.gks)))) &&
+         (((uintptr_t)a.qo | (uintptr_t)a.ko | (uintptr_t)a.cs | (uintptr_t)a.sn) & 15) == 0;
+}
+
 hipError_t qk_norm_rope(const QkRows& a, bool bwd, int dtype, hipStream_t st) {
-  const long long n = (long long)a.B * a.T * (a.Hq + a.Hk);
+  const long long tokens = (long long)a.B * a.T, n = tokens * (a.Hq + a.Hk);
   if (n == 0) return hipSuccess;
   if ((n + 3) / 4 > 0x7fffffffLL) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((n + 3) / 4)), block(256);
+  const dim3 block(256);
+  if (qk_words(a, bwd, dtype == 0 ? 4 : 2) && tokens < (1LL << 31)) {
+    const dim3 grid((unsigned)((tokens + 3) / 4));
+#define ANN_QK(TY, D)                                                                          \
+  if (bwd) hipLaunchKernelGGL((k_qk_rope<TY, D, true>), grid, block, 0, st, a, (int)tokens);  \
+  else hipLaunchKernelGGL((k_qk_rope<TY, D, false>), grid, block, 0, st, a, (int)tokens)
+    if (dtype == 0) {
+      if (a.D == 64) { ANN_QK(float, 64); } else { ANN_QK(float, 128); }
+    } else {
+      if (a.D == 64) { ANN_QK(bf16_t, 64); } else { ANN_QK(bf16_t, 128); }
+    }
+#undef ANN_QK
+    return hipGetLastError();
+  }
+  const dim3 grid((unsigned)((n + 3) / 4));
 #define ANN_QK(TY)                                                                     \
   if (bwd) hipLaunchKernelGGL((k_qk_rope_any<TY, true>), grid, block, 0, st, a, n);   \
   else hipLaunchKernelGGL((k_qk_rope_any<TY, false>), grid, block, 0, st, a, n)

@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._stream import current_stream
+from ._stream import current_stream, on_device
 
 
 def _dt(x):
@@ -76,55 +76,73 @@ def rms(x, eps=1e-6):
     return y
 
 
-def _qk_struct(q, k, cs, sn, pos, eps, grads=()):
-    """AnnQkRows of (B, T, H, D) rows, and what has to outlive the call."""
-    rows = []
-    for x in (q, k, *grads):
-        if not (isinstance(x, torch.Tensor) and x.is_cuda):
-            raise ValueError("expected a GPU tensor")
+def _table(x, d):
+    """cs or sn as the kernel reads it: fp32, contiguous."""
+    if not isinstance(x, torch.Tensor) or x.get_device() != d:
+        raise ValueError("the tables must be GPU tensors on the rows' device")
+    if x.dim() != 2:
+        raise ValueError("the tables must be (rows, D/4)")
+    if x.dtype is not torch.float32 or not x.is_contiguous():
+        x = x.float().contiguous()
+    return x
+
+
+def _qk_struct(q, k, cs, sn, pos, eps, gq=None, gk=None):
+    """AnnQkRows of (B, T, H, D) rows, its outputs, the device, and what has to
+    outlive the call."""
+    rows = (q, k) if gq is None else (q, k, gq, gk)
+    d = q.get_device() if isinstance(q, torch.Tensor) else -1
+    copied = None
+    for i, x in enumerate(rows):
+        if not isinstance(x, torch.Tensor) or x.get_device() != d or d < 0:
+            raise ValueError("expected GPU tensors on one device")
         if x.dim() != 4:
             raise ValueError("rows must be (B, T, H, D)")
-        rows.append(x if x.stride(3) == 1 else x.contiguous())
-    q, k = rows[:2]
-    B, T, Hq, D = q.shape
-    Hk = k.shape[2]
-    if k.shape[:2] != (B, T) or k.shape[3] != D:
-        raise ValueError(f"k {tuple(k.shape)} must be (B, T, Hk, D) of q {tuple(q.shape)}")
-    for x, like in zip(rows[2:], (q, k)):
-        if x.shape != like.shape:
-            raise ValueError(f"gradient {tuple(x.shape)} must match {tuple(like.shape)}")
-    dt = _dt(q)
-    cs, sn = _gpu(cs).float(), _gpu(sn).float()
-    if D % 4 or cs.dim() != 2 or cs.shape[1] != D // 4 or sn.shape != cs.shape:
-        raise ValueError("D must be a multiple of 4 and the tables (rows, D/4)")
-    a = _lib.AnnQkRows()
-    if isinstance(pos, torch.Tensor):
-        if pos.dtype != torch.int32 or tuple(pos.shape) not in ((B,), (B, T)):
-            raise ValueError("pos must be a number or int32 of shape (B,) or (B, T)")
-        pos = _gpu(pos)
-        a.pos, a.pos_each = pos.data_ptr(), int(pos.dim() == 2)
-        rows.append(pos)
-    else:
-        a.pos0 = pos
-        if B and T and (pos < 0 or pos + T > cs.shape[0]):
-            raise ValueError("tables must be (>= pos + T, D/4)")
-    for x in rows[1:] + [cs, sn]:
-        if x.device != q.device:
-            raise ValueError(f"tensors on {q.device} and {x.device}")
-    for x in rows[1:2 + len(grads)]:
-        if x.dtype != q.dtype:
+        if x.dtype is not q.dtype:
             raise TypeError(f"dtypes {q.dtype} and {x.dtype} differ")
-    a.q, a.k = q.data_ptr(), k.data_ptr()
-    a.q_stride[:], a.k_stride[:] = q.stride()[:3], k.stride()[:3]
-    if grads:
-        a.gq, a.gk = rows[2].data_ptr(), rows[3].data_ptr()
-        a.gq_stride[:], a.gk_stride[:] = rows[2].stride()[:3], rows[3].stride()[:3]
-    a.cs, a.sn, a.table_rows = cs.data_ptr(), sn.data_ptr(), cs.shape[0]
-    a.B, a.T, a.Hq, a.Hk, a.D, a.dtype, a.eps = B, T, Hq, Hk, D, dt, eps
-    qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    ko = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-    a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
-    return a, (rows, cs, sn), qo, ko
+        if x.stride(3) != 1:
+            copied = copied or list(rows)
+            copied[i] = x.contiguous()
+    if copied:
+        rows = copied
+        q, k = rows[:2]
+    dt = _dt(q)
+    B, T, Hq, D = q.shape
+    Bk, Tk, Hk, Dk = k.shape
+    if Bk != B or Tk != T or Dk != D:
+        raise ValueError(f"k {tuple(k.shape)} must be (B, T, Hk, D) of q {tuple(q.shape)}")
+    cs, sn = _table(cs, d), _table(sn, d)
+    n = cs.shape[0]
+    if D % 4 or cs.shape[1] != D // 4 or sn.shape != cs.shape:
+        raise ValueError("D must be a multiple of 4 and the tables (rows, D/4)")
+    at, each, pos0 = 0, 0, 0
+    if isinstance(pos, torch.Tensor):
+        if pos.dtype is not torch.int32 or tuple(pos.shape) not in ((B,), (B, T)):
+            raise ValueError("pos must be a number or int32 of shape (B,) or (B, T)")
+        if pos.get_device() != d:
+            raise ValueError("pos must be on the rows' device")
+        pos = pos.contiguous()
+        at, each = pos.data_ptr(), int(pos.dim() == 2)
+    else:
+        pos0 = int(pos)
+        if B and T and (pos0 < 0 or pos0 + T > n):
+            raise ValueError("tables must be (>= pos + T, D/4)")
+    g = (0, 0, 0, 0, 0, 0)
+    gp = (0, 0)
+    if gq is not None:
+        gq, gk = rows[2:]
+        if gq.shape != q.shape or gk.shape != k.shape:
+            raise ValueError(f"gradients {tuple(gq.shape)}, {tuple(gk.shape)} must match "
+                             f"{tuple(q.shape)}, {tuple(k.shape)}")
+        g = (*gq.stride()[:3], *gk.stride()[:3])
+        gp = (gq.data_ptr(), gk.data_ptr())
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    a = _lib.AnnQkRows.from_values(
+        q.data_ptr(), k.data_ptr(), 0, *gp, qo.data_ptr(), ko.data_ptr(), *q.stride()[:3],
+        *k.stride()[:3], 0, 0, 0, *g, cs.data_ptr(), sn.data_ptr(), at, each, pos0, n, B, T, Hq, Hk,
+        D, dt, eps)
+    return a, d, qo, ko, (rows, cs, sn, pos)
 
 
 def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
@@ -138,14 +156,14 @@ def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
     ``pos`` is the position of token 0, or an int32 GPU tensor: (B,) one start
     for each batch row, (B, T) one position for each token (a value outside the
     tables takes their nearest row)."""
-    a, keep, qo, ko = _qk_struct(q, k, cs, sn, pos, eps)
-    _lib.launch(qo.device, _lib.lib().ann_op_qk_norm_rope, a)
+    a, d, qo, ko, keep = _qk_struct(q, k, cs, sn, pos, eps)
+    _lib.check(on_device(d, _lib.lib().ann_op_qk_norm_rope, a))
     return qo, ko
 
 
 def qk_norm_rope_bwd(gq, gk, q, k, cs, sn, pos=0, eps=1e-6):
     """Gradients of ``qk_norm_rope``'s inputs from those of its outputs -> (dq, dk).
     ``q`` and ``k`` are its inputs."""
-    a, keep, qo, ko = _qk_struct(q, k, cs, sn, pos, eps, (gq, gk))
-    _lib.launch(qo.device, _lib.lib().ann_op_qk_norm_rope_bwd, a)
+    a, d, qo, ko, keep = _qk_struct(q, k, cs, sn, pos, eps, gq, gk)
+    _lib.check(on_device(d, _lib.lib().ann_op_qk_norm_rope_bwd, a))
     return qo, ko

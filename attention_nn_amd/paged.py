@@ -30,77 +30,103 @@ its current stream.
 import torch
 
 from . import _lib
+from ._stream import on_device
 
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+_Tensor, _empty = torch.Tensor, torch.empty
 
 
-def _check(name, x, dtype, dim, device=None):
-    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+def _refuse(name, x, dtype, dim, d):
+    if not isinstance(x, _Tensor) or x.get_device() < 0:
         raise ValueError(f"{name}: expected a GPU tensor")
     if x.dtype != dtype:
         raise TypeError(f"{name}: {x.dtype}, expected {dtype}")
     if x.dim() != dim:
         raise ValueError(f"{name}: expected {dim} dimensions, got shape {tuple(x.shape)}")
-    if device is not None and x.device != device:
-        raise ValueError(f"{name} is on {x.device}, not on {device}")
-    return x
+    raise ValueError(f"{name} is on {x.device}, not on cuda:{d}")
 
 
-def _rows(name, x, device):
+def _check(name, x, dtype, dim, d):
+    if not isinstance(x, _Tensor) or x.get_device() != d or x.dtype is not dtype or x.dim() != dim:
+        _refuse(name, x, dtype, dim, d)
+
+
+def _pool(k_cache):
+    """The GPU that the cache is on."""
+    if not isinstance(k_cache, _Tensor) or k_cache.get_device() < 0:
+        raise ValueError("k_cache: expected a GPU tensor")
+    return k_cache.get_device()
+
+
+def _rows(name, x, d):
     """(rows, heads, head_dim) bf16 that 16-byte loads can read: x, or a copy."""
-    _check(name, x, _BF16, 3, device)
-    st = x.stride()
-    if st[2] != 1 or (st[0] | st[1]) & 7 or x.data_ptr() & 15:
+    _check(name, x, _BF16, 3, d)
+    a, b, c = x.stride()
+    if c != 1 or (a | b) & 7 or x.data_ptr() & 15:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
-def _column(name, x, n, device):
-    _check(name, x, _I32, 1, device)
+def _column(name, x, n, d):
+    _check(name, x, _I32, 1, d)
     if x.shape[0] != n:
         raise ValueError(f"{name} has {x.shape[0]} elements, expected {n}")
-    return x if x.stride(0) == 1 or n <= 1 else x.contiguous()
+    return x if n <= 1 or x.stride(0) == 1 else x.contiguous()
 
 
-def _cache(k_cache, v_cache, table, lens, starts=None, rows=0):
-    """AnnPaged of the call, and what has to outlive it."""
-    device = _check("k_cache", k_cache, _BF16, 4).device
+def _out(out, like):
+    _check("out", out, _BF16, 3, like.get_device())
+    if out.shape != like.shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {tuple(like.shape)}")
+    return out
+
+
+def _cache(d, k_cache, v_cache, table, lens, starts=None, rows=0):
+    """AnnPaged of the call, (sequences, table columns, kv heads, page size, head
+    dimension), the table, and what has to outlive the call."""
+    _check("k_cache", k_cache, _BF16, 4, d)
+    _check("table", table, _I32, 2, d)
     pages, heads, page, dim = k_cache.shape
-    _check("table", table, _I32, 2, device)
     S, cols = table.shape
-    if cols > 1 and table.stride(1) != 1:
+    ts, tc = table.stride()
+    if tc != 1 and cols > 1:
         table = table.contiguous()
-    lens = _column("lens", lens, S, device)
-    c = _lib.AnnPaged()
-    keep = [table, lens]
-    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if x is None:
-            continue
-        _check(name, x, _BF16, 4, device)
-        if tuple(x.shape) != (pages, heads, page, dim):
-            raise ValueError(f"{name} {tuple(x.shape)} differs from {(pages, heads, page, dim)}")
-        if x.stride(3) != 1:
-            raise ValueError(f"{name}: the head dimension must be contiguous")
-    c.k = k_cache.data_ptr()
-    c.k_page, c.k_head, c.k_slot = k_cache.stride()[:3]
+        ts = cols
+    lens = _column("lens", lens, S, d)
+    kp, kh, ks, kd = k_cache.stride()
+    v, vp, vh, vs, vd = 0, 0, 0, 0, 1
     if v_cache is not None:
-        c.v = v_cache.data_ptr()
-        c.v_page, c.v_head, c.v_slot = v_cache.stride()[:3]
+        _check("v_cache", v_cache, _BF16, 4, d)
+        if v_cache.shape != k_cache.shape:
+            raise ValueError(f"v_cache {tuple(v_cache.shape)} differs from {tuple(k_cache.shape)}")
+        v = v_cache.data_ptr()
+        vp, vh, vs, vd = v_cache.stride()
+    if kd != 1 or vd != 1:
+        raise ValueError("the caches' head dimension must be contiguous")
+    first = 0
     if starts is not None:
-        starts = _column("starts", starts, S + 1, device)
-        c.starts = starts.data_ptr()
-        keep.append(starts)
-    c.table, c.table_row, c.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
-    c.pages, c.page_size, c.heads, c.head_dim = pages, page, heads, dim
-    c.seqs, c.cols, c.rows = S, cols, rows
-    return c, device, keep
+        starts = _column("starts", starts, S + 1, d)
+        first = starts.data_ptr()
+    c = _lib.AnnPaged.from_values(k_cache.data_ptr(), v, kp, kh, ks, vp, vh, vs, table.data_ptr(),
+                                  ts, first, lens.data_ptr(), pages, page, heads, dim, S, cols, rows)
+    return c, (S, cols, heads, page, dim), table, (lens, starts)
 
 
-def _weight(name, weight, S, cap, device):
-    _check(name, weight, _F32, 2, device)
+def _weight(name, weight, S, cap, d):
+    _check(name, weight, _F32, 2, d)
     if tuple(weight.shape) != (S, cap):
         raise ValueError(f"{name} {tuple(weight.shape)} must be (sequences, table entries) = {(S, cap)}")
-    return weight if weight.stride(1) == 1 or cap <= 1 else weight.contiguous()
+    return weight if cap <= 1 or weight.stride(1) == 1 else weight.contiguous()
+
+
+def _angles(name, x, dim, d):
+    _check(name, x, _F32, 2, d)
+    n, m = x.shape
+    if m != dim // 4 or n < 1:
+        raise ValueError(f"{name} {tuple(x.shape)} must be (positions, {dim // 4})")
+    if not x.is_contiguous() or x.data_ptr() & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
 
 
 def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps=1e-6, out=None):
@@ -112,46 +138,41 @@ def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps
     A token's position is its entry, or ``pos`` (rows,) int32 (after an eviction
     the positions run ahead of the entries); the tables ``cs``, ``sn`` (positions,
     head_dim / 4) end there (a position outside takes their nearest row)."""
-    q = _rows("q", q, _check("k_cache", k_cache, _BF16, 4).device)
+    d = _pool(k_cache)
+    q, k, v = _rows("q", q, d), _rows("k", k, d), _rows("v", v, d)
     N, H, D = q.shape
-    c, device, keep = _cache(k_cache, v_cache, table, lens, starts, N)
-    k, v = _rows("k", k, device), _rows("v", v, device)
-    if tuple(k.shape) != (N, c.heads, c.head_dim) or k.shape != v.shape or D != c.head_dim:
+    c, (S, _, heads, _, dim), table, keep = _cache(d, k_cache, v_cache, table, lens, starts, N)
+    if k.shape != (N, heads, dim) or v.shape != (N, heads, dim) or D != dim:
         raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} must be (rows, kv_heads, head_dim) "
-                         f"= {(N, c.heads, c.head_dim)} beside q {tuple(q.shape)}")
-    tabs = []
-    for name, x in (("cs", cs), ("sn", sn)):
-        _check(name, x, _F32, 2, device)
-        if x.shape[1] != D // 4 or x.shape[0] < 1 or x.shape != cs.shape:
-            raise ValueError(f"{name} {tuple(x.shape)} must be (positions, {D // 4})")
-        tabs.append(x if x.is_contiguous() and not x.data_ptr() & 15 else
-                    x.clone(memory_format=torch.contiguous_format))
-    if out is None:
-        out = torch.empty((N, H, D), dtype=_BF16, device=device)
-    else:
-        _check("out", out, _BF16, 3, device)
-        if out.shape != q.shape or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous {tuple(q.shape)}")
-    a = _lib.AnnQkRows()
+                         f"= {(N, heads, dim)} beside q {tuple(q.shape)}")
+    cs, sn = _angles("cs", cs, D, d), _angles("sn", sn, D, d)
+    if cs.shape != sn.shape:
+        raise ValueError(f"cs {tuple(cs.shape)} and sn {tuple(sn.shape)} differ")
+    out = _empty((N, H, D), dtype=_BF16, device=q.device) if out is None else _out(out, q)
+    at = 0
     if pos is not None:
-        pos = _column("pos", pos, N, device)
-        a.pos, a.pos_each = pos.data_ptr(), 1
-    a.q, a.k, a.v, a.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.q_stride[1], a.q_stride[2] = q.stride()[:2]
-    a.k_stride[1], a.k_stride[2] = k.stride()[:2]
-    a.v_stride[1], a.v_stride[2] = v.stride()[:2]
-    a.cs, a.sn, a.table_rows = tabs[0].data_ptr(), tabs[1].data_ptr(), cs.shape[0]
-    a.B, a.T, a.Hq, a.Hk, a.D, a.dtype, a.eps = 1, N, H, c.heads, D, _lib.DTYPE_BF16, eps
-    _lib.launch(device, _lib.lib().ann_op_paged_append, c, a)
+        pos = _column("pos", pos, N, d)
+        at = pos.data_ptr()
+    qt, qh, _ = q.stride()
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    a = _lib.AnnQkRows.from_values(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, out.data_ptr(), 0,
+                                   0, qt, qh, 0, kt, kh, 0, vt, vh, 0, 0, 0, 0, 0, 0, cs.data_ptr(),
+                                   sn.data_ptr(), at, 1, 0, cs.shape[0], 1, N, H, heads, D,
+                                   _lib.DTYPE_BF16, eps)
+    rc = on_device(d, _lib.lib().ann_op_paged_append, c, a)
+    if rc:
+        _lib.check(rc)
     return out
 
 
 def _queries(q, k_cache, v_cache, table, starts, lens):
-    q = _rows("q", q, _check("k_cache", k_cache, _BF16, 4).device)
-    c, device, keep = _cache(k_cache, v_cache, table, lens, starts, q.shape[0])
-    if q.shape[2] != c.head_dim:
-        raise ValueError(f"q {tuple(q.shape)}: the cache's head dimension is {c.head_dim}")
-    return q, c, device, keep
+    d = _pool(k_cache)
+    q = _rows("q", q, d)
+    c, sizes, table, keep = _cache(d, k_cache, v_cache, table, lens, starts, q.shape[0])
+    if q.shape[2] != sizes[4]:
+        raise ValueError(f"q {tuple(q.shape)}: the cache's head dimension is {sizes[4]}")
+    return q, d, c, sizes, (table, keep)
 
 
 def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_lse=False, out=None):
@@ -162,22 +183,20 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     (rows, heads) fp32, the log of each softmax sum.  A token that sees nothing
     gets 0 and -inf.  Weights enter the product with the values in bf16, as the
     framework's attention forms it; scores, softmax and sums are fp32."""
-    q, c, device, keep = _queries(q, k_cache, v_cache, table, starts, lens)
+    q, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
     N, H, D = q.shape
-    if out is None:
-        out = torch.empty((N, H, D), dtype=_BF16, device=device)
-    else:
-        _check("out", out, _BF16, 3, device)
-        if out.shape != q.shape or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous {tuple(q.shape)}")
-    lse = torch.empty((N, H), dtype=_F32, device=device) if want_lse else None
+    device = q.device
+    out = _empty((N, H, D), dtype=_BF16, device=device) if out is None else _out(out, q)
     L = _lib.lib()
     nws = L.ann_op_paged_attention_ws_bytes(c, H, window)
-    ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
-    st = q.stride()
-    _lib.launch(device, L.ann_op_paged_attention, c, q.data_ptr(), st[0], st[1], H, scale,
-                window, out.data_ptr(), lse.data_ptr() if want_lse else None,
-                ws.data_ptr() if nws else None, nws)
+    lse = _empty((N, H), dtype=_F32, device=device) if want_lse else None
+    ws = _empty(nws, dtype=torch.uint8, device=device) if nws else None
+    qt, qh, _ = q.stride()
+    rc = on_device(d, L.ann_op_paged_attention, c, q.data_ptr(), qt, qh, H, scale, window,
+                   out.data_ptr(), lse.data_ptr() if want_lse else None,
+                   ws.data_ptr() if nws else None, nws)
+    if rc:
+        _lib.check(rc)
     return (out, lse) if want_lse else out
 
 
@@ -186,24 +205,27 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
     each entry receives from the new tokens ``q``, over all their heads; ``lse`` as
     ``attention`` returned it for the same tokens.  -> a new tensor, or ``out``,
     which may be ``weight``.  Entries behind a sequence keep their weight."""
-    q, c, device, keep = _queries(q, k_cache, None, table, starts, lens)
+    q, d, c, (S, cols, _, page, _), keep = _queries(q, k_cache, None, table, starts, lens)
     N, H, _ = q.shape
-    _check("lse", lse, _F32, 2, device)
-    if tuple(lse.shape) != (N, H):
+    _check("lse", lse, _F32, 2, d)
+    if lse.shape != (N, H):
         raise ValueError(f"lse {tuple(lse.shape)} must be {(N, H)}")
-    lse = lse.contiguous()
-    weight = _weight("weight", weight, c.seqs, c.cols * c.page_size, device)
+    if not lse.is_contiguous():
+        lse = lse.contiguous()
+    weight = _weight("weight", weight, S, cols * page, d)
     if out is None:
-        out = torch.empty(weight.shape, dtype=_F32, device=device)
-    elif _weight("out", out, c.seqs, c.cols * c.page_size, device) is not out:
+        out = _empty((S, cols * page), dtype=_F32, device=q.device)
+    elif _weight("out", out, S, cols * page, d) is not out:
         raise ValueError("out: rows must be contiguous")
     L = _lib.lib()
     nws = L.ann_op_paged_weight_ws_bytes(c, H)
-    ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
-    st = q.stride()
-    _lib.launch(device, L.ann_op_paged_weight, c, q.data_ptr(), st[0], st[1], H, lse.data_ptr(),
-                scale, window, weight.data_ptr(), weight.stride(0), out.data_ptr(),
-                out.stride(0), ws.data_ptr() if nws else None, nws)
+    ws = _empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    qt, qh, _ = q.stride()
+    rc = on_device(d, L.ann_op_paged_weight, c, q.data_ptr(), qt, qh, H, lse.data_ptr(), scale,
+                   window, weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
+                   ws.data_ptr() if nws else None, nws)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -218,23 +240,30 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
     ``out_table`` names pages that ``table`` does not (or is ``table``).  Keys hold
     their rotation, so later tokens go on at their own positions: pass ``pos`` to
     ``append``."""
-    c, device, held = _cache(k_cache, v_cache, table, lens)
-    cap = c.cols * c.page_size
-    weight = _weight("weight", weight, c.seqs, cap, device)
-    to = held[0] if out_table is None else _check("out_table", out_table, _I32, 2, device)
-    if to.shape[0] != c.seqs:
-        raise ValueError(f"out_table {tuple(to.shape)} must have {c.seqs} rows")
-    if to.shape[1] > 1 and to.stride(1) != 1:
-        to = to.contiguous()
+    d = _pool(k_cache)
+    c, (S, cols, _, page, _), table, held = _cache(d, k_cache, v_cache, table, lens)
+    cap = cols * page
+    weight = _weight("weight", weight, S, cap, d)
+    if out_table is None:
+        out_table = table
+    else:
+        _check("out_table", out_table, _I32, 2, d)
+        if out_table.shape[0] != S:
+            raise ValueError(f"out_table {tuple(out_table.shape)} must have {S} rows")
+        if out_table.shape[1] > 1 and out_table.stride(1) != 1:
+            out_table = out_table.contiguous()
     keep, recent = int(keep), int(recent)
     if keep < 1:
         raise ValueError(f"keep={keep} must be at least 1")
-    if keep > to.shape[1] * c.page_size:
-        raise ValueError(f"{to.shape[1]} pages of {c.page_size} do not hold keep={keep} entries")
-    index = torch.empty((c.seqs, keep), dtype=_I32, device=device)
-    left = torch.empty((c.seqs,), dtype=_I32, device=device)
-    out = torch.empty((c.seqs, cap), dtype=_F32, device=device)
-    _lib.launch(device, _lib.lib().ann_op_paged_evict, c, to.data_ptr(), to.stride(0), to.shape[1],
-                weight.data_ptr(), weight.stride(0), keep, recent, index.data_ptr(),
-                left.data_ptr(), out.data_ptr(), out.stride(0))
+    if keep > out_table.shape[1] * page:
+        raise ValueError(f"{out_table.shape[1]} pages of {page} do not hold keep={keep} entries")
+    device = k_cache.device
+    index = _empty((S, keep), dtype=_I32, device=device)
+    left = _empty((S,), dtype=_I32, device=device)
+    out = _empty((S, cap), dtype=_F32, device=device)
+    rc = on_device(d, _lib.lib().ann_op_paged_evict, c, out_table.data_ptr(), out_table.stride(0),
+                   out_table.shape[1], weight.data_ptr(), weight.stride(0), keep, recent,
+                   index.data_ptr(), left.data_ptr(), out.data_ptr(), cap)
+    if rc:
+        _lib.check(rc)
     return index, left, out
