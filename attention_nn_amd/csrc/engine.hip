@@ -1198,6 +1198,9 @@ int paged_args(const ann_paged* c, bool kv, bool tokens, PagedArgs* a) {
   if (((uintptr_t)c->k | (kv ? (uintptr_t)c->v : 0)) & 15 ||
       (c->k_page | c->k_head | c->k_slot) & 7 || (kv && ((c->v_page | c->v_head | c->v_slot) & 7)))
     return fail(ANN_E_ARG, "cache rows must be 16-byte aligned");
+  const int64_t far = 1 << 25;   // 16 slots within 32 bits of bytes
+  if (c->k_slot < 0 || c->k_slot > far || (kv && (c->v_slot < 0 || c->v_slot > far)))
+    return fail(ANN_E_ARG, "slots must lie at most 2^25 elements apart");
   *a = PagedArgs{(uint16_t*)c->k, (uint16_t*)c->v, c->k_page, c->k_head, c->k_slot, c->v_page,
                  c->v_head, c->v_slot, c->table, c->table_row, c->starts, c->lens, c->pages, sh,
                  c->heads, c->seqs, c->cols, c->rows};
@@ -1210,6 +1213,8 @@ int paged_query(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head
   if (heads < 1 || heads > 65535 || heads % c->heads)
     return fail(ANN_E_ARG, "%d query heads over %d cache heads", heads, c->heads);
   if (c->rows && !q) return fail(ANN_E_ARG, "null argument");
+  if ((long long)c->rows * heads > 0x7fffffffLL)
+    return fail(ANN_E_ARG, "%d rows of %d heads pass 2^31", c->rows, heads);
   if (((uintptr_t)q & 15) || ((q_row | q_head) & 7))
     return fail(ANN_E_ARG, "query rows must be 16-byte aligned");
   if (!(scale == scale) || scale - scale != 0.f) return fail(ANN_E_ARG, "scale must be finite");

@@ -59,6 +59,21 @@ ANN_HD long long pg_slot(int e, int sh, long long slot) {
   return (long long)(e & ((1 << sh) - 1)) * slot;
 }
 
+// n / d for 0 <= n < 2^31 by a product: m = ceil(2^s / d) with s = 31 + ceil(log2 d)
+// is below 2^32 for d > 1, and n (m d - 2^s) < 2^31 d <= 2^s keeps the quotient.
+struct FastDiv {
+  uint32_t m;
+  int s;   // 0: d is 1
+  ANN_HD int div(int n) const { return s ? (int)(((uint64_t)(uint32_t)n * m) >> s) : n; }
+  static inline FastDiv of(int d) {
+    if (d <= 1) return {0, 0};
+    int l = 0;
+    while ((1LL << l) < d) ++l;
+    const int s = 31 + l;
+    return {(uint32_t)(((1ULL << s) + d - 1) / d), s};
+  }
+};
+
 #if defined(__HIPCC__)
 // The sequence whose new tokens row n belongs to, by a whole wave: the last s
 // with starts[s] <= n, found among 64 of them at a time (two loads in a row up

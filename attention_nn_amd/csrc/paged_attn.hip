@@ -252,6 +252,17 @@ __device__ __forceinline__ bf16x8_t pa_query(const bf16_t* p, int neg) {
   return __builtin_bit_cast(bf16x8_t, w);
 }
 
+__device__ __forceinline__ bf16x8_t pa_join(pa_v4i16 a, pa_v4i16 b) {
+  return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The 16 entries of a cache from entry k0 on (a multiple of 16): a uniform
+// address, to which a lane adds its row's and column's 32 bits.
+__device__ __forceinline__ const unsigned char* pa_group(const bf16_t* head, int id, long long page,
+                                                         long long slot, int k0, int sh) {
+  return (const unsigned char*)(head + id * page + pg_slot(k0, sh, slot));
+}
+
 // Page ids ahead of their use: lane i of a wave holds the id of its i-th group of
 // 16 entries.
 struct PaPages {
@@ -335,17 +346,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
         // entries inside [a0, b0): where the whole group lies outside, the nearest one's page
         const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
         const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
-        const bf16_t* kp = kh + id * a.c.kp + pg_slot(k0, a.c.sh, a.c.ks);
-        const bf16_t* vp = vh + id * a.c.vp + pg_slot(k0, a.c.sh, a.c.vs);
-        const bf16_t* kr = kp + min(max(r16, rl), rh) * a.c.ks + g4 * 8;
+        const unsigned char* kp = pa_group(kh, id, a.c.kp, a.c.ks, k0, a.c.sh);
+        const unsigned char* vp = pa_group(vh, id, a.c.vp, a.c.vs, k0, a.c.sh);
+        const unsigned ko = (unsigned)(min(max(r16, rl), rh) * (int)a.c.ks * 2 + g4 * 16);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) kf[slot][g][ks] = *(const bf16x8_t*)(kr + ks * 32);
+        for (int ks = 0; ks < NKS; ++ks) kf[slot][g][ks] = *(const bf16x8_t*)(kp + ko + ks * 64);
 #pragma unroll
         for (int u = 0; u < LPW / 2; ++u) {
           const int r = u * RPL + lane / (RB / 16);   // row of the group
-          const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(16 * g + r)) * 8;
-          __builtin_amdgcn_global_load_lds(vp + min(max(r, rl), rh) * a.c.vs + col,
-                                           (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
+          const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
+          const unsigned vo = (unsigned)(min(max(r, rl), rh) * (int)a.c.vs * 2 + col);
+          __builtin_amdgcn_global_load_lds(vp + vo, (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
         }
       }
     };
@@ -394,9 +405,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
         constexpr int db = decltype(dc)::value;
         pa_wait_lgkm<2 * (NDB - 1 - db)>(v0[db]);
         pa_wait_lgkm<2 * (NDB - 1 - db)>(v1[db]);
-        const short a8[8] = {v0[db][0], v0[db][1], v0[db][2], v0[db][3],
-                             v1[db][0], v1[db][1], v1[db][2], v1[db][3]};
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8_t*)a8, pf, o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_join(v0[db], v1[db]), pf, o[db], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
     };
@@ -482,6 +491,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
   const int tile = w % tiles, kvh = (w / tiles) % a.c.heads, part = w / tiles / a.c.heads;
   int s = 0, row0 = 0;
   if (!pg_tile(a.c.starts, a.c.seqs, a.c.rows, a.heads / a.c.heads, a.few, BR, tile, s, row0)) return;
+  s = __builtin_amdgcn_readfirstlane(s);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
   const PaSeq q = pa_seq(a, s);
   const int nrow = min(BR, q.rows - row0);
   int lo, hi;
@@ -529,6 +540,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     return pg_read(table[min(max(key, a0), b0 - 1) >> a.c.sh], a.c.pages);
   };
   PaPages pg = {nt ? ids(0) : 0, nt > TPB ? ids(1) : 0};
+  // load x of a tile is rows x RPL .. of it: this lane's row of its group of 16 and column
+  int lrow[LPW], lcol[LPW];
+  unsigned koff[LPW], voff[LPW];
+#pragma unroll
+  for (int u = 0; u < LPW; ++u) {
+    const int r = (wv * LPW + u) * RPL + lane / (RB / 16);
+    lrow[u] = r % 16;
+    lcol[u] = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
+    koff[u] = (unsigned)(lrow[u] * (int)a.c.ks * 2 + lcol[u]);
+    voff[u] = (unsigned)(lrow[u] * (int)a.c.vs * 2 + lcol[u]);
+  }
   auto issue = [&](int t) {
     if (t && t % TPB == 0) {
       pg.now = pg.next;
@@ -536,33 +558,45 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     }
     const int kb = kb0 + BK * t;
     unsigned char* st = smem + (t & 1) * 2 * TB;
+    const bool inside = kb >= a0 && kb + BK <= b0;
 #pragma unroll
     for (int u = 0; u < LPW; ++u) {
       const int x = wv * LPW + u, g = x * RPL / 16;   // the load, and its group of 16 entries
       const int id = __builtin_amdgcn_readlane(pg.now, GPT * (t % TPB) + g);
-      const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
-      const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
-      const int r = x * RPL % 16 + lane / (RB / 16), rc = min(max(r, rl), rh);
-      const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(16 * g + r)) * 8;
-      __builtin_amdgcn_global_load_lds(kh + id * a.c.kp + pg_slot(k0, a.c.sh, a.c.ks) + rc * a.c.ks + col,
+      int k0 = kb + 16 * g;
+      unsigned ko = koff[u], vo = voff[u];
+      if (!inside) {   // rows outside [a0, b0) take the nearest inside
+        k0 = min(max(k0, a0 & ~15), (b0 - 1) & ~15);
+        const int rc = min(max(lrow[u], a0 - k0), b0 - 1 - k0);
+        ko = (unsigned)(rc * (int)a.c.ks * 2 + lcol[u]);
+        vo = (unsigned)(rc * (int)a.c.vs * 2 + lcol[u]);
+      }
+      __builtin_amdgcn_global_load_lds(pa_group(kh, id, a.c.kp, a.c.ks, k0, a.c.sh) + ko,
                                        (pa_lds_void*)(st + x * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vh + id * a.c.vp + pg_slot(k0, a.c.sh, a.c.vs) + rc * a.c.vs + col,
+      __builtin_amdgcn_global_load_lds(pa_group(vh, id, a.c.vp, a.c.vs, k0, a.c.sh) + vo,
                                        (pa_lds_void*)(st + TB + x * 1024), 16, 0, 0);
     }
   };
-  const int kx = pa_swz<DH>(r16);
-  const int trow = 4 * g4 + (r16 >> 2), tcol = 4 * (r16 & 3), vx = pa_swz<DH>(trow);
+  // fragment addresses of the first stage; the second lies 2 TB behind
+  const int trow = 4 * g4 + (r16 >> 2), tcol = 4 * (r16 & 3);
+  pa_lds_cchar* kadr[NKS];
+  pa_lds_cchar* vadr[NDB];
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks)
+    kadr[ks] = (pa_lds_cchar*)smem + r16 * RB + (((ks * 4 + g4) ^ pa_swz<DH>(r16)) << 4);
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+    vadr[db] = (pa_lds_cchar*)smem + TB + trow * RB + (tcol & 7) * 2 +
+               (((2 * db + (tcol >> 3)) ^ pa_swz<DH>(trow)) << 4);
 
-  if (nt) issue(0);
-  for (int t = 0; t < nt; ++t) {
+  auto step = [&](int t, auto stage) __attribute__((always_inline)) {
+    constexpr int ST = decltype(stage)::value * 2 * TB;
     const int kb = kb0 + BK * t;
     pa_wait_vm<0>();   // this wave's part of tile t is in LDS
     __syncthreads();   // every wave's; the other stage is free
     if (t + 1 < nt) issue(t + 1);
-    if (!(some && kb <= eh && el - (kb + BK - 1) < a.window)) continue;   // nothing in it for this wave
+    if (!(some && kb <= eh && el - (kb + BK - 1) < a.window)) return;   // nothing in it for this wave
     const bool full = kb >= a0 && kb + BK - 1 < b0 && kb + BK - 1 <= el && eh - kb < a.window;
-    const unsigned char* st = smem + (t & 1) * 2 * TB;
-    pa_lds_cchar* kst = (pa_lds_cchar*)st + r16 * RB;
 
     floatx4_t sacc[QB][NBLK];
 #pragma unroll
@@ -573,14 +607,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     bf16x8_t kf[2][NBLK];
     pa_static_for<0, NBLK>([&](auto bc) __attribute__((always_inline)) {
       constexpr int i = decltype(bc)::value;
-      kf[0][i] = pa_rd_b128<i * 16 * RB>(kst + ((g4 ^ kx) << 4));
+      kf[0][i] = pa_rd_b128<ST + i * 16 * RB>(kadr[0]);
     });
     pa_static_for<0, NKS>([&](auto kc) __attribute__((always_inline)) {
       constexpr int ks = decltype(kc)::value;
       if constexpr (ks + 1 < NKS) {
         pa_static_for<0, NBLK>([&](auto bc) __attribute__((always_inline)) {
           constexpr int i = decltype(bc)::value;
-          kf[(ks + 1) & 1][i] = pa_rd_b128<i * 16 * RB>(kst + ((((ks + 1) * 4 + g4) ^ kx) << 4));
+          kf[(ks + 1) & 1][i] = pa_rd_b128<ST + i * 16 * RB>(kadr[ks + 1]);
         });
       }
       constexpr int ahead = ks + 1 < NKS ? NBLK : 0;
@@ -595,10 +629,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     });
 
     float p[QB][NBLK][4];
+    if (full) {
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      float lm = -INFINITY;
-      if (full) {
+      for (int b = 0; b < QB; ++b) {
+        float lm = sacc[b][0][0];
 #pragma unroll
         for (int i = 0; i < NBLK; ++i)
 #pragma unroll
@@ -609,39 +643,45 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             p[b][i][r] = __builtin_amdgcn_exp2f(sacc[b][i][r] * a.sl2 - msl[b]);
-      } else {
-        unsigned ok = 0;
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        // entries jl .. jh of this lane's four of each block; a masked one's score is -inf
+        const int jl = max(a0, e[b] < a.window ? 0 : e[b] - a.window + 1) - kb - 4 * g4;
+        const int jh = min(b0 - 1, e[b]) - kb - 4 * g4;
+        float lm = -INFINITY;
 #pragma unroll
         for (int i = 0; i < NBLK; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int j = kb + 16 * i + 4 * g4 + r;
-            const bool v = j >= a0 && j < b0 && j <= e[b] && e[b] - j < a.window;
-            ok |= (unsigned)v << (4 * i + r);
-            lm = fmaxf(lm, v ? sacc[b][i][r] : -INFINITY);
+            const bool ok = 16 * i + r >= jl && 16 * i + r <= jh;
+            sacc[b][i][r] = ok ? sacc[b][i][r] : -INFINITY;
+            lm = fmaxf(lm, sacc[b][i][r]);
           }
         pa_raise<NDB>(lm, a.thr, a.sl2, m[b], msl[b], lsum[b], o[b]);
 #pragma unroll
         for (int i = 0; i < NBLK; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            p[b][i][r] = (ok >> (4 * i + r)) & 1
-                             ? __builtin_amdgcn_exp2f(sacc[b][i][r] * a.sl2 - msl[b]) : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const float v = __builtin_amdgcn_exp2f(sacc[b][i][r] * a.sl2 - msl[b]);
+            const bool ok = 16 * i + r >= jl && 16 * i + r <= jh;
+            p[b][i][r] = ok ? v : 0.f;
+          }
       }
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b)
 #pragma unroll
       for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lsum[b] += p[b][i][r];
-    }
-    pa_lds_cchar* vst = (pa_lds_cchar*)st + TB + trow * RB + (tcol & 7) * 2;
+        lsum[b] += (p[b][i][0] + p[b][i][1]) + (p[b][i][2] + p[b][i][3]);
     pa_static_for<0, NI>([&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value;
       pa_v4i16 v0[NDB], v1[NDB];
       pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
         constexpr int db = decltype(dc)::value;
-        pa_lds_cchar* src = vst + (((2 * db + (tcol >> 3)) ^ vx) << 4);
-        v0[db] = pa_rd_tr<32 * i * RB>(src);
-        v1[db] = pa_rd_tr<(32 * i + 16) * RB>(src);
+        v0[db] = pa_rd_tr<ST + 32 * i * RB>(vadr[db]);
+        v1[db] = pa_rd_tr<ST + (32 * i + 16) * RB>(vadr[db]);
       });
       bf16x8_t pf[QB];
 #pragma unroll
@@ -656,15 +696,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
         constexpr int db = decltype(dc)::value;
         pa_wait_lgkm<2 * (NDB - 1 - db)>(v0[db]);
         pa_wait_lgkm<2 * (NDB - 1 - db)>(v1[db]);
-        const short a8[8] = {v0[db][0], v0[db][1], v0[db][2], v0[db][3],
-                             v1[db][0], v1[db][1], v1[db][2], v1[db][3]};
-        const bf16x8_t vf = *(const bf16x8_t*)a8;
+        const bf16x8_t vf = pa_join(v0[db], v1[db]);
 #pragma unroll
         for (int b = 0; b < QB; ++b)
           o[b][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], o[b][db], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
     });
+  };
+  if (nt) issue(0);
+  for (int t = 0; t < nt; t += 2) {
+    step(t, std::integral_constant<int, 0>{});
+    if (t + 1 < nt) step(t + 1, std::integral_constant<int, 1>{});
   }
   pa_wait_vm<0>();
   if (!some) return;
@@ -830,105 +873,112 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 
 // ---- weight of the entries -------------------------------------------------------
 //
-// A work-group takes 64 entries of a sequence and all rows (token, head) that see
-// any of them; a wave takes 64 rows of one cache head at a time, its keys in
-// registers.  S = K Q^T, entries x rows, 16 x 16 a product: a lane adds the weights
-// of its row's column for its four entries of each block, and only at the end are
-// the 16 columns and the eight waves added, in a fixed order, so a sum does not
-// depend on what else is in the call.
+// A work-group takes WE entries of a sequence and all rows (token, head) that see
+// any of them, its waves an equal share of them each: in the order of the cache
+// heads, so that a wave's keys stay in registers from one 16 rows to the next.
+// S = K Q^T, entries x rows, 16 x 16 a product: a lane adds the weights of its
+// row's column for its four entries of each block, and only at the end are the 16
+// columns and the waves added, in a fixed order, so a sum does not depend on what
+// else is in the call.
+constexpr int PW_E = 32;   // entries a work-group
 template <int DH>
-__global__ __launch_bounds__(512) void k_paged_weight(PagedArgs c, const bf16_t* __restrict__ q,
-                                                      long long qt, long long qh, int heads,
-                                                      const float* __restrict__ lse, float sl2,
-                                                      int neg, int window, const float* w,
-                                                      long long wrow, float* out, long long orow,
-                                                      int cap) {
-  constexpr int NKS = DH / 32, RC = 64;
-  __shared__ float part[8][64];
+__global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16_t* __restrict__ q,
+                                                         long long qt, long long qh, int heads,
+                                                         FastDiv group,
+                                                         const float* __restrict__ lse, float sl2,
+                                                         int neg, int window, const float* w,
+                                                         long long wrow, float* out, long long orow,
+                                                         int cap) {
+  constexpr int NKS = DH / 32, NB = PW_E / 16;
+  __shared__ float part[8][PW_E];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = blockIdx.y, j0 = blockIdx.x * 64;
+  const int s = blockIdx.y, j0 = blockIdx.x * PW_E, j = j0 + tid;
   const int len = pg_len(c.lens[s], c.cols, c.sh);
   const PgRange r = pg_range(c.starts[s], c.starts[s + 1], c.rows);
-  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + 63, len - 1);
+  const float was = tid < PW_E && j < cap ? w[s * wrow + j] : 0.f;
+  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + PW_E - 1, len - 1);
   // tokens t0 .. t1 - 1 see one of the entries j0 .. jl
   const int t0 = max(0, j0 - e0), t1 = jl - e0 < r.n - window ? jl - e0 + window : r.n;
-  float acc[4][4];
+  float acc[NB][4];
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
   if (j0 < len && t1 > t0) {
-    const int lo = t0 * G, hi = t1 * G, chunks = (hi - lo + RC - 1) / RC;
-    const int32_t* table = c.table + s * c.trow;
-    for (int u = wv; u < c.heads * chunks; u += 8) {
-      const int kvh = u / chunks, c0 = lo + u % chunks * RC, c1 = min(c0 + RC, hi);
-      bf16x8_t kf[4][NKS];
+    const int lo = t0 * G, hi = t1 * G;
+    const int tiles = (hi - lo + 15) / 16, all = tiles * c.heads, per = (all + 7) / 8;
+    const bf16_t* kr[NB];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int k0 = min(j0 + 16 * b, jl & ~15);
-        const int id = pg_read(table[k0 >> c.sh], c.pages);
-        const bf16_t* kr = c.k + id * c.kp + kvh * c.kh + pg_slot(k0, c.sh, c.ks) +
-                           min(r16, jl - k0) * c.ks + g4 * 8;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) kf[b][ks] = *(const bf16x8_t*)(kr + ks * 32);
-      }
-      auto load = [&](int row0, bf16x8_t* qf, float& l2, int& e) {
-        const int row = min(row0 + r16, hi - 1), t = row / G;
-        const int h = kvh * G + row % G;
-        const bf16_t* qr = q + (r.first + t) * qt + h * qh + g4 * 8;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_query(qr + ks * 32, neg);
-        l2 = lse[(long long)(r.first + t) * heads + h] * PA_LOG2E;
-        e = row0 + r16 < c1 ? e0 + t : -1;   // a row past the chunk sees nothing
-      };
-      bf16x8_t qf[NKS];
+    for (int b = 0; b < NB; ++b) {
+      const int k0 = min(j0 + 16 * b, jl & ~15);
+      const int id = pg_read(c.table[s * c.trow + (k0 >> c.sh)], c.pages);
+      kr[b] = c.k + id * c.kp + pg_slot(k0, c.sh, c.ks) + min(r16, jl - k0) * c.ks + g4 * 8;
+    }
+    int u = wv * per;
+    const int end = min(u + per, all);
+    while (u < end) {   // the wave's rows of one cache head
+      const int kvh = u / tiles, first = u - kvh * tiles, n = min(tiles - first, end - u);
+      u += n;
+      bf16x8_t kf[NB][NKS], qf[NKS];
+      const bf16_t* qb = q + r.first * qt + (long long)kvh * G * qh + g4 * 8;
+      const float* lb = lse + (long long)r.first * heads + kvh * G;
       float l2;
       int e;
-      load(c0, qf, l2, e);
-      for (int row0 = c0; row0 < c1; row0 += 16) {
-        floatx4_t sc[4];
+      auto load = [&](int tile) {
+        const int at = lo + tile * 16 + r16, row = min(at, hi - 1), t = group.div(row), h = row - t * G;
+        const bf16_t* qr = qb + t * qt + h * qh;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) sc[b] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+        for (int ks = 0; ks < NKS; ++ks) qf[ks] = *(const bf16x8_t*)(qr + ks * 32);
+        l2 = lb[(long long)t * heads + h];
+        e = at < hi ? e0 + t : -1;   // a row past the last sees nothing
+      };
+      load(first);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+          kf[b][ks] = pa_query(kr[b] + kvh * c.kh + ks * 32, neg);
+      for (int i = 0; i < n; ++i) {
+        floatx4_t sc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) sc[b] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int b = 0; b < NB; ++b)
             sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], sc[b], 0, 0, 0);
-        const float base = l2;
-        const int at = e;
-        if (row0 + 16 < c1) load(row0 + 16, qf, l2, e);
-        // entry jl is the last that any row here sees or the tile holds
-        const bool full = row0 + 16 <= c1 && e0 + row0 / G >= j0 + 63 &&
-                          e0 + (row0 + 15) / G - j0 < window;
+        const float base = l2 * PA_LOG2E;
+        const int at = e, row0 = lo + (first + i) * 16;
+        if (i + 1 < n) load(first + i + 1);
+        const bool full = row0 + 16 <= hi && e0 + group.div(row0) >= j0 + PW_E - 1 &&
+                          e0 + group.div(row0 + 15) - j0 < window;
         if (full) {
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[b][i] += __builtin_amdgcn_exp2f(sc[b][i] * sl2 - base);
+            for (int k = 0; k < 4; ++k) acc[b][k] += __builtin_amdgcn_exp2f(sc[b][k] * sl2 - base);
         } else {
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = j0 + 16 * b + 4 * g4 + i;
-              acc[b][i] += j <= at && at - j < window ? __builtin_amdgcn_exp2f(sc[b][i] * sl2 - base) : 0.f;
+            for (int k = 0; k < 4; ++k) {
+              const int x = j0 + 16 * b + 4 * g4 + k;
+              acc[b][k] += x <= at && at - x < window ? __builtin_amdgcn_exp2f(sc[b][k] * sl2 - base) : 0.f;
             }
         }
       }
     }
   }
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float v = group_sum<16>(acc[b][i]);
       if (r16 == 0) part[wv][16 * b + 4 * g4 + i] = v;
     }
   __syncthreads();
-  const int j = j0 + tid;
-  if (tid >= 64 || j >= cap) return;
-  const float was = w[s * wrow + j];
+  if (tid >= PW_E || j >= cap) return;
   if (j < len) {
     float v = part[0][tid];
 #pragma unroll
@@ -948,9 +998,10 @@ hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long 
   if (c.seqs == 0 || cap == 0) return hipSuccess;
   (void)ws;
   const int win = window > 0 ? window : 0x7fffffff;
-  const dim3 grid((unsigned)((cap + 63) / 64), (unsigned)c.seqs), block(512);
+  const dim3 grid((unsigned)((cap + PW_E - 1) / PW_E), (unsigned)c.seqs), block(512);
 #define ANN_PW(D)                                                                               \
-  hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads, lse,           \
+  hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads,                 \
+                     FastDiv::of(heads / c.heads), lse,                                         \
                      fabsf(scale) * PA_LOG2E, (int)(scale < 0.f), win, w, wrow, out, orow, cap)
   if (Dh == 64) ANN_PW(64);
   else if (Dh == 128) ANN_PW(128);

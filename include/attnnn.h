@@ -288,7 +288,8 @@ int ann_op_qk_norm_rope_bwd(const ann_qk_rows* r, void* stream);
  * so the last new token is entry lens[s] - 1.  table, starts and lens are
  * device arrays: ids that are no page are never written to and read page 0,
  * lengths outside the table end at it.  Rows of queries, keys, values and
- * cache slots are 16-byte aligned (strides multiples of 8).  A head of the
+ * cache slots are 16-byte aligned (strides multiples of 8, slots at most 2^25
+ * elements apart).  A head of the
  * cache serves heads / cache heads query heads behind one another. */
 typedef struct ann_paged {
   void* k;               /* bf16, (pages, heads, page_size, head_dim) by the strides */

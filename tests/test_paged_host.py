@@ -47,6 +47,15 @@ int main() {
     }
   // slots, past 2^31 elements
   if (pg_slot(35, 4, 128) != 3 * 128 || pg_slot(1023, 10, 1LL << 40) != 1023LL << 40) return 6;
+  // quotients
+  for (int d = 1; d < 70000; d = d < 300 ? d + 1 : d * 3 / 2 + 1) {
+    const FastDiv f = FastDiv::of(d);
+    for (int n : {0, 1, 2, 1000, 65535, 1 << 20, INT_MAX - 1, INT_MAX}) {
+      if (f.div(n) != n / d) return 7;
+      const int k = n / d * d;   // and on both sides of a multiple
+      if (f.div(k) != k / d || (k && f.div(k - 1) != (k - 1) / d)) return 8;
+    }
+  }
   return 0;
 }
 """
@@ -83,6 +92,7 @@ def _attention(c, heads=6, q=FAKE, row=768, head=128, scale=0.1, window=0, out=F
     ("page_size", 24, "power of two"), ("page_size", 2048, "power of two"), ("cols", 1 << 27, "2^30"),
     ("k", None, "null"), ("v", None, "null"), ("lens", None, "null"), ("table", None, "null"),
     ("starts", None, "null"), ("k", FAKE + 8, "aligned"), ("k_slot", 132, "aligned"), ("v_head", 4, "aligned"),
+    ("k_slot", (1 << 25) + 8, "2^25"), ("v_slot", -8, "2^25"),
 ])
 def test_cache_refusals(field, value, msg):
     assert _attention(_paged(**{field: value})) == _lib.ANN_E_ARG
@@ -93,10 +103,10 @@ def test_cache_refusals(field, value, msg):
     ({"heads": 8}, "8 query heads over 6"), ({"heads": 0}, "query heads"), ({"q": None}, "null"),
     ({"q": FAKE + 2}, "aligned"), ({"row": 770}, "aligned"), ({"scale": float("nan")}, "finite"),
     ({"scale": float("inf")}, "finite"), ({"window": -1}, "window"), ({"out": None}, "out is null"),
-    ({"out": FAKE + 4}, "aligned"),
+    ({"out": FAKE + 4}, "aligned"), ({"heads": 600}, "2^31"),
 ])
 def test_attention_refusals(kw, msg):
-    assert _attention(_paged(), **kw) == _lib.ANN_E_ARG
+    assert _attention(_paged(rows=1 << 22 if kw == {"heads": 600} else 4), **kw) == _lib.ANN_E_ARG
     assert msg in _lib.lib().ann_last_error().decode()
     assert _lib.lib().ann_op_paged_attention(None, FAKE, 768, 128, 6, 0.1, 0, FAKE, None, None, 0, None) == _lib.ANN_E_ARG
 
