@@ -88,8 +88,15 @@ typedef short pa_v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void pa_lds_void;
 typedef __attribute__((address_space(3))) const unsigned char pa_lds_cchar;
 
-// 16-byte chunk c of LDS row r is stored at chunk c ^ swz(r): conflict-free for
-// the fragment reads of the keys and the transposed ones of the values.
+// 16-byte chunk c of LDS row r is stored at chunk c ^ kswz(r) of a key tile and c
+// ^ swz(r) of a value tile.  A fragment of keys is 16 rows of one chunk each,
+// which the hardware reads 16 lanes at a time from two neighbouring chunks; one of
+// values 8 rows of two chunks.  Measured, cycles for 1 KB of keys: 5 with kswz, 8
+// with swz, 32 unswizzled; for 512 bytes of values 4.25 and 16.
+template <int DH>
+__device__ __forceinline__ int pa_kswz(int r) {
+  return DH == 128 ? r & 15 : r & 7;
+}
 template <int DH>
 __device__ __forceinline__ int pa_swz(int r) {
   return DH == 128 ? (((r & 7) << 1) | ((r >> 3) & 1)) : ((r >> 1) & 7);
@@ -115,6 +122,10 @@ __device__ __forceinline__ pa_v4i16 pa_rd_tr(pa_lds_cchar* p) {
 template <int N, typename X>
 __device__ __forceinline__ void pa_wait_lgkm(X& x) {
   asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(x) : "i"(N));
+}
+template <int N, typename X>
+__device__ __forceinline__ void pa_wait_lgkm2(X& x, X& y) {
+  asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(x), "+v"(y) : "i"(N));
 }
 template <int I, int N, typename F>
 __device__ __forceinline__ void pa_static_for(F&& f) {
@@ -147,15 +158,16 @@ struct PaArgs {
   long long qt, qh;
   int heads, window;   // window: none is INT_MAX
   float sl2, thr;      // |scale| log2(e); 8 / sl2, the rise of m's that is let pass
-  int neg;             // scale < 0: the queries enter negated
+  float ssl2;          // scale log2(e)
+  uint32_t keep, flip; // of the queries' words: all bits, signs of a negative scale, none of scale 0 (sl2 is 1 then)
   bf16_t* out;
   float* lse;
   float* po;           // partial sums (rows, heads, parts, DH), or null: one part
   float2* pml;         // (rows, heads, parts): m in log2 units, sum
   int ns_few, ns_many; // most parts of a tile of each kind
   int nsmax;           // the larger, the stride of the partials
-  int few;             // rows of a sequence up to which k_paged_few takes it
-  int br;              // rows of k_paged_many's tiles
+  int few;             // rows of a sequence up to which pa_few takes it
+  int br;              // rows of pa_many's tiles
 };
 
 // One sequence's new tokens as a call sees them.
@@ -207,7 +219,7 @@ __device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, const 
   const int t = row / q.G, e = q.e0 + t, n = q.first + t, h = kvh * q.G + row % q.G;
   const int lo = max(a0, e < a.window ? 0 : e - a.window + 1), hi = min(b0, e + 1);
   float m, l, o[DL];
-  pa_row<DH>(a.c, table, a.q + n * a.qt + h * a.qh, kvh, lo, hi, a.neg ? -a.sl2 : a.sl2, m, l, o);
+  pa_row<DH>(a.c, table, a.q + n * a.qt + h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
   // lane i holds dims i DL ..: four lanes' (two's) values to the one that stores them
   float4 v;
   if constexpr (DL == 1) {
@@ -225,12 +237,11 @@ __device__ __forceinline__ bool pa_finite(const floatx4_t& v) {
   return z == 0.f;
 }
 
-// The running maximum raised where a lane's largest score lm passes it by more
-// than thr; the four lanes of a row agree on it.
+// The running maximum raised to the largest score, of which each of a row's four
+// lanes knows its own: where one passes it by more than a.thr.
 template <int NDB>
-__device__ __forceinline__ void pa_raise(float lm, float thr, float sl2, float& m, float& msl,
-                                         float& lsum, floatx4_t* o) {
-  if (!__any(lm > m + thr)) return;
+__device__ __forceinline__ void pa_raise(float lm, float sl2, float& m, float& msl, float& lsum,
+                                         floatx4_t* o) {
   lm = fmaxf(lm, __shfl_xor(lm, 16, 64));
   lm = fmaxf(lm, __shfl_xor(lm, 32, 64));
   const float mn = fmaxf(m, lm);
@@ -242,13 +253,14 @@ __device__ __forceinline__ void pa_raise(float lm, float thr, float sl2, float& 
   for (int i = 0; i < NDB; ++i) o[i] *= f;
 }
 
-__device__ __forceinline__ bf16x8_t pa_query(const bf16_t* p, int neg) {
+// 8 values with the scale's sign: products are with |scale| then, whose largest
+// score is the largest product.
+__device__ __forceinline__ bf16x8_t pa_signed(const bf16_t* p, uint32_t keep, uint32_t flip) {
   uint4 w = *(const uint4*)p;
-  const uint32_t x = neg ? 0x80008000u : 0u;
-  w.x ^= x;
-  w.y ^= x;
-  w.z ^= x;
-  w.w ^= x;
+  w.x = (w.x & keep) ^ flip;
+  w.y = (w.y & keep) ^ flip;
+  w.z = (w.z & keep) ^ flip;
+  w.w = (w.w & keep) ^ flip;
   return __builtin_bit_cast(bf16x8_t, w);
 }
 
@@ -272,24 +284,29 @@ struct PaPages {
 // ---- sequences of few rows ----------------------------------------------------------
 //
 // A work-group takes a part of a sequence's entries for one cache head, 16 rows at
-// a time (one row of a decoding sequence without shared heads).  Its four waves
+// a time (one row of a decoding sequence without shared heads).  Its NW waves
 // take chunks of 32 entries in turn and meet only at the end: keys from memory
-// straight into the fragments of the product, two chunks ahead; values into the
-// wave's own ring of LDS stages.
-template <int DH>
-__global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
+// straight into the fragments of the product, a chunk ahead; values into the
+// wave's own ring of two LDS stages.  The products have time to spare here, and the
+// weights enter as two bf16 halves (2^-17 of each).
+template <int DH, int NW>
+constexpr size_t pa_few_lds() {
+  // the rings; after them the waves' sums, their maxima and totals, rows to form again
+  const size_t ring = (size_t)NW * 2 * 32 * DH * 2;
+  const size_t sums = ((size_t)NW * 16 * (DH + 4) + 2 * NW * 16 + 16) * 4;
+  return ring > sums ? ring : sums;
+}
+template <int DH, int NW>
+__device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part,
+                                       unsigned char* smem) {
   constexpr int RB = DH * 2, TB = 32 * RB;      // bytes of an LDS row, of a chunk's values
   constexpr int LPW = TB / 1024, RPL = 1024 / RB;   // loads of a chunk's values, rows of each
   constexpr int NKS = DH / 32, NDB = DH / 16, PW = DH + 4;
-  // the rings; after them the waves' sums, their maxima and totals, rows to form again
-  constexpr int RING = 4 * 2 * TB, SUMS = 4 * 16 * PW * 4 + (2 * 64 + 16) * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[RING > SUMS ? RING : SUMS];
   float* sums = (float*)smem;
-  float* s_m = sums + 4 * 16 * PW;
-  float* s_l = s_m + 64;
-  int* s_bad = (int*)(s_l + 64);
+  float* s_m = sums + NW * 16 * PW;
+  float* s_l = s_m + NW * 16;
+  int* s_bad = (int*)(s_l + NW * 16);
 
-  const int s = blockIdx.y, kvh = blockIdx.x % a.c.heads, part = blockIdx.x / a.c.heads;
   const PaSeq q = pa_seq(a, s);
   if (q.rows == 0 || q.rows > a.few) return;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -310,7 +327,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
     const int a0 = max(pt.begin + part * pt.per, lo), b0 = min(pt.begin + (part + 1) * pt.per, hi);
     const int kb0 = pt.begin + part * pt.per;
     const int nch = b0 > a0 ? (b0 - kb0 + 31) / 32 : 0;
-    const int nt = nch > wv ? (nch - wv + 3) / 4 : 0;   // chunks of this wave
+    const int nt = nch > wv ? (nch - wv + NW - 1) / NW : 0;   // chunks of this wave
 
     const int row = row0 + min(r16, nrow - 1), tok = row / q.G;
     const int e = q.e0 + tok;
@@ -318,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
     const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row % q.G) * a.qh + g4 * 8;
     bf16x8_t qf[NKS];
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_query(qr + ks * 32, a.neg);
+    for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
 
     floatx4_t o[NDB];
 #pragma unroll
@@ -327,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
 
     // ids of chunks 32 b .. 32 b + 31 of this wave: lane i group i & 1 of chunk i >> 1
     auto ids = [&](int b) {
-      const int key = kb0 + 32 * (wv + 4 * (32 * b + (lane >> 1))) + 16 * (lane & 1);
+      const int key = kb0 + 32 * (wv + NW * (32 * b + (lane >> 1))) + 16 * (lane & 1);
       return pg_read(table[min(max(key, a0), b0 - 1) >> a.c.sh], a.c.pages);
     };
     PaPages pg = {nt ? ids(0) : 0, nt > 32 ? ids(1) : 0};
@@ -338,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
         pg.now = pg.next;
         if (t + 32 < nt) pg.next = ids(t / 32 + 1);
       }
-      const int kb = kb0 + 32 * (wv + 4 * t);
+      const int kb = kb0 + 32 * (wv + NW * t);
       unsigned char* st = ring + (t & 1) * TB;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -361,7 +378,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
       }
     };
     auto compute = [&](int t, int slot) {
-      const int kb = kb0 + 32 * (wv + 4 * t);
+      const int kb = kb0 + 32 * (wv + NW * t);
       floatx4_t sacc[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -381,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
           ok[g][r] = full || (j >= a0 && j < b0 && j <= e && e - j < a.window);
           lm = fmaxf(lm, ok[g][r] ? sacc[g][r] : -INFINITY);
         }
-      pa_raise<NDB>(lm, a.thr, a.sl2, m, msl, lsum, o);
+      if (__any(lm > m + a.thr)) pa_raise<NDB>(lm, a.sl2, m, msl, lsum, o);
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -389,10 +406,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
           p[g][r] = ok[g][r] ? __builtin_amdgcn_exp2f(sacc[g][r] * a.sl2 - msl) : 0.f;
           lsum += p[g][r];
         }
-      uint32_t pw[4];
+      uint32_t pw[4], pl[4];   // the weights in bf16, and what that leaves of them
 #pragma unroll
-      for (int x = 0; x < 4; ++x) pw[x] = pack2(p[x >> 1][(x & 1) * 2], p[x >> 1][(x & 1) * 2 + 1]);
-      const bf16x8_t pf = *(const bf16x8_t*)pw;
+      for (int x = 0; x < 4; ++x) {
+        const float u = p[x >> 1][(x & 1) * 2], v = p[x >> 1][(x & 1) * 2 + 1];
+        pw[x] = pack2(u, v);
+        pl[x] = pack2(u - lo_f(pw[x]), v - hi_f(pw[x]));
+      }
+      const bf16x8_t pf = *(const bf16x8_t*)pw, pr = *(const bf16x8_t*)pl;
       pa_lds_cchar* vst = (pa_lds_cchar*)(ring + (t & 1) * TB) + trow * RB + (tcol & 7) * 2;
       pa_v4i16 v0[NDB], v1[NDB];
       pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
@@ -403,9 +424,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
       });
       pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
         constexpr int db = decltype(dc)::value;
-        pa_wait_lgkm<2 * (NDB - 1 - db)>(v0[db]);
-        pa_wait_lgkm<2 * (NDB - 1 - db)>(v1[db]);
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_join(v0[db], v1[db]), pf, o[db], 0, 0, 0);
+        pa_wait_lgkm2<2 * (NDB - 1 - db)>(v0[db], v1[db]);
+        const bf16x8_t vf = pa_join(v0[db], v1[db]);
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr, o[db], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
     };
@@ -441,11 +463,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
     if (tid < 16) s_bad[tid] = 0;
     __syncthreads();
     auto joined = [&](int r, int d, float& M, float& L) {
-      M = fmaxf(fmaxf(s_m[r], s_m[16 + r]), fmaxf(s_m[32 + r], s_m[48 + r]));
+      M = s_m[r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w * 16 + r]);
       L = 0.f;
       floatx4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w * 16 + r] - M);
         L += s_l[w * 16 + r] * f;
         v += *(const floatx4_t*)(sums + (w * 16 + r) * PW + d) * f;
@@ -454,21 +478,27 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
     };
     float M, L;
     if (nrow > 1) {   // one row alone sees all that its part reads
-      for (int i = tid; i < nrow * (DH / 4); i += 256)
+      for (int i = tid; i < nrow * (DH / 4); i += 64 * NW)
         if (!pa_finite(joined(i / (DH / 4), i % (DH / 4) * 4, M, L))) s_bad[i / (DH / 4)] = 1;
       __syncthreads();
     }
-    for (int i = tid; i < nrow * (DH / 4); i += 256) {
+    for (int i = tid; i < nrow * (DH / 4); i += 64 * NW) {
       const int r = i / (DH / 4), d = i % (DH / 4) * 4, rr = row0 + r;
       if (s_bad[r]) continue;
       const floatx4_t v = joined(r, d, M, L);
       pa_store4<DH>(a, q.first + rr / q.G, kvh * q.G + rr % q.G, part, pt.n, d,
                     make_float4(v[0], v[1], v[2], v[3]), M, L);
     }
-    for (int r = wv; r < nrow; r += 4)
+    for (int r = wv; r < nrow; r += NW)
       if (s_bad[r]) pa_again<DH>(a, q, table, kvh, row0 + r, a0, b0, part, pt.n);
     __syncthreads();   // the sums are read before the next rows' chunks arrive
   }
+}
+
+template <int DH, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
+  pa_few<DH, NW>(a, blockIdx.y, blockIdx.x % a.c.heads, blockIdx.x / a.c.heads, pa_smem);
 }
 
 // ---- sequences of many rows -----------------------------------------------------------
@@ -477,18 +507,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PaArgs a) {
 // entries, which pass through a ring of two LDS stages shared by its waves: loaded
 // straight into LDS a step ahead, one barrier a step.  A key or value fragment
 // read from LDS serves QB products.
+constexpr int PM_AHEAD = 1;   // steps that loads run ahead (odd: a step's parity is its stage's)
+template <int LPW>
+struct PaWalk {
+  const unsigned char* head;
+  long long page, slot;
+  int lo, hi, next;    // lane i: offset of group i in bytes; page id of group i of the next batch
+  unsigned off[LPW];   // this lane's row and column in the group of load u, bytes
+};
+template <int DH, int BK>
+constexpr size_t pa_many_lds() { return (size_t)2 * (PM_AHEAD + 1) * BK * DH * 2; }
 template <int DH, int BK, int QB>
-__global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
+__device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int part,
+                                        unsigned char* smem) {
   constexpr int BR = 64 * QB, RB = DH * 2, TB = BK * RB;
   constexpr int LPW = TB / 1024 / 4, RPL = 1024 / RB;   // loads a wave makes of K (and of V), rows of each
-  constexpr int NKS = DH / 32, NDB = DH / 16, NBLK = BK / 16, NI = BK / 32, GPT = BK / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * 2 * TB];
+  constexpr int NKS = DH / 32, NDB = DH / 16, NBLK = BK / 16, NI = BK / 32;
+  constexpr int NS = PM_AHEAD + 1;   // stages of keys, and of values
 
-  // tiles of one (cache head, part) run together on one XCD and share its L2:
-  // work-group L runs on XCD L % 8
-  const int total = gridDim.x, L = blockIdx.x;
-  const int w = total % 8 == 0 ? (L % 8) * (total / 8) + L / 8 : L;
-  const int tile = w % tiles, kvh = (w / tiles) % a.c.heads, part = w / tiles / a.c.heads;
   int s = 0, row0 = 0;
   if (!pg_tile(a.c.starts, a.c.seqs, a.c.rows, a.heads / a.c.heads, a.few, BR, tile, s, row0)) return;
   s = __builtin_amdgcn_readfirstlane(s);
@@ -507,8 +543,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
   const int32_t* table = a.c.table + s * a.c.trow;
-  const bf16_t* kh = a.c.k + kvh * a.c.kh;
-  const bf16_t* vh = a.c.v + kvh * a.c.vh;
 
   // this wave's rows, past the last one copies of it; their entries el .. eh
   const int wr0 = row0 + wv * 16 * QB, last = q.rows - 1;
@@ -522,7 +556,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     e[b] = q.e0 + tok;
     const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row % q.G) * a.qh + g4 * 8;
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[b][ks] = pa_query(qr + ks * 32, a.neg);
+    for (int ks = 0; ks < NKS; ++ks) qf[b][ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
   }
   floatx4_t o[QB][NDB];
   float m[QB], msl[QB], lsum[QB];
@@ -534,181 +568,208 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
     for (int i = 0; i < NDB; ++i) o[b][i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
   }
 
-  constexpr int TPB = 64 / GPT;   // tiles whose page ids a wave holds
-  auto ids = [&](int b) {
-    const int key = kb0 + BK * TPB * b + 16 * lane;
-    return pg_read(table[min(max(key, a0), b0 - 1) >> a.c.sh], a.c.pages);
+  // A wave's loads of a tile lie in one group of 16 entries, group gw.  Lane i
+  // holds the offset in bytes within a head of that group of tile i of a batch of
+  // 64, from one table entry each; the next batch's page ids come ahead.  Keys and
+  // values walk apart by a tile.
+  static_assert(LPW * RPL <= 16, "one group a wave");
+  const int gw = wv * LPW * RPL / 16;
+  auto slot0 = [&](int b) {
+    return min(max(kb0 + BK * (64 * b + lane) + 16 * gw, a0 & ~15), (b0 - 1) & ~15);
   };
-  PaPages pg = {nt ? ids(0) : 0, nt > TPB ? ids(1) : 0};
-  // load x of a tile is rows x RPL .. of it: this lane's row of its group of 16 and column
-  int lrow[LPW], lcol[LPW];
-  unsigned koff[LPW], voff[LPW];
+  PaWalk<LPW> wk, wx;
+  wk.head = (const unsigned char*)(a.c.k + kvh * a.c.kh);
+  wk.page = a.c.kp;
+  wk.slot = a.c.ks;
+  wx.head = (const unsigned char*)(a.c.v + kvh * a.c.vh);
+  wx.page = a.c.vp;
+  wx.slot = a.c.vs;
+  int lrow[LPW], kcol[LPW], vcol[LPW];   // load u: this lane's row of its group, its columns in bytes
 #pragma unroll
   for (int u = 0; u < LPW; ++u) {
-    const int r = (wv * LPW + u) * RPL + lane / (RB / 16);
+    const int r = (wv * LPW + u) * RPL + lane / (RB / 16), ch = lane % (RB / 16);
     lrow[u] = r % 16;
-    lcol[u] = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
-    koff[u] = (unsigned)(lrow[u] * (int)a.c.ks * 2 + lcol[u]);
-    voff[u] = (unsigned)(lrow[u] * (int)a.c.vs * 2 + lcol[u]);
+    kcol[u] = (ch ^ pa_kswz<DH>(r)) * 16;
+    vcol[u] = (ch ^ pa_swz<DH>(r)) * 16;
+    wk.off[u] = (unsigned)(lrow[u] * (int)a.c.ks * 2 + kcol[u]);
+    wx.off[u] = (unsigned)(lrow[u] * (int)a.c.vs * 2 + vcol[u]);
   }
-  auto issue = [&](int t) {
-    if (t && t % TPB == 0) {
-      pg.now = pg.next;
-      if (t + TPB < nt) pg.next = ids(t / TPB + 1);
-    }
-    const int kb = kb0 + BK * t;
-    unsigned char* st = smem + (t & 1) * 2 * TB;
-    const bool inside = kb >= a0 && kb + BK <= b0;
+  auto turn = [&](PaWalk<LPW>& w, int b) {   // to batch b, whose ids have arrived
+    const long long off =
+        (pg_read(w.next, a.c.pages) * w.page + pg_slot(slot0(b), a.c.sh, w.slot)) * 2;
+    w.lo = (int)off;
+    w.hi = (int)(off >> 32);
+    if ((b + 1) * 64 < nt) w.next = table[slot0(b + 1) >> a.c.sh];
+  };
+  // tile t to stage st; edge: rows outside [a0, b0) take the nearest inside
+  auto issue = [&](PaWalk<LPW>& w, const int* col, int t, unsigned char* st, bool edge)
+                   __attribute__((always_inline)) {
+    if (t % 64 == 0) turn(w, t / 64);
+    const unsigned lo = __builtin_amdgcn_readlane(w.lo, t % 64);
+    const unsigned char* base =
+        w.head + (((long long)__builtin_amdgcn_readlane(w.hi, t % 64) << 32) | lo);
 #pragma unroll
     for (int u = 0; u < LPW; ++u) {
-      const int x = wv * LPW + u, g = x * RPL / 16;   // the load, and its group of 16 entries
-      const int id = __builtin_amdgcn_readlane(pg.now, GPT * (t % TPB) + g);
-      int k0 = kb + 16 * g;
-      unsigned ko = koff[u], vo = voff[u];
-      if (!inside) {   // rows outside [a0, b0) take the nearest inside
-        k0 = min(max(k0, a0 & ~15), (b0 - 1) & ~15);
-        const int rc = min(max(lrow[u], a0 - k0), b0 - 1 - k0);
-        ko = (unsigned)(rc * (int)a.c.ks * 2 + lcol[u]);
-        vo = (unsigned)(rc * (int)a.c.vs * 2 + lcol[u]);
+      unsigned off = w.off[u];
+      if (edge) {
+        const int k0 = min(max(kb0 + BK * t + 16 * gw, a0 & ~15), (b0 - 1) & ~15);
+        off = (unsigned)(min(max(lrow[u], a0 - k0), b0 - 1 - k0) * (int)w.slot * 2 + col[u]);
       }
-      __builtin_amdgcn_global_load_lds(pa_group(kh, id, a.c.kp, a.c.ks, k0, a.c.sh) + ko,
-                                       (pa_lds_void*)(st + x * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(pa_group(vh, id, a.c.vp, a.c.vs, k0, a.c.sh) + vo,
-                                       (pa_lds_void*)(st + TB + x * 1024), 16, 0, 0);
+      const unsigned char* src = base + off;
+      __builtin_amdgcn_global_load_lds(src, (pa_lds_void*)(st + (wv * LPW + u) * 1024), 16, 0, 0);
     }
   };
-  // fragment addresses of the first stage; the second lies 2 TB behind
+  // fragment addresses of the first key and value stage
   const int trow = 4 * g4 + (r16 >> 2), tcol = 4 * (r16 & 3);
   pa_lds_cchar* kadr[NKS];
   pa_lds_cchar* vadr[NDB];
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks)
-    kadr[ks] = (pa_lds_cchar*)smem + r16 * RB + (((ks * 4 + g4) ^ pa_swz<DH>(r16)) << 4);
+    kadr[ks] = (pa_lds_cchar*)smem + r16 * RB + (((ks * 4 + g4) ^ pa_kswz<DH>(r16)) << 4);
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
-    vadr[db] = (pa_lds_cchar*)smem + TB + trow * RB + (tcol & 7) * 2 +
+    vadr[db] = (pa_lds_cchar*)smem + NS * TB + trow * RB + (tcol & 7) * 2 +
                (((2 * db + (tcol >> 3)) ^ pa_swz<DH>(trow)) << 4);
-
-  auto step = [&](int t, auto stage) __attribute__((always_inline)) {
-    constexpr int ST = decltype(stage)::value * 2 * TB;
+  auto live = [&](int t) {   // whether this wave's rows see any of tile t
     const int kb = kb0 + BK * t;
-    pa_wait_vm<0>();   // this wave's part of tile t is in LDS
-    __syncthreads();   // every wave's; the other stage is free
-    if (t + 1 < nt) issue(t + 1);
-    if (!(some && kb <= eh && el - (kb + BK - 1) < a.window)) return;   // nothing in it for this wave
-    const bool full = kb >= a0 && kb + BK - 1 < b0 && kb + BK - 1 <= el && eh - kb < a.window;
+    return some && t < nt && kb <= eh && el - (kb + BK - 1) < a.window;
+  };
 
-    floatx4_t sacc[QB][NBLK];
+  // A step's scores were formed in the step before: its products with the next
+  // keys run beside its exponentials, both in groups of one key fragment, and the
+  // values' fragments arrive behind them for the products with P.  Steps f0 .. f1
+  // - 1 are free of every edge: all their entries are seen by all rows, and what
+  // they load ahead is there.
+  constexpr int KG = NKS * NBLK, VG = NI * NDB, PG = NBLK * 4 / KG;   // PG weights a group and row block
+  static_assert(KG == 8 && KG == VG && PG * KG == NBLK * 4, "one value fragment beside each key fragment");
+  int f0 = max(a0 - kb0, eh - a.window + 1 - kb0);
+  f0 = f0 > 0 ? (f0 + BK - 1) / BK : 0;
+  const int f1 = some ? min((min(b0, el + 1) - kb0) / BK, (b0 - kb0) / BK - 1 - PM_AHEAD) : 0;
+  floatx4_t sc[2][QB][NBLK];
+  auto step = [&](int t, auto stage, auto free) __attribute__((always_inline)) {
+    constexpr bool FREE = decltype(free)::value;
+    constexpr int ST = decltype(stage)::value, P = ST & 1;   // t % NS, t % 2
+    constexpr int KO = (ST + 1) % NS * TB, VO = ST * TB;
+    // this wave's part of keys t + 1 and values t is in LDS: all but the last
+    // PM_AHEAD - 1 steps' loads, or near the end all
+    if (FREE || t + PM_AHEAD < nt) pa_wait_vm<(PM_AHEAD - 1) * 2 * LPW>();
+    else pa_wait_vm<0>();
+    __syncthreads();   // every wave's; keys t and values t - 1 are used up
+    if (FREE || t + 1 + PM_AHEAD < nt) issue(wk, kcol, t + 1 + PM_AHEAD, smem + ST * TB, !FREE);
+    if (FREE || t + PM_AHEAD < nt)
+      issue(wx, vcol, t + PM_AHEAD, smem + (NS + (ST + NS - 1) % NS) * TB, !FREE);
+    floatx4_t(&s0)[QB][NBLK] = sc[P];
+    floatx4_t(&s1)[QB][NBLK] = sc[1 - P];
+    if constexpr (!FREE) {
+      const bool now = live(t);
+      if (!now && !live(t + 1)) return;
+      const int kb = kb0 + BK * t;
 #pragma unroll
-    for (int b = 0; b < QB; ++b)
-#pragma unroll
-      for (int i = 0; i < NBLK; ++i) sacc[b][i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
-    // key fragments: one k-step (NBLK reads) ahead of its products
-    bf16x8_t kf[2][NBLK];
-    pa_static_for<0, NBLK>([&](auto bc) __attribute__((always_inline)) {
-      constexpr int i = decltype(bc)::value;
-      kf[0][i] = pa_rd_b128<ST + i * 16 * RB>(kadr[0]);
-    });
-    pa_static_for<0, NKS>([&](auto kc) __attribute__((always_inline)) {
-      constexpr int ks = decltype(kc)::value;
-      if constexpr (ks + 1 < NKS) {
-        pa_static_for<0, NBLK>([&](auto bc) __attribute__((always_inline)) {
-          constexpr int i = decltype(bc)::value;
-          kf[(ks + 1) & 1][i] = pa_rd_b128<ST + i * 16 * RB>(kadr[ks + 1]);
-        });
-      }
-      constexpr int ahead = ks + 1 < NKS ? NBLK : 0;
-      pa_static_for<0, NBLK>([&](auto bc) __attribute__((always_inline)) {
-        constexpr int i = decltype(bc)::value;
-        pa_wait_lgkm<ahead + NBLK - 1 - i>(kf[ks & 1][i]);
-#pragma unroll
-        for (int b = 0; b < QB; ++b)
-          sacc[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[ks & 1][i], qf[b][ks], sacc[b][i], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    });
-
-    float p[QB][NBLK][4];
-    if (full) {
-#pragma unroll
-      for (int b = 0; b < QB; ++b) {
-        float lm = sacc[b][0][0];
-#pragma unroll
-        for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) lm = fmaxf(lm, sacc[b][i][r]);
-        pa_raise<NDB>(lm, a.thr, a.sl2, m[b], msl[b], lsum[b], o[b]);
+      for (int b = 0; b < QB; ++b) {   // what is masked scores -inf
+        const int jl = max(a0, e[b] < a.window ? 0 : e[b] - a.window + 1) - kb - 4 * g4;
+        const int jh = now ? min(b0 - 1, e[b]) - kb - 4 * g4 : -64;
 #pragma unroll
         for (int i = 0; i < NBLK; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            p[b][i][r] = __builtin_amdgcn_exp2f(sacc[b][i][r] * a.sl2 - msl[b]);
-      }
-    } else {
-#pragma unroll
-      for (int b = 0; b < QB; ++b) {
-        // entries jl .. jh of this lane's four of each block; a masked one's score is -inf
-        const int jl = max(a0, e[b] < a.window ? 0 : e[b] - a.window + 1) - kb - 4 * g4;
-        const int jh = min(b0 - 1, e[b]) - kb - 4 * g4;
-        float lm = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool ok = 16 * i + r >= jl && 16 * i + r <= jh;
-            sacc[b][i][r] = ok ? sacc[b][i][r] : -INFINITY;
-            lm = fmaxf(lm, sacc[b][i][r]);
-          }
-        pa_raise<NDB>(lm, a.thr, a.sl2, m[b], msl[b], lsum[b], o[b]);
-#pragma unroll
-        for (int i = 0; i < NBLK; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float v = __builtin_amdgcn_exp2f(sacc[b][i][r] * a.sl2 - msl[b]);
-            const bool ok = 16 * i + r >= jl && 16 * i + r <= jh;
-            p[b][i][r] = ok ? v : 0.f;
-          }
+            s0[b][i][r] = 16 * i + r >= jl && 16 * i + r <= jh ? s0[b][i][r] : -INFINITY;
       }
     }
+    float lm[QB];
+    bool over = false;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      lm[b] = s0[b][0][0];
+#pragma unroll
+      for (int i = 0; i < NBLK; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lm[b] = fmaxf(lm[b], s0[b][i][r]);
+      over = over || lm[b] > m[b] + a.thr;
+    }
+    if (__any(over))
+#pragma unroll
+      for (int b = 0; b < QB; ++b) pa_raise<NDB>(lm[b], a.sl2, m[b], msl[b], lsum[b], o[b]);
+    bf16x8_t kf[KG];
+    pa_v4i16 v0[VG], v1[VG];
 #pragma unroll
     for (int b = 0; b < QB; ++b)
 #pragma unroll
-      for (int i = 0; i < NBLK; ++i)
-        lsum[b] += (p[b][i][0] + p[b][i][1]) + (p[b][i][2] + p[b][i][3]);
-    pa_static_for<0, NI>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value;
-      pa_v4i16 v0[NDB], v1[NDB];
-      pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
-        constexpr int db = decltype(dc)::value;
-        v0[db] = pa_rd_tr<ST + 32 * i * RB>(vadr[db]);
-        v1[db] = pa_rd_tr<ST + (32 * i + 16) * RB>(vadr[db]);
-      });
-      bf16x8_t pf[QB];
+      for (int i = 0; i < NBLK; ++i) s1[b][i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+    // four key fragments ahead; behind group x's the values' pair x, so that group x
+    // waits for all but what was read after its own fragment
+    pa_static_for<0, 4>([&](auto xc) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value, ks = x / NBLK, i = x % NBLK;
+      kf[x] = pa_rd_b128<KO + i * 16 * RB>(kadr[ks]);
+    });
+    uint32_t pw[QB][NBLK][2];
+    pa_static_for<0, KG>([&](auto xc) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value, ks = x / NBLK, i = x % NBLK, vi = x / NDB, db = x % NDB;
+      pa_wait_lgkm<(x < 4 ? 3 + 2 * x : 15 - x)>(kf[x]);
+#pragma unroll
+      for (int b = 0; b < QB; ++b)
+        s1[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[x], qf[b][ks], s1[b][i], 0, 0, 0);
+      if constexpr (x + 4 < KG) {
+        constexpr int y = x + 4;
+        kf[y] = pa_rd_b128<KO + y % NBLK * 16 * RB>(kadr[y / NBLK]);
+      }
+      v0[x] = pa_rd_tr<VO + 32 * vi * RB>(vadr[db]);
+      v1[x] = pa_rd_tr<VO + (32 * vi + 16) * RB>(vadr[db]);
 #pragma unroll
       for (int b = 0; b < QB; ++b) {
-        uint32_t pw[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          pw[x] = pack2(p[b][2 * i + (x >> 1)][(x & 1) * 2], p[b][2 * i + (x >> 1)][(x & 1) * 2 + 1]);
-        pf[b] = *(const bf16x8_t*)pw;
+        for (int g = 0; g < PG; ++g) {
+          const int k = x * PG + g;
+          const float v = __builtin_amdgcn_exp2f(s0[b][k / 4][k % 4] * a.sl2 - msl[b]);
+          s0[b][k / 4][k % 4] = v;
+          lsum[b] += v;
+          if (k % 2 == 1) pw[b][k / 4][(k % 4) / 2] = pack2(s0[b][k / 4][k % 4 - 1], v);
+        }
       }
-      pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
-        constexpr int db = decltype(dc)::value;
-        pa_wait_lgkm<2 * (NDB - 1 - db)>(v0[db]);
-        pa_wait_lgkm<2 * (NDB - 1 - db)>(v1[db]);
-        const bf16x8_t vf = pa_join(v0[db], v1[db]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    pa_static_for<0, VG>([&](auto xc) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value, i = x / NDB, db = x % NDB;
+      pa_wait_lgkm2<2 * (VG - 1 - x)>(v0[x], v1[x]);
+      const bf16x8_t vf = pa_join(v0[x], v1[x]);
 #pragma unroll
-        for (int b = 0; b < QB; ++b)
-          o[b][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], o[b][db], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      });
+      for (int b = 0; b < QB; ++b) {
+        const uint32_t w4[4] = {pw[b][2 * i][0], pw[b][2 * i][1], pw[b][2 * i + 1][0], pw[b][2 * i + 1][1]};
+        o[b][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *(const bf16x8_t*)w4, o[b][db], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     });
   };
-  if (nt) issue(0);
-  for (int t = 0; t < nt; t += 2) {
-    step(t, std::integral_constant<int, 0>{});
-    if (t + 1 < nt) step(t + 1, std::integral_constant<int, 1>{});
+  if (nt) {
+    wk.next = wx.next = table[slot0(0) >> a.c.sh];
+    issue(wk, kcol, 0, smem, true);
+#pragma unroll
+    for (int d = 0; d < PM_AHEAD; ++d) {
+      if (d + 1 < nt) issue(wk, kcol, d + 1, smem + (d + 1) * TB, true);
+      if (d < nt) issue(wx, vcol, d, smem + (NS + d) * TB, true);
+    }
+    if (PM_AHEAD < nt) pa_wait_vm<PM_AHEAD * 2 * LPW>();
+    else pa_wait_vm<0>();
+    __syncthreads();
+    pa_static_for<0, KG>([&](auto xc) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value, ks = x / NBLK, i = x % NBLK;
+      bf16x8_t kf = pa_rd_b128<i * 16 * RB>(kadr[ks]);
+      pa_wait_lgkm<0>(kf);
+#pragma unroll
+      for (int b = 0; b < QB; ++b)
+        sc[0][b][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            kf, qf[b][ks], ks ? sc[0][b][i] : (floatx4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    });
   }
+  const auto steps = [&](int t, auto free) __attribute__((always_inline)) {
+    pa_static_for<0, NS>([&](auto st) __attribute__((always_inline)) {
+      constexpr int i = decltype(st)::value;
+      if (decltype(free)::value || t + i < nt) step(t + i, st, free);
+    });
+  };
+  int t = 0;
+  for (; t < nt && (t < f0 || t + NS > f1); t += NS) steps(t, std::false_type{});
+  for (; t + NS <= f1; t += NS) steps(t, std::true_type{});
+  for (; t < nt; t += NS) steps(t, std::false_type{});
   pa_wait_vm<0>();
   if (!some) return;
 #pragma unroll
@@ -736,73 +797,152 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles) {
   }
 }
 
-// The parts of each row joined, in part order: one wave for each (token, head).
+// Tiles of many rows, then (where a call has both) sequences of few, each by a
+// work-group of its own: the short ones fill the CUs that the long ones leave.
+template <int DH, int QB>
+__global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles, int blocks) {
+  constexpr int BK = DH == 64 ? 64 : 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
+  const int L = blockIdx.x;
+  if (L < blocks) {
+    // tiles of one (cache head, part) run together on one XCD and share its L2:
+    // work-group L runs on XCD L % 8
+    const int w = blocks % 8 == 0 ? (L % 8) * (blocks / 8) + L / 8 : L;
+    pa_many<DH, BK, QB>(a, w % tiles, (w / tiles) % a.c.heads, w / tiles / a.c.heads, pa_smem);
+  } else {
+    const int w = L - blocks, i = w / a.c.heads;
+    pa_few<DH, 4>(a, i % a.c.seqs, w % a.c.heads, i / a.c.seqs, pa_smem);
+  }
+}
+
+// The parts of each row joined, in part order: a wave takes HPW heads of a token,
+// W lanes of four dims each; of all tokens or (each) of the first ones of every
+// sequence with few rows.
 template <int DH>
-__global__ __launch_bounds__(256) void k_paged_join(PaArgs a) {
-  constexpr int DL = DH / 64;
-  const int lane = threadIdx.x & 63;
-  const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = (int)(w / a.heads), h = (int)(w % a.heads);
-  if (n >= a.c.rows) return;
-  const int s = pg_sequence(a.c.starts, a.c.seqs, n);
-  if (s < 0) return;
+__global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int groups) {
+  constexpr int W = DH / 4, HPW = 64 / W, NP = 64 / W;   // NP: parts a lane weighs, 64 in all
+  const int lane = threadIdx.x & 63, l = lane % W;
+  const int wv = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int n = wv / groups;   // the token, or its place in its sequence
+  const int h = wv % groups * HPW + lane / W;
+  int s = blockIdx.y;
+  if (!each) {
+    if (n >= a.c.rows) return;
+    s = __builtin_amdgcn_readfirstlane(pg_sequence(a.c.starts, a.c.seqs, n));
+    if (s < 0) return;
+  }
   const PaSeq q = pa_seq(a, s);
+  if (each) n += q.first;
   if (n - q.first >= q.n) return;
   const bool few = q.rows <= a.few;
+  if (each && !few) return;
   const int br = few ? 16 : a.br;
-  const int row0 = ((n - q.first) * q.G + h % q.G) / br * br;
+  const int row0 = ((n - q.first) * q.G + min(h, a.heads - 1) % q.G) / br * br;
   int lo, hi;
   pa_span(q, row0, min(br, q.rows - row0), a.window, lo, hi);
   const int np = pa_parts(lo, hi, few ? a.ns_few : a.ns_many).n;
-  if (np == 1) return;
-  const float2* ml = a.pml + w * a.nsmax;
-  const float* po = a.po + w * a.nsmax * DH + lane * DL;
-  float M = -INFINITY;
-  for (int i = 0; i < np; ++i) M = fmaxf(M, ml[i].x);
-  const float base = M == -INFINITY ? 0.f : M;
-  float l = 0.f, o[DL] = {};
-  for (int i = 0; i < np; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[i].x - base);
-    l += ml[i].y * f;
+  // heads of one token may lie in two tiles, of other numbers of parts
+  const bool mine = h < a.heads && np > 1;
+  if (!__any(mine)) return;
+  const long long r = (long long)n * a.heads + min(h, a.heads - 1);
+  const float* po = a.po + r * a.nsmax * DH + l * 4;
+  float m[NP], f[NP], M = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int d = 0; d < DL; ++d) o[d] += po[i * DH + d] * f;
+  for (int k = 0; k < NP; ++k) {
+    const float2 ml = mine && l + W * k < np ? a.pml[r * a.nsmax + l + W * k] : make_float2(-INFINITY, 0.f);
+    m[k] = ml.x;
+    f[k] = ml.y;
+    M = fmaxf(M, m[k]);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  M = group_max<W>(M);
+  const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int d = 0; d < DL; ++d) a.out[w * DH + lane * DL + d] = f2bf(o[d] * inv);
-  if (a.lse && lane == 0) a.lse[w] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * PA_LN2;
+  for (int k = 0; k < NP; ++k) {
+    m[k] = __builtin_amdgcn_exp2f(m[k] - base);
+    sum += f[k] * m[k];
+  }
+  sum = group_sum<W>(sum);
+  floatx4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    for (int i0 = 0; i0 < W; i0 += 8) {
+      if (!__any(mine && W * k + i0 < np)) break;
+      floatx4_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = *(const floatx4_t*)(po + (mine ? min(W * k + i0 + i, np - 1) : 0) * DH);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __shfl(m[k], i0 + i, W);
+        if (W * k + i0 + i < np) o += v[i] * w;
+      }
+    }
+  }
+  if (!mine) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *(uint2*)(a.out + r * DH + l * 4) =
+      make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+  if (a.lse && l == 0) a.lse[r] = sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * PA_LN2;
 }
 
 // What a call launches, from what the host knows: rows and sequences, not how
 // the rows are shared out among them.
 struct PaPlan {
-  int few;             // rows of a sequence up to which k_paged_few takes it
-  bool many;           // k_paged_many runs too
+  int few;             // rows of a sequence up to which pa_few takes it
+  bool many;           // pa_many takes the others
   int qb, tiles;       // its row blocks and (at most) its tiles
   int ns_few, ns_many;
+  bool wide;           // pa_few by eight waves
 };
-static PaPlan pa_plan(const PagedArgs& c, int heads, int window) {
+static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   static const int cus = device_cus();
   PaPlan p{};
   const int G = heads / c.heads;
-  const long long rows = (long long)c.rows * G;
-  long long keys = (long long)c.cols << c.sh;
-  if (window > 0 && keys > window + 31LL) keys = window + 31LL;
+  const long long rows = (long long)c.rows * G, pairs = (long long)c.seqs * c.heads;
+  // entries that a tile of br rows sees at most
+  const auto span = [&](long long br) {
+    const long long all = (long long)c.cols << c.sh;
+    return window > 0 && window + br < all ? window + br : all;
+  };
   const auto clamp = [](long long v, long long hi) { return (int)(v < 1 ? 1 : v > hi ? hi : v); };
-  const long long most = clamp((keys + 127) / 128, 64);
   p.many = rows > 16 && c.rows > c.seqs;
   p.few = !p.many ? 0x7fffffff : c.seqs == 1 ? 0 : 16;
-  p.ns_few = clamp((2LL * cus + (long long)c.seqs * c.heads - 1) / ((long long)c.seqs * c.heads), most);
+  // Few rows: one part, and one launch, up to 1024 entries (us with parts and
+  // without, 6 heads of 128: 1 sequence of 400 entries 18.8 / 14.3, of 1024 18.5 /
+  // 15.4, of 2048 17.9 / 24.9; 64 of 400 23.8 / 18.5, of 1024 43.8 / 42.1), else two
+  // work-groups for each CU; by eight waves where there are CUs to spare (1024
+  // entries, 1 sequence 15.4 against 16.7 by four, 64 of them 46.2 against 42.1).
+  p.ns_few = p.few == 0 || span(16) <= 1024
+                 ? 1 : clamp((2LL * cus + pairs - 1) / pairs, clamp((span(16) + 127) / 128, 64));
+  p.wide = !p.many && p.ns_few == 1 && pairs <= cus;
+  // Many rows: the tile and the number of parts that the figures below put
+  // first.  A step of 32 entries (64 at head dim 64) takes a work-group of 64 rows
+  // 0.475 us, two on one CU 0.68, of 128 rows 0.65 and 0.88; parts cost another
+  // launch and their sums' way to memory and back.  us measured at 12 heads of 128,
+  // 2048 rows on 16384 entries: 64 rows 351 / 274 / 270 in 1 / 2 / 4 parts, 128 rows
+  // 350 / 240 / 230; 6 heads, 512 rows on 8192: 64 rows 122 / 71 / 43 / 35 / 39 in 1
+  // .. 16 parts, 128 rows 160 / 91 / 54 / 38 / 36.
+  p.ns_many = 1;
   if (p.many) {
-    p.qb = rows >= 96LL * c.seqs ? 2 : 1;
-    const int br = 64 * p.qb;
-    const long long bands = c.seqs < c.rows ? c.seqs : c.rows;
-    p.tiles = (int)(rows / br + bands);
-    long long k2 = (long long)c.cols << c.sh;
-    if (window > 0 && k2 > window + br + 31LL) k2 = window + br + 31LL;
-    p.ns_many = clamp((2LL * cus) / ((long long)p.tiles * c.heads), clamp((k2 + 127) / 128, 16));
-  } else {
-    p.ns_many = 1;
+    const float alone[2] = {0.475f, 0.65f}, both[2] = {0.68f, 0.88f};
+    float best = 0.f;
+    for (int qb = 1; qb <= 2; ++qb) {
+      const int br = 64 * qb, step = Dh == 64 ? 64 : 32;
+      const long long keys = span(br);
+      const float tiles = (float)((rows + br - 1) / br) + 0.5f * (float)((c.seqs < c.rows ? c.seqs : c.rows) - 1);
+      for (int ns = 1; ns <= 64 && (ns == 1 || keys / ns >= 256); ns *= 2) {
+        const int each = (int)ceilf(tiles * (float)(c.heads * ns) / (float)cus);   // of a CU's work-groups
+        const float steps = (float)((keys + (long long)step * ns - 1) / ((long long)step * ns));
+        float us = steps * ((float)(each / 2) * both[qb - 1] + (float)(each % 2) * alone[qb - 1]);
+        if (ns > 1) us += 5.f + (float)c.rows * (float)heads * (float)ns * (float)(Dh + 4) * 8.f / 4e6f;
+        if (best == 0.f || us < best) {
+          best = us;
+          p.qb = qb;
+          p.ns_many = ns;
+        }
+      }
+    }
+    p.tiles = (int)(rows / (64 * p.qb) + (c.seqs < c.rows ? c.seqs : c.rows));
   }
   return p;
 }
@@ -812,15 +952,55 @@ static size_t pa_ws(const PagedArgs& c, int heads, int Dh, const PaPlan& p) {
 }
 
 size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh, int window) {
-  return c.rows == 0 || c.seqs == 0 ? 0 : pa_ws(c, heads, Dh, pa_plan(c, heads, window));
+  return c.rows == 0 || c.seqs == 0 ? 0 : pa_ws(c, heads, Dh, pa_plan(c, heads, Dh, window));
+}
+
+template <int DH, int NW>
+static hipError_t pa_launch_few(const PaArgs& a, hipStream_t st) {
+  constexpr size_t lds = pa_few_lds<DH, NW>();
+  if (lds > 64 * 1024) {
+    static PerDevice limit;
+    const hipError_t e = lds_limit(limit, (const void*)k_paged_few<DH, NW>, lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((k_paged_few<DH, NW>), dim3((unsigned)(a.c.heads * a.ns_few), (unsigned)a.c.seqs),
+                     dim3(64 * NW), lds, st, a);
+  return hipGetLastError();
+}
+
+template <int DH>
+static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
+  hipError_t e;
+  if (p.many) {
+    constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>(), f = pa_few_lds<DH, 4>();
+    const long long blocks = (long long)p.tiles * a.c.heads * a.ns_many;
+    const long long more = p.few ? (long long)a.c.seqs * a.c.heads * a.ns_few : 0;
+    if (blocks + more > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(blocks + more));
+    const size_t lds = p.few && f > m ? f : m;
+    if (p.qb == 2)
+      hipLaunchKernelGGL((k_paged_many<DH, 2>), grid, dim3(256), lds, st, a, p.tiles, (int)blocks);
+    else
+      hipLaunchKernelGGL((k_paged_many<DH, 1>), grid, dim3(256), lds, st, a, p.tiles, (int)blocks);
+    e = hipGetLastError();
+  } else {
+    e = p.wide ? pa_launch_few<DH, 8>(a, st) : pa_launch_few<DH, 4>(a, st);
+  }
+  if (e != hipSuccess || a.nsmax == 1) return e;
+  // only rows of sequences with few come in parts where the tiles do not
+  const int G = a.heads / a.c.heads, groups = (a.heads * (DH / 4) + 63) / 64;
+  const int each = p.many && a.ns_many == 1 ? (16 + G - 1) / G : 0;
+  const dim3 grid = each ? dim3((unsigned)((each * groups + 3) / 4), (unsigned)a.c.seqs)
+                         : dim3((unsigned)(((long long)a.c.rows * groups + 3) / 4));
+  hipLaunchKernelGGL(k_paged_join<DH>, grid, dim3(256), 0, st, a, each, groups);
+  return hipGetLastError();
 }
 
 hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
                            int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
                            void* ws, hipStream_t st) {
   if (c.rows == 0 || c.seqs == 0) return hipSuccess;
-  if (Dh != 64 && Dh != 128) return hipErrorInvalidValue;
-  const PaPlan p = pa_plan(c, heads, window);
+  const PaPlan p = pa_plan(c, heads, Dh, window);
   PaArgs a{};
   a.c = c;
   a.q = q;
@@ -828,9 +1008,11 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.qh = qh;
   a.heads = heads;
   a.window = window > 0 ? window : 0x7fffffff;
-  a.sl2 = fabsf(scale) * PA_LOG2E;
+  a.ssl2 = scale * PA_LOG2E;
+  a.sl2 = scale == 0.f ? 1.f : fabsf(a.ssl2);
   a.thr = fminf(8.f / a.sl2, 3e38f);
-  a.neg = scale < 0.f;
+  a.keep = scale == 0.f ? 0u : ~0u;
+  a.flip = scale < 0.f ? 0x80008000u : 0u;
   a.out = out;
   a.lse = lse;
   a.ns_few = p.ns_few;
@@ -840,35 +1022,9 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.br = 64 * p.qb;
   a.po = (float*)ws;
   a.pml = (float2*)((float*)ws + (size_t)c.rows * heads * a.nsmax * Dh);
-  const dim3 block(256);
-  if (p.many) {
-    const long long n = (long long)p.tiles * c.heads * p.ns_many;
-    if (n > 0x7fffffffLL) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)n);
-#define ANN_PM(D, BK, QB) \
-  hipLaunchKernelGGL((k_paged_many<D, BK, QB>), grid, block, 0, st, a, p.tiles)
-    if (Dh == 64) {
-      if (p.qb == 2) ANN_PM(64, 64, 2); else ANN_PM(64, 64, 1);
-    } else {
-      if (p.qb == 2) ANN_PM(128, 32, 2); else ANN_PM(128, 32, 1);
-    }
-#undef ANN_PM
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (p.few > 0) {
-    const dim3 grid((unsigned)(c.heads * p.ns_few), (unsigned)c.seqs);
-    if (Dh == 64) hipLaunchKernelGGL(k_paged_few<64>, grid, block, 0, st, a);
-    else hipLaunchKernelGGL(k_paged_few<128>, grid, block, 0, st, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (a.nsmax > 1) {
-    const dim3 grid((unsigned)(((long long)c.rows * heads + 3) / 4));
-    if (Dh == 64) hipLaunchKernelGGL(k_paged_join<64>, grid, block, 0, st, a);
-    else hipLaunchKernelGGL(k_paged_join<128>, grid, block, 0, st, a);
-  }
-  return hipGetLastError();
+  if (Dh == 64) return pa_launch<64>(a, p, st);
+  if (Dh == 128) return pa_launch<128>(a, p, st);
+  return hipErrorInvalidValue;
 }
 
 // ---- weight of the entries -------------------------------------------------------
@@ -886,7 +1042,7 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
                                                          long long qt, long long qh, int heads,
                                                          FastDiv group,
                                                          const float* __restrict__ lse, float sl2,
-                                                         int neg, int window, const float* w,
+                                                         int window, const float* w,
                                                          long long wrow, float* out, long long orow,
                                                          int cap) {
   constexpr int NKS = DH / 32, NB = PW_E / 16;
@@ -938,7 +1094,7 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
-          kf[b][ks] = pa_query(kr[b] + kvh * c.kh + ks * 32, neg);
+          kf[b][ks] = *(const bf16x8_t*)(kr[b] + kvh * c.kh + ks * 32);
       for (int i = 0; i < n; ++i) {
         floatx4_t sc[NB];
 #pragma unroll
@@ -1002,7 +1158,7 @@ hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long 
 #define ANN_PW(D)                                                                               \
   hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads,                 \
                      FastDiv::of(heads / c.heads), lse,                                         \
-                     fabsf(scale) * PA_LOG2E, (int)(scale < 0.f), win, w, wrow, out, orow, cap)
+                     scale * PA_LOG2E, win, w, wrow, out, orow, cap)
   if (Dh == 64) ANN_PW(64);
   else if (Dh == 128) ANN_PW(128);
   else return hipErrorInvalidValue;

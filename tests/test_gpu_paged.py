@@ -99,7 +99,7 @@ def _setup(case, seed=0):
     return s, case.get("window", 0)
 
 
-@pytest.mark.parametrize("scale", [0.1, -1.5])
+@pytest.mark.parametrize("scale", [0.1, -1.5, 0.0])
 @pytest.mark.parametrize("i", range(len(CASES)))
 def test_attention(i, scale):
     from attention_nn_amd import paged
