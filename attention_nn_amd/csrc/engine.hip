@@ -1217,6 +1217,9 @@ int paged_query(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head
     return fail(ANN_E_ARG, "%d rows of %d heads pass 2^31", c->rows, heads);
   if (((uintptr_t)q & 15) || ((q_row | q_head) & 7))
     return fail(ANN_E_ARG, "query rows must be 16-byte aligned");
+  // a tile's rows within 32 bits of bytes
+  if (q_row < 0 || q_row > (1 << 25) || q_head < 0 || q_head * heads > (1 << 28))
+    return fail(ANN_E_ARG, "query strides %lld, %lld out of range", (long long)q_row, (long long)q_head);
   if (!(scale == scale) || scale - scale != 0.f) return fail(ANN_E_ARG, "scale must be finite");
   return ANN_OK;
 }

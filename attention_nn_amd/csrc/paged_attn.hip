@@ -12,6 +12,9 @@
 
 namespace ann {
 
+// The kernels' window: INT_MAX for none, as for one past the largest table.
+static int pa_window(int window) { return window > 0 && window <= 1 << 30 ? window : 0x7fffffff; }
+
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 
 // One row (token, head) by one wave: 64 entries at a time, a lane for each
@@ -933,7 +936,8 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
       for (int ns = 1; ns <= 64 && (ns == 1 || keys / ns >= 256); ns *= 2) {
         const int each = (int)ceilf(tiles * (float)(c.heads * ns) / (float)cus);   // of a CU's work-groups
         const float steps = (float)((keys + (long long)step * ns - 1) / ((long long)step * ns));
-        float us = steps * ((float)(each / 2) * both[qb - 1] + (float)(each % 2) * alone[qb - 1]);
+        float us = 4.f * (float)((each + 1) / 2) +   // to find the tile and its first entries
+                   steps * ((float)(each / 2) * both[qb - 1] + (float)(each % 2) * alone[qb - 1]);
         if (ns > 1) us += 5.f + (float)c.rows * (float)heads * (float)ns * (float)(Dh + 4) * 8.f / 4e6f;
         if (best == 0.f || us < best) {
           best = us;
@@ -1007,7 +1011,7 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.qt = qt;
   a.qh = qh;
   a.heads = heads;
-  a.window = window > 0 ? window : 0x7fffffff;
+  a.window = pa_window(window);
   a.ssl2 = scale * PA_LOG2E;
   a.sl2 = scale == 0.f ? 1.f : fabsf(a.ssl2);
   a.thr = fminf(8.f / a.sl2, 3e38f);
@@ -1029,31 +1033,40 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 
 // ---- weight of the entries -------------------------------------------------------
 //
-// A work-group takes WE entries of a sequence and all rows (token, head) that see
-// any of them, its waves an equal share of them each: in the order of the cache
-// heads, so that a wave's keys stay in registers from one 16 rows to the next.
-// S = K Q^T, entries x rows, 16 x 16 a product: a lane adds the weights of its
-// row's column for its four entries of each block, and only at the end are the 16
-// columns and the waves added, in a fixed order, so a sum does not depend on what
-// else is in the call.
-constexpr int PW_E = 32;   // entries a work-group
-template <int DH>
-__global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16_t* __restrict__ q,
-                                                         long long qt, long long qh, int heads,
-                                                         FastDiv group,
-                                                         const float* __restrict__ lse, float sl2,
-                                                         int window, const float* w,
-                                                         long long wrow, float* out, long long orow,
-                                                         int cap) {
-  constexpr int NKS = DH / 32, NB = PW_E / 16;
-  __shared__ float part[8][PW_E];
+// A wave takes 16 NB entries of a sequence, `share` of a work-group's NW waves the
+// same ones, and of the rows (token, head) that see any of them, in the order of
+// the cache heads, an equal share each.  S = K Q^T, entries x rows, 16 x 16 a
+// product: a lane adds the weights of its row's column for its four entries of
+// each block, and only at the end are the 16 columns and the waves added, in a
+// fixed order, so a sum does not depend on what else is in the call.
+//
+// FEW: calls of sixteen rows a head or so (decoding), where the keys change from
+// head to head and the next head's are loaded ahead.  Otherwise the keys stay, and
+// the next sixteen rows are.
+template <int DH, bool FEW>
+struct PwShape {
+  static constexpr int NW = FEW ? 4 : 8, NB = 2, E = 16 * NB;
+};
+template <int DH, bool FEW>
+__global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
+    PagedArgs c, const bf16_t* __restrict__ q, long long qt, long long qh, int heads, FastDiv group,
+    const float* __restrict__ lse, float sl2, int window, const float* w, long long wrow, float* out,
+    long long orow, int cap, int share) {
+  constexpr int NW = PwShape<DH, FEW>::NW, NB = PwShape<DH, FEW>::NB, E = PwShape<DH, FEW>::E;
+  constexpr int NKS = DH / 32;
+  __shared__ float part[NW][E];
+  extern __shared__ __attribute__((aligned(16))) unsigned char pw_smem[];   // NW * 2 * 16 rows
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = blockIdx.y, j0 = blockIdx.x * PW_E, j = j0 + tid;
+  const int blocks = NW / share, s = blockIdx.y;
+  const int j0 = (blockIdx.x * blocks + wv / share) * E;
+  // the entry whose sum this thread writes
+  const int j = blockIdx.x * blocks * E + tid;
+  const bool mine = tid < blocks * E && j < cap;
+  const float was = mine ? w[s * wrow + j] : 0.f;
   const int len = pg_len(c.lens[s], c.cols, c.sh);
   const PgRange r = pg_range(c.starts[s], c.starts[s + 1], c.rows);
-  const float was = tid < PW_E && j < cap ? w[s * wrow + j] : 0.f;
-  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + PW_E - 1, len - 1);
+  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + E - 1, len - 1);
   // tokens t0 .. t1 - 1 see one of the entries j0 .. jl
   const int t0 = max(0, j0 - e0), t1 = jl - e0 < r.n - window ? jl - e0 + window : r.n;
   float acc[NB][4];
@@ -1062,8 +1075,8 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
   if (j0 < len && t1 > t0) {
-    const int lo = t0 * G, hi = t1 * G;
-    const int tiles = (hi - lo + 15) / 16, all = tiles * c.heads, per = (all + 7) / 8;
+    const int hi = (t1 - t0) * G;   // rows, from token t0 on
+    const int tiles = (hi + 15) / 16, all = tiles * c.heads, per = (all + share - 1) / share;
     const bf16_t* kr[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -1071,59 +1084,172 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
       const int id = pg_read(c.table[s * c.trow + (k0 >> c.sh)], c.pages);
       kr[b] = c.k + id * c.kp + pg_slot(k0, c.sh, c.ks) + min(r16, jl - k0) * c.ks + g4 * 8;
     }
-    int u = wv * per;
-    const int end = min(u + per, all);
-    while (u < end) {   // the wave's rows of one cache head
-      const int kvh = u / tiles, first = u - kvh * tiles, n = min(tiles - first, end - u);
-      u += n;
-      bf16x8_t kf[NB][NKS], qf[NKS];
-      const bf16_t* qb = q + r.first * qt + (long long)kvh * G * qh + g4 * 8;
-      const float* lb = lse + (long long)r.first * heads + kvh * G;
+    const bf16_t* q0 = q + (r.first + t0) * qt;
+    const float* l0 = lse + (long long)(r.first + t0) * heads;
+    // tiles of whole tokens: a lane's token and head of each are the same
+    const bool whole = 16 % G == 0;
+    const int tg = 16 / G;
+    struct Rows {
+      bf16x8_t q[NKS];
       float l2;
       int e;
-      auto load = [&](int tile) {
-        const int at = lo + tile * 16 + r16, row = min(at, hi - 1), t = group.div(row), h = row - t * G;
-        const bf16_t* qr = qb + t * qt + h * qh;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) qf[ks] = *(const bf16x8_t*)(qr + ks * 32);
-        l2 = lb[(long long)t * heads + h];
-        e = at < hi ? e0 + t : -1;   // a row past the last sees nothing
-      };
-      load(first);
+    };
+    auto keys = [&](bf16x8_t (&kf)[NB][NKS], int kvh) __attribute__((always_inline)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-          kf[b][ks] = *(const bf16x8_t*)(kr[b] + kvh * c.kh + ks * 32);
-      for (int i = 0; i < n; ++i) {
-        floatx4_t sc[NB];
+        for (int ks = 0; ks < NKS; ++ks) kf[b][ks] = *(const bf16x8_t*)(kr[b] + kvh * c.kh + ks * 32);
+    };
+    auto rows = [&](Rows& x, int kvh, int tile) __attribute__((always_inline)) {
+      const unsigned char* qb = (const unsigned char*)(q0 + (long long)kvh * G * qh);
+      const unsigned char* lb = (const unsigned char*)(l0 + kvh * G);
+      const int at = tile * 16 + r16, row = min(at, hi - 1), t = group.div(row), h = row - t * G;
+      const unsigned qx = (unsigned)(t * (int)qt + h * (int)qh + g4 * 8) * 2, lx = (unsigned)(t * heads + h) * 4;
+      x.e = at < hi ? e0 + t0 + t : -1;   // a row past the last sees nothing
 #pragma unroll
-        for (int b = 0; b < NB; ++b) sc[b] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+      for (int ks = 0; ks < NKS; ++ks) x.q[ks] = *(const bf16x8_t*)(qb + qx + ks * 64);
+      x.l2 = *(const float*)(lb + lx);
+    };
+    auto add = [&](const bf16x8_t (&kf)[NB][NKS], const Rows& x, bool full) __attribute__((always_inline)) {
+      floatx4_t sc[NB];
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
+      for (int b = 0; b < NB; ++b) sc[b] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
-            sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], qf[ks], sc[b], 0, 0, 0);
-        const float base = l2 * PA_LOG2E;
-        const int at = e, row0 = lo + (first + i) * 16;
-        if (i + 1 < n) load(first + i + 1);
-        const bool full = row0 + 16 <= hi && e0 + group.div(row0) >= j0 + PW_E - 1 &&
-                          e0 + group.div(row0 + 15) - j0 < window;
-        if (full) {
+      for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][ks], x.q[ks], sc[b], 0, 0, 0);
+      const float base = x.l2 * PA_LOG2E;
+      const int yl = x.e < window ? 0 : x.e - window + 1;   // entries yl .. x.e are seen
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[b][k] += __builtin_amdgcn_exp2f(sc[b][k] * sl2 - base);
-        } else {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int x = j0 + 16 * b + 4 * g4 + k;
-              acc[b][k] += x <= at && at - x < window ? __builtin_amdgcn_exp2f(sc[b][k] * sl2 - base) : 0.f;
-            }
+        for (int k = 0; k < 4; ++k) {
+          const int y = j0 + 16 * b + 4 * g4 + k;
+          const float p = __builtin_amdgcn_exp2f(sc[b][k] * sl2 - base);
+          acc[b][k] += full || (y <= x.e && y >= yl) ? p : 0.f;
         }
+    };
+    int u = wv % share * per;
+    const int end = min(u + per, all);
+    bool done = false;
+    if constexpr (FEW) {
+      if (tiles == 1) {
+        done = true;
+        bf16x8_t kf[2][NB][NKS];
+        Rows x[2];
+        if (u < end) {
+          rows(x[0], u, 0);
+          keys(kf[0], u);
+        }
+        for (; u < end; u += 2)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (u + i >= end) break;
+            if (u + i + 1 < end) {
+              rows(x[1 - i], u + i + 1, 0);
+              keys(kf[1 - i], u + i + 1);
+            }
+            add(kf[i], x[i], false);
+          }
       }
+    }
+    // Sixteens of rows pass through the wave's own two LDS stages, loaded 1 KB at a
+    // time: a fragment's lanes side by side belong to different rows, and read from
+    // memory each is an access of its own (64 for 1 KB instead of 16).  Tiles f0 ..
+    // f1 - 1 are of whole tokens that all see all the entries.
+    constexpr int RB = DH * 2, LPT = 16 * RB / 1024, RPL = 1024 / RB;
+    unsigned char* ring = pw_smem + wv * 2 * 16 * RB;
+    int f0 = 0, f1 = 0;
+    if (whole) {
+      f0 = max(0, (j0 + E - 1 - e0 - t0 + tg - 1) / tg);
+      f1 = min(hi / 16, window == 0x7fffffff ? 0x7fffffff : (window + j0 - e0 - t0) / tg);
+    }
+    unsigned qoff[LPT];
+    int qrow[LPT], qcol[LPT];   // load u: this lane's row of the tile and column in bytes
+#pragma unroll
+    for (int k = 0; k < LPT; ++k) {
+      qrow[k] = k * RPL + lane / (RB / 16);
+      qcol[k] = ((lane % (RB / 16)) ^ pa_kswz<DH>(qrow[k])) * 16;
+      const int t = group.div(qrow[k]);
+      qoff[k] = (unsigned)(t * (int)qt + (qrow[k] - t * G) * (int)qh) * 2 + qcol[k];
+    }
+    auto issue = [&](int kvh, int tile, int stage, bool in) __attribute__((always_inline)) {
+      const int tb = in ? tile * tg : group.div(tile * 16);
+      const unsigned char* qb = (const unsigned char*)(q0 + (long long)kvh * G * qh + tb * qt);
+#pragma unroll
+      for (int k = 0; k < LPT; ++k) {
+        unsigned off = qoff[k];
+        if (!in) {
+          const int row = min(tile * 16 + qrow[k], hi - 1), t = group.div(row);
+          off = (unsigned)((t - tb) * (int)qt + (row - t * G) * (int)qh) * 2 + qcol[k];
+        }
+        const unsigned char* src = qb + off;
+        __builtin_amdgcn_global_load_lds(src, (pa_lds_void*)(ring + stage * 16 * RB + k * 1024), 16, 0, 0);
+      }
+    };
+    pa_lds_cchar* qadr[NKS];
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks)
+      qadr[ks] = (pa_lds_cchar*)ring + r16 * RB + (((ks * 4 + g4) ^ pa_kswz<DH>(r16)) << 4);
+    auto fetch = [&](Rows& x, auto stage) __attribute__((always_inline)) {   // a stage that has arrived
+      constexpr int ST = decltype(stage)::value;
+      pa_static_for<0, NKS>([&](auto kc) __attribute__((always_inline)) {
+        x.q[decltype(kc)::value] = pa_rd_b128<ST * 16 * RB>(qadr[decltype(kc)::value]);
+      });
+      pa_static_for<0, NKS>([&](auto kc) __attribute__((always_inline)) {
+        pa_wait_lgkm<NKS - 1 - decltype(kc)::value>(x.q[decltype(kc)::value]);
+      });
+      asm volatile("" ::: "memory");   // the stage's next load comes behind
+    };
+    // the log sums of 64 rows from `tile` on, a lane each
+    auto sums = [&](int kvh, int tile) __attribute__((always_inline)) {
+      const int row = min(tile * 16 + lane, hi - 1), t = group.div(row);
+      return l0[(long long)t * heads + kvh * G + row - t * G];
+    };
+    while (!done && u < end) {   // the wave's rows of one cache head
+      const int kvh = u / tiles, first = u - kvh * tiles, n = min(tiles - first, end - u);
+      u += n;
+      bf16x8_t kf[NB][NKS];
+      keys(kf, kvh);
+      int i = first;
+      const int stop = first + n, g0 = min(max(f0, first), stop), g1 = min(f1, stop);
+      Rows x;
+      const auto some = [&](int to) __attribute__((always_inline)) {
+        for (; i < to; ++i) {
+          issue(kvh, i, 0, false);
+          const int at = i * 16 + r16, t = group.div(min(at, hi - 1));
+          x.e = at < hi ? e0 + t0 + t : -1;   // a row past the last sees nothing
+          x.l2 = __shfl(sums(kvh, i), r16, 64);
+          pa_wait_vm<0>();
+          fetch(x, std::integral_constant<int, 0>{});
+          add(kf, x, false);
+        }
+      };
+      some(g0);
+      if (i < g1) {
+        issue(kvh, i, 0, true);
+        float ls = sums(kvh, i), ln = 0.f;
+        for (; i < g1; i += 4) {
+          if (i + 4 < g1) ln = sums(kvh, i + 4);
+          pa_static_for<0, 4>([&](auto kc) __attribute__((always_inline)) {
+            constexpr int k = decltype(kc)::value;
+            if (i + k >= g1) return;
+            if (i + k + 1 < g1) {
+              issue(kvh, i + k + 1, (k + 1) & 1, true);
+              pa_wait_vm<LPT>();
+            } else {
+              pa_wait_vm<0>();
+            }
+            fetch(x, std::integral_constant<int, k & 1>{});
+            x.l2 = __shfl(ls, 16 * k + r16, 64);
+            add(kf, x, true);
+          });
+          ls = ln;
+        }
+        i = g1;
+      }
+      some(stop);
     }
   }
 #pragma unroll
@@ -1134,11 +1260,11 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
       if (r16 == 0) part[wv][16 * b + 4 * g4 + i] = v;
     }
   __syncthreads();
-  if (tid >= PW_E || j >= cap) return;
+  if (!mine) return;
   if (j < len) {
-    float v = part[0][tid];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) v += part[k][tid];
+    const int k0 = tid / E * share;
+    float v = part[k0][tid % E];
+    for (int k = 1; k < share; ++k) v += part[k0 + k][tid % E];
     out[s * orow + j] = was + v;
   } else if (out != w) {
     out[s * orow + j] = was;
@@ -1147,23 +1273,50 @@ __global__ __launch_bounds__(512, 4) void k_paged_weight(PagedArgs c, const bf16
 
 size_t paged_weight_ws_bytes(const PagedArgs&, int, int) { return 0; }
 
+template <int DH, bool FEW>
+static hipError_t pw_launch(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
+                            int heads, const float* lse, float sl2, int window, const float* w,
+                            long long wrow, float* out, long long orow, int cap, hipStream_t st) {
+  using S = PwShape<DH, FEW>;
+  static const int cus = device_cus();
+  const long long blocks = (long long)c.seqs * ((cap + S::E - 1) / S::E);
+  // waves that share their entries, while the call's stay below eight (sixteen)
+  // for each CU: 864 tokens of 8 heads of 64 on 4 x 4096 entries 48.0 / 27.0 / 17.8
+  // us with 2 / 4 / 8, one token each on 16 x 4096 (6 x 128) 17.9 / 19.8 / 20.8 with
+  // 1 / 2 / 4
+  int share = 1;
+  while (share < S::NW && blocks * share * 2 <= (FEW ? 8LL : 16LL) * cus) share *= 2;
+  const int per = S::NW / share * S::E;
+  const dim3 grid((unsigned)((cap + per - 1) / per), (unsigned)c.seqs);
+  constexpr size_t lds = (size_t)S::NW * 2 * 16 * DH * 2;
+  if (lds > 32 * 1024) {
+    static PerDevice limit;
+    const hipError_t e = lds_limit(limit, (const void*)k_paged_weight<DH, FEW>, lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((k_paged_weight<DH, FEW>), grid, dim3(64 * S::NW), lds, st, c, q, qt, qh, heads,
+                     FastDiv::of(heads / c.heads), lse, sl2, window, w, wrow, out, orow, cap, share);
+  return hipGetLastError();
+}
+
 hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads,
                         int Dh, const float* lse, float scale, int window, const float* w,
                         long long wrow, float* out, long long orow, void* ws, hipStream_t st) {
   const int cap = c.cols << c.sh;
   if (c.seqs == 0 || cap == 0) return hipSuccess;
   (void)ws;
-  const int win = window > 0 ? window : 0x7fffffff;
-  const dim3 grid((unsigned)((cap + PW_E - 1) / PW_E), (unsigned)c.seqs), block(512);
-#define ANN_PW(D)                                                                               \
-  hipLaunchKernelGGL(k_paged_weight<D>, grid, block, 0, st, c, q, qt, qh, heads,                 \
-                     FastDiv::of(heads / c.heads), lse,                                         \
-                     scale * PA_LOG2E, win, w, wrow, out, orow, cap)
-  if (Dh == 64) ANN_PW(64);
-  else if (Dh == 128) ANN_PW(128);
-  else return hipErrorInvalidValue;
+  const int win = pa_window(window);
+  const bool few = (long long)c.rows * (heads / c.heads) <= 16LL * c.seqs;
+#define ANN_PW(D, F)                                                                             \
+  return pw_launch<D, F>(c, q, qt, qh, heads, lse, scale * PA_LOG2E, win, w, wrow, out, orow, cap, st)
+  if (Dh == 64) {
+    if (few) ANN_PW(64, true); else ANN_PW(64, false);
+  }
+  if (Dh == 128) {
+    if (few) ANN_PW(128, true); else ANN_PW(128, false);
+  }
 #undef ANN_PW
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 }  // namespace ann

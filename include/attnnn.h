@@ -315,7 +315,7 @@ int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream);
  * window: out = softmax(scale q.k_j) v_j (rows, heads, head_dim) bf16, lse
  * (rows, heads) fp32 the natural log of the softmax sum, or null.  A token that
  * sees nothing gets 0 and -infinity.  q (rows, heads, head_dim) bf16 by
- * strides; ws: ann_op_paged_attention_ws_bytes bytes (16-byte aligned). */
+ * strides (q_row at most 2^25, heads * q_head at most 2^28); ws: ann_op_paged_attention_ws_bytes bytes (16-byte aligned). */
 size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads, int32_t window);
 int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
                            int32_t heads, float scale, int32_t window, void* out, float* lse,

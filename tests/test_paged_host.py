@@ -103,6 +103,7 @@ def test_cache_refusals(field, value, msg):
     ({"heads": 8}, "8 query heads over 6"), ({"heads": 0}, "query heads"), ({"q": None}, "null"),
     ({"q": FAKE + 2}, "aligned"), ({"row": 770}, "aligned"), ({"scale": float("nan")}, "finite"),
     ({"scale": float("inf")}, "finite"), ({"window": -1}, "window"), ({"out": None}, "out is null"),
+    ({"row": 1 << 26}, "strides"), ({"head": 1 << 27}, "strides"), ({"row": -768}, "strides"),
     ({"out": FAKE + 4}, "aligned"), ({"heads": 600}, "2^31"),
 ])
 def test_attention_refusals(kw, msg):
