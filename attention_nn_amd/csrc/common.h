@@ -36,6 +36,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_hw));
 }
 
+// A 16-byte store of what the kernel does not read again (non-temporal).
+typedef uint32_t uint4_hw __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void st_once(void* p, const uint4& w) {
+  __builtin_nontemporal_store(__builtin_bit_cast(uint4_hw, w), (uint4_hw*)p);
+}
+
 template <int W>
 __device__ __forceinline__ float group_sum(float v) {
   // butterfly over groups of W consecutive lanes (W a power of two <= 64)

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(NT) void k_evict_move(PagedArgs c, const int32_t* _
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const long long t = s_to[b][u * RP + tid / W];
-      if (t >= 0) *(uint4*)(base + t) = w[u];
+      if (t >= 0) st_once(base + t, w[u]);
     }
     if (i0 + ROWS < end) __syncthreads();   // s_to[b] is read before the next places take it
   }

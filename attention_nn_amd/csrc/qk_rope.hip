@@ -115,7 +115,7 @@ struct QrWord<float> {
     f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
   }
   static __device__ __forceinline__ void store(float* p, const float* f) {
-    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+    st_once(p, __builtin_bit_cast(uint4, make_float4(f[0], f[1], f[2], f[3])));
   }
   static __device__ __forceinline__ void angles(const float* p, float* f) {
     const float2 w = *(const float2*)p;
@@ -127,7 +127,7 @@ struct QrWord<bf16_t> {
   static constexpr int NV = 8;
   static __device__ __forceinline__ void load(const bf16_t* p, float* f) { unpack8(*(const uint4*)p, f); }
   static __device__ __forceinline__ void store(bf16_t* p, const float* f) {
-    *(uint4*)p = make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+    st_once(p, make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7])));
   }
   static __device__ __forceinline__ void angles(const float* p, float* f) {
     const float4 w = *(const float4*)p;
@@ -298,11 +298,11 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedArgs c, QkRows a,
     if (!isv) w = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
     if (!on) continue;
     if (isv) {
-      if (store) *(uint4*)(vd + i_ * c.vh) = w;
+      if (store) st_once(vd + i_ * c.vh, w);
     } else if (isk) {
-      if (store) *(uint4*)(kd + i_ * c.kh) = w;
+      if (store) st_once(kd + i_ * c.kh, w);
     } else {
-      *(uint4*)((bf16_t*)a.qo + ((long long)n * a.Hq + i_) * DH + l * 8) = w;
+      st_once((bf16_t*)a.qo + ((long long)n * a.Hq + i_) * DH + l * 8, w);
     }
   }
 }
