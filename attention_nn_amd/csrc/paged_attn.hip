@@ -139,17 +139,21 @@ __device__ __forceinline__ void pa_static_for(F&& f) {
 }
 
 // How a tile's entries [lo, hi) are shared out: n parts of `per` entries from lo
-// rounded down to 32.  per is a multiple of 64; up to most parts, of 128 entries
-// at least.
+// rounded down to 32, per a multiple of 64.  As many as the call is split into, of
+// 128 entries at least and 4096 at most where `most` parts allow it: a sequence far
+// longer than the others does not keep one work-group.
+struct PaSplit {
+  int split, most;
+};
 struct PaParts {
   int begin, per, n;
 };
-__device__ __forceinline__ PaParts pa_parts(int lo, int hi, int most) {
+__device__ __forceinline__ PaParts pa_parts(int lo, int hi, PaSplit sp) {
   PaParts p;
   p.begin = lo & ~31;
   const int total = hi - p.begin;
   if (hi <= lo) return {0, 64, 1};
-  const int n = min(most, (total + 127) / 128);
+  const int n = min(sp.most, max(min(sp.split, (total + 127) / 128), (total + 4095) / 4096));
   p.per = ((total + n - 1) / n + 63) & ~63;
   p.n = (total + p.per - 1) / p.per;
   return p;
@@ -165,11 +169,14 @@ struct PaArgs {
   uint32_t keep, flip; // of the queries' words: all bits, signs of a negative scale, none of scale 0 (sl2 is 1 then)
   bf16_t* out;
   float* lse;
-  float* po;           // partial sums (rows, heads, parts, DH), or null: one part
-  float2* pml;         // (rows, heads, parts): m in log2 units, sum
-  int ns_few, ns_many; // most parts of a tile of each kind
-  int nsmax;           // the larger, the stride of the partials
+  // parts of a row's sums (slots, most, DH), and (slots, most): m in log2 units, sum
+  float* po_few;
+  float* po_many;
+  float2* ml_few;
+  float2* ml_many;
+  PaSplit sp_few, sp_many;
   int few;             // rows of a sequence up to which pa_few takes it
+  int packed;          // slots of pa_few: 16 a (sequence, cache head), else as pa_many's, (rows, heads)
   int br;              // rows of pa_many's tiles
 };
 
@@ -195,11 +202,28 @@ __device__ __forceinline__ void pa_span(const PaSeq& q, int row0, int n, int win
   hi = max(eh + 1, 0);
 }
 
-// Final or partial result of one row (token, head) part: 4 dims from d on.
-template <int DH>
-__device__ __forceinline__ void pa_store4(const PaArgs& a, int n, int h, int part, int parts, int d,
-                                          float4 o, float m, float l) {
-  const long long r = (long long)n * a.heads + h;
+// A row of a tile: its token and head, and where the sums of its part go.
+struct PaRow {
+  int n, h;
+  long long at;   // slot * most + part
+};
+template <bool FEW>
+__device__ __forceinline__ PaRow pa_place(const PaArgs& a, const PaSeq& q, int s, int kvh, int row,
+                                          int part) {
+  PaRow r;
+  r.n = q.first + row / q.G;
+  r.h = kvh * q.G + row % q.G;
+  const long long slot = FEW && a.packed ? ((long long)s * a.c.heads + kvh) * 16 + row
+                                         : (long long)r.n * a.heads + r.h;
+  r.at = slot * (FEW ? a.sp_few.most : a.sp_many.most) + part;
+  return r;
+}
+
+// Final (parts == 1) or partial result of a row: 4 dims from d on.
+template <int DH, bool FEW>
+__device__ __forceinline__ void pa_store4(const PaArgs& a, const PaRow& w, int parts, int d, float4 o,
+                                          float m, float l) {
+  const long long r = (long long)w.n * a.heads + w.h;
   if (parts == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *(uint2*)(a.out + r * DH + d) =
@@ -207,30 +231,31 @@ __device__ __forceinline__ void pa_store4(const PaArgs& a, int n, int h, int par
     if (d == 0 && a.lse)
       a.lse[r] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * PA_LN2;
   } else {
-    const long long x = r * a.nsmax + part;
-    *(float4*)(a.po + x * DH + d) = o;
-    if (d == 0) a.pml[x] = make_float2(m, l);
+    *(float4*)((FEW ? a.po_few : a.po_many) + w.at * DH + d) = o;
+    if (d == 0) (FEW ? a.ml_few : a.ml_many)[w.at] = make_float2(m, l);
   }
 }
 
 // A row formed entry by entry, over the part [a0, b0) of what it sees.
-template <int DH>
-__device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, const int32_t* table,
-                                         int kvh, int row, int a0, int b0, int part, int parts) {
+template <int DH, bool FEW>
+__device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, int s,
+                                         const int32_t* table, int kvh, int row, int a0, int b0,
+                                         int part, int parts) {
   constexpr int DL = DH / 64;
   const int lane = threadIdx.x & 63;
-  const int t = row / q.G, e = q.e0 + t, n = q.first + t, h = kvh * q.G + row % q.G;
+  const PaRow w = pa_place<FEW>(a, q, s, kvh, row, part);
+  const int e = q.e0 + row / q.G;
   const int lo = max(a0, e < a.window ? 0 : e - a.window + 1), hi = min(b0, e + 1);
   float m, l, o[DL];
-  pa_row<DH>(a.c, table, a.q + n * a.qt + h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
+  pa_row<DH>(a.c, table, a.q + w.n * a.qt + w.h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
   // lane i holds dims i DL ..: four lanes' (two's) values to the one that stores them
   float4 v;
   if constexpr (DL == 1) {
     v = make_float4(o[0], __shfl_down(o[0], 1, 64), __shfl_down(o[0], 2, 64), __shfl_down(o[0], 3, 64));
-    if (lane % 4 == 0) pa_store4<DH>(a, n, h, part, parts, lane, v, m, l);
+    if (lane % 4 == 0) pa_store4<DH, FEW>(a, w, parts, lane, v, m, l);
   } else {
     v = make_float4(o[0], o[1], __shfl_down(o[0], 1, 64), __shfl_down(o[1], 1, 64));
-    if (lane % 2 == 0) pa_store4<DH>(a, n, h, part, parts, lane * 2, v, m, l);
+    if (lane % 2 == 0) pa_store4<DH, FEW>(a, w, parts, lane * 2, v, m, l);
   }
 }
 
@@ -325,7 +350,7 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     const int nrow = min(16, q.rows - row0);
     int lo, hi;
     pa_span(q, row0, nrow, a.window, lo, hi);
-    const PaParts pt = pa_parts(lo, hi, a.ns_few);
+    const PaParts pt = pa_parts(lo, hi, a.sp_few);
     if (part >= pt.n) continue;
     const int a0 = max(pt.begin + part * pt.per, lo), b0 = min(pt.begin + (part + 1) * pt.per, hi);
     const int kb0 = pt.begin + part * pt.per;
@@ -489,11 +514,11 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
       const int r = i / (DH / 4), d = i % (DH / 4) * 4, rr = row0 + r;
       if (s_bad[r]) continue;
       const floatx4_t v = joined(r, d, M, L);
-      pa_store4<DH>(a, q.first + rr / q.G, kvh * q.G + rr % q.G, part, pt.n, d,
-                    make_float4(v[0], v[1], v[2], v[3]), M, L);
+      pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, rr, part), pt.n, d,
+                          make_float4(v[0], v[1], v[2], v[3]), M, L);
     }
     for (int r = wv; r < nrow; r += NW)
-      if (s_bad[r]) pa_again<DH>(a, q, table, kvh, row0 + r, a0, b0, part, pt.n);
+      if (s_bad[r]) pa_again<DH, true>(a, q, s, table, kvh, row0 + r, a0, b0, part, pt.n);
     __syncthreads();   // the sums are read before the next rows' chunks arrive
   }
 }
@@ -536,7 +561,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   const int nrow = min(BR, q.rows - row0);
   int lo, hi;
   pa_span(q, row0, nrow, a.window, lo, hi);
-  const PaParts pt = pa_parts(lo, hi, a.ns_many);
+  const PaParts pt = pa_parts(lo, hi, a.sp_many);
   if (part >= pt.n) return;
   const int kb0 = pt.begin + part * pt.per;
   const int a0 = max(kb0, lo), b0 = min(kb0 + pt.per, hi);
@@ -777,7 +802,8 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   if (!some) return;
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
-    const int row = wr0 + 16 * b + r16, tok = min(row, last) / q.G;
+    const int row = wr0 + 16 * b + r16;
+    const PaRow w = pa_place<false>(a, q, s, kvh, min(row, last), part);
     float l = lsum[b];
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -790,12 +816,12 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
     if (row <= last && !((bad >> r16) & 1))
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
-        pa_store4<DH>(a, q.first + tok, kvh * q.G + row % q.G, part, pt.n, db * 16 + g4 * 4,
-                      make_float4(o[b][db][0], o[b][db][1], o[b][db][2], o[b][db][3]), M, l);
+        pa_store4<DH, false>(a, w, pt.n, db * 16 + g4 * 4,
+                             make_float4(o[b][db][0], o[b][db][1], o[b][db][2], o[b][db][3]), M, l);
     while (bad) {
       const int r = __builtin_ctzll(bad);
       bad &= bad - 1;
-      pa_again<DH>(a, q, table, kvh, wr0 + 16 * b + r, a0, b0, part, pt.n);
+      pa_again<DH, false>(a, q, s, table, kvh, wr0 + 16 * b + r, a0, b0, part, pt.n);
     }
   }
 }
@@ -803,15 +829,26 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
 // Tiles of many rows, then (where a call has both) sequences of few, each by a
 // work-group of its own: the short ones fill the CUs that the long ones leave.
 template <int DH, int QB>
-__global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles, int blocks) {
+__global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles, int full, int blocks) {
   constexpr int BK = DH == 64 ? 64 : 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
   const int L = blockIdx.x;
   if (L < blocks) {
-    // tiles of one (cache head, part) run together on one XCD and share its L2:
-    // work-group L runs on XCD L % 8
-    const int w = blocks % 8 == 0 ? (L % 8) * (blocks / 8) + L / 8 : L;
-    pa_many<DH, BK, QB>(a, w % tiles, (w / tiles) % a.c.heads, w / tiles / a.c.heads, pa_smem);
+    // Tiles of one (cache head, part) run together on one XCD and share its L2:
+    // work-group L runs on XCD L % 8.  That many tiles as the rows fill go first; of
+    // the others, one for each sequence, many are none, and among the first they
+    // would leave CUs to them alone (64 rows on 16384 entries, 12 heads: 47 us).
+    const int pairs = a.c.heads * a.sp_many.most, first = full * pairs;
+    int tile, w = L;
+    if (L < first) {
+      if (first % 8 == 0) w = (L % 8) * (first / 8) + L / 8;
+      tile = w % full;
+      w /= full;
+    } else {
+      tile = full + (L - first) / pairs;
+      w = (L - first) % pairs;
+    }
+    pa_many<DH, BK, QB>(a, tile, w % a.c.heads, w / a.c.heads, pa_smem);
   } else {
     const int w = L - blocks, i = w / a.c.heads;
     pa_few<DH, 4>(a, i % a.c.seqs, w % a.c.heads, i / a.c.seqs, pa_smem);
@@ -840,19 +877,23 @@ __global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int grou
   const bool few = q.rows <= a.few;
   if (each && !few) return;
   const int br = few ? 16 : a.br;
-  const int row0 = ((n - q.first) * q.G + min(h, a.heads - 1) % q.G) / br * br;
+  const int kvh = min(h, a.heads - 1) / q.G, row = (n - q.first) * q.G + min(h, a.heads - 1) % q.G;
+  const int row0 = row / br * br;
   int lo, hi;
   pa_span(q, row0, min(br, q.rows - row0), a.window, lo, hi);
-  const int np = pa_parts(lo, hi, few ? a.ns_few : a.ns_many).n;
+  const PaSplit sp = few ? a.sp_few : a.sp_many;
+  const int np = pa_parts(lo, hi, sp).n;
   // heads of one token may lie in two tiles, of other numbers of parts
   const bool mine = h < a.heads && np > 1;
   if (!__any(mine)) return;
   const long long r = (long long)n * a.heads + min(h, a.heads - 1);
-  const float* po = a.po + r * a.nsmax * DH + l * 4;
+  const long long at = few ? pa_place<true>(a, q, s, kvh, row, 0).at : pa_place<false>(a, q, s, kvh, row, 0).at;
+  const float* po = (few ? a.po_few : a.po_many) + at * DH + l * 4;
+  const float2* pml = (few ? a.ml_few : a.ml_many) + at;
   float m[NP], f[NP], M = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const float2 ml = mine && l + W * k < np ? a.pml[r * a.nsmax + l + W * k] : make_float2(-INFINITY, 0.f);
+    const float2 ml = mine && l + W * k < np ? pml[l + W * k] : make_float2(-INFINITY, 0.f);
     m[k] = ml.x;
     f[k] = ml.y;
     M = fmaxf(M, m[k]);
@@ -893,8 +934,8 @@ __global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int grou
 struct PaPlan {
   int few;             // rows of a sequence up to which pa_few takes it
   bool many;           // pa_many takes the others
-  int qb, tiles;       // its row blocks and (at most) its tiles
-  int ns_few, ns_many;
+  int qb, tiles, full; // its row blocks, its tiles at most and where one sequence has all rows
+  PaSplit sp_few, sp_many;
   bool wide;           // pa_few by eight waves
 };
 static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
@@ -912,22 +953,28 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   p.few = !p.many ? 0x7fffffff : c.seqs == 1 ? 0 : 16;
   // Few rows: one part, and one launch, up to 1024 entries (us with parts and
   // without, 6 heads of 128: 1 sequence of 400 entries 18.8 / 14.3, of 1024 18.5 /
-  // 15.4, of 2048 17.9 / 24.9; 64 of 400 23.8 / 18.5, of 1024 43.8 / 42.1), else two
-  // work-groups for each CU; by eight waves where there are CUs to spare (1024
+  // 15.4, of 2048 17.9 / 24.9; 64 of 400 23.8 / 18.5, of 1024 43.8 / 42.1) or with a
+  // (sequence, head) for each CU (32 x 4096 of 8 heads of 64: 42.3 in one part, 46.6
+  // in two), else what two work-groups a CU take at once (16 x 8192: 77.7 in 5 parts,
+  // 480 work-groups, 87.3 in 6); by eight waves where there are CUs to spare (1024
   // entries, 1 sequence 15.4 against 16.7 by four, 64 of them 46.2 against 42.1).
-  p.ns_few = p.few == 0 || span(16) <= 1024
-                 ? 1 : clamp((2LL * cus + pairs - 1) / pairs, clamp((span(16) + 127) / 128, 64));
-  p.wide = !p.many && p.ns_few == 1 && pairs <= cus;
+  const bool one = p.few == 0 || span(16) <= 1024;
+  p.sp_few.split = one || pairs >= cus ? 1 : clamp(2LL * cus / pairs, clamp((span(16) + 127) / 128, 64));
+  p.sp_few.most = one ? 1 : clamp((span(16) + 4095) / 4096, 64);
+  if (p.sp_few.most < p.sp_few.split) p.sp_few.most = p.sp_few.split;
+  p.wide = !p.many && p.sp_few.most == 1 && pairs <= cus;
   // Many rows: the tile and the number of parts that the figures below put
-  // first.  A step of 32 entries (64 at head dim 64) takes a work-group of 64 rows
-  // 0.475 us, two on one CU 0.68, of 128 rows 0.65 and 0.88; parts cost another
-  // launch and their sums' way to memory and back.  us measured at 12 heads of 128,
+  // first.  A step of 32 entries takes a work-group of 64 rows 0.475 us, two on one
+  // CU 0.68, of 128 rows 0.65 and 0.88 (of 64 entries at head dim 64 0.5, 0.86, 0.75
+  // and 1.4); parts cost another launch and their sums' way to memory and back.  us measured at 12 heads of 128,
   // 2048 rows on 16384 entries: 64 rows 351 / 274 / 270 in 1 / 2 / 4 parts, 128 rows
   // 350 / 240 / 230; 6 heads, 512 rows on 8192: 64 rows 122 / 71 / 43 / 35 / 39 in 1
   // .. 16 parts, 128 rows 160 / 91 / 54 / 38 / 36.
-  p.ns_many = 1;
+  p.sp_many = {1, 1};
   if (p.many) {
-    const float alone[2] = {0.475f, 0.65f}, both[2] = {0.68f, 0.88f};
+    const bool h = Dh == 64;
+    const float alone[2] = {h ? 0.5f : 0.475f, h ? 0.75f : 0.65f};
+    const float both[2] = {h ? 0.86f : 0.68f, h ? 1.4f : 0.88f};
     float best = 0.f;
     for (int qb = 1; qb <= 2; ++qb) {
       const int br = 64 * qb, step = Dh == 64 ? 64 : 32;
@@ -942,21 +989,33 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
         if (best == 0.f || us < best) {
           best = us;
           p.qb = qb;
-          p.ns_many = ns;
+          p.sp_many = {ns, ns};
         }
       }
     }
+    p.full = (int)(rows / (64 * p.qb));
+    if (p.full < 1) p.full = 1;
     p.tiles = (int)(rows / (64 * p.qb) + (c.seqs < c.rows ? c.seqs : c.rows));
   }
   return p;
 }
-static size_t pa_ws(const PagedArgs& c, int heads, int Dh, const PaPlan& p) {
-  const int ns = p.ns_few > p.ns_many ? p.ns_few : p.ns_many;
-  return ns == 1 ? 0 : (size_t)c.rows * heads * ns * (Dh + 2) * 4;
+// Slots of the parts' sums, and the workspace they take: none where all rows come
+// in one part.
+struct PaSlots {
+  size_t few, many;
+};
+static PaSlots pa_slots(const PagedArgs& c, int heads, const PaPlan& p) {
+  PaSlots n = {0, 0};
+  if (p.few && p.sp_few.most > 1)
+    n.few = (p.many ? (size_t)c.seqs * c.heads * 16 : (size_t)c.rows * heads) * p.sp_few.most;
+  if (p.many && p.sp_many.most > 1) n.many = (size_t)c.rows * heads * p.sp_many.most;
+  return n;
 }
 
 size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh, int window) {
-  return c.rows == 0 || c.seqs == 0 ? 0 : pa_ws(c, heads, Dh, pa_plan(c, heads, Dh, window));
+  if (c.rows == 0 || c.seqs == 0) return 0;
+  const PaSlots n = pa_slots(c, heads, pa_plan(c, heads, Dh, window));
+  return (n.few + n.many) * (Dh + 2) * sizeof(float);
 }
 
 template <int DH, int NW>
@@ -967,7 +1026,7 @@ static hipError_t pa_launch_few(const PaArgs& a, hipStream_t st) {
     const hipError_t e = lds_limit(limit, (const void*)k_paged_few<DH, NW>, lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_paged_few<DH, NW>), dim3((unsigned)(a.c.heads * a.ns_few), (unsigned)a.c.seqs),
+  hipLaunchKernelGGL((k_paged_few<DH, NW>), dim3((unsigned)(a.c.heads * a.sp_few.most), (unsigned)a.c.seqs),
                      dim3(64 * NW), lds, st, a);
   return hipGetLastError();
 }
@@ -977,23 +1036,23 @@ static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   hipError_t e;
   if (p.many) {
     constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>(), f = pa_few_lds<DH, 4>();
-    const long long blocks = (long long)p.tiles * a.c.heads * a.ns_many;
-    const long long more = p.few ? (long long)a.c.seqs * a.c.heads * a.ns_few : 0;
+    const long long blocks = (long long)p.tiles * a.c.heads * a.sp_many.most;
+    const long long more = p.few ? (long long)a.c.seqs * a.c.heads * a.sp_few.most : 0;
     if (blocks + more > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(blocks + more));
     const size_t lds = p.few && f > m ? f : m;
     if (p.qb == 2)
-      hipLaunchKernelGGL((k_paged_many<DH, 2>), grid, dim3(256), lds, st, a, p.tiles, (int)blocks);
+      hipLaunchKernelGGL((k_paged_many<DH, 2>), grid, dim3(256), lds, st, a, p.tiles, p.full, (int)blocks);
     else
-      hipLaunchKernelGGL((k_paged_many<DH, 1>), grid, dim3(256), lds, st, a, p.tiles, (int)blocks);
+      hipLaunchKernelGGL((k_paged_many<DH, 1>), grid, dim3(256), lds, st, a, p.tiles, p.full, (int)blocks);
     e = hipGetLastError();
   } else {
     e = p.wide ? pa_launch_few<DH, 8>(a, st) : pa_launch_few<DH, 4>(a, st);
   }
-  if (e != hipSuccess || a.nsmax == 1) return e;
+  if (e != hipSuccess || (a.sp_few.most == 1 && a.sp_many.most == 1)) return e;
   // only rows of sequences with few come in parts where the tiles do not
   const int G = a.heads / a.c.heads, groups = (a.heads * (DH / 4) + 63) / 64;
-  const int each = p.many && a.ns_many == 1 ? (16 + G - 1) / G : 0;
+  const int each = p.many && a.sp_many.most == 1 ? (16 + G - 1) / G : 0;
   const dim3 grid = each ? dim3((unsigned)((each * groups + 3) / 4), (unsigned)a.c.seqs)
                          : dim3((unsigned)(((long long)a.c.rows * groups + 3) / 4));
   hipLaunchKernelGGL(k_paged_join<DH>, grid, dim3(256), 0, st, a, each, groups);
@@ -1019,13 +1078,16 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.flip = scale < 0.f ? 0x80008000u : 0u;
   a.out = out;
   a.lse = lse;
-  a.ns_few = p.ns_few;
-  a.ns_many = p.ns_many;
-  a.nsmax = p.ns_few > p.ns_many ? p.ns_few : p.ns_many;
+  a.sp_few = p.sp_few;
+  a.sp_many = p.sp_many;
   a.few = p.few;
+  a.packed = p.many;
   a.br = 64 * p.qb;
-  a.po = (float*)ws;
-  a.pml = (float2*)((float*)ws + (size_t)c.rows * heads * a.nsmax * Dh);
+  const PaSlots n = pa_slots(c, heads, p);
+  a.po_few = (float*)ws;
+  a.po_many = a.po_few + n.few * Dh;
+  a.ml_few = (float2*)(a.po_many + n.many * Dh);
+  a.ml_many = a.ml_few + n.few;
   if (Dh == 64) return pa_launch<64>(a, p, st);
   if (Dh == 128) return pa_launch<128>(a, p, st);
   return hipErrorInvalidValue;
