@@ -1193,7 +1193,8 @@ int paged_args(const ann_paged* c, bool kv, bool tokens, PagedArgs* a) {
     return fail(ANN_E_ARG, "page_size %d must be a power of two from 16 to 1024", c->page_size);
   if (((long long)c->cols << sh) > (1LL << 30))
     return fail(ANN_E_ARG, "a table row of %d pages of %d passes 2^30 entries", c->cols, c->page_size);
-  if (!c->k || !c->lens || (c->cols && !c->table) || (kv && !c->v) || (tokens && !c->starts))
+  if (!c->k || (kv && !c->v) || (c->seqs && (!c->lens || (c->cols && !c->table))) ||
+      (tokens && !c->starts))
     return fail(ANN_E_ARG, "null argument");
   if (((uintptr_t)c->k | (kv ? (uintptr_t)c->v : 0)) & 15 ||
       (c->k_page | c->k_head | c->k_slot) & 7 || (kv && ((c->v_page | c->v_head | c->v_slot) & 7)))
@@ -1329,7 +1330,7 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
   if (c->seqs == 0) return ANN_OK;
   if (!out_table || !index || !new_lens || (c->cols && (!weight || !weight_out)))
     return fail(ANN_E_ARG, "null argument");
-  if (weight == weight_out && w_row != wo_row)
+  if (c->cols && weight == weight_out && w_row != wo_row)
     return fail(ANN_E_ARG, "weight in place with another row stride");
   HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,
                      index, new_lens, weight_out, wo_row, (hipStream_t)stream));

@@ -33,7 +33,8 @@ from . import _lib
 from ._stream import on_device
 
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
-_Tensor, _empty = torch.Tensor, torch.empty
+_Tensor, _empty, _empty_strided = torch.Tensor, torch.empty, torch.empty_strided
+_paged, _qk_rows = _lib.AnnPaged.from_values, _lib.AnnQkRows.from_values
 
 
 def _refuse(name, x, dtype, dim, d):
@@ -59,19 +60,32 @@ def _pool(k_cache):
 
 
 def _rows(name, x, d):
-    """(rows, heads, head_dim) bf16 that 16-byte loads can read: x, or a copy."""
+    """(rows, heads, head_dim) bf16 that 16-byte loads can read, x or a copy; and
+    its address, row and head stride."""
     _check(name, x, _BF16, 3, d)
     a, b, c = x.stride()
-    if c != 1 or (a | b) & 7 or x.data_ptr() & 15:
+    at = x.data_ptr()
+    if c != 1 or (a | b) & 7 or at & 15:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        a, b, c = x.stride()
+        at = x.data_ptr()
+    return x, at, a, b
 
 
 def _column(name, x, n, d):
     _check(name, x, _I32, 1, d)
     if x.shape[0] != n:
         raise ValueError(f"{name} has {x.shape[0]} elements, expected {n}")
-    return x if n <= 1 or x.stride(0) == 1 else x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def _new(shape, dtype, device):
+    """A contiguous tensor (by its strides: a quarter faster than torch.empty)."""
+    if len(shape) == 3:
+        a, b, c = shape
+        return _empty_strided(shape, (b * c, c, 1), dtype=dtype, device=device)
+    a, b = shape
+    return _empty_strided(shape, (b, 1), dtype=dtype, device=device)
 
 
 def _out(out, like):
@@ -84,21 +98,30 @@ def _out(out, like):
 def _cache(d, k_cache, v_cache, table, lens, starts=None, rows=0):
     """AnnPaged of the call, (sequences, table columns, kv heads, page size, head
     dimension), the table, and what has to outlive the call."""
-    _check("k_cache", k_cache, _BF16, 4, d)
-    _check("table", table, _I32, 2, d)
-    pages, heads, page, dim = k_cache.shape
+    # one expression for what is nearly always so; what is not is named below
+    if not (k_cache.dtype is _BF16 and k_cache.dim() == 4 and isinstance(table, _Tensor)
+            and table.dtype is _I32 and table.dim() == 2 and table.get_device() == d
+            and isinstance(lens, _Tensor) and lens.dtype is _I32 and lens.dim() == 1
+            and lens.get_device() == d):
+        _check("k_cache", k_cache, _BF16, 4, d)
+        _check("table", table, _I32, 2, d)
+        _check("lens", lens, _I32, 1, d)
+    shape = k_cache.shape
+    pages, heads, page, dim = shape
     S, cols = table.shape
     ts, tc = table.stride()
     if tc != 1 and cols > 1:
         table = table.contiguous()
         ts = cols
-    lens = _column("lens", lens, S, d)
+    if lens.shape[0] != S or not lens.is_contiguous():
+        lens = _column("lens", lens, S, d)
     kp, kh, ks, kd = k_cache.stride()
-    v, vp, vh, vs, vd = 0, 0, 0, 0, 1
-    if v_cache is not None:
+    if v_cache is None:
+        v, vp, vh, vs, vd = 0, 0, 0, 0, 1
+    else:
         _check("v_cache", v_cache, _BF16, 4, d)
-        if v_cache.shape != k_cache.shape:
-            raise ValueError(f"v_cache {tuple(v_cache.shape)} differs from {tuple(k_cache.shape)}")
+        if v_cache.shape != shape:
+            raise ValueError(f"v_cache {tuple(v_cache.shape)} differs from {tuple(shape)}")
         v = v_cache.data_ptr()
         vp, vh, vs, vd = v_cache.stride()
     if kd != 1 or vd != 1:
@@ -107,14 +130,14 @@ def _cache(d, k_cache, v_cache, table, lens, starts=None, rows=0):
     if starts is not None:
         starts = _column("starts", starts, S + 1, d)
         first = starts.data_ptr()
-    c = _lib.AnnPaged.from_values(k_cache.data_ptr(), v, kp, kh, ks, vp, vh, vs, table.data_ptr(),
-                                  ts, first, lens.data_ptr(), pages, page, heads, dim, S, cols, rows)
+    c = _paged(k_cache.data_ptr(), v, kp, kh, ks, vp, vh, vs, table.data_ptr(), ts, first,
+               lens.data_ptr(), pages, page, heads, dim, S, cols, rows)
     return c, (S, cols, heads, page, dim), table, (lens, starts)
 
 
 def _weight(name, weight, S, cap, d):
     _check(name, weight, _F32, 2, d)
-    if tuple(weight.shape) != (S, cap):
+    if weight.shape != (S, cap):
         raise ValueError(f"{name} {tuple(weight.shape)} must be (sequences, table entries) = {(S, cap)}")
     return weight if cap <= 1 or weight.stride(1) == 1 else weight.contiguous()
 
@@ -139,7 +162,9 @@ def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps
     the positions run ahead of the entries); the tables ``cs``, ``sn`` (positions,
     head_dim / 4) end there (a position outside takes their nearest row)."""
     d = _pool(k_cache)
-    q, k, v = _rows("q", q, d), _rows("k", k, d), _rows("v", v, d)
+    q, qp, qt, qh = _rows("q", q, d)
+    k, kp, kt, kh = _rows("k", k, d)
+    v, vp, vt, vh = _rows("v", v, d)
     N, H, D = q.shape
     c, (S, _, heads, _, dim), table, keep = _cache(d, k_cache, v_cache, table, lens, starts, N)
     if k.shape != (N, heads, dim) or v.shape != (N, heads, dim) or D != dim:
@@ -148,18 +173,14 @@ def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps
     cs, sn = _angles("cs", cs, D, d), _angles("sn", sn, D, d)
     if cs.shape != sn.shape:
         raise ValueError(f"cs {tuple(cs.shape)} and sn {tuple(sn.shape)} differ")
-    out = _empty((N, H, D), dtype=_BF16, device=q.device) if out is None else _out(out, q)
+    out = _new((N, H, D), _BF16, q.device) if out is None else _out(out, q)
     at = 0
     if pos is not None:
         pos = _column("pos", pos, N, d)
         at = pos.data_ptr()
-    qt, qh, _ = q.stride()
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
-    a = _lib.AnnQkRows.from_values(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, out.data_ptr(), 0,
-                                   0, qt, qh, 0, kt, kh, 0, vt, vh, 0, 0, 0, 0, 0, 0, cs.data_ptr(),
-                                   sn.data_ptr(), at, 1, 0, cs.shape[0], 1, N, H, heads, D,
-                                   _lib.DTYPE_BF16, eps)
+    a = _qk_rows(qp, kp, vp, 0, 0, out.data_ptr(), 0, 0, qt, qh, 0, kt, kh, 0, vt, vh, 0, 0, 0, 0, 0, 0,
+                 cs.data_ptr(), sn.data_ptr(), at, 1, 0, cs.shape[0], 1, N, H, heads, D,
+                 _lib.DTYPE_BF16, eps)
     rc = on_device(d, _lib.lib().ann_op_paged_append, c, a)
     if rc:
         _lib.check(rc)
@@ -168,11 +189,12 @@ def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps
 
 def _queries(q, k_cache, v_cache, table, starts, lens):
     d = _pool(k_cache)
-    q = _rows("q", q, d)
-    c, sizes, table, keep = _cache(d, k_cache, v_cache, table, lens, starts, q.shape[0])
-    if q.shape[2] != sizes[4]:
+    rows = _rows("q", q, d)
+    N, H, D = rows[0].shape
+    c, sizes, table, keep = _cache(d, k_cache, v_cache, table, lens, starts, N)
+    if D != sizes[4]:
         raise ValueError(f"q {tuple(q.shape)}: the cache's head dimension is {sizes[4]}")
-    return q, d, c, sizes, (table, keep)
+    return rows, N, H, D, d, c, sizes, (table, keep)
 
 
 def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_lse=False, out=None):
@@ -183,16 +205,14 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     (rows, heads) fp32, the log of each softmax sum.  A token that sees nothing
     gets 0 and -inf.  Weights enter the product with the values in bf16, as the
     framework's attention forms it; scores, softmax and sums are fp32."""
-    q, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
-    N, H, D = q.shape
+    (q, qp, qt, qh), N, H, D, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
     device = q.device
-    out = _empty((N, H, D), dtype=_BF16, device=device) if out is None else _out(out, q)
+    out = _new((N, H, D), _BF16, device) if out is None else _out(out, q)
     L = _lib.lib()
     nws = L.ann_op_paged_attention_ws_bytes(c, H, window)
-    lse = _empty((N, H), dtype=_F32, device=device) if want_lse else None
+    lse = _new((N, H), _F32, device) if want_lse else None
     ws = _empty(nws, dtype=torch.uint8, device=device) if nws else None
-    qt, qh, _ = q.stride()
-    rc = on_device(d, L.ann_op_paged_attention, c, q.data_ptr(), qt, qh, H, scale, window,
+    rc = on_device(d, L.ann_op_paged_attention, c, qp, qt, qh, H, scale, window,
                    out.data_ptr(), lse.data_ptr() if want_lse else None,
                    ws.data_ptr() if nws else None, nws)
     if rc:
@@ -205,8 +225,8 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
     each entry receives from the new tokens ``q``, over all their heads; ``lse`` as
     ``attention`` returned it for the same tokens.  -> a new tensor, or ``out``,
     which may be ``weight``.  Entries behind a sequence keep their weight."""
-    q, d, c, (S, cols, _, page, _), keep = _queries(q, k_cache, None, table, starts, lens)
-    N, H, _ = q.shape
+    (q, qp, qt, qh), N, H, _, d, c, (S, cols, _, page, _), keep = _queries(q, k_cache, None, table,
+                                                                           starts, lens)
     _check("lse", lse, _F32, 2, d)
     if lse.shape != (N, H):
         raise ValueError(f"lse {tuple(lse.shape)} must be {(N, H)}")
@@ -214,15 +234,13 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
         lse = lse.contiguous()
     weight = _weight("weight", weight, S, cols * page, d)
     if out is None:
-        out = _empty((S, cols * page), dtype=_F32, device=q.device)
+        out = _new((S, cols * page), _F32, q.device)
     elif _weight("out", out, S, cols * page, d) is not out:
         raise ValueError("out: rows must be contiguous")
     L = _lib.lib()
     nws = L.ann_op_paged_weight_ws_bytes(c, H)
     ws = _empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    qt, qh, _ = q.stride()
-    rc = on_device(d, L.ann_op_paged_weight, c, q.data_ptr(), qt, qh, H, lse.data_ptr(), scale,
-                   window, weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
+    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, window, weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
                    ws.data_ptr() if nws else None, nws)
     if rc:
         _lib.check(rc)
@@ -258,9 +276,9 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
     if keep > out_table.shape[1] * page:
         raise ValueError(f"{out_table.shape[1]} pages of {page} do not hold keep={keep} entries")
     device = k_cache.device
-    index = _empty((S, keep), dtype=_I32, device=device)
-    left = _empty((S,), dtype=_I32, device=device)
-    out = _empty((S, cap), dtype=_F32, device=device)
+    index = _new((S, keep), _I32, device)
+    left = _empty(S, dtype=_I32, device=device)
+    out = _new((S, cap), _F32, device)
     rc = on_device(d, _lib.lib().ann_op_paged_evict, c, out_table.data_ptr(), out_table.stride(0),
                    out_table.shape[1], weight.data_ptr(), weight.stride(0), keep, recent,
                    index.data_ptr(), left.data_ptr(), out.data_ptr(), cap)

@@ -448,6 +448,43 @@ def test_chunks_join():
         assert ((y - ref).abs() <= 2 * tol + 2.0 ** -8).all()
 
 
+def test_nothing_there():
+    """No sequences, no rows, a table without pages, sequences without entries."""
+    from attention_nn_amd import paged
+    kc = torch.full((3, 2, 16, 64), 7.0, dtype=BF, device="cuda")
+    vc = kc.clone()
+    ang = torch.zeros((8, 16), device="cuda")
+
+    def i32(*v, shape=None):
+        t = torch.tensor(v, dtype=I32, device="cuda")
+        return t if shape is None else t.view(shape)
+
+    q = torch.ones((4, 2, 64), dtype=BF, device="cuda")
+    for table, starts, lens in ((i32(shape=(0, 2)), i32(0), i32()), (i32(shape=(2, 0)), i32(0, 1, 4), i32(1, 3)),
+                                (i32(0, 1, 2, 0, shape=(2, 2)), i32(0, 0, 0), i32(9, 0)),
+                                (i32(0, 1, 2, 0, shape=(2, 2)), i32(0, 1, 4), i32(0, 0))):
+        S, cap = table.shape[0], table.shape[1] * 16
+        end = int(starts[-1])
+        out = torch.full_like(q, 5.0)
+        paged.append(q, q, q, ang, ang, kc, vc, table, starts, lens, out=out)
+        assert (out[end:] == 5.0).all() and (kc == 7.0).all() and (vc == 7.0).all()
+        out = torch.full_like(q, 5.0)
+        lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, 0, True, out)[1]
+        assert (out[end:] == 5.0).all() and (out[:end] == 0).all() and (lse[:end] == -math.inf).all()
+        w = torch.rand((S, cap), device="cuda")
+        assert torch.equal(paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1), w)
+        n = i32(*([0] * S))
+        k, new, w2 = paged.evict(kc, vc, table, n, w, 5, 2, i32(*([1] * S), shape=(S, 1)))
+        assert (k == -1).all() and (new == 0).all() and (w2 == 0).all() and (kc == 7.0).all()
+    table, starts, lens = i32(0, 1, shape=(1, 2)), i32(0, 0), i32(20)
+    none = q[:0]
+    assert paged.append(none, none, none, ang, ang, kc, vc, table, starts, lens).shape == none.shape
+    out, lse = paged.attention(none, kc, vc, table, starts, lens, 0.1, want_lse=True)
+    assert out.shape == none.shape and lse.shape == (0, 2)
+    w = torch.rand((1, 32), device="cuda")
+    assert torch.equal(paged.attention_weight(none, lse, kc, table, starts, lens, w, 0.1), w)
+
+
 def test_refusals():
     """Wrong types, shapes and sizes are refused before any launch."""
     from attention_nn_amd import paged
