@@ -71,13 +71,19 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int co
   const int old = len - last;           // those that are ranked
   const int want = left - last;         // and how many of them stay
   const int segs = (old + SEG - 1) / SEG;
-  float x[NPT];                         // entry seg * SEG + k * EV_T + tid
+  // weight and word of entry seg * SEG + k * EV_T + tid, bit k of here: it is ranked
+  float x[NPT];
+  uint32_t u[NPT], here;
   auto load = [&](int seg) {
+    here = 0;
 #pragma unroll
     for (int k = 0; k < NPT; ++k) {
       const int i = seg * SEG + k * EV_T + tid;
-      x[k] = i < old ? ws[i] : 0.f;
+      x[k] = ws[min(i, old - 1)];
+      here |= (unsigned)(i < old) << k;
     }
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) u[k] = ev_key(x[k]);
   };
   if (segs == 1) load(0);
   uint32_t edge = 0;                    // smallest word that stays
@@ -95,9 +101,8 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int co
         if (segs > 1) load(seg);
 #pragma unroll
         for (int k = 0; k < NPT; ++k) {
-          const uint32_t u = ev_key(x[k]);
-          if (seg * SEG + k * EV_T + tid < old && (u & mask) == prefix)
-            atomicAdd(&hist[(u >> (8 * byte)) & 255], 1u);
+          if ((here >> k) & 1 && (u[k] & mask) == prefix)
+            atomicAdd(&hist[(u[k] >> (8 * byte)) & 255], 1u);
         }
       }
       __syncthreads();
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int co
     if (!all) {   // ranks among the words equal to the edge
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
-        be[k] = __ballot(seg * SEG + k * EV_T + tid < old && ev_key(x[k]) == edge);
+        be[k] = __ballot((here >> k) & 1 && u[k] == edge);
         if (lane == 0) s_cnt[k * EV_W + wv] = __popcll(be[k]);
       }
       __syncthreads();
@@ -148,10 +153,9 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int co
     unsigned stays = 0;
 #pragma unroll
     for (int k = 0; k < NPT; ++k) {
-      const int i = seg * SEG + k * EV_T + tid;
-      const uint32_t u = ev_key(x[k]);
-      const bool in = i < old && (all || u > edge ||
-                                  (u == edge && tied + s_cnt[k * EV_W + wv] + __popcll(be[k] & below) < ties));
+      const bool in = (here >> k) & 1 &&
+                      (all || u[k] > edge ||
+                       (u[k] == edge && tied + s_cnt[k * EV_W + wv] + __popcll(be[k] & below) < ties));
       stays |= (unsigned)in << k;
     }
     if (!all) tied += s_total;
