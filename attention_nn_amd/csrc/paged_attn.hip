@@ -855,16 +855,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles, int 
   }
 }
 
-// The parts of each row joined, in part order: a wave takes HPW heads of a token,
-// W lanes of four dims each; of all tokens or (each) of the first ones of every
-// sequence with few rows.
-template <int DH>
-__global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int groups) {
+// The parts of each row joined, in part order.  A wave takes a token, its heads HPW
+// at a time, W lanes of four dims each: GP such groups, whose parts' sums are on
+// their way together, and then the next GP * step.  Of all tokens or (each) of the
+// first ones of every sequence with few rows.
+template <int DH, int GP>
+__global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int groups, int waves) {
   constexpr int W = DH / 4, HPW = 64 / W, NP = 64 / W;   // NP: parts a lane weighs, 64 in all
   const int lane = threadIdx.x & 63, l = lane % W;
   const int wv = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int n = wv / groups;   // the token, or its place in its sequence
-  const int h = wv % groups * HPW + lane / W;
+  int n = wv / waves;   // the token, or its place in its sequence
   int s = blockIdx.y;
   if (!each) {
     if (n >= a.c.rows) return;
@@ -877,56 +877,75 @@ __global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int grou
   const bool few = q.rows <= a.few;
   if (each && !few) return;
   const int br = few ? 16 : a.br;
-  const int kvh = min(h, a.heads - 1) / q.G, row = (n - q.first) * q.G + min(h, a.heads - 1) % q.G;
-  const int row0 = row / br * br;
-  int lo, hi;
-  pa_span(q, row0, min(br, q.rows - row0), a.window, lo, hi);
   const PaSplit sp = few ? a.sp_few : a.sp_many;
-  const int np = pa_parts(lo, hi, sp).n;
-  // heads of one token may lie in two tiles, of other numbers of parts
-  const bool mine = h < a.heads && np > 1;
-  if (!__any(mine)) return;
-  const long long r = (long long)n * a.heads + min(h, a.heads - 1);
-  const long long at = few ? pa_place<true>(a, q, s, kvh, row, 0).at : pa_place<false>(a, q, s, kvh, row, 0).at;
-  const float* po = (few ? a.po_few : a.po_many) + at * DH + l * 4;
-  const float2* pml = (few ? a.ml_few : a.ml_many) + at;
-  float m[NP], f[NP], M = -INFINITY, sum = 0.f;
+  for (int g0 = wv % waves * GP; g0 < groups; g0 += waves * GP) {
+    const float* po[GP];
+    int np[GP], most = 0;
+    float m[GP][NP], sum[GP], M[GP];
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const float2 ml = mine && l + W * k < np ? pml[l + W * k] : make_float2(-INFINITY, 0.f);
-    m[k] = ml.x;
-    f[k] = ml.y;
-    M = fmaxf(M, m[k]);
-  }
-  M = group_max<W>(M);
-  const float base = M == -INFINITY ? 0.f : M;
+    for (int g = 0; g < GP; ++g) {
+      const int h = (g0 + g) * HPW + lane / W, hc = min(h, a.heads - 1);
+      const int kvh = hc / q.G, row = (n - q.first) * q.G + hc % q.G, row0 = row / br * br;
+      int lo, hi;
+      pa_span(q, row0, min(br, q.rows - row0), a.window, lo, hi);
+      // heads of one token may lie in two tiles, of other numbers of parts
+      np[g] = h < a.heads ? pa_parts(lo, hi, sp).n : 1;
+      if (np[g] == 1) np[g] = 0;
+      const long long at = few ? pa_place<true>(a, q, s, kvh, row, 0).at : pa_place<false>(a, q, s, kvh, row, 0).at;
+      po[g] = (few ? a.po_few : a.po_many) + at * DH + l * 4;
+      const float2* pml = (few ? a.ml_few : a.ml_many) + at;
+      float f[NP];
+      M[g] = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    m[k] = __builtin_amdgcn_exp2f(m[k] - base);
-    sum += f[k] * m[k];
-  }
-  sum = group_sum<W>(sum);
-  floatx4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    for (int i0 = 0; i0 < W; i0 += 8) {
-      if (!__any(mine && W * k + i0 < np)) break;
-      floatx4_t v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = *(const floatx4_t*)(po + (mine ? min(W * k + i0 + i, np - 1) : 0) * DH);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = __shfl(m[k], i0 + i, W);
-        if (W * k + i0 + i < np) o += v[i] * w;
+      for (int k = 0; k < NP; ++k) {
+        const float2 ml = l + W * k < np[g] ? pml[l + W * k] : make_float2(-INFINITY, 0.f);
+        m[g][k] = ml.x;
+        f[k] = ml.y;
+        M[g] = fmaxf(M[g], m[g][k]);
       }
+      M[g] = group_max<W>(M[g]);
+      const float base = M[g] == -INFINITY ? 0.f : M[g];
+      sum[g] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        m[g][k] = __builtin_amdgcn_exp2f(m[g][k] - base);
+        sum[g] += f[k] * m[g][k];
+      }
+      sum[g] = group_sum<W>(sum[g]);
+      most = max(most, np[g]);
+    }
+    floatx4_t o[GP];
+#pragma unroll
+    for (int g = 0; g < GP; ++g) o[g] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      for (int i0 = 0; i0 < W; i0 += 4) {
+        if (!__any(W * k + i0 < most)) break;
+        floatx4_t v[GP][4];
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)   // of a row that came in one part: its slot, not added
+            v[g][i] = *(const floatx4_t*)(po[g] + max(min(W * k + i0 + i, np[g] - 1), 0) * DH);
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = __shfl(m[g][k], i0 + i, W);
+            if (W * k + i0 + i < np[g]) o[g] += v[g][i] * w;
+          }
+      }
+#pragma unroll
+    for (int g = 0; g < GP; ++g) {
+      if (!np[g]) continue;
+      const long long r = (long long)n * a.heads + (g0 + g) * HPW + lane / W;
+      const float inv = sum[g] == 0.f ? 0.f : 1.f / sum[g];
+      *(uint2*)(a.out + r * DH + l * 4) =
+          make_uint2(pack2(o[g][0] * inv, o[g][1] * inv), pack2(o[g][2] * inv, o[g][3] * inv));
+      if (a.lse && l == 0)
+        a.lse[r] = sum[g] == 0.f ? -INFINITY : (M[g] + __builtin_amdgcn_logf(sum[g])) * PA_LN2;
     }
   }
-  if (!mine) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *(uint2*)(a.out + r * DH + l * 4) =
-      make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
-  if (a.lse && l == 0) a.lse[r] = sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * PA_LN2;
 }
 
 // What a call launches, from what the host knows: rows and sequences, not how
@@ -1053,9 +1072,15 @@ static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   // only rows of sequences with few come in parts where the tiles do not
   const int G = a.heads / a.c.heads, groups = (a.heads * (DH / 4) + 63) / 64;
   const int each = p.many && a.sp_many.most == 1 ? (16 + G - 1) / G : 0;
-  const dim3 grid = each ? dim3((unsigned)((each * groups + 3) / 4), (unsigned)a.c.seqs)
-                         : dim3((unsigned)(((long long)a.c.rows * groups + 3) / 4));
-  hipLaunchKernelGGL(k_paged_join<DH>, grid, dim3(256), 0, st, a, each, groups);
+  // a wave for each group of heads of few tokens, for all those of many (2048 tokens
+  // of 12 heads in 4 parts: 18.3 and 15.4 us)
+  const long long tokens = each ? (long long)each * a.c.seqs : a.c.rows;
+  const bool wide = tokens * groups <= 4096;
+  const int waves = wide ? groups : 1;
+  const dim3 grid = each ? dim3((unsigned)((each * waves + 3) / 4), (unsigned)a.c.seqs)
+                         : dim3((unsigned)(((long long)a.c.rows * waves + 3) / 4));
+  if (wide) hipLaunchKernelGGL((k_paged_join<DH, 1>), grid, dim3(256), 0, st, a, each, groups, waves);
+  else hipLaunchKernelGGL((k_paged_join<DH, 3>), grid, dim3(256), 0, st, a, each, groups, waves);
   return hipGetLastError();
 }
 
