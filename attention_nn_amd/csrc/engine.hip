@@ -1214,15 +1214,31 @@ int paged_query(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head
   if (heads < 1 || heads > 65535 || heads % c->heads)
     return fail(ANN_E_ARG, "%d query heads over %d cache heads", heads, c->heads);
   if (c->rows && !q) return fail(ANN_E_ARG, "null argument");
-  if ((long long)c->rows * heads > 0x7fffffffLL)
-    return fail(ANN_E_ARG, "%d rows of %d heads pass 2^31", c->rows, heads);
+  if ((long long)c->rows * heads > 1 << 30)
+    return fail(ANN_E_ARG, "%d rows of %d heads pass 2^30", c->rows, heads);
   if (((uintptr_t)q & 15) || ((q_row | q_head) & 7))
     return fail(ANN_E_ARG, "query rows must be 16-byte aligned");
   // a tile's rows within 32 bits of bytes
   if (q_row < 0 || q_row > (1 << 25) || q_head < 0 || q_head * heads > (1 << 28))
     return fail(ANN_E_ARG, "query strides %lld, %lld out of range", (long long)q_row, (long long)q_head);
-  if (!(scale == scale) || scale - scale != 0.f) return fail(ANN_E_ARG, "scale must be finite");
+  if (!(scale >= -2e38f && scale <= 2e38f))   // times log2(e) too
+    return fail(ANN_E_ARG, "scale must be finite, at most 2e38");
   return ANN_OK;
+}
+
+// Whether the contiguous rows of out (rows, heads, dim; bf16) share memory with
+// rows x of x_heads heads by strides; not (same_too) where they are the same rows.
+// An x with gaps that out would fit into may lie around it.
+bool paged_overlap(const void* out, int heads, const void* x, int64_t row, int64_t head, int x_heads,
+                   int rows, int dim, bool same_too) {
+  const int64_t n = (int64_t)rows * heads * dim;
+  const int64_t span = (rows - 1LL) * row + (x_heads - 1LL) * head + dim;
+  const uintptr_t o = (uintptr_t)out, p = (uintptr_t)x;
+  if (rows < 1 || o >= p + (uintptr_t)span * 2 || p >= o + (uintptr_t)n * 2) return false;
+  if (same_too && o == p && (rows == 1 || row == (int64_t)heads * dim) &&
+      (heads == 1 || head == dim))
+    return false;
+  return row < n + (int64_t)x_heads * dim && head < n + dim;
 }
 
 int paged_ws(const void* ws, size_t have, size_t need) {
@@ -1261,6 +1277,14 @@ int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream) 
       (r->q_stride[1] | r->q_stride[2] | r->k_stride[1] | r->k_stride[2] | r->v_stride[1] |
        r->v_stride[2]) & 7)
     return fail(ANN_E_ARG, "query, key, value and table rows must be 16-byte aligned");
+  if ((long long)c->rows * r->Hq > 1 << 30)
+    return fail(ANN_E_ARG, "%d rows of %d heads pass 2^30", c->rows, r->Hq);
+  const auto over = [&](const void* x, const int64_t* by, int heads, bool same_too) {
+    return paged_overlap(r->q_out, r->Hq, x, by[1], by[2], heads, c->rows, r->D, same_too);
+  };
+  if (over(r->q, r->q_stride, r->Hq, true) || over(r->k, r->k_stride, r->Hk, false) ||
+      over(r->v, r->v_stride, r->Hk, false))
+    return fail(ANN_E_ARG, "out overlaps the queries, keys or values");
   HIPCHK(paged_append(p, a, (const bf16_t*)r->v, r->v_stride[1], r->v_stride[2],
                       (hipStream_t)stream));
   return ANN_OK;
@@ -1283,6 +1307,8 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
   if (c->rows == 0) return ANN_OK;
   if (!out) return fail(ANN_E_ARG, "out is null");
   if ((uintptr_t)out & 15) return fail(ANN_E_ARG, "out must be 16-byte aligned");
+  if (paged_overlap(out, heads, q, q_row, q_head, heads, c->rows, c->head_dim, true))
+    return fail(ANN_E_ARG, "out overlaps the queries");
   rc = paged_ws(ws, ws_bytes, paged_attention_ws_bytes(p, heads, c->head_dim, window));
   if (rc) return rc;
   HIPCHK(paged_attention(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, scale, window,
@@ -1307,6 +1333,8 @@ int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_
   if (rc) return rc;
   if (c->seqs == 0 || c->cols == 0) return ANN_OK;
   if ((c->rows && !lse) || !weight || !weight_out) return fail(ANN_E_ARG, "null argument");
+  if (c->seqs > 1 && out_row < (int64_t)c->cols * c->page_size)
+    return fail(ANN_E_ARG, "rows of out overlap");
   if (weight == weight_out && w_row != out_row)
     return fail(ANN_E_ARG, "weight in place with another row stride");
   rc = paged_ws(ws, ws_bytes, paged_weight_ws_bytes(p, heads, c->head_dim));
@@ -1330,6 +1358,8 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
   if (c->seqs == 0) return ANN_OK;
   if (!out_table || !index || !new_lens || (c->cols && (!weight || !weight_out)))
     return fail(ANN_E_ARG, "null argument");
+  if (c->seqs > 1 && wo_row < (int64_t)c->cols * c->page_size)
+    return fail(ANN_E_ARG, "rows of weight_out overlap");
   if (c->cols && weight == weight_out && w_row != wo_row)
     return fail(ANN_E_ARG, "weight in place with another row stride");
   HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,

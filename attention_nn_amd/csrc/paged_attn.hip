@@ -670,7 +670,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   // they load ahead is there.
   constexpr int KG = NKS * NBLK, VG = NI * NDB, PG = NBLK * 4 / KG;   // PG weights a group and row block
   static_assert(KG == 8 && KG == VG && PG * KG == NBLK * 4, "one value fragment beside each key fragment");
-  int f0 = max(a0 - kb0, eh - a.window + 1 - kb0);
+  int f0 = max(a0 - kb0, eh < a.window ? 0 : eh - a.window + 1 - kb0);
   f0 = f0 > 0 ? (f0 + BK - 1) / BK : 0;
   const int f1 = some ? min((min(b0, el + 1) - kb0) / BK, (b0 - kb0) / BK - 1 - PM_AHEAD) : 0;
   floatx4_t sc[2][QB][NBLK];

@@ -261,8 +261,7 @@ template <int DH, int NT>
 static void evict_move(const PagedArgs& c, const int32_t* out_table, long long out_row, int out_cols,
                        const int32_t* index, const int32_t* new_lens, int keep, hipStream_t st) {
   constexpr int ROWS = 8 * NT / (DH / 8);
-  const bool same = out_table == c.table;
-  const dim3 grid(same ? 1u : (unsigned)((keep + ROWS - 1) / ROWS), (unsigned)(2 * c.heads),
+  const dim3 grid(NT == 1024 ? 1u : (unsigned)((keep + ROWS - 1) / ROWS), (unsigned)(2 * c.heads),
                   (unsigned)c.seqs);
   hipLaunchKernelGGL((k_evict_move<DH, NT>), grid, dim3(NT), 0, st, c, out_table, out_row, out_cols,
                      index, new_lens, keep);
@@ -284,9 +283,9 @@ hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, lon
 #undef ANN_EP
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  // in place a sequence's tiles follow one another: large work-groups
+  // in place a sequence's tiles follow one another: one large work-group
 #define ANN_EM(D, NT) evict_move<D, NT>(c, out_table, out_row, out_cols, index, new_lens, keep, st)
-  if (out_table == c.table) {
+  if (out_table == c.table && (out_row == c.trow || c.seqs == 1)) {
     if (Dh == 64) ANN_EM(64, 1024); else ANN_EM(128, 1024);
   } else {
     if (Dh == 64) ANN_EM(64, 256); else ANN_EM(128, 256);

@@ -89,6 +89,7 @@ CASES = [
     dict(new=[1], lens=[1100], H=1, Hk=1, page=1024),
     dict(new=[33], lens=[2100], H=1, Hk=1, D=64, page=128),
     dict(new=[150, 1, 200], lens=[150, 400, 260], H=2, Hk=1, window=64),
+    dict(new=[300, 1], lens=[40, 40], H=2, Hk=2),              # tiles of rows that see nothing
 ]
 
 
@@ -485,6 +486,65 @@ def test_nothing_there():
     assert torch.equal(paged.attention_weight(none, lse, kc, table, starts, lens, w, 0.1), w)
 
 
+@pytest.mark.parametrize("new,lens", [([1, 1], [900, 40]), ([1], [9000]), ([150, 1], [170, 60]),
+                                      ([513], [5000])])
+def test_out_is_the_queries(new, lens):
+    """The result in the queries' own memory, in one part and in several."""
+    from attention_nn_amd import paged
+    s = Setup(new, lens, H=4, Hk=2, D=64, garbage=False)
+    kc, vc, table, starts, ends = s.dev()
+    q = s.q.cuda()
+    want, wlse = paged.attention(q, kc, vc, table, starts, ends, 0.1, want_lse=True)
+    x = q.clone()
+    got, lse = paged.attention(x, kc, vc, table, starts, ends, 0.1, want_lse=True, out=x)
+    assert got is x and torch.equal(got, want) and torch.equal(lse, wlse)
+    ang = torch.rand((s.cols * 16, 16), generator=_gen(3)).cuda()
+    k = torch.randn((s.N, 2, 64), generator=_gen(4)).to(BF).cuda()
+    want = paged.append(q, k, k, ang.cos(), ang.sin(), kc, vc, table, starts, ends)
+    x = q.clone()
+    assert torch.equal(paged.append(x, k, k, ang.cos(), ang.sin(), kc, vc, table, starts, ends, out=x), want)
+
+
+def test_shared_pages():
+    """A prefix that two sequences share, read by both; evicted to pages of their own."""
+    from attention_nn_amd import paged
+    s = Setup([1, 20], [100, 130], H=4, Hk=2, D=64, garbage=False, more_cols=1, out_cols=4)
+    s.table[1, :5] = s.table[0, :5]
+    kc, vc, table, starts, lens = s.dev()
+    q = s.q.cuda()
+    ref, _, tol, _ = R.attention(s.q, s.k, s.v, s.table, s.starts, s.lens, 0.1, 0)
+    got, lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, want_lse=True)
+    assert ((got.double().cpu() - ref).abs() <= tol).all()
+    w = paged.attention_weight(q, lse, kc, table, starts, lens, torch.zeros((2, s.cols * 16), device="cuda"), 0.1)
+    ref = R.evict(s.k, s.v, s.table, s.lens, w.cpu(), 60, 20, s.out_table)
+    got = paged.evict(kc, vc, table, lens, w, 60, 20, s.out_table.cuda())
+    assert torch.equal(got[0].cpu(), ref[0])
+    assert torch.equal(kc.cpu(), ref[3]) and torch.equal(vc.cpu(), ref[4])
+
+
+def test_evict_within_a_larger_table():
+    """Pages to go to that begin where the table does and go on elsewhere: the first
+    sequence in place, the others not."""
+    from attention_nn_amd import paged
+    lens, keep = [1500, 1400, 1300], 1200
+    s = Setup([0] * 3, lens, H=1, Hk=1, D=128, garbage=False, out_cols=80)
+    n = s.cols
+    both = torch.empty(4 * 2 * n, dtype=I32)   # rows 2 n apart, and n apart
+    both[:2 * n].view(2, n)[0] = s.table[0]
+    both[n:3 * n] = s.out_table.flatten()[:2 * n]
+    both[2 * n:3 * n] = s.table[1]
+    both[4 * n:5 * n] = s.table[2]
+    dev = both.cuda()
+    table = dev.as_strided((3, n), (2 * n, 1))
+    for seqs, out in ((1, dev.as_strided((1, n), (n, 1))), (2, dev.as_strided((2, n), (n, 1)))):
+        kc, vc = s.cache(s.k), s.cache(s.v)
+        w = torch.rand((3, n * 16), generator=_gen(5))
+        ref = R.evict(s.k, s.v, table[:seqs].cpu(), lens[:seqs], w[:seqs], keep, 100, out.cpu())
+        paged.evict(kc, vc, table[:seqs], torch.tensor(lens[:seqs], dtype=I32, device="cuda"), w[:seqs].cuda(),
+                    keep, 100, out)
+        assert torch.equal(kc.cpu(), ref[3]) and torch.equal(vc.cpu(), ref[4])
+
+
 def test_refusals():
     """Wrong types, shapes and sizes are refused before any launch."""
     from attention_nn_amd import paged
@@ -513,10 +573,14 @@ def test_refusals():
     bad(ValueError, at, q, kc[:, :, :15], vc[:, :, :15], table, starts, lens, 0.1)
     bad(ValueError, at, q, kc, vc, table, starts, lens, 0.1, out=torch.empty_like(q)[:2])
     bad(ValueError, at, q, kc, vc, table.cpu(), starts, lens, 0.1)
+    bad(ValueError, at, q, kc, vc, table, starts, lens, 3e38)
+    two = torch.zeros((4, 4, 64), dtype=BF, device="cuda")
+    bad(ValueError, at, two[1:], kc, vc, table, starts, lens, 0.1, out=two[:-1])
     we = paged.attention_weight
     bad(ValueError, we, q, lse[:2], kc, table, starts, lens, w, 0.1)
     bad(ValueError, we, q, lse, kc, table, starts, lens, w[:, :-1], 0.1)
     bad(TypeError, we, q, lse, kc, table, starts, lens, w.double(), 0.1)
+    bad(ValueError, we, q, lse, kc, table, starts, lens, w, 0.1, out=w[:1].expand(2, -1))
     ev = paged.evict
     bad(ValueError, ev, kc, vc, table, lens, w, 0)
     bad(ValueError, ev, kc, vc, table, lens, w, 8, 9)
@@ -528,3 +592,7 @@ def test_refusals():
     bad(ValueError, ap, q, q[:, :2], q[:2, :2], ang, ang, kc, vc, table, starts, lens)
     bad(ValueError, ap, q, q[:, :2], q[:, :2], ang[:, :8], ang, kc, vc, table, starts, lens)
     bad(TypeError, ap, q, q[:, :2], q[:, :2], ang.double(), ang, kc, vc, table, starts, lens)
+    ang, fused = torch.zeros((40, 16), device="cuda"), torch.zeros((3, 6, 64), dtype=BF, device="cuda")
+    flat = fused.view(-1)[:3 * 4 * 64].view(3, 4, 64)   # the first rows of queries, keys and values
+    bad(ValueError, ap, q, fused[:, 2:4], q[:, :2], ang, ang, kc, vc, table, starts, lens, out=flat)
+    bad(ValueError, ap, fused[:, :4], q[:, :2], q[:, :2], ang, ang, kc, vc, table, starts, lens, out=flat)

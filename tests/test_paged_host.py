@@ -104,7 +104,9 @@ def test_cache_refusals(field, value, msg):
     ({"q": FAKE + 2}, "aligned"), ({"row": 770}, "aligned"), ({"scale": float("nan")}, "finite"),
     ({"scale": float("inf")}, "finite"), ({"window": -1}, "window"), ({"out": None}, "out is null"),
     ({"row": 1 << 26}, "strides"), ({"head": 1 << 27}, "strides"), ({"row": -768}, "strides"),
-    ({"out": FAKE + 4}, "aligned"), ({"heads": 600}, "2^31"),
+    ({"out": FAKE + 4}, "aligned"), ({"heads": 600}, "2^30"),
+    ({"scale": 3e38}, "finite"), ({"out": FAKE + 16}, "overlaps"), ({"out": FAKE + 4 * 768 * 2 - 16}, "overlaps"),
+    ({"out": FAKE - 16}, "overlaps"), ({"row": 1536}, "overlaps"), ({"row": 0}, "overlaps"),
 ])
 def test_attention_refusals(kw, msg):
     assert _attention(_paged(rows=1 << 22 if kw == {"heads": 600} else 4), **kw) == _lib.ANN_E_ARG
@@ -118,7 +120,7 @@ def test_weight_and_evict_refusals():
     def weight(c, lse=FAKE, w=FAKE, wrow=128, out=FAKE, orow=128, heads=6):
         return L.ann_op_paged_weight(c, FAKE, 768, 128, heads, lse, 0.1, 0, w, wrow, out, orow, FAKE, 1 << 40, None)
 
-    for kw in ({"lse": None}, {"w": None}, {"out": None}, {"orow": 256}, {"heads": 9}):
+    for kw in ({"lse": None}, {"w": None}, {"out": None}, {"orow": 256}, {"heads": 9}, {"out": FAKE + 4096, "orow": 120}):
         assert weight(_paged(), **kw) == _lib.ANN_E_ARG
     assert weight(_paged(starts=None)) == _lib.ANN_E_ARG
 
@@ -126,7 +128,7 @@ def test_weight_and_evict_refusals():
         return L.ann_op_paged_evict(c, table, 8, cols, w, wrow, keep, recent, index, lens, out, orow, None)
 
     for kw in ({"keep": 0}, {"recent": -1}, {"recent": 101}, {"table": None}, {"w": None}, {"index": None},
-               {"lens": None}, {"out": None}, {"orow": 64}):
+               {"lens": None}, {"out": None}, {"orow": 64}, {"out": FAKE + 4096, "orow": 120}):
         assert evict(_paged(), **kw) == _lib.ANN_E_ARG, kw
     for kw in ({"cols": 6}, {"cols": -1}, {"keep": 129}):
         assert evict(_paged(), **kw) == _lib.ANN_E_CAPACITY
@@ -152,7 +154,7 @@ def test_rows_refusals():
     assert L.ann_op_qk_norm_rope_bwd(rows(gq=None), None) == _lib.ANN_E_ARG
     assert L.ann_op_qk_norm_rope(None, None) == _lib.ANN_E_ARG
     for kw in [{"D": 64}, {"Hk": 3}, {"Hq": 0}, {"B": 2}, {"T": 5}, {"dtype": 0}, {"v": None}, {"pos": FAKE},
-               {"q": FAKE + 4}, {"cs": FAKE + 4}, {"eps": -1.0}]:
+               {"q": FAKE + 4}, {"cs": FAKE + 4}, {"eps": -1.0}, {"q_out": FAKE + 16}, {"q_out": FAKE - 16}]:
         assert L.ann_op_paged_append(_paged(), rows(**kw), None) == _lib.ANN_E_ARG, kw
     odd = rows()
     odd.k_stride[1] = 4
