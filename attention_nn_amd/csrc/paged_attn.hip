@@ -153,6 +153,7 @@ __device__ __forceinline__ PaParts pa_parts(int lo, int hi, PaSplit sp) {
   p.begin = lo & ~31;
   const int total = hi - p.begin;
   if (hi <= lo) return {0, 64, 1};
+  if (sp.most == 1) return {p.begin, (total + 63) & ~63, 1};
   const int n = min(sp.most, max(min(sp.split, (total + 127) / 128), (total + 4095) / 4096));
   p.per = ((total + n - 1) / n + 63) & ~63;
   p.n = (total + p.per - 1) / p.per;
@@ -164,6 +165,8 @@ struct PaArgs {
   const bf16_t* q;
   long long qt, qh;
   int heads, window;   // window: none is INT_MAX
+  int G;               // heads / cache heads
+  FastDiv by;          // division by G
   float sl2, thr;      // |scale| log2(e); 8 / sl2, the rise of m's that is let pass
   float ssl2;          // scale log2(e)
   uint32_t keep, flip; // of the queries' words: all bits, signs of a negative scale, none of scale 0 (sl2 is 1 then)
@@ -183,6 +186,7 @@ struct PaArgs {
 // One sequence's new tokens as a call sees them.
 struct PaSeq {
   int first, n, len, rows, G, e0;   // e0: entry of token 0
+  FastDiv by;                       // division by G
 };
 __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int s) {
   const PgRange r = pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows);
@@ -190,14 +194,15 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int s) {
   q.first = r.first;
   q.n = r.n;
   q.len = pg_len(a.c.lens[s], a.c.cols, a.c.sh);
-  q.G = a.heads / a.c.heads;
+  q.G = a.G;
+  q.by = a.by;
   q.rows = r.n * q.G;
   q.e0 = q.len - r.n;
   return q;
 }
 // The entries that rows row0 .. row0 + n - 1 see.
 __device__ __forceinline__ void pa_span(const PaSeq& q, int row0, int n, int window, int& lo, int& hi) {
-  const int el = q.e0 + row0 / q.G, eh = q.e0 + (row0 + n - 1) / q.G;
+  const int el = q.e0 + q.by.div(row0), eh = q.e0 + q.by.div(row0 + n - 1);
   lo = el < window ? 0 : el - window + 1;
   hi = max(eh + 1, 0);
 }
@@ -211,8 +216,9 @@ template <bool FEW>
 __device__ __forceinline__ PaRow pa_place(const PaArgs& a, const PaSeq& q, int s, int kvh, int row,
                                           int part) {
   PaRow r;
-  r.n = q.first + row / q.G;
-  r.h = kvh * q.G + row % q.G;
+  const int tok = q.by.div(row);
+  r.n = q.first + tok;
+  r.h = kvh * q.G + row - tok * q.G;
   const long long slot = FEW && a.packed ? ((long long)s * a.c.heads + kvh) * 16 + row
                                          : (long long)r.n * a.heads + r.h;
   r.at = slot * (FEW ? a.sp_few.most : a.sp_many.most) + part;
@@ -244,7 +250,7 @@ __device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, int s,
   constexpr int DL = DH / 64;
   const int lane = threadIdx.x & 63;
   const PaRow w = pa_place<FEW>(a, q, s, kvh, row, part);
-  const int e = q.e0 + row / q.G;
+  const int e = q.e0 + q.by.div(row);
   const int lo = max(a0, e < a.window ? 0 : e - a.window + 1), hi = min(b0, e + 1);
   float m, l, o[DL];
   pa_row<DH>(a.c, table, a.q + w.n * a.qt + w.h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
@@ -335,12 +341,14 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
   float* s_l = s_m + NW * 16;
   int* s_bad = (int*)(s_l + NW * 16);
 
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int32_t* table = a.c.table + s * a.c.trow;
+  // the first 64 page ids, on their way before the sequence's length is known
+  const int first = a.c.cols ? table[min(lane, a.c.cols - 1)] : 0;
   const PaSeq q = pa_seq(a, s);
   if (q.rows == 0 || q.rows > a.few) return;
-  const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
-  const int32_t* table = a.c.table + s * a.c.trow;
   const bf16_t* kh = a.c.k + kvh * a.c.kh;
   const bf16_t* vh = a.c.v + kvh * a.c.vh;
   unsigned char* ring = smem + wv * 2 * TB;
@@ -357,10 +365,11 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     const int nch = b0 > a0 ? (b0 - kb0 + 31) / 32 : 0;
     const int nt = nch > wv ? (nch - wv + NW - 1) / NW : 0;   // chunks of this wave
 
-    const int row = row0 + min(r16, nrow - 1), tok = row / q.G;
+    const int row = row0 + min(r16, nrow - 1), tok = q.by.div(row);
+    // the entries that this lane's row sees of its part, from the lane's first one on
     const int e = q.e0 + tok;
-    const int el = q.e0 + row0 / q.G, eh = q.e0 + (row0 + nrow - 1) / q.G;
-    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row % q.G) * a.qh + g4 * 8;
+    const int jl = max(a0, e < a.window ? 0 : e - a.window + 1) - 4 * g4, jh = min(b0 - 1, e) - 4 * g4;
+    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
     bf16x8_t qf[NKS];
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
@@ -373,7 +382,8 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     // ids of chunks 32 b .. 32 b + 31 of this wave: lane i group i & 1 of chunk i >> 1
     auto ids = [&](int b) {
       const int key = kb0 + 32 * (wv + NW * (32 * b + (lane >> 1))) + 16 * (lane & 1);
-      return pg_read(table[min(max(key, a0), b0 - 1) >> a.c.sh], a.c.pages);
+      const int col = min(max(key, a0), b0 - 1) >> a.c.sh;
+      return pg_read((b0 - 1) >> a.c.sh < 64 ? __shfl(first, col, 64) : table[col], a.c.pages);
     };
     PaPages pg = {nt ? ids(0) : 0, nt > 32 ? ids(1) : 0};
     bf16x8_t kf[2][2][NKS];
@@ -415,23 +425,21 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
         for (int ks = 0; ks < NKS; ++ks)
           sacc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[slot][g][ks], qf[ks], sacc[g], 0, 0, 0);
       }
-      const bool full = kb >= a0 && kb + 31 < b0 && kb + 31 <= el && eh - kb < a.window;
       float p[2][4], lm = -INFINITY;
-      bool ok[2][4];
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = kb + 16 * g + 4 * g4 + r;
-          ok[g][r] = full || (j >= a0 && j < b0 && j <= e && e - j < a.window);
-          lm = fmaxf(lm, ok[g][r] ? sacc[g][r] : -INFINITY);
+        for (int r = 0; r < 4; ++r) {   // what is masked scores -inf
+          const int j = kb + 16 * g + r;
+          p[g][r] = j >= jl && j <= jh ? sacc[g][r] : -INFINITY;
+          lm = fmaxf(lm, p[g][r]);
         }
       if (__any(lm > m + a.thr)) pa_raise<NDB>(lm, a.sl2, m, msl, lsum, o);
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[g][r] = ok[g][r] ? __builtin_amdgcn_exp2f(sacc[g][r] * a.sl2 - msl) : 0.f;
+          p[g][r] = __builtin_amdgcn_exp2f(p[g][r] * a.sl2 - msl);
           lsum += p[g][r];
         }
       uint32_t pw[4], pl[4];   // the weights in bf16, and what that leaves of them
@@ -554,7 +562,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   constexpr int NS = PM_AHEAD + 1;   // stages of keys, and of values
 
   int s = 0, row0 = 0;
-  if (!pg_tile(a.c.starts, a.c.seqs, a.c.rows, a.heads / a.c.heads, a.few, BR, tile, s, row0)) return;
+  if (!pg_tile(a.c.starts, a.c.seqs, a.c.rows, a.G, a.few, BR, tile, s, row0)) return;
   s = __builtin_amdgcn_readfirstlane(s);
   row0 = __builtin_amdgcn_readfirstlane(row0);
   const PaSeq q = pa_seq(a, s);
@@ -575,14 +583,14 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   // this wave's rows, past the last one copies of it; their entries el .. eh
   const int wr0 = row0 + wv * 16 * QB, last = q.rows - 1;
   const bool some = wr0 <= last;
-  const int el = q.e0 + min(wr0, last) / q.G, eh = q.e0 + min(wr0 + 16 * QB - 1, last) / q.G;
+  const int el = q.e0 + q.by.div(min(wr0, last)), eh = q.e0 + q.by.div(min(wr0 + 16 * QB - 1, last));
   bf16x8_t qf[QB][NKS];
   int e[QB];
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
-    const int row = min(wr0 + 16 * b + r16, last), tok = row / q.G;
+    const int row = min(wr0 + 16 * b + r16, last), tok = q.by.div(row);
     e[b] = q.e0 + tok;
-    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row % q.G) * a.qh + g4 * 8;
+    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qf[b][ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
   }
@@ -885,7 +893,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int grou
 #pragma unroll
     for (int g = 0; g < GP; ++g) {
       const int h = (g0 + g) * HPW + lane / W, hc = min(h, a.heads - 1);
-      const int kvh = hc / q.G, row = (n - q.first) * q.G + hc % q.G, row0 = row / br * br;
+      const int kvh = q.by.div(hc), row = (n - q.first) * q.G + hc - kvh * q.G, row0 = row & ~(br - 1);
       int lo, hi;
       pa_span(q, row0, min(br, q.rows - row0), a.window, lo, hi);
       // heads of one token may lie in two tiles, of other numbers of parts
@@ -1070,7 +1078,7 @@ static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   }
   if (e != hipSuccess || (a.sp_few.most == 1 && a.sp_many.most == 1)) return e;
   // only rows of sequences with few come in parts where the tiles do not
-  const int G = a.heads / a.c.heads, groups = (a.heads * (DH / 4) + 63) / 64;
+  const int G = a.G, groups = (a.heads * (DH / 4) + 63) / 64;
   const int each = p.many && a.sp_many.most == 1 ? (16 + G - 1) / G : 0;
   // a wave for each group of heads of few tokens, for all those of many (2048 tokens
   // of 12 heads in 4 parts: 18.3 and 15.4 us)
@@ -1095,6 +1103,8 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.qt = qt;
   a.qh = qh;
   a.heads = heads;
+  a.G = heads / c.heads;
+  a.by = FastDiv::of(a.G);
   a.window = pa_window(window);
   a.ssl2 = scale * PA_LOG2E;
   a.sl2 = scale == 0.f ? 1.f : fabsf(a.ssl2);
