@@ -322,7 +322,12 @@ struct PaPages {
 // take chunks of 32 entries in turn and meet only at the end: keys from memory
 // straight into the fragments of the product, a chunk ahead; values into the
 // wave's own ring of two LDS stages.  The products have time to spare here, and the
-// weights enter as two bf16 halves (2^-17 of each).
+// weights enter as two bf16 halves (2^-17 of each).  Bound by memory on long caches
+// (one token on 16 x 8192 entries of 6 heads of 128 in 5 parts: 59 us and 5 to join
+// them, 290 MB, 4.5 TB/s of a copy's 5.2), by the wait for one read after another and
+// a chunk's some 370 instructions a wave on short ones (777 entries: 11.9 us; 13.0
+// with the page ids read only behind the length, divisions by the group and four
+// compares a mask).
 template <int DH, int NW>
 constexpr size_t pa_few_lds() {
   // the rings; after them the waves' sums, their maxima and totals, rows to form again
@@ -542,7 +547,14 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
 // A work-group takes BR = 64 QB rows (four waves of QB x 16) and a part of the
 // entries, which pass through a ring of two LDS stages shared by its waves: loaded
 // straight into LDS a step ahead, one barrier a step.  A key or value fragment
-// read from LDS serves QB products.
+// read from LDS serves QB products.  Bound by the matrix units and the vector units
+// beside them (an exponential costs four instructions' time, a weight seven in all):
+// 2048 tokens of 12 heads of 128 on 16384 entries 229 us, 193 GFLOP at 0.84 PFLOP/s,
+// the matrix units busy 45% of the time and the vector units 50%, no bank conflicts;
+// a large product of the same card reaches 1.38.  24 ragged sequences on a window of
+// 384, 50 MB and 4 GFLOP, take 20.5 us: a dozen steps behind the search for the tile.
+// No faster: three steps ahead, higher priority of waves in the products (230 and
+// 233), parts by thirds.
 constexpr int PM_AHEAD = 1;   // steps that loads run ahead (odd: a step's parity is its stage's)
 template <int LPW>
 struct PaWalk {
@@ -1139,7 +1151,9 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 //
 // FEW: calls of sixteen rows a head or so (decoding), where the keys change from
 // head to head and the next head's are loaded ahead.  Otherwise the keys stay, and
-// the next sixteen rows are.
+// the next sixteen rows are.  FEW is bound by memory (one token on 16 x 4096 entries of
+// 6 heads of 128: 17.7 us, 4.3 TB/s), the other by the vector units' exponentials (4 x
+// 512 tokens of 8 heads of 64 on up to 4096 entries: 16.9 us, 156 TFLOP/s of products).
 template <int DH, bool FEW>
 struct PwShape {
   static constexpr int NW = FEW ? 4 : 8, NB = 2, E = 16 * NB;

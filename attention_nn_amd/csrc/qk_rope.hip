@@ -104,7 +104,12 @@ __global__ __launch_bounds__(256) void k_qk_rope_any(QkRows a, long long n) {
 
 // The same for head dims 64 and 128 of 16-byte aligned rows: one wave for each
 // token, whose heads pass four (or so) at a time, W lanes of 16 bytes each, with
-// the token's angles read once.
+// the token's angles read once.  Bound by memory: a value is read (twice with its
+// gradient) and written once, for 5 (10) operations.  U groups of heads are on
+// their way together.  Measured: 64 x 512 tokens of 6 + 6 heads of 128 in bf16, of a
+// fused projection, 32.6 us, 6.2 TB/s; the gradient at 16 x 1023 tokens of 8 + 8
+// heads of 64 in fp32 36.3 us, 5.6 TB/s (a 1 GiB copy: 5.2 TB/s).  A wave for each
+// row (above) takes 118 and 107 us there.
 template <typename T>
 struct QrWord;
 template <>
@@ -241,6 +246,10 @@ hipError_t qk_norm_rope(const QkRows& a, bool bwd, int dtype, hipStream_t st) {
 // Queries and keys are normalised and turned; a key and a value go to their
 // entry's slot, a query to its row of the output.  A token behind the last
 // sequence's, an entry outside the table and a page that is none are left alone.
+// Bound by memory where there is enough of it: 4,200 tokens of 3 x 12 heads of 128, 15.0 us,
+// 5.2 TB/s; a decoding step of 64 sequences (0.6 MB) takes
+// 6.2 us, a launch and three reads that wait for one another (starts, then length
+// and table, beside the rows; then the angles).
 template <int DH>
 __global__ __launch_bounds__(256) void k_paged_append(PagedArgs c, QkRows a,
                                                       const bf16_t* __restrict__ v, long long vt,
