@@ -547,14 +547,18 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
 // A work-group takes BR = 64 QB rows (four waves of QB x 16) and a part of the
 // entries, which pass through a ring of two LDS stages shared by its waves: loaded
 // straight into LDS a step ahead, one barrier a step.  A key or value fragment
-// read from LDS serves QB products.  Bound by the matrix units and the vector units
-// beside them (an exponential costs four instructions' time, a weight seven in all):
-// 2048 tokens of 12 heads of 128 on 16384 entries 229 us, 193 GFLOP at 0.84 PFLOP/s,
-// the matrix units busy 45% of the time and the vector units 50%, no bank conflicts;
-// a large product of the same card reaches 1.38.  24 ragged sequences on a window of
-// 384, 50 MB and 4 GFLOP, take 20.5 us: a dozen steps behind the search for the tile.
-// No faster: three steps ahead, higher priority of waves in the products (230 and
-// 233), parts by thirds.
+// read from LDS serves QB products.  Bound by three units that a step needs for about
+// as long, in cycles for one wave on each SIMD: the matrix units 512, the vector units
+// some 600 (an exponential takes four instructions' time), LDS 560 (430 of reads).  A
+// model of the step without its LDS reads takes 196 ns a wave, with them 317, with
+// barrier and loads 358; here it is 440, and 650 where a CU has one work-group alone.
+// 2048 tokens of 12 heads of 128 on 16384 entries: 229 us, 193 GFLOP at 0.84 PFLOP/s
+// (a large product of the same card: 1.38), matrix units busy 40% of the time, no bank
+// conflicts; its 768 work-groups fill 512 places once and half again.  24 ragged
+// sequences on a window of 384, 50 MB and 4 GFLOP, take 20.5 us: a dozen steps behind
+// the search for the tile.  No faster: three steps ahead, higher priority of waves in
+// the products (230 and 233), sums and maxima beside the products with P (228), parts
+// by thirds, fifths and sixths.
 constexpr int PM_AHEAD = 1;   // steps that loads run ahead (odd: a step's parity is its stage's)
 template <int LPW>
 struct PaWalk {
