@@ -169,7 +169,7 @@ struct PaArgs {
   FastDiv by;          // division by G
   float sl2, thr;      // |scale| log2(e); 8 / sl2, the rise of m's that is let pass
   float ssl2;          // scale log2(e)
-  uint32_t keep, flip; // of the queries' words: all bits, signs of a negative scale, none of scale 0 (sl2 is 1 then)
+  uint32_t keep, flip; // of the queries' words: the bits kept (scale 0: none, sl2 is 1) and turned (below 0: signs)
   bf16_t* out;
   float* lse;
   // parts of a row's sums (slots, most, DH), and (slots, most): m in log2 units, sum
@@ -1009,9 +1009,9 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   // Many rows: the tile and the number of parts that the figures below put
   // first.  A step of 32 entries takes a work-group of 64 rows 0.475 us, two on one
   // CU 0.68, of 128 rows 0.65 and 0.88 (of 64 entries at head dim 64 0.5, 0.86, 0.75
-  // and 1.4); parts cost another launch and their sums' way to memory and back.  us measured at 12 heads of 128,
-  // 2048 rows on 16384 entries: 64 rows 351 / 274 / 270 in 1 / 2 / 4 parts, 128 rows
-  // 350 / 240 / 230; 6 heads, 512 rows on 8192: 64 rows 122 / 71 / 43 / 35 / 39 in 1
+  // and 1.4); parts cost another launch and their sums' way to memory and back.  us
+  // measured at 12 heads of 128, 2048 rows on 16384 entries: 64 rows 351 / 274 / 270
+  // in 1 / 2 / 4 parts, 128 rows 350 / 240 / 230; 6 heads, 512 rows on 8192: 64 rows 122 / 71 / 43 / 35 / 39 in 1
   // .. 16 parts, 128 rows 160 / 91 / 54 / 38 / 36.
   p.sp_many = {1, 1};
   if (p.many) {
@@ -1156,8 +1156,11 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 // FEW: calls of sixteen rows a head or so (decoding), where the keys change from
 // head to head and the next head's are loaded ahead.  Otherwise the keys stay, and
 // the next sixteen rows are.  FEW is bound by memory (one token on 16 x 4096 entries of
-// 6 heads of 128: 17.7 us, 4.3 TB/s), the other by the vector units' exponentials (4 x
-// 512 tokens of 8 heads of 64 on up to 4096 entries: 16.9 us, 156 TFLOP/s of products).
+// 6 heads of 128: 17.7 us, 4.3 TB/s), the other by its vector instructions on
+// the CUs whose sequences have the most rows (864 tokens of 8 heads of 64, 462 of them
+// on one of four sequences of up to 4096 entries: 16.9 us; all CUs' vector units are
+// busy 55% of 13 us).  No faster: rows three tiles ahead (16.4, but 30 to 34 us for 29
+// at head dim 128), 16 or 64 entries a wave (16.9 and 21.6), four waves (22.7).
 template <int DH, bool FEW>
 struct PwShape {
   static constexpr int NW = FEW ? 4 : 8, NB = 2, E = 16 * NB;

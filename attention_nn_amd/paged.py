@@ -25,6 +25,9 @@ The cache may have any strides over page, head and slot (multiples of 8), and a
 head of it serves ``heads / kv_heads`` query heads behind one another.
 Tensors live on one GPU, which need not be the current device; the work goes to
 its current stream.
+
+A page that a call writes belongs to one sequence; pages that are only read may
+be shared by several (a common prefix).
 """
 
 import torch
@@ -156,7 +159,7 @@ def append(q, k, v, cs, sn, k_cache, v_cache, table, starts, lens, pos=None, eps
     """New tokens enter the cache: queries ``q`` (rows, heads, head_dim) and keys
     ``k`` (rows, kv_heads, head_dim) normalised and rotated as
     ``kernels.qk_norm_rope`` does, keys and values ``v`` to their entries.
-    -> the queries, contiguous (``out``, where given).
+    -> the queries, contiguous (``out``, where given; it may be ``q``).
 
     A token's position is its entry, or ``pos`` (rows,) int32 (after an eviction
     the positions run ahead of the entries); the tables ``cs``, ``sn`` (positions,
@@ -203,8 +206,10 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     entries ``j <= e`` and, with ``window`` > 0, ``e - j < window``.
     -> (rows, heads, head_dim) bf16 (``out``, where given); with ``want_lse`` also
     (rows, heads) fp32, the log of each softmax sum.  A token that sees nothing
-    gets 0 and -inf.  Weights enter the product with the values in bf16, as the
-    framework's attention forms it; scores, softmax and sums are fp32."""
+    gets 0 and -inf.  ``out`` may be ``q``.  Scores, softmax and sums are fp32; the
+    weights enter the product with the values in two bf16 halves where a sequence
+    has up to 16 rows (tokens times shared heads), else in bf16, as in the
+    framework's other attention."""
     (q, qp, qt, qh), N, H, D, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
     device = q.device
     out = _new((N, H, D), _BF16, device) if out is None else _out(out, q)
@@ -240,7 +245,8 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
     L = _lib.lib()
     nws = L.ann_op_paged_weight_ws_bytes(c, H)
     ws = _empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, window, weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
+    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, window,
+                   weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
                    ws.data_ptr() if nws else None, nws)
     if rc:
         _lib.check(rc)
@@ -255,7 +261,8 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
     -> (index, lens, weight): the entry that each came from (sequences, keep)
     int32, -1 behind them; the new lengths; their weights, 0 behind them.
 
-    ``out_table`` names pages that ``table`` does not (or is ``table``).  Keys hold
+    ``out_table`` names pages that ``table`` does not, each once (or is ``table``); in
+    place, no two sequences share a page.  ``recent`` is at most ``keep``.  Keys hold
     their rotation, so later tokens go on at their own positions: pass ``pos`` to
     ``append``."""
     d = _pool(k_cache)

@@ -289,8 +289,9 @@ int ann_op_qk_norm_rope_bwd(const ann_qk_rows* r, void* stream);
  * device arrays: ids that are no page are never written to and read page 0,
  * lengths outside the table end at it.  Rows of queries, keys, values and
  * cache slots are 16-byte aligned (strides multiples of 8, slots at most 2^25
- * elements apart).  A head of the
- * cache serves heads / cache heads query heads behind one another. */
+ * elements apart).  A head of the cache serves heads / cache heads query heads
+ * behind one another.  Pages that a call writes belong to one sequence; pages
+ * that are only read may be shared. */
 typedef struct ann_paged {
   void* k;               /* bf16, (pages, heads, page_size, head_dim) by the strides */
   void* v;
@@ -315,7 +316,9 @@ int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream);
  * window: out = softmax(scale q.k_j) v_j (rows, heads, head_dim) bf16, lse
  * (rows, heads) fp32 the natural log of the softmax sum, or null.  A token that
  * sees nothing gets 0 and -infinity.  q (rows, heads, head_dim) bf16 by
- * strides (q_row at most 2^25, heads * q_head at most 2^28); ws: ann_op_paged_attention_ws_bytes bytes (16-byte aligned). */
+ * strides (q_row at most 2^25, heads * q_head at most 2^28; rows * heads at most
+ * 2^30); out may be q, by contiguous rows.  ws: ann_op_paged_attention_ws_bytes
+ * bytes (16-byte aligned), one for each call in flight. */
 size_t ann_op_paged_attention_ws_bytes(const ann_paged* c, int32_t heads, int32_t window);
 int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
                            int32_t heads, float scale, int32_t window, void* out, float* lse,
@@ -337,11 +340,11 @@ int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_
  * `recent` and, of the others, those of the largest weight (of equal ones the
  * lower entry; NaN below every number), min(len, keep) in all, moved in order
  * to entries 0 .. of the pages in out_table (seqs, out_cols; rows out_row
- * elements apart).  out_table is the table itself (in place) or names pages
- * that the table does not.  index (seqs, keep): the entry each came from, -1
- * behind them; new_lens (seqs); weight_out (seqs, cols * page_size): their
- * weights, 0 behind them; it may be weight, and new_lens may be c->lens.
- * c->starts is not read. */
+ * elements apart).  out_table is the table itself (in place: no two sequences
+ * share a page) or names pages that the table does not, each once.  index (seqs,
+ * keep): the entry each came from, -1 behind them; new_lens (seqs); weight_out
+ * (seqs, cols * page_size): their weights, 0 behind them; it may be weight, and
+ * new_lens may be c->lens.  c->starts is not read. */
 int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out_row,
                        int32_t out_cols, const float* weight, int64_t w_row, int32_t keep,
                        int32_t recent, int32_t* index, int32_t* new_lens, float* weight_out,
