@@ -96,18 +96,26 @@ __device__ __forceinline__ int pg_sequence(const int32_t* __restrict__ starts, i
 }
 
 // The tile-th tile of br rows of the sequences with more than `few` rows (g rows
-// for each new token), by a whole wave: its sequence and first row, or false where
-// there are fewer tiles.
-__device__ __forceinline__ bool pg_tile(const int32_t* __restrict__ starts, int seqs, int rows,
-                                        int g, int few, int br, int tile, int& seq, int& row0) {
+// for each new token), by a whole wave: its sequence and first row, the sequence's
+// new tokens and length (read beside its rows); seq -1 where there are fewer tiles.
+struct PgTile {
+  int seq, row0;
+  PgRange r;
+  int len;
+};
+__device__ __forceinline__ PgTile pg_tile(const int32_t* __restrict__ starts,
+                                          const int32_t* __restrict__ lens, int seqs, int rows,
+                                          int g, int few, int br, int tile) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int s0 = 0; s0 < seqs; s0 += 64) {
     const int s = s0 + lane;
-    int n = 0;
+    int n = 0, len = 0;
+    PgRange r = {0, 0};
     if (s < seqs) {
-      const int r = pg_range(starts[s], starts[s + 1], rows).n * g;
-      n = r > few ? (r + br - 1) / br : 0;
+      len = lens[s];
+      r = pg_range(starts[s], starts[s + 1], rows);
+      n = r.n * g > few ? (r.n * g + br - 1) / br : 0;
     }
     int sum = n;   // of this lane's sequence and those before it
 #pragma unroll
@@ -118,13 +126,13 @@ __device__ __forceinline__ bool pg_tile(const int32_t* __restrict__ starts, int 
     const unsigned long long past = __ballot(before + sum > tile);
     if (past) {
       const int at = __builtin_ctzll(past);
-      seq = s0 + at;
-      row0 = (tile - before - __shfl(sum - n, at, 64)) * br;
-      return true;
+      return {s0 + at, (tile - before - __builtin_amdgcn_readlane(sum - n, at)) * br,
+              {__builtin_amdgcn_readlane(r.first, at), __builtin_amdgcn_readlane(r.n, at)},
+              __builtin_amdgcn_readlane(len, at)};
     }
     before += __shfl(sum, 63, 64);
   }
-  return false;
+  return {-1, 0, {0, 0}, 0};
 }
 #endif
 

@@ -188,17 +188,19 @@ struct PaSeq {
   int first, n, len, rows, G, e0;   // e0: entry of token 0
   FastDiv by;                       // division by G
 };
-__device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int s) {
-  const PgRange r = pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows);
+__device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, PgRange r, int len) {
   PaSeq q;
   q.first = r.first;
   q.n = r.n;
-  q.len = pg_len(a.c.lens[s], a.c.cols, a.c.sh);
+  q.len = pg_len(len, a.c.cols, a.c.sh);
   q.G = a.G;
   q.by = a.by;
   q.rows = r.n * q.G;
   q.e0 = q.len - r.n;
   return q;
+}
+__device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int s) {
+  return pa_seq(a, pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows), a.c.lens[s]);
 }
 // The entries that rows row0 .. row0 + n - 1 see.
 __device__ __forceinline__ void pa_span(const PaSeq& q, int row0, int n, int window, int& lo, int& hi) {
@@ -552,10 +554,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
 // some 600 (an exponential takes four instructions' time), LDS 560 (430 of reads).  A
 // model of the step without its LDS reads takes 196 ns a wave, with them 317, with
 // barrier and loads 358; here it is 440, and 650 where a CU has one work-group alone.
-// 2048 tokens of 12 heads of 128 on 16384 entries: 229 us, 193 GFLOP at 0.84 PFLOP/s
+// 2048 tokens of 12 heads of 128 on 16384 entries: 227 us, 193 GFLOP at 0.85 PFLOP/s
 // (a large product of the same card: 1.38), matrix units busy 40% of the time, no bank
 // conflicts; its 768 work-groups fill 512 places once and half again.  24 ragged
-// sequences on a window of 384, 50 MB and 4 GFLOP, take 20.5 us: a dozen steps behind
+// sequences on a window of 384, 50 MB and 4 GFLOP, take 20.2 us: a dozen steps behind
 // the search for the tile.  No faster: three steps ahead, higher priority of waves in
 // the products (230 and 233), sums and maxima beside the products with P (228), parts
 // by thirds, fifths and sixths.
@@ -577,11 +579,10 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   constexpr int NKS = DH / 32, NDB = DH / 16, NBLK = BK / 16, NI = BK / 32;
   constexpr int NS = PM_AHEAD + 1;   // stages of keys, and of values
 
-  int s = 0, row0 = 0;
-  if (!pg_tile(a.c.starts, a.c.seqs, a.c.rows, a.G, a.few, BR, tile, s, row0)) return;
-  s = __builtin_amdgcn_readfirstlane(s);
-  row0 = __builtin_amdgcn_readfirstlane(row0);
-  const PaSeq q = pa_seq(a, s);
+  const PgTile pl = pg_tile(a.c.starts, a.c.lens, a.c.seqs, a.c.rows, a.G, a.few, BR, tile);
+  if (pl.seq < 0) return;
+  const int s = __builtin_amdgcn_readfirstlane(pl.seq), row0 = __builtin_amdgcn_readfirstlane(pl.row0);
+  const PaSeq q = pa_seq(a, pl.r, pl.len);
   const int nrow = min(BR, q.rows - row0);
   int lo, hi;
   pa_span(q, row0, nrow, a.window, lo, hi);
