@@ -283,7 +283,10 @@ EVICT = [dict(lens=[5], keep=3), dict(lens=[5], keep=5, recent=2), dict(lens=[5,
          dict(lens=[300], keep=200, recent=200), dict(lens=[40, 60], keep=1, recent=0),
          dict(lens=[2500, 1100], keep=1024, recent=1), dict(lens=[90, 64], keep=64, recent=9, page=64, D=64, Hk=3),
          dict(lens=[200, 130], keep=77, recent=30, page=32, layout="slots"),
-         dict(lens=[200, 130], keep=77, recent=30, layout="wide", D=64)]
+         dict(lens=[200, 130], keep=77, recent=30, layout="wide", D=64),
+         # longer than a work-group holds at once
+         dict(lens=[9000, 12], keep=4000, recent=300, D=64, Hk=1, page=1024),
+         dict(lens=[17000, 30000], keep=5000, recent=100, D=64, Hk=1, page=1024)]
 
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "few", "odd"])
