@@ -145,6 +145,11 @@ def _weight(name, weight, S, cap, d):
     return weight if cap <= 1 or weight.stride(1) == 1 else weight.contiguous()
 
 
+def _window(window):
+    """As the C ABI's 32 bits hold it: 2^30 is past every table, -1 is refused there."""
+    return window if 0 <= window < 1 << 30 else -1 if window < 0 else 1 << 30
+
+
 def _angles(name, x, dim, d):
     _check(name, x, _F32, 2, d)
     n, m = x.shape
@@ -213,6 +218,7 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     (q, qp, qt, qh), N, H, D, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
     device = q.device
     out = _new((N, H, D), _BF16, device) if out is None else _out(out, q)
+    window = _window(window)
     L = _lib.lib()
     nws = L.ann_op_paged_attention_ws_bytes(c, H, window)
     lse = _new((N, H), _F32, device) if want_lse else None
@@ -245,7 +251,7 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
     L = _lib.lib()
     nws = L.ann_op_paged_weight_ws_bytes(c, H)
     ws = _empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, window,
+    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, _window(window),
                    weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
                    ws.data_ptr() if nws else None, nws)
     if rc:
@@ -278,8 +284,8 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
         if out_table.shape[1] > 1 and out_table.stride(1) != 1:
             out_table = out_table.contiguous()
     keep, recent = int(keep), int(recent)
-    if keep < 1:
-        raise ValueError(f"keep={keep} must be at least 1")
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"keep={keep} must be at least 1 and recent={recent} lie in [0, keep]")
     if keep > out_table.shape[1] * page:
         raise ValueError(f"{out_table.shape[1]} pages of {page} do not hold keep={keep} entries")
     device = k_cache.device

@@ -508,6 +508,19 @@ def test_out_is_the_queries(new, lens):
     assert torch.equal(paged.append(x, k, k, ang.cos(), ang.sin(), kc, vc, table, starts, ends, out=x), want)
 
 
+def test_windows_past_the_table():
+    """A window of more entries than there are is none, in 32 bits and past them."""
+    from attention_nn_amd import paged
+    s = Setup([1, 30], [200, 90], H=2, Hk=1, D=64, garbage=False)
+    kc, vc, table, starts, lens = s.dev()
+    q, w = s.q.cuda(), torch.zeros((2, s.cols * 16), device="cuda")
+    want, lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, want_lse=True)
+    seen = paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1)
+    for window in (200, 1 << 30, (1 << 31) - 1, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(paged.attention(q, kc, vc, table, starts, lens, 0.1, window), want)
+        assert torch.equal(paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1, window), seen)
+
+
 def test_shared_pages():
     """A prefix that two sequences share, read by both; evicted to pages of their own."""
     from attention_nn_amd import paged
@@ -577,6 +590,7 @@ def test_refusals():
     bad(ValueError, at, q, kc, vc, table, starts, lens, 0.1, out=torch.empty_like(q)[:2])
     bad(ValueError, at, q, kc, vc, table.cpu(), starts, lens, 0.1)
     bad(ValueError, at, q, kc, vc, table, starts, lens, 3e38)
+    bad(ValueError, at, q, kc, vc, table, starts, lens, 0.1, -(1 << 32) + 5)
     two = torch.zeros((4, 4, 64), dtype=BF, device="cuda")
     bad(ValueError, at, two[1:], kc, vc, table, starts, lens, 0.1, out=two[:-1])
     we = paged.attention_weight
@@ -587,6 +601,7 @@ def test_refusals():
     ev = paged.evict
     bad(ValueError, ev, kc, vc, table, lens, w, 0)
     bad(ValueError, ev, kc, vc, table, lens, w, 8, 9)
+    bad(ValueError, ev, kc, vc, table, lens, w, 8, 1 << 32)
     bad(ValueError, ev, kc, vc, table, lens, w, 1000)
     bad(ValueError, ev, kc, vc, table, lens, w[:1], 8)
     ang = torch.zeros((40, 16), device="cuda")
