@@ -21,8 +21,8 @@ a length past the table ends at it; ``starts`` must not fall.  Rows from
 ``starts[-1]`` on belong to no sequence and are left as they were.
 
 The page size is a power of two from 16 to 1024, the head dimension 64 or 128.
-The cache may have any strides over page, head and slot (multiples of 8), and a
-head of it serves ``heads / kv_heads`` query heads behind one another.
+The cache may have any strides over page, head and slot (multiples of 8, slots at
+most 2^25 elements apart), and a head of it serves ``heads / kv_heads`` query heads behind one another.
 Tensors live on one GPU, which need not be the current device; the work goes to
 its current stream.
 
@@ -199,6 +199,8 @@ def _queries(q, k_cache, v_cache, table, starts, lens):
     d = _pool(k_cache)
     rows = _rows("q", q, d)
     N, H, D = rows[0].shape
+    if rows[2] > 1 << 25 or rows[3] * H > 1 << 28:   # a tile's offsets are 32 bits
+        rows = _rows("q", rows[0].clone(memory_format=torch.contiguous_format), d)
     c, sizes, table, keep = _cache(d, k_cache, v_cache, table, lens, starts, N)
     if D != sizes[4]:
         raise ValueError(f"q {tuple(q.shape)}: the cache's head dimension is {sizes[4]}")

@@ -508,6 +508,22 @@ def test_out_is_the_queries(new, lens):
     assert torch.equal(paged.append(x, k, k, ang.cos(), ang.sin(), kc, vc, table, starts, ends, out=x), want)
 
 
+@pytest.mark.parametrize("far", [(1 << 25) + 8, 0])
+def test_far_queries(far):
+    """Queries whose rows (or heads) lie further apart than a tile's offsets reach."""
+    from attention_nn_amd import paged
+    s = Setup([1, 2], [60, 20], H=4, Hk=2, D=64, garbage=False)
+    kc, vc, table, starts, lens = s.dev()
+    q, w = s.q.cuda(), torch.zeros((2, s.cols * 16), device="cuda")
+    buf = torch.empty(3 * (1 << 25) + 1024 if far else 3 * (1 << 26) + 1024, dtype=BF, device="cuda")
+    x = buf.as_strided((3, 4, 64), (far, 64, 1) if far else (64, (1 << 26) + 8, 1))
+    x.copy_(q)
+    want, lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, want_lse=True)
+    assert torch.equal(paged.attention(x, kc, vc, table, starts, lens, 0.1), want)
+    assert torch.equal(paged.attention_weight(x, lse, kc, table, starts, lens, w, 0.1),
+                       paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1))
+
+
 def test_windows_past_the_table():
     """A window of more entries than there are is none, in 32 bits and past them."""
     from attention_nn_amd import paged
