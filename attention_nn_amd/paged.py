@@ -36,7 +36,7 @@ from . import _lib
 from ._stream import on_device
 
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
-_Tensor, _empty, _empty_strided = torch.Tensor, torch.empty, torch.empty_strided
+_Tensor, _empty_strided = torch.Tensor, torch.empty_strided
 _paged, _qk_rows = _lib.AnnPaged.from_values, _lib.AnnQkRows.from_values
 
 
@@ -85,10 +85,10 @@ def _column(name, x, n, d):
 def _new(shape, dtype, device):
     """A contiguous tensor (by its strides: a quarter faster than torch.empty)."""
     if len(shape) == 3:
-        a, b, c = shape
-        return _empty_strided(shape, (b * c, c, 1), dtype=dtype, device=device)
-    a, b = shape
-    return _empty_strided(shape, (b, 1), dtype=dtype, device=device)
+        strides = (shape[1] * shape[2], shape[2], 1)
+    else:
+        strides = (shape[1], 1) if len(shape) == 2 else (1,)
+    return _empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def _out(out, like):
@@ -224,7 +224,7 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     L = _lib.lib()
     nws = L.ann_op_paged_attention_ws_bytes(c, H, window)
     lse = _new((N, H), _F32, device) if want_lse else None
-    ws = _empty(nws, dtype=torch.uint8, device=device) if nws else None
+    ws = _new((nws,), torch.uint8, device) if nws else None
     rc = on_device(d, L.ann_op_paged_attention, c, qp, qt, qh, H, scale, window,
                    out.data_ptr(), lse.data_ptr() if want_lse else None,
                    ws.data_ptr() if nws else None, nws)
@@ -252,7 +252,7 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
         raise ValueError("out: rows must be contiguous")
     L = _lib.lib()
     nws = L.ann_op_paged_weight_ws_bytes(c, H)
-    ws = _empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    ws = _new((nws,), torch.uint8, q.device) if nws else None
     rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, _window(window),
                    weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
                    ws.data_ptr() if nws else None, nws)
@@ -292,7 +292,7 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
         raise ValueError(f"{out_table.shape[1]} pages of {page} do not hold keep={keep} entries")
     device = k_cache.device
     index = _new((S, keep), _I32, device)
-    left = _empty(S, dtype=_I32, device=device)
+    left = _new((S,), _I32, device)
     out = _new((S, cap), _F32, device)
     rc = on_device(d, _lib.lib().ann_op_paged_evict, c, out_table.data_ptr(), out_table.stride(0),
                    out_table.shape[1], weight.data_ptr(), weight.stride(0), keep, recent,
