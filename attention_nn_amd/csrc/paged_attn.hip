@@ -304,19 +304,6 @@ __device__ __forceinline__ bf16x8_t pa_join(pa_v4i16 a, pa_v4i16 b) {
   return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// The 16 entries of a cache from entry k0 on (a multiple of 16): a uniform
-// address, to which a lane adds its row's and column's 32 bits.
-__device__ __forceinline__ const unsigned char* pa_group(const bf16_t* head, int id, long long page,
-                                                         long long slot, int k0, int sh) {
-  return (const unsigned char*)(head + id * page + pg_slot(k0, sh, slot));
-}
-
-// Page ids ahead of their use: lane i of a wave holds the id of its i-th group of
-// 16 entries.
-struct PaPages {
-  int now, next;
-};
-
 // ---- sequences of few rows ----------------------------------------------------------
 //
 // A work-group takes a part of a sequence's entries for one cache head, 16 rows at
@@ -327,9 +314,9 @@ struct PaPages {
 // weights enter as two bf16 halves (2^-17 of each).  Bound by memory on long caches
 // (one token on 16 x 8192 entries of 6 heads of 128 in 5 parts: 59 us and 5 to join
 // them, 290 MB, 4.5 TB/s of a copy's 5.2), by the wait for one read after another and
-// a chunk's some 370 instructions a wave on short ones (777 entries: 11.9 us; 13.0
-// with the page ids read only behind the length, divisions by the group and four
-// compares a mask).
+// a chunk's some 270 instructions a wave on short ones (777 entries: 11.5 us a call;
+// 13.0 with the page ids read only behind the length, divisions by the group, every
+// chunk's addresses formed from its page id and every chunk masked).
 template <int DH, int NW>
 constexpr size_t pa_few_lds() {
   // the rings; after them the waves' sums, their maxima and totals, rows to form again
@@ -376,6 +363,9 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     // the entries that this lane's row sees of its part, from the lane's first one on
     const int e = q.e0 + tok;
     const int jl = max(a0, e < a.window ? 0 : e - a.window + 1) - 4 * g4, jh = min(b0 - 1, e) - 4 * g4;
+    // and those that all rows see
+    const int el = q.e0 + q.by.div(row0), eh = q.e0 + q.by.div(row0 + nrow - 1);
+    const int seen0 = max(a0, eh < a.window ? 0 : eh - a.window + 1), seen1 = min(b0 - 1, el);
     const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
     bf16x8_t qf[NKS];
 #pragma unroll
@@ -386,39 +376,63 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     for (int i = 0; i < NDB; ++i) o[i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, msl = 0.f, lsum = 0.f;
 
-    // ids of chunks 32 b .. 32 b + 31 of this wave: lane i group i & 1 of chunk i >> 1
-    auto ids = [&](int b) {
+    // Of chunks 32 b .. 32 b + 31 of this wave lane i has group i & 1 of chunk i >> 1:
+    // its first entry (where all of it lies outside [a0, b0), the nearest group's), the
+    // page id, and the offsets in bytes within a head that come of them.  The next 32
+    // chunks' ids come ahead.
+    auto place = [&](int b) {
       const int key = kb0 + 32 * (wv + NW * (32 * b + (lane >> 1))) + 16 * (lane & 1);
-      const int col = min(max(key, a0), b0 - 1) >> a.c.sh;
+      return min(max(key, a0 & ~15), (b0 - 1) & ~15);
+    };
+    auto ids = [&](int b) {
+      const int col = place(b) >> a.c.sh;
       return pg_read((b0 - 1) >> a.c.sh < 64 ? __shfl(first, col, 64) : table[col], a.c.pages);
     };
-    PaPages pg = {nt ? ids(0) : 0, nt > 32 ? ids(1) : 0};
+    int klo = 0, khi = 0, vlo = 0, vhi = 0, next = nt ? ids(0) : 0;
+    auto turn = [&](int b) {
+      const int k0 = place(b);
+      const long long ko = (next * a.c.kp + pg_slot(k0, a.c.sh, a.c.ks)) * 2;
+      const long long vo = (next * a.c.vp + pg_slot(k0, a.c.sh, a.c.vs)) * 2;
+      klo = (int)ko;
+      khi = (int)(ko >> 32);
+      vlo = (int)vo;
+      vhi = (int)(vo >> 32);
+      if (32 * (b + 1) < nt) next = ids(b + 1);
+    };
+    const auto group = [&](const bf16_t* head, int lo, int hi, int i) {
+      const unsigned l = __builtin_amdgcn_readlane(lo, i);
+      return (const unsigned char*)head + (((long long)__builtin_amdgcn_readlane(hi, i) << 32) | l);
+    };
     bf16x8_t kf[2][2][NKS];
     auto issue = [&](int t, int slot) {
       asm volatile("" ::: "memory");   // behind the reads of the stage it fills
-      if (t && t % 32 == 0) {
-        pg.now = pg.next;
-        if (t + 32 < nt) pg.next = ids(t / 32 + 1);
-      }
-      const int kb = kb0 + 32 * (wv + NW * t);
+      if (t % 32 == 0) turn(t / 32);
+      const int kb = kb0 + 32 * (wv + NW * t), i = 2 * (t % 32);
       unsigned char* st = ring + (t & 1) * TB;
+      const bool edge = kb < a0 || kb + 32 > b0;   // rows outside take the nearest inside
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int id = __builtin_amdgcn_readlane(pg.now, 2 * (t % 32) + g);
-        // entries inside [a0, b0): where the whole group lies outside, the nearest one's page
-        const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
-        const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
-        const unsigned char* kp = pa_group(kh, id, a.c.kp, a.c.ks, k0, a.c.sh);
-        const unsigned char* vp = pa_group(vh, id, a.c.vp, a.c.vs, k0, a.c.sh);
-        const unsigned ko = (unsigned)(min(max(r16, rl), rh) * (int)a.c.ks * 2 + g4 * 16);
+        const unsigned char* kp = group(kh, klo, khi, i + g);
+        const unsigned char* vp = group(vh, vlo, vhi, i + g);
+        int kr = r16, vr[LPW / 2];
+#pragma unroll
+        for (int u = 0; u < LPW / 2; ++u) vr[u] = u * RPL + lane / (RB / 16);   // row of the group
+        if (edge) {
+          const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
+          const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
+          kr = min(max(kr, rl), rh);
+#pragma unroll
+          for (int u = 0; u < LPW / 2; ++u) vr[u] = min(max(vr[u], rl), rh);
+        }
+        const unsigned ko = (unsigned)(kr * (int)a.c.ks * 2 + g4 * 16);
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) kf[slot][g][ks] = *(const bf16x8_t*)(kp + ko + ks * 64);
 #pragma unroll
         for (int u = 0; u < LPW / 2; ++u) {
-          const int r = u * RPL + lane / (RB / 16);   // row of the group
+          const int r = u * RPL + lane / (RB / 16);
           const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
-          const unsigned vo = (unsigned)(min(max(r, rl), rh) * (int)a.c.vs * 2 + col);
-          __builtin_amdgcn_global_load_lds(vp + vo, (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
+          const unsigned char* src = vp + (unsigned)(vr[u] * (int)a.c.vs * 2 + col);
+          __builtin_amdgcn_global_load_lds(src, (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
         }
       }
     };
@@ -432,21 +446,25 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
         for (int ks = 0; ks < NKS; ++ks)
           sacc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[slot][g][ks], qf[ks], sacc[g], 0, 0, 0);
       }
-      float p[2][4], lm = -INFINITY;
+      if (kb < seen0 || kb + 31 > seen1)   // what is masked scores -inf
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = kb + 16 * g + r;
+            sacc[g][r] = j >= jl && j <= jh ? sacc[g][r] : -INFINITY;
+          }
+      float p[2][4], lm = sacc[0][0];
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {   // what is masked scores -inf
-          const int j = kb + 16 * g + r;
-          p[g][r] = j >= jl && j <= jh ? sacc[g][r] : -INFINITY;
-          lm = fmaxf(lm, p[g][r]);
-        }
+        for (int r = 0; r < 4; ++r) lm = fmaxf(lm, sacc[g][r]);
       if (__any(lm > m + a.thr)) pa_raise<NDB>(lm, a.sl2, m, msl, lsum, o);
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[g][r] = __builtin_amdgcn_exp2f(p[g][r] * a.sl2 - msl);
+          p[g][r] = __builtin_amdgcn_exp2f(sacc[g][r] * a.sl2 - msl);
           lsum += p[g][r];
         }
       uint32_t pw[4], pl[4];   // the weights in bf16, and what that leaves of them
