@@ -94,8 +94,9 @@ typedef __attribute__((address_space(3))) const unsigned char pa_lds_cchar;
 // 16-byte chunk c of LDS row r is stored at chunk c ^ kswz(r) of a key tile and c
 // ^ swz(r) of a value tile.  A fragment of keys is 16 rows of one chunk each,
 // which the hardware reads 16 lanes at a time from two neighbouring chunks; one of
-// values 8 rows of two chunks.  Measured, cycles for 1 KB of keys: 5 with kswz, 8
-// with swz, 32 unswizzled; for 512 bytes of values 4.25 and 16.
+// values 8 rows of two chunks.  Measured with one wave, cycles for 1 KB of keys: 5
+// with kswz, 8 with swz, 32 unswizzled; for 512 bytes of values 4.25 and 16 (with
+// all waves 4.4 and 2.6, as for reads in a row).
 template <int DH>
 __device__ __forceinline__ int pa_kswz(int r) {
   return DH == 128 ? r & 15 : r & 7;
@@ -569,16 +570,18 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
 // straight into LDS a step ahead, one barrier a step.  A key or value fragment
 // read from LDS serves QB products.  Bound by three units that a step needs for about
 // as long, in cycles for one wave on each SIMD: the matrix units 512, the vector units
-// some 600 (an exponential takes four instructions' time), LDS 560 (430 of reads).  A
-// model of the step without its LDS reads takes 196 ns a wave, with them 317, with
-// barrier and loads 358; here it is 440, and 650 where a CU has one work-group alone.
+// some 600 (an exponential takes four instructions' time), LDS 430 (300 of reads).  A
+// model of the step without its LDS reads takes 196 ns a wave at 2.4 GHz, with them
+// 317, with barrier and loads 358; here it is 440 at the 2.0 GHz that the card holds
+// under real data, and 650 where a CU has one work-group alone.
 // 2048 tokens of 12 heads of 128 on 16384 entries: 227 us, 193 GFLOP at 0.85 PFLOP/s
 // (a large product of the same card: 1.38), matrix units busy 40% of the time, no bank
 // conflicts; its 768 work-groups fill 512 places once and half again.  24 ragged
 // sequences on a window of 384, 50 MB and 4 GFLOP, take 20.2 us: a dozen steps behind
 // the search for the tile.  No faster: three steps ahead, higher priority of waves in
-// the products (230 and 233), sums and maxima beside the products with P (228), parts
-// by thirds, fifths and sixths.
+// the products (230 and 233), sums and maxima beside the products with P (228), the
+// first key fragments read a step ahead (226, and 21.9 for the ragged ones), parts by
+// thirds, fifths and sixths.
 constexpr int PM_AHEAD = 1;   // steps that loads run ahead (odd: a step's parity is its stage's)
 template <int LPW>
 struct PaWalk {
