@@ -1178,35 +1178,36 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 // FEW: calls of sixteen rows a head or so (decoding), where the keys change from
 // head to head and the next head's are loaded ahead.  Otherwise the keys stay, and
 // the next sixteen rows are.  FEW is bound by memory (one token on 16 x 4096 entries of
-// 6 heads of 128: 17.7 us, 4.3 TB/s), the other by its vector instructions on
-// the CUs whose sequences have the most rows (864 tokens of 8 heads of 64, 462 of them
-// on one of four sequences of up to 4096 entries: 16.9 us; all CUs' vector units are
-// busy 55% of 13 us).  No faster: rows three tiles ahead (16.4, but 30 to 34 us for 29
-// at head dim 128), 16 or 64 entries a wave (16.9 and 21.6), four waves (22.7).
+// 6 heads of 128: 17.4 us, 4.4 TB/s), the other by its vector instructions on the
+// CUs whose sequences have the most rows (864 tokens of 8 heads of 64, 462 of them on
+// one of four sequences of up to 4096 entries: 16.6 us; all CUs' vector units are busy
+// 55% of 13 us).  No faster: rows three tiles ahead (16.4, but 30 to 34 us for 29 at
+// head dim 128), 16 or 64 entries a wave (16.9 and 21.6), four or sixteen waves (22.7
+// and 18.7), page ids ahead of the length (16.6).
 template <int DH, bool FEW>
 struct PwShape {
   static constexpr int NW = FEW ? 4 : 8, NB = 2, E = 16 * NB;
 };
 template <int DH, bool FEW>
 __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
-    PagedArgs c, const bf16_t* __restrict__ q, long long qt, long long qh, int heads, FastDiv group,
+    PagedArgs c, const bf16_t* __restrict__ q, long long qt, long long qh, int heads, int G, FastDiv group,
     const float* __restrict__ lse, float sl2, int window, const float* w, long long wrow, float* out,
-    long long orow, int cap, int share) {
+    long long orow, int cap, int share2, int tg2) {   // log2 of share, and of whole tokens a tile (or -1)
   constexpr int NW = PwShape<DH, FEW>::NW, NB = PwShape<DH, FEW>::NB, E = PwShape<DH, FEW>::E;
   constexpr int NKS = DH / 32;
   __shared__ float part[NW][E];
   extern __shared__ __attribute__((aligned(16))) unsigned char pw_smem[];   // NW * 2 * 16 rows
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int blocks = NW / share, s = blockIdx.y;
-  const int j0 = (blockIdx.x * blocks + wv / share) * E;
+  const int share = 1 << share2, blocks = NW >> share2, s = blockIdx.y;
+  const int j0 = (blockIdx.x * blocks + (wv >> share2)) * E;
   // the entry whose sum this thread writes
   const int j = blockIdx.x * blocks * E + tid;
   const bool mine = tid < blocks * E && j < cap;
   const float was = mine ? w[s * wrow + j] : 0.f;
   const int len = pg_len(c.lens[s], c.cols, c.sh);
   const PgRange r = pg_range(c.starts[s], c.starts[s + 1], c.rows);
-  const int G = heads / c.heads, e0 = len - r.n, jl = min(j0 + E - 1, len - 1);
+  const int e0 = len - r.n, jl = min(j0 + E - 1, len - 1);
   // tokens t0 .. t1 - 1 see one of the entries j0 .. jl
   const int t0 = max(0, j0 - e0), t1 = jl - e0 < r.n - window ? jl - e0 + window : r.n;
   float acc[NB][4];
@@ -1216,7 +1217,7 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
   if (j0 < len && t1 > t0) {
     const int hi = (t1 - t0) * G;   // rows, from token t0 on
-    const int tiles = (hi + 15) / 16, all = tiles * c.heads, per = (all + share - 1) / share;
+    const int tiles = (hi + 15) / 16, all = tiles * c.heads, per = (all + share - 1) >> share2;
     const bf16_t* kr[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -1226,9 +1227,6 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
     }
     const bf16_t* q0 = q + (r.first + t0) * qt;
     const float* l0 = lse + (long long)(r.first + t0) * heads;
-    // tiles of whole tokens: a lane's token and head of each are the same
-    const bool whole = 16 % G == 0;
-    const int tg = 16 / G;
     struct Rows {
       bf16x8_t q[NKS];
       float l2;
@@ -1270,7 +1268,7 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
           acc[b][k] += full || (y <= x.e && y >= yl) ? p : 0.f;
         }
     };
-    int u = wv % share * per;
+    int u = (wv & (share - 1)) * per;
     const int end = min(u + per, all);
     bool done = false;
     if constexpr (FEW) {
@@ -1301,9 +1299,9 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
     constexpr int RB = DH * 2, LPT = 16 * RB / 1024, RPL = 1024 / RB;
     unsigned char* ring = pw_smem + wv * 2 * 16 * RB;
     int f0 = 0, f1 = 0;
-    if (whole) {
-      f0 = max(0, (j0 + E - 1 - e0 - t0 + tg - 1) / tg);
-      f1 = min(hi / 16, window == 0x7fffffff ? 0x7fffffff : (window + j0 - e0 - t0) / tg);
+    if (tg2 >= 0) {
+      f0 = max(0, (j0 + E - 1 - e0 - t0 + (1 << tg2) - 1) >> tg2);
+      f1 = min(hi / 16, window == 0x7fffffff ? 0x7fffffff : (window + j0 - e0 - t0) >> tg2);
     }
     unsigned qoff[LPT];
     int qrow[LPT], qcol[LPT];   // load u: this lane's row of the tile and column in bytes
@@ -1315,7 +1313,7 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
       qoff[k] = (unsigned)(t * (int)qt + (qrow[k] - t * G) * (int)qh) * 2 + qcol[k];
     }
     auto issue = [&](int kvh, int tile, int stage, bool in) __attribute__((always_inline)) {
-      const int tb = in ? tile * tg : group.div(tile * 16);
+      const int tb = in ? tile << tg2 : group.div(tile * 16);
       const unsigned char* qb = (const unsigned char*)(q0 + (long long)kvh * G * qh + tb * qt);
 #pragma unroll
       for (int k = 0; k < LPT; ++k) {
@@ -1424,9 +1422,10 @@ static hipError_t pw_launch(const PagedArgs& c, const bf16_t* q, long long qt, l
   // for each CU: 864 tokens of 8 heads of 64 on 4 x 4096 entries 48.0 / 27.0 / 17.8
   // us with 2 / 4 / 8, one token each on 16 x 4096 (6 x 128) 17.9 / 19.8 / 20.8 with
   // 1 / 2 / 4
-  int share = 1;
-  while (share < S::NW && blocks * share * 2 <= (FEW ? 8LL : 16LL) * cus) share *= 2;
-  const int per = S::NW / share * S::E;
+  int share2 = 0;
+  while (1 << share2 < S::NW && blocks << (share2 + 1) <= (FEW ? 8LL : 16LL) * cus) ++share2;
+  const int per = (S::NW >> share2) * S::E;
+  const int G = heads / c.heads, tg2 = 16 % G ? -1 : __builtin_ctz(16 / G);
   const dim3 grid((unsigned)((cap + per - 1) / per), (unsigned)c.seqs);
   constexpr size_t lds = (size_t)S::NW * 2 * 16 * DH * 2;
   if (lds > 32 * 1024) {
@@ -1434,8 +1433,8 @@ static hipError_t pw_launch(const PagedArgs& c, const bf16_t* q, long long qt, l
     const hipError_t e = lds_limit(limit, (const void*)k_paged_weight<DH, FEW>, lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_paged_weight<DH, FEW>), grid, dim3(64 * S::NW), lds, st, c, q, qt, qh, heads,
-                     FastDiv::of(heads / c.heads), lse, sl2, window, w, wrow, out, orow, cap, share);
+  hipLaunchKernelGGL((k_paged_weight<DH, FEW>), grid, dim3(64 * S::NW), lds, st, c, q, qt, qh, heads, G,
+                     FastDiv::of(G), lse, sl2, window, w, wrow, out, orow, cap, share2, tg2);
   return hipGetLastError();
 }
 
