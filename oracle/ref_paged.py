@@ -72,6 +72,50 @@ def attention(q, kc, vc, table, starts, lens, scale, window):
     return out, lse, tol, ltol
 
 
+def attention_whole(q, kc, vc, table, starts, lens, scale, window):
+    """``attention`` a sequence and cache head at a time, for long ones.  Its bounds
+    take the weights in two bf16 halves (2^-16 of each, the second rounded to 2^-8
+    of at most 2^-8 of the first) where a sequence has up to 16 rows."""
+    N, H, D = q.shape
+    Hk, page, cap = kc.shape[1], kc.shape[2], table.shape[1] * kc.shape[2]
+    G = H // Hk
+    out = torch.full((N, H, D), math.nan, dtype=torch.float64)
+    lse = torch.full((N, H), math.nan, dtype=torch.float64)
+    tol, ltol = torch.zeros(N, H, D).double(), torch.zeros(N, H).double()
+    for s in range(len(lens)):
+        a, n = starts[s], starts[s + 1] - starts[s]
+        length = min(max(lens[s], 0), cap)
+        if not n:
+            continue
+        ids = table[s, :-(-length // page)].long()
+        ids = torch.where((ids >= 0) & (ids < kc.shape[0]), ids, 0)
+        k, v = (x[ids].transpose(1, 2).reshape(-1, Hk, D)[:length] for x in (kc, vc))
+        e = torch.arange(length - n, length)[:, None]
+        j = torch.arange(length)[None, :]
+        sees = (j <= e) & (e - j < window) if window else j <= e
+        some = sees.any(1)
+        rounding = 2.0 ** -16 if n * G <= 16 else 2.0 ** -8
+        for h in range(H):
+            kh, vh, qh = k[:, h // G].double(), v[:, h // G].double(), q[a:a + n, h].double()
+            x = torch.where(sees, scale * (qh @ kh.t()), -math.inf)
+            size = torch.where(sees, abs(scale) * (qh.abs() @ kh.abs().t()), 0.0)
+            lse[a:a + n, h] = torch.logsumexp(x, 1) if length else -math.inf
+            p = torch.where(some[:, None], torch.softmax(x, 1), 0.0)
+            o, mass = p @ vh, p @ vh.abs()
+            # NaN and infinities of entries that some rows see
+            for i in torch.nonzero(~torch.isfinite(o).all(1)).flatten().tolist():
+                o[i], mass[i] = p[i, sees[i]] @ vh[sees[i]], p[i, sees[i]] @ vh[sees[i]].abs()
+            out[a:a + n, h] = o
+            if not length:
+                continue
+            top = torch.where(sees, x.abs(), 0.0).amax(1)
+            d = (size.amax(1) * (D + 4) + top * 2 + 4) * 2.0 ** -24
+            sums = (sees.sum(1) + 16) * 2.0 ** -24
+            tol[a:a + n, h] = 2.0 ** -8 * o.abs() + (rounding + 2 * d + 2 * sums)[:, None] * mass + 1e-30
+            ltol[a:a + n, h] = d + sums + 2.0 ** -22 * (1 + lse[a:a + n, h].abs())
+    return out, lse, tol, ltol
+
+
 def weight(q, lse, kc, table, starts, lens, w, scale, window):
     """-> the new weights and the bounds of an fp32 result."""
     N, H, D = q.shape
@@ -93,6 +137,37 @@ def weight(q, lse, kc, table, starts, lens, w, scale, window):
             terms[s, lo:e + 1] += 1
             tol[s, lo:e + 1] += p * (size * (D + 4) + (x.abs() + lse[n, h].abs() + y.abs()) * 2 + 8) * 2.0 ** -24
     # the sum of the terms in fp32, in any order
+    return out, tol + out.abs() * (terms + 4) * 2.0 ** -24 + 1e-30
+
+
+def weight_whole(q, lse, kc, table, starts, lens, w, scale, window):
+    """``weight`` a sequence and cache head at a time, for long ones."""
+    H, D = q.shape[1:]
+    Hk, page, cap = kc.shape[1], kc.shape[2], w.shape[1]
+    out = w.double().clone()
+    tol, terms = torch.zeros_like(out), torch.zeros_like(out)
+    for s in range(len(lens)):
+        a, n = starts[s], starts[s + 1] - starts[s]
+        length = min(max(lens[s], 0), cap)
+        if not n or not length:
+            continue
+        ids = table[s, :-(-length // page)].long()
+        ids = torch.where((ids >= 0) & (ids < kc.shape[0]), ids, 0)
+        k = kc[ids].transpose(1, 2).reshape(-1, Hk, D)[:length]
+        e = torch.arange(length - n, length)[:, None]
+        j = torch.arange(length)[None, :]
+        sees = (j <= e) & (e - j < window) if window else j <= e
+        for h in range(H):
+            kh, qh = k[:, h * Hk // H].double(), q[a:a + n, h].double()
+            l = lse[a:a + n, h].double()[:, None]
+            x = scale * (qh @ kh.t())
+            size = abs(scale) * (qh.abs() @ kh.abs().t())
+            y = x - l
+            p = torch.where(sees, torch.exp(y), 0.0)
+            d = torch.where(sees, size * (D + 4) + (x.abs() + l.abs() + y.abs()) * 2 + 8, 0.0)
+            out[s, :length] += p.sum(0)
+            terms[s, :length] += sees.sum(0)
+            tol[s, :length] += torch.where(sees, p * d, 0.0).sum(0) * 2.0 ** -24
     return out, tol + out.abs() * (terms + 4) * 2.0 ** -24 + 1e-30
 
 
