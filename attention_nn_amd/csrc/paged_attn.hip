@@ -524,32 +524,35 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
     }
     if (tid < 16) s_bad[tid] = 0;
     __syncthreads();
-    auto joined = [&](int r, int d, float& M, float& L) {
-      M = s_m[r];
+    // a thread's four dims of up to NI rows; one row alone may see an infinity too,
+    // which the halves of its weight, or the zeros behind a chunk's end, make a NaN
+    constexpr int NI = (16 * (DH / 4) + 64 * NW - 1) / (64 * NW);
+    floatx4_t v[NI];
+    float M[NI], L[NI];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w * 16 + r]);
-      L = 0.f;
-      floatx4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < NI; ++k) {
+      const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
+      if (r >= nrow) break;
+      M[k] = s_m[r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M[k] = fmaxf(M[k], s_m[w * 16 + r]);
+      L[k] = 0.f;
+      v[k] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w * 16 + r] - M);
-        L += s_l[w * 16 + r] * f;
-        v += *(const floatx4_t*)(sums + (w * 16 + r) * PW + d) * f;
+        const float f = M[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w * 16 + r] - M[k]);
+        L[k] += s_l[w * 16 + r] * f;
+        v[k] += *(const floatx4_t*)(sums + (w * 16 + r) * PW + d) * f;
       }
-      return v;
-    };
-    float M, L;
-    if (nrow > 1) {   // one row alone sees all that its part reads
-      for (int i = tid; i < nrow * (DH / 4); i += 64 * NW)
-        if (!pa_finite(joined(i / (DH / 4), i % (DH / 4) * 4, M, L))) s_bad[i / (DH / 4)] = 1;
-      __syncthreads();
+      if (!pa_finite(v[k])) s_bad[r] = 1;
     }
-    for (int i = tid; i < nrow * (DH / 4); i += 64 * NW) {
-      const int r = i / (DH / 4), d = i % (DH / 4) * 4, rr = row0 + r;
-      if (s_bad[r]) continue;
-      const floatx4_t v = joined(r, d, M, L);
-      pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, rr, part), pt.n, d,
-                          make_float4(v[0], v[1], v[2], v[3]), M, L);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
+      if (r >= nrow || s_bad[r]) continue;
+      pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, row0 + r, part), pt.n, d,
+                          make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), M[k], L[k]);
     }
     for (int r = wv; r < nrow; r += NW)
       if (s_bad[r]) pa_again<DH, true>(a, q, s, table, kvh, row0 + r, a0, b0, part, pt.n);

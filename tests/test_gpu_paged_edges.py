@@ -1,0 +1,38 @@
+"""The paged cache's operators where values leave the ordinary: infinities that a
+token sees, alone in its sequence or beside others."""
+
+import math
+
+import pytest
+import torch
+
+import oracle.ref_paged as R
+from tests.test_gpu_paged import Setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("H,Hk,D", [(2, 2, 128), (2, 1, 64)])
+@pytest.mark.parametrize("new,length", [(1, 1), (1, 5), (1, 33), (1, 777), (1, 3000), (2, 40), (2, 3000), (40, 100),
+                                        (40, 3000)])
+def test_infinities_that_a_token_sees(new, length, H, Hk, D):
+    """An infinite value makes its dimension infinite for the tokens that see it, two
+    of unlike sign or a NaN make it NaN, as the sum of the products does; the other
+    dimensions are as they were."""
+    from attention_nn_amd import paged
+    s = Setup([new], [length], H=H, Hk=Hk, D=D, garbage=False)
+    first, last = max(0, length - new - 2), length - 1
+    for e, dim, value in ((first, 3, math.inf), (last, 60, -math.inf), (first, 17, math.inf), (last, 17, -math.inf),
+                          (first, 33, math.nan)):
+        s.v[int(s.table[0, e // 16]), :, e % 16, dim] = value
+    if first == last:
+        s.v[int(s.table[0, 0]), :, last % 16, 17] = math.nan
+    kc, vc, table, starts, lens = s.dev()
+    ref, rlse, tol, ltol = R.attention_whole(s.q, s.k, s.v, s.table, s.starts, s.lens, 0.1, 0)
+    got, lse = paged.attention(s.q.cuda(), kc, vc, table, starts, lens, 0.1, want_lse=True)
+    got = got.cpu().double()
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    assert torch.equal(got[got.abs() == math.inf], ref[ref.abs() == math.inf])
+    assert ((got - ref).abs()[fine] <= tol[fine]).all()
+    assert ((lse.cpu().double() - rlse).abs() <= ltol).all()
