@@ -39,11 +39,11 @@ __device__ __forceinline__ QkRow<T> qk_row(const QkRows& a, int b, int t, int h)
 }
 
 // The table row of token (b, t); a position the table does not have takes the
-// nearest it has.
+// nearest it has.  64 bits: a start may be any of 32, and t goes on from there.
 __device__ __forceinline__ int qk_position(const QkRows& a, int b, int t) {
-  int p = a.pos0 + t;
-  if (a.pos) p = a.pos_each ? a.pos[(long long)b * a.T + t] : a.pos[b] + t;
-  return min(max(p, 0), a.table_rows - 1);
+  long long p = (long long)a.pos0 + t;
+  if (a.pos) p = a.pos_each ? a.pos[(long long)b * a.T + t] : (long long)a.pos[b] + t;
+  return (int)min(max(p, 0LL), a.table_rows - 1LL);
 }
 
 // One wave for each row, any D that is a multiple of 4 and any alignment.
