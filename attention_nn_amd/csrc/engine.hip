@@ -21,6 +21,7 @@
 #include <vector>
 #include "attnnn.h"
 #include "launch.h"
+#include "overlap.h"
 
 using namespace ann;
 
@@ -1228,17 +1229,12 @@ int paged_query(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head
 
 // Whether the contiguous rows of out (rows, heads, dim; bf16) share memory with
 // rows x of x_heads heads by strides; not (same_too) where they are the same rows.
-// An x with gaps that out would fit into may lie around it.
 bool paged_overlap(const void* out, int heads, const void* x, int64_t row, int64_t head, int x_heads,
                    int rows, int dim, bool same_too) {
-  const int64_t n = (int64_t)rows * heads * dim;
-  const int64_t span = (rows - 1LL) * row + (x_heads - 1LL) * head + dim;
-  const uintptr_t o = (uintptr_t)out, p = (uintptr_t)x;
-  if (rows < 1 || o >= p + (uintptr_t)span * 2 || p >= o + (uintptr_t)n * 2) return false;
-  if (same_too && o == p && (rows == 1 || row == (int64_t)heads * dim) &&
-      (heads == 1 || head == dim))
+  if (same_too && out == x && (rows == 1 || row == (int64_t)heads * dim) && (heads == 1 || head == dim))
     return false;
-  return row < n + (int64_t)x_heads * dim && head < n + dim;
+  return overlap({x, rows, row * 2, x_heads, head * 2, dim * 2LL},
+                 {out, 1, 0, 1, 0, (int64_t)rows * heads * dim * 2});
 }
 
 int paged_ws(const void* ws, size_t have, size_t need) {

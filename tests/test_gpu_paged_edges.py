@@ -36,3 +36,22 @@ def test_infinities_that_a_token_sees(new, length, H, Hk, D):
     assert torch.equal(got[got.abs() == math.inf], ref[ref.abs() == math.inf])
     assert ((got - ref).abs()[fine] <= tol[fine]).all()
     assert ((lse.cpu().double() - rlse).abs() <= ltol).all()
+
+
+def test_a_result_in_the_queries_gaps():
+    """Rows of queries far enough apart hold the result between them; on one of them
+    it is refused."""
+    from attention_nn_amd import paged
+    s = Setup([2, 1], [20, 30], H=4, Hk=2, D=64, garbage=False)
+    kc, vc, table, starts, lens = s.dev()
+    want = paged.attention(s.q.cuda(), kc, vc, table, starts, lens, 0.1)
+    buf = torch.zeros(3 * 2048, dtype=torch.bfloat16, device="cuda")
+    q = buf.as_strided((3, 4, 64), (2048, 64, 1))
+    q.copy_(s.q)
+    at = lambda i: buf[i:i + 3 * 4 * 64].view(3, 4, 64)
+    for i in (2048 + 256, 4096 - 768, 5120):
+        assert torch.equal(paged.attention(q, kc, vc, table, starts, lens, 0.1, out=at(i)), want)
+        assert torch.equal(q.cpu(), s.q)
+    for i in (0, 2048, 2048 + 248, 4096 - 760):
+        with pytest.raises(ValueError, match="overlaps"):
+            paged.attention(q, kc, vc, table, starts, lens, 0.1, out=at(i))
