@@ -1237,6 +1237,14 @@ bool paged_overlap(const void* out, int heads, const void* x, int64_t row, int64
                  {out, 1, 0, 1, 0, (int64_t)rows * heads * dim * 2});
 }
 
+// Whether rows of fp32 weights may not be written by way of out: they share memory,
+// and are not the same rows.
+bool weights_overlap(const float* w, int64_t w_row, const float* out, int64_t out_row, int64_t seqs,
+                     int64_t cap) {
+  if (w == out && (w_row == out_row || seqs == 1)) return false;
+  return overlap({w, seqs, w_row * 4, 1, 0, cap * 4}, {out, seqs, out_row * 4, 1, 0, cap * 4});
+}
+
 int paged_ws(const void* ws, size_t have, size_t need) {
   if (have < need) return fail(ANN_E_CAPACITY, "workspace %zu < %zu bytes", have, need);
   if (need && (!ws || ((uintptr_t)ws & 15)))
@@ -1333,6 +1341,11 @@ int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_
     return fail(ANN_E_ARG, "rows of out overlap");
   if (weight == weight_out && w_row != out_row)
     return fail(ANN_E_ARG, "weight in place with another row stride");
+  const int64_t cap = (int64_t)c->cols * c->page_size;
+  if (weights_overlap(weight, w_row, weight_out, out_row, c->seqs, cap))
+    return fail(ANN_E_ARG, "out overlaps weight and is not the same rows");
+  if (overlap({weight_out, c->seqs, out_row * 4, 1, 0, cap * 4}, {lse, 1, 0, 1, 0, (int64_t)c->rows * heads * 4}))
+    return fail(ANN_E_ARG, "out overlaps lse");
   rc = paged_ws(ws, ws_bytes, paged_weight_ws_bytes(p, heads, c->head_dim));
   if (rc) return rc;
   HIPCHK(paged_weight(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, lse, scale, window,
@@ -1358,6 +1371,8 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
     return fail(ANN_E_ARG, "rows of weight_out overlap");
   if (c->cols && weight == weight_out && w_row != wo_row)
     return fail(ANN_E_ARG, "weight in place with another row stride");
+  if (c->cols && weights_overlap(weight, w_row, weight_out, wo_row, c->seqs, (int64_t)c->cols * c->page_size))
+    return fail(ANN_E_ARG, "weight_out overlaps weight and is not the same rows");
   HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,
                      index, new_lens, weight_out, wo_row, (hipStream_t)stream));
   return ANN_OK;

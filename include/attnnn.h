@@ -328,8 +328,9 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
  * entry j and over heads of exp(scale q.k_j - lse), lse as
  * ann_op_paged_attention gives it; entries behind the sequence keep their
  * weight.  weight and weight_out (seqs, cols * page_size) fp32, rows w_row and
- * out_row elements apart; they may be the same.  c->v is not read.  The sums'
- * order does not depend on what else runs: results are reproducible. */
+ * out_row elements apart; they may be the same, or share nothing.  c->v is not
+ * read.  The sums' order does not depend on what else runs: results are
+ * reproducible. */
 size_t ann_op_paged_weight_ws_bytes(const ann_paged* c, int32_t heads);
 int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
                         int32_t heads, const float* lse, float scale, int32_t window,

@@ -55,3 +55,26 @@ def test_a_result_in_the_queries_gaps():
     for i in (0, 2048, 2048 + 248, 4096 - 760):
         with pytest.raises(ValueError, match="overlaps"):
             paged.attention(q, kc, vc, table, starts, lens, 0.1, out=at(i))
+
+
+def test_weights_beside_the_new_ones():
+    """Old and new weights as column halves of one tensor, and a broadcast row of old
+    ones; what shares some of the rows is refused."""
+    from attention_nn_amd import paged
+    s = Setup([2, 1], [20, 30], H=4, Hk=2, D=64, garbage=False)
+    kc, vc, table, starts, lens = s.dev()
+    q, cap = s.q.cuda(), s.cols * 16
+    lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, want_lse=True)[1]
+    both = torch.rand((2, 2 * cap), device="cuda")
+    old, new = both[:, :cap], both[:, cap:]
+    was = old.clone()
+    want = paged.attention_weight(q, lse, kc, table, starts, lens, was, 0.1)
+    assert paged.attention_weight(q, lse, kc, table, starts, lens, old, 0.1, out=new) is new
+    assert torch.equal(new, want) and torch.equal(old, was)
+    one = was[:1].expand(2, -1)
+    assert torch.equal(paged.attention_weight(q, lse, kc, table, starts, lens, one, 0.1),
+                       paged.attention_weight(q, lse, kc, table, starts, lens, one.contiguous(), 0.1))
+    rows = torch.rand((3, cap), device="cuda")
+    for w, out in ((rows[:2], rows[1:]), (rows[1:], rows[:2]), (old, both[:, cap - 1:-1]), (one, was)):
+        with pytest.raises(ValueError, match="overlaps|in place"):
+            paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1, out=out)

@@ -76,3 +76,31 @@ def test_results_on_a_row_between_gaps_are_refused():
                 s[1], s[2] = row, 128
             assert L.ann_op_paged_append(c, r, None) == _lib.ANN_E_ARG
             assert "overlaps" in L.ann_last_error().decode()
+
+
+def test_weights_that_overlap_in_part_are_refused():
+    """New weights into memory that shares some rows with the old ones, or parts of
+    rows, and into the log sums."""
+    from attention_nn_amd import _lib
+    L = _lib.lib()
+    c = _lib.AnnPaged(k=FAKE, v=FAKE, k_page=6 * 16 * 128, k_head=16 * 128, k_slot=128, v_page=6 * 16 * 128,
+                      v_head=16 * 128, v_slot=128, table=FAKE, table_row=8, starts=FAKE, lens=FAKE, pages=64,
+                      page_size=16, heads=6, head_dim=128, seqs=4, cols=8, rows=4)
+
+    def weight(w, wrow, out, orow, lse=FAKE << 2):
+        return L.ann_op_paged_weight(c, FAKE, 768, 128, 6, lse, 0.1, 0, w, wrow, out, orow, None, 0, None)
+
+    def evict(w, wrow, out, orow):
+        return L.ann_op_paged_evict(c, FAKE, 8, 8, w, wrow, 100, 10, FAKE << 2, FAKE << 3, out, orow, None)
+
+    # rows of 128 weights: one row on, half a row, the last one, a row of a broadcast
+    # one, other strides that meet in row 2
+    for w, wrow, out, orow in ((FAKE, 128, FAKE + 512, 128), (FAKE, 128, FAKE - 256, 128), (FAKE, 256, FAKE + 508, 256),
+                               (FAKE, 128, FAKE + 3 * 512 + 508, 128), (FAKE, 0, FAKE - 1024, 128),
+                               (FAKE, 300, FAKE + 800, 128), (FAKE, 128, FAKE, 128 + 4)):
+        for call in (weight, evict):
+            assert call(w, wrow, out, orow) == _lib.ANN_E_ARG, (w, wrow, out, orow)
+            assert "weight" in L.ann_last_error().decode()
+    for lse in (FAKE, FAKE + 2048 - 4, FAKE - 92):
+        assert weight(FAKE << 3, 128, FAKE, 128, lse) == _lib.ANN_E_ARG
+        assert "lse" in L.ann_last_error().decode()
