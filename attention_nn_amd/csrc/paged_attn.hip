@@ -307,8 +307,8 @@ __device__ __forceinline__ bf16x8_t pa_join(pa_v4i16 a, pa_v4i16 b) {
 
 // ---- sequences of few rows ----------------------------------------------------------
 //
-// A work-group takes a part of a sequence's entries for one cache head, 16 rows at
-// a time (one row of a decoding sequence without shared heads).  Its NW waves
+// A work-group takes a part of a sequence's entries for one cache head and 16 rows
+// (one row of a decoding sequence without shared heads).  Its NW waves
 // take chunks of 32 entries in turn and meet only at the end: keys from memory
 // straight into the fragments of the product, a chunk ahead; values into the
 // wave's own ring of two LDS stages.  The products have time to spare here, and the
@@ -326,7 +326,7 @@ constexpr size_t pa_few_lds() {
   return ring > sums ? ring : sums;
 }
 template <int DH, int NW>
-__device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part,
+__device__ __forceinline__ void pa_few(const PaArgs& a, int s, int row0, int kvh, int part,
                                        unsigned char* smem) {
   constexpr int RB = DH * 2, TB = 32 * RB;      // bytes of an LDS row, of a chunk's values
   constexpr int LPW = TB / 1024, RPL = 1024 / RB;   // loads of a chunk's values, rows of each
@@ -341,7 +341,7 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
   // the first 64 page ids, on their way before the sequence's length is known
   const int first = a.c.cols ? table[min(lane, a.c.cols - 1)] : 0;
   const PaSeq q = pa_seq(a, s);
-  if (q.rows == 0 || q.rows > a.few) return;
+  if (row0 >= q.rows || q.rows > a.few) return;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
   const bf16_t* kh = a.c.k + kvh * a.c.kh;
@@ -349,221 +349,235 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int kvh, int part
   unsigned char* ring = smem + wv * 2 * TB;
   const int trow = 4 * g4 + (r16 >> 2), tcol = 4 * (r16 & 3), vx = pa_swz<DH>(trow);
 
-  for (int row0 = 0; row0 < q.rows; row0 += 16) {
-    const int nrow = min(16, q.rows - row0);
-    int lo, hi;
-    pa_span(q, row0, nrow, a.window, lo, hi);
-    const PaParts pt = pa_parts(lo, hi, a.sp_few);
-    if (part >= pt.n) continue;
-    const int a0 = max(pt.begin + part * pt.per, lo), b0 = min(pt.begin + (part + 1) * pt.per, hi);
-    const int kb0 = pt.begin + part * pt.per;
-    const int nch = b0 > a0 ? (b0 - kb0 + 31) / 32 : 0;
-    const int nt = nch > wv ? (nch - wv + NW - 1) / NW : 0;   // chunks of this wave
+  const int nrow = min(16, q.rows - row0);
+  int lo, hi;
+  pa_span(q, row0, nrow, a.window, lo, hi);
+  const PaParts pt = pa_parts(lo, hi, a.sp_few);
+  if (part >= pt.n) return;
+  const int a0 = max(pt.begin + part * pt.per, lo), b0 = min(pt.begin + (part + 1) * pt.per, hi);
+  const int kb0 = pt.begin + part * pt.per;
+  const int nch = b0 > a0 ? (b0 - kb0 + 31) / 32 : 0;
+  const int nt = nch > wv ? (nch - wv + NW - 1) / NW : 0;   // chunks of this wave
 
-    const int row = row0 + min(r16, nrow - 1), tok = q.by.div(row);
-    // the entries that this lane's row sees of its part, from the lane's first one on
-    const int e = q.e0 + tok;
-    const int jl = max(a0, e < a.window ? 0 : e - a.window + 1) - 4 * g4, jh = min(b0 - 1, e) - 4 * g4;
-    // and those that all rows see
-    const int el = q.e0 + q.by.div(row0), eh = q.e0 + q.by.div(row0 + nrow - 1);
-    const int seen0 = max(a0, eh < a.window ? 0 : eh - a.window + 1), seen1 = min(b0 - 1, el);
-    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
-    bf16x8_t qf[NKS];
+  const int row = row0 + min(r16, nrow - 1), tok = q.by.div(row);
+  // the entries that this lane's row sees of its part, from the lane's first one on
+  const int e = q.e0 + tok;
+  const int jl = max(a0, e < a.window ? 0 : e - a.window + 1) - 4 * g4, jh = min(b0 - 1, e) - 4 * g4;
+  // and those that all rows see
+  const int el = q.e0 + q.by.div(row0), eh = q.e0 + q.by.div(row0 + nrow - 1);
+  const int seen0 = max(a0, eh < a.window ? 0 : eh - a.window + 1), seen1 = min(b0 - 1, el);
+  const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
+  bf16x8_t qf[NKS];
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
+  for (int ks = 0; ks < NKS; ++ks) qf[ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
 
-    floatx4_t o[NDB];
+  floatx4_t o[NDB];
 #pragma unroll
-    for (int i = 0; i < NDB; ++i) o[i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, msl = 0.f, lsum = 0.f;
+  for (int i = 0; i < NDB; ++i) o[i] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, msl = 0.f, lsum = 0.f;
 
-    // Of chunks 32 b .. 32 b + 31 of this wave lane i has group i & 1 of chunk i >> 1:
-    // its first entry (where all of it lies outside [a0, b0), the nearest group's), the
-    // page id, and the offsets in bytes within a head that come of them.  The next 32
-    // chunks' ids come ahead.
-    auto place = [&](int b) {
-      const int key = kb0 + 32 * (wv + NW * (32 * b + (lane >> 1))) + 16 * (lane & 1);
-      return min(max(key, a0 & ~15), (b0 - 1) & ~15);
-    };
-    auto ids = [&](int b) {
-      const int col = place(b) >> a.c.sh;
-      return pg_read((b0 - 1) >> a.c.sh < 64 ? __shfl(first, col, 64) : table[col], a.c.pages);
-    };
-    int klo = 0, khi = 0, vlo = 0, vhi = 0, next = nt ? ids(0) : 0;
-    auto turn = [&](int b) {
-      const int k0 = place(b);
-      const long long ko = (next * a.c.kp + pg_slot(k0, a.c.sh, a.c.ks)) * 2;
-      const long long vo = (next * a.c.vp + pg_slot(k0, a.c.sh, a.c.vs)) * 2;
-      klo = (int)ko;
-      khi = (int)(ko >> 32);
-      vlo = (int)vo;
-      vhi = (int)(vo >> 32);
-      if (32 * (b + 1) < nt) next = ids(b + 1);
-    };
-    const auto group = [&](const bf16_t* head, int lo, int hi, int i) {
-      const unsigned l = __builtin_amdgcn_readlane(lo, i);
-      return (const unsigned char*)head + (((long long)__builtin_amdgcn_readlane(hi, i) << 32) | l);
-    };
-    bf16x8_t kf[2][2][NKS];
-    auto issue = [&](int t, int slot) {
-      asm volatile("" ::: "memory");   // behind the reads of the stage it fills
-      if (t % 32 == 0) turn(t / 32);
-      const int kb = kb0 + 32 * (wv + NW * t), i = 2 * (t % 32);
-      unsigned char* st = ring + (t & 1) * TB;
-      const bool edge = kb < a0 || kb + 32 > b0;   // rows outside take the nearest inside
+  // Of chunks 32 b .. 32 b + 31 of this wave lane i has group i & 1 of chunk i >> 1:
+  // its first entry (where all of it lies outside [a0, b0), the nearest group's), the
+  // page id, and the offsets in bytes within a head that come of them.  The next 32
+  // chunks' ids come ahead.
+  auto place = [&](int b) {
+    const int key = kb0 + 32 * (wv + NW * (32 * b + (lane >> 1))) + 16 * (lane & 1);
+    return min(max(key, a0 & ~15), (b0 - 1) & ~15);
+  };
+  auto ids = [&](int b) {
+    const int col = place(b) >> a.c.sh;
+    return pg_read((b0 - 1) >> a.c.sh < 64 ? __shfl(first, col, 64) : table[col], a.c.pages);
+  };
+  int klo = 0, khi = 0, vlo = 0, vhi = 0, next = nt ? ids(0) : 0;
+  auto turn = [&](int b) {
+    const int k0 = place(b);
+    const long long ko = (next * a.c.kp + pg_slot(k0, a.c.sh, a.c.ks)) * 2;
+    const long long vo = (next * a.c.vp + pg_slot(k0, a.c.sh, a.c.vs)) * 2;
+    klo = (int)ko;
+    khi = (int)(ko >> 32);
+    vlo = (int)vo;
+    vhi = (int)(vo >> 32);
+    if (32 * (b + 1) < nt) next = ids(b + 1);
+  };
+  const auto group = [&](const bf16_t* head, int lo, int hi, int i) {
+    const unsigned l = __builtin_amdgcn_readlane(lo, i);
+    return (const unsigned char*)head + (((long long)__builtin_amdgcn_readlane(hi, i) << 32) | l);
+  };
+  bf16x8_t kf[2][2][NKS];
+  auto issue = [&](int t, int slot) {
+    asm volatile("" ::: "memory");   // behind the reads of the stage it fills
+    if (t % 32 == 0) turn(t / 32);
+    const int kb = kb0 + 32 * (wv + NW * t), i = 2 * (t % 32);
+    unsigned char* st = ring + (t & 1) * TB;
+    const bool edge = kb < a0 || kb + 32 > b0;   // rows outside take the nearest inside
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const unsigned char* kp = group(kh, klo, khi, i + g);
-        const unsigned char* vp = group(vh, vlo, vhi, i + g);
-        int kr = r16, vr[LPW / 2];
+    for (int g = 0; g < 2; ++g) {
+      const unsigned char* kp = group(kh, klo, khi, i + g);
+      const unsigned char* vp = group(vh, vlo, vhi, i + g);
+      int kr = r16, vr[LPW / 2];
 #pragma unroll
-        for (int u = 0; u < LPW / 2; ++u) vr[u] = u * RPL + lane / (RB / 16);   // row of the group
-        if (edge) {
-          const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
-          const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
-          kr = min(max(kr, rl), rh);
+      for (int u = 0; u < LPW / 2; ++u) vr[u] = u * RPL + lane / (RB / 16);   // row of the group
+      if (edge) {
+        const int k0 = min(max(kb + 16 * g, a0 & ~15), (b0 - 1) & ~15);
+        const int rl = max(a0 - k0, 0), rh = min(b0 - 1 - k0, 15);
+        kr = min(max(kr, rl), rh);
 #pragma unroll
-          for (int u = 0; u < LPW / 2; ++u) vr[u] = min(max(vr[u], rl), rh);
-        }
-        const unsigned ko = (unsigned)(kr * (int)a.c.ks * 2 + g4 * 16);
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) kf[slot][g][ks] = *(const bf16x8_t*)(kp + ko + ks * 64);
-#pragma unroll
-        for (int u = 0; u < LPW / 2; ++u) {
-          const int r = u * RPL + lane / (RB / 16);
-          const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
-          const unsigned char* src = vp + (unsigned)(vr[u] * (int)a.c.vs * 2 + col);
-          __builtin_amdgcn_global_load_lds(src, (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
-        }
+        for (int u = 0; u < LPW / 2; ++u) vr[u] = min(max(vr[u], rl), rh);
       }
-    };
-    auto compute = [&](int t, int slot) {
-      const int kb = kb0 + 32 * (wv + NW * t);
-      floatx4_t sacc[2];
+      const unsigned ko = (unsigned)(kr * (int)a.c.ks * 2 + g4 * 16);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        sacc[g] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+      for (int ks = 0; ks < NKS; ++ks) kf[slot][g][ks] = *(const bf16x8_t*)(kp + ko + ks * 64);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-          sacc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[slot][g][ks], qf[ks], sacc[g], 0, 0, 0);
+      for (int u = 0; u < LPW / 2; ++u) {
+        const int r = u * RPL + lane / (RB / 16);
+        const int col = ((lane % (RB / 16)) ^ pa_swz<DH>(r)) * 16;
+        const unsigned char* src = vp + (unsigned)(vr[u] * (int)a.c.vs * 2 + col);
+        __builtin_amdgcn_global_load_lds(src, (pa_lds_void*)(st + (g * LPW / 2 + u) * 1024), 16, 0, 0);
       }
-      if (kb < seen0 || kb + 31 > seen1)   // what is masked scores -inf
+    }
+  };
+  auto compute = [&](int t, int slot) {
+    const int kb = kb0 + 32 * (wv + NW * t);
+    floatx4_t sacc[2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+    for (int g = 0; g < 2; ++g) {
+      sacc[g] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = kb + 16 * g + r;
-            sacc[g][r] = j >= jl && j <= jh ? sacc[g][r] : -INFINITY;
-          }
-      float p[2][4], lm = sacc[0][0];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lm = fmaxf(lm, sacc[g][r]);
-      if (__any(lm > m + a.thr)) pa_raise<NDB>(lm, a.sl2, m, msl, lsum, o);
+      for (int ks = 0; ks < NKS; ++ks)
+        sacc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[slot][g][ks], qf[ks], sacc[g], 0, 0, 0);
+    }
+    if (kb < seen0 || kb + 31 > seen1)   // what is masked scores -inf
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[g][r] = __builtin_amdgcn_exp2f(sacc[g][r] * a.sl2 - msl);
-          lsum += p[g][r];
+          const int j = kb + 16 * g + r;
+          sacc[g][r] = j >= jl && j <= jh ? sacc[g][r] : -INFINITY;
         }
-      uint32_t pw[4], pl[4];   // the weights in bf16, and what that leaves of them
+    float p[2][4], lm = sacc[0][0];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float u = p[x >> 1][(x & 1) * 2], v = p[x >> 1][(x & 1) * 2 + 1];
-        pw[x] = pack2(u, v);
-        pl[x] = pack2(u - lo_f(pw[x]), v - hi_f(pw[x]));
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lm = fmaxf(lm, sacc[g][r]);
+    if (__any(lm > m + a.thr)) pa_raise<NDB>(lm, a.sl2, m, msl, lsum, o);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[g][r] = __builtin_amdgcn_exp2f(sacc[g][r] * a.sl2 - msl);
+        lsum += p[g][r];
       }
-      const bf16x8_t pf = *(const bf16x8_t*)pw, pr = *(const bf16x8_t*)pl;
-      pa_lds_cchar* vst = (pa_lds_cchar*)(ring + (t & 1) * TB) + trow * RB + (tcol & 7) * 2;
-      pa_v4i16 v0[NDB], v1[NDB];
-      pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
-        constexpr int db = decltype(dc)::value;
-        pa_lds_cchar* src = vst + (((2 * db + (tcol >> 3)) ^ vx) << 4);
-        v0[db] = pa_rd_tr<0>(src);
-        v1[db] = pa_rd_tr<16 * RB>(src);
-      });
-      pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
-        constexpr int db = decltype(dc)::value;
-        pa_wait_lgkm2<2 * (NDB - 1 - db)>(v0[db], v1[db]);
-        const bf16x8_t vf = pa_join(v0[db], v1[db]);
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[db], 0, 0, 0);
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr, o[db], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    };
-    if (nt) issue(0, 0);
-    for (int t = 0; t < nt; t += 2) {
+    uint32_t pw[4], pl[4];   // the weights in bf16, and what that leaves of them
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (t + u < nt) {
-          if (t + u + 1 < nt) {
-            issue(t + u + 1, (u + 1) & 1);
-            pa_wait_vm<LPW + 2 * NKS>();   // all but the next chunk's
-          } else {
-            pa_wait_vm<0>();
-          }
-          compute(t + u, u);
+    for (int x = 0; x < 4; ++x) {
+      const float u = p[x >> 1][(x & 1) * 2], v = p[x >> 1][(x & 1) * 2 + 1];
+      pw[x] = pack2(u, v);
+      pl[x] = pack2(u - lo_f(pw[x]), v - hi_f(pw[x]));
+    }
+    const bf16x8_t pf = *(const bf16x8_t*)pw, pr = *(const bf16x8_t*)pl;
+    pa_lds_cchar* vst = (pa_lds_cchar*)(ring + (t & 1) * TB) + trow * RB + (tcol & 7) * 2;
+    pa_v4i16 v0[NDB], v1[NDB];
+    pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
+      constexpr int db = decltype(dc)::value;
+      pa_lds_cchar* src = vst + (((2 * db + (tcol >> 3)) ^ vx) << 4);
+      v0[db] = pa_rd_tr<0>(src);
+      v1[db] = pa_rd_tr<16 * RB>(src);
+    });
+    pa_static_for<0, NDB>([&](auto dc) __attribute__((always_inline)) {
+      constexpr int db = decltype(dc)::value;
+      pa_wait_lgkm2<2 * (NDB - 1 - db)>(v0[db], v1[db]);
+      const bf16x8_t vf = pa_join(v0[db], v1[db]);
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[db], 0, 0, 0);
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr, o[db], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  if (nt) issue(0, 0);
+  for (int t = 0; t < nt; t += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (t + u < nt) {
+        if (t + u + 1 < nt) {
+          issue(t + u + 1, (u + 1) & 1);
+          pa_wait_vm<LPW + 2 * NKS>();   // all but the next chunk's
+        } else {
+          pa_wait_vm<0>();
         }
+        compute(t + u, u);
       }
     }
-
-    // the four waves' sums, brought to their largest maximum, in wave order
-    lsum += __shfl_xor(lsum, 16, 64);
-    lsum += __shfl_xor(lsum, 32, 64);
-    __syncthreads();   // every wave is done with the ring
-    if (r16 < nrow) {
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        *(floatx4_t*)(sums + (wv * 16 + r16) * PW + db * 16 + g4 * 4) = o[db];
-      if (g4 == 0) {
-        s_m[wv * 16 + r16] = m == -INFINITY ? -INFINITY : m * a.sl2;
-        s_l[wv * 16 + r16] = lsum;
-      }
-    }
-    if (tid < 16) s_bad[tid] = 0;
-    __syncthreads();
-    // a thread's four dims of up to NI rows; one row alone may see an infinity too,
-    // which the halves of its weight, or the zeros behind a chunk's end, make a NaN
-    constexpr int NI = (16 * (DH / 4) + 64 * NW - 1) / (64 * NW);
-    floatx4_t v[NI];
-    float M[NI], L[NI];
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
-      if (r >= nrow) break;
-      M[k] = s_m[r];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) M[k] = fmaxf(M[k], s_m[w * 16 + r]);
-      L[k] = 0.f;
-      v[k] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float f = M[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w * 16 + r] - M[k]);
-        L[k] += s_l[w * 16 + r] * f;
-        v[k] += *(const floatx4_t*)(sums + (w * 16 + r) * PW + d) * f;
-      }
-      if (!pa_finite(v[k])) s_bad[r] = 1;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
-      if (r >= nrow || s_bad[r]) continue;
-      pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, row0 + r, part), pt.n, d,
-                          make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), M[k], L[k]);
-    }
-    for (int r = wv; r < nrow; r += NW)
-      if (s_bad[r]) pa_again<DH, true>(a, q, s, table, kvh, row0 + r, a0, b0, part, pt.n);
-    __syncthreads();   // the sums are read before the next rows' chunks arrive
   }
+
+  // the four waves' sums, brought to their largest maximum, in wave order
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  __syncthreads();   // every wave is done with the ring
+  if (r16 < nrow) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      *(floatx4_t*)(sums + (wv * 16 + r16) * PW + db * 16 + g4 * 4) = o[db];
+    if (g4 == 0) {
+      s_m[wv * 16 + r16] = m == -INFINITY ? -INFINITY : m * a.sl2;
+      s_l[wv * 16 + r16] = lsum;
+    }
+  }
+  if (tid < 16) s_bad[tid] = 0;
+  __syncthreads();
+  // a thread's four dims of up to NI rows; one row alone may see an infinity too,
+  // which the halves of its weight, or the zeros behind a chunk's end, make a NaN
+  constexpr int NI = (16 * (DH / 4) + 64 * NW - 1) / (64 * NW);
+  floatx4_t v[NI];
+  float M[NI], L[NI];
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
+    if (r >= nrow) break;
+    M[k] = s_m[r];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M[k] = fmaxf(M[k], s_m[w * 16 + r]);
+    L[k] = 0.f;
+    v[k] = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = M[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w * 16 + r] - M[k]);
+      L[k] += s_l[w * 16 + r] * f;
+      v[k] += *(const floatx4_t*)(sums + (w * 16 + r) * PW + d) * f;
+    }
+    if (!pa_finite(v[k])) s_bad[r] = 1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
+    if (r >= nrow || s_bad[r]) continue;
+    pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, row0 + r, part), pt.n, d,
+                        make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), M[k], L[k]);
+  }
+  for (int r = wv; r < nrow; r += NW)
+    if (s_bad[r]) pa_again<DH, true>(a, q, s, table, kvh, row0 + r, a0, b0, part, pt.n);
 }
 
+// Work-groups past the sequences' take the sixteens of rows behind a sequence's first:
+// in the order of all the call's rows (token, head of the group), number x the one
+// that begins among rows 16 x .. 16 x + 15, of which there is one at most, its
+// sequence having begun at least 16 rows before.  A call with as many sequences as
+// tokens may still bring most of them to one (a captured step of many slots): 512
+// tokens on 2000 entries beside 511 empty sequences 42 us (one work-group for all of a
+// sequence's rows: 619), where every sequence has one token nothing is lost.
 template <int DH, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a, int blocks) {
   extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
-  pa_few<DH, NW>(a, blockIdx.y, blockIdx.x % a.c.heads, blockIdx.x / a.c.heads, pa_smem);
+  const int i = blockIdx.z * gridDim.y + blockIdx.y;
+  if (i >= blocks) return;
+  int s = i, row0 = 0;
+  if (i >= a.c.seqs) {
+    const int at = 16 * (i - a.c.seqs + 1);
+    s = __builtin_amdgcn_readfirstlane(pg_sequence(a.c.starts, a.c.seqs, a.by.div(at)));
+    if (s < 0) return;
+    row0 = (at - pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows).first * a.G + 15) & ~15;
+    if (row0 == 0) return;
+  }
+  pa_few<DH, NW>(a, s, row0, blockIdx.x % a.c.heads, blockIdx.x / a.c.heads, pa_smem);
 }
 
 // ---- sequences of many rows -----------------------------------------------------------
@@ -900,7 +914,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_many(PaArgs a, int tiles, int 
     pa_many<DH, BK, QB>(a, tile, w % a.c.heads, w / a.c.heads, pa_smem);
   } else {
     const int w = L - blocks, i = w / a.c.heads;
-    pa_few<DH, 4>(a, i % a.c.seqs, w % a.c.heads, i / a.c.seqs, pa_smem);
+    pa_few<DH, 4>(a, i % a.c.seqs, 0, w % a.c.heads, i / a.c.seqs, pa_smem);
   }
 }
 
@@ -1094,8 +1108,12 @@ static hipError_t pa_launch_few(const PaArgs& a, hipStream_t st) {
     const hipError_t e = lds_limit(limit, (const void*)k_paged_few<DH, NW>, lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_paged_few<DH, NW>), dim3((unsigned)(a.c.heads * a.sp_few.most), (unsigned)a.c.seqs),
-                     dim3(64 * NW), lds, st, a);
+  // the first sixteen rows of each sequence, and what may be behind them
+  const long long blocks = a.c.seqs + ((long long)a.c.rows * a.G - 1) / 16;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  const unsigned z = (unsigned)((blocks + 65534) / 65535);
+  const dim3 grid((unsigned)(a.c.heads * a.sp_few.most), (unsigned)((blocks + z - 1) / z), z);
+  hipLaunchKernelGGL((k_paged_few<DH, NW>), grid, dim3(64 * NW), lds, st, a, (int)blocks);
   return hipGetLastError();
 }
 

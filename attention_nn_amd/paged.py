@@ -215,8 +215,8 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     (rows, heads) fp32, the log of each softmax sum.  A token that sees nothing
     gets 0 and -inf.  ``out`` may be ``q``.  Scores, softmax and sums are fp32; the
     weights enter the product with the values in two bf16 halves where a sequence
-    has up to 16 rows (tokens times shared heads), else in bf16, as in the
-    framework's other attention."""
+    has up to 16 rows (tokens times shared heads) or the call no more tokens than
+    sequences, else in bf16, as in the framework's other attention."""
     (q, qp, qt, qh), N, H, D, d, c, _, keep = _queries(q, k_cache, v_cache, table, starts, lens)
     device = q.device
     out = _new((N, H, D), _BF16, device) if out is None else _out(out, q)
