@@ -1019,7 +1019,17 @@ struct PaPlan {
   int qb, tiles, full; // its row blocks, its tiles at most and where one sequence has all rows
   PaSplit sp_few, sp_many;
   bool wide;           // pa_few by eight waves
+  bool packed;         // slots of pa_few: 16 a (sequence, cache head), else one a row
 };
+// Slots of the parts' sums of few rows.
+static size_t pa_slots_few(const PagedArgs& c, int heads, bool packed) {
+  return packed ? (size_t)c.seqs * c.heads * 16 : (size_t)c.rows * heads;
+}
+// Bytes that the parts of few rows, and those of many, may take: many times what fills
+// the card's places (512 of 128 rows of 128 dims: 34 MB), and less than the table's
+// width asks for where few of its sequences are long (1024 of up to 131072 entries, 8
+// heads, 1535 rows: 2.2 GB by 16 slots a sequence and a part for every 4096).
+constexpr size_t PA_WS_MAX = (size_t)1 << 28;
 static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   static const int cus = device_cus();
   PaPlan p{};
@@ -1044,6 +1054,10 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   p.sp_few.split = one || pairs >= cus ? 1 : clamp(2LL * cus / pairs, clamp((span(16) + 127) / 128, 64));
   p.sp_few.most = one ? 1 : clamp((span(16) + 4095) / 4096, 64);
   if (p.sp_few.most < p.sp_few.split) p.sp_few.most = p.sp_few.split;
+  p.packed = p.many && pairs * 16 < (long long)c.rows * heads;
+  const size_t part = (size_t)(Dh + 2) * sizeof(float);   // of a slot
+  p.sp_few.most = clamp((long long)(PA_WS_MAX / (pa_slots_few(c, heads, p.packed) * part)), p.sp_few.most);
+  if (p.sp_few.split > p.sp_few.most) p.sp_few.split = p.sp_few.most;
   p.wide = !p.many && p.sp_few.most == 1 && pairs <= cus;
   // Many rows: the tile and the number of parts that the figures below put
   // first.  A step of 32 entries takes a work-group of 64 rows 0.475 us, two on one
@@ -1062,7 +1076,8 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
       const int br = 64 * qb, step = Dh == 64 ? 64 : 32;
       const long long keys = span(br);
       const float tiles = (float)((rows + br - 1) / br) + 0.5f * (float)((c.seqs < c.rows ? c.seqs : c.rows) - 1);
-      for (int ns = 1; ns <= 64 && (ns == 1 || keys / ns >= 256); ns *= 2) {
+      for (int ns = 1; ns <= 64 && (ns == 1 || (keys / ns >= 256 && (size_t)c.rows * heads * ns * part <= PA_WS_MAX));
+           ns *= 2) {
         const int each = (int)ceilf(tiles * (float)(c.heads * ns) / (float)cus);   // of a CU's work-groups
         const float steps = (float)((keys + (long long)step * ns - 1) / ((long long)step * ns));
         float us = 4.f * (float)((each + 1) / 2) +   // to find the tile and its first entries
@@ -1081,15 +1096,14 @@ static PaPlan pa_plan(const PagedArgs& c, int heads, int Dh, int window) {
   }
   return p;
 }
-// Slots of the parts' sums, and the workspace they take: none where all rows come
-// in one part.
+// Slots times parts: none where all rows come in one part.
 struct PaSlots {
   size_t few, many;
 };
 static PaSlots pa_slots(const PagedArgs& c, int heads, const PaPlan& p) {
   PaSlots n = {0, 0};
   if (p.few && p.sp_few.most > 1)
-    n.few = (p.many ? (size_t)c.seqs * c.heads * 16 : (size_t)c.rows * heads) * p.sp_few.most;
+    n.few = pa_slots_few(c, heads, p.packed) * p.sp_few.most;
   if (p.many && p.sp_many.most > 1) n.many = (size_t)c.rows * heads * p.sp_many.most;
   return n;
 }
@@ -1175,7 +1189,7 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.sp_few = p.sp_few;
   a.sp_many = p.sp_many;
   a.few = p.few;
-  a.packed = p.many;
+  a.packed = p.packed;
   a.br = 64 * p.qb;
   const PaSlots n = pa_slots(c, heads, p);
   a.po_few = (float*)ws;
