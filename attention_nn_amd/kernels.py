@@ -145,6 +145,34 @@ def _qk_struct(q, k, cs, sn, pos, eps, gq=None, gk=None):
     return a, d, qo, ko, (rows, cs, sn, pos)
 
 
+def _qk_norm_rope(q, k, cs, sn, pos, eps):
+    a, d, qo, ko, keep = _qk_struct(q, k, cs, sn, pos, eps)
+    _lib.check(on_device(d, _lib.lib().ann_op_qk_norm_rope, a))
+    return qo, ko
+
+
+class _QkNormRope(torch.autograd.Function):
+    """``qk_norm_rope`` of rows that require a gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, cs, sn, pos, eps):
+        tensor = isinstance(pos, torch.Tensor)
+        ctx.save_for_backward(q, k, cs, sn, pos if tensor else None)
+        ctx.pos, ctx.eps = None if tensor else pos, eps
+        return _qk_norm_rope(q, k, cs, sn, pos, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        # captured, an accumulation into leaves that an eager graph holds too would
+        # end the process: by hand there is none
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("qk_norm_rope: in a captured backward pass call qk_norm_rope_bwd")
+        q, k, cs, sn, pos = ctx.saved_tensors
+        d = qk_norm_rope_bwd(gq, gk, q, k, cs, sn, ctx.pos if pos is None else pos, ctx.eps)
+        return (*(x if need else None for x, need in zip(d, ctx.needs_input_grad)), None, None, None, None)
+
+
 def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
     """Queries (B, T, Hq, D) and keys (B, T, Hk, D) as the attention takes them:
     each head's row over sqrt(mean(x^2) + eps), its first half rotated as
@@ -155,15 +183,18 @@ def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
     any strides over batch, token and head (of a fused projection, say).
     ``pos`` is the position of token 0, or an int32 GPU tensor: (B,) one start
     for each batch row, (B, T) one position for each token (a value outside the
-    tables takes their nearest row)."""
-    a, d, qo, ko, keep = _qk_struct(q, k, cs, sn, pos, eps)
-    _lib.check(on_device(d, _lib.lib().ann_op_qk_norm_rope, a))
-    return qo, ko
+    tables takes their nearest row).
+
+    Autograd passes through to ``q`` and ``k`` (once, by ``qk_norm_rope_bwd``; the
+    tables get no gradient), but not in a captured backward pass."""
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k)):
+        return _QkNormRope.apply(q, k, cs, sn, pos, eps)
+    return _qk_norm_rope(q, k, cs, sn, pos, eps)
 
 
 def qk_norm_rope_bwd(gq, gk, q, k, cs, sn, pos=0, eps=1e-6):
     """Gradients of ``qk_norm_rope``'s inputs from those of its outputs -> (dq, dk).
-    ``q`` and ``k`` are its inputs."""
+    ``q`` and ``k`` are its inputs.  Autograd does not see this call."""
     a, d, qo, ko, keep = _qk_struct(q, k, cs, sn, pos, eps, gq, gk)
     _lib.check(on_device(d, _lib.lib().ann_op_qk_norm_rope_bwd, a))
     return qo, ko

@@ -28,6 +28,8 @@ its current stream.
 
 A page that a call writes belongs to one sequence; pages that are only read may
 be shared by several (a common prefix).
+
+These calls serve: autograd does not see them, and their results require no gradient.
 """
 
 import torch
