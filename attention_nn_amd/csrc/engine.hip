@@ -1320,16 +1320,12 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
   return ANN_OK;
 }
 
-size_t ann_op_paged_weight_ws_bytes(const ann_paged* c, int32_t heads) {
-  PagedArgs p;
-  if (paged_args(c, false, true, &p) || heads < 1 || heads % c->heads) return 0;
-  return paged_weight_ws_bytes(p, heads, c->head_dim);
-}
+size_t ann_op_paged_weight_ws_bytes(const ann_paged*, int32_t) { return 0; }
 
 int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
                         int32_t heads, const float* lse, float scale, int32_t window,
                         const float* weight, int64_t w_row, float* weight_out, int64_t out_row,
-                        void* ws, size_t ws_bytes, void* stream) {
+                        void*, size_t, void* stream) {
   PagedArgs p;
   int rc = paged_args(c, false, true, &p);
   if (rc) return rc;
@@ -1346,10 +1342,8 @@ int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_
     return fail(ANN_E_ARG, "out overlaps weight and is not the same rows");
   if (overlap({weight_out, c->seqs, out_row * 4, 1, 0, cap * 4}, {lse, 1, 0, 1, 0, (int64_t)c->rows * heads * 4}))
     return fail(ANN_E_ARG, "out overlaps lse");
-  rc = paged_ws(ws, ws_bytes, paged_weight_ws_bytes(p, heads, c->head_dim));
-  if (rc) return rc;
   HIPCHK(paged_weight(p, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, lse, scale, window,
-                      weight, w_row, weight_out, out_row, ws, (hipStream_t)stream));
+                      weight, w_row, weight_out, out_row, (hipStream_t)stream));
   return ANN_OK;
 }
 

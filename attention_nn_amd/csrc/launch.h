@@ -424,10 +424,9 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
                            int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
                            void* ws, hipStream_t st);
 // out[s][j] = w[s][j] + the weight entry j receives (j < len), else w[s][j].
-size_t paged_weight_ws_bytes(const PagedArgs& c, int heads, int Dh);
 hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads,
                         int Dh, const float* lse, float scale, int window, const float* w,
-                        long long wrow, float* out, long long orow, void* ws, hipStream_t st);
+                        long long wrow, float* out, long long orow, hipStream_t st);
 hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, long long out_row,
                        int out_cols, const float* w, long long wrow, int keep, int recent,
                        int32_t* index, int32_t* new_lens, float* out, long long orow,

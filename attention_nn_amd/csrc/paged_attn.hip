@@ -1208,7 +1208,8 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 // the cache heads, an equal share each.  S = K Q^T, entries x rows, 16 x 16 a
 // product: a lane adds the weights of its row's column for its four entries of
 // each block, and only at the end are the 16 columns and the waves added, in a
-// fixed order, so a sum does not depend on what else is in the call.
+// fixed order: the same call gives the same bits.  (How many waves share entries goes
+// by the call's sequences, rows and table, so another call may add in another order.)
 //
 // FEW: calls of sixteen rows a head or so (decoding), where the keys change from
 // head to head and the next head's are loaded ahead.  Otherwise the keys stay, and
@@ -1444,8 +1445,6 @@ __global__ __launch_bounds__(FEW ? 256 : 512, FEW ? 3 : 4) void k_paged_weight(
   }
 }
 
-size_t paged_weight_ws_bytes(const PagedArgs&, int, int) { return 0; }
-
 template <int DH, bool FEW>
 static hipError_t pw_launch(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
                             int heads, const float* lse, float sl2, int window, const float* w,
@@ -1475,10 +1474,9 @@ static hipError_t pw_launch(const PagedArgs& c, const bf16_t* q, long long qt, l
 
 hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads,
                         int Dh, const float* lse, float scale, int window, const float* w,
-                        long long wrow, float* out, long long orow, void* ws, hipStream_t st) {
+                        long long wrow, float* out, long long orow, hipStream_t st) {
   const int cap = c.cols << c.sh;
   if (c.seqs == 0 || cap == 0) return hipSuccess;
-  (void)ws;
   const int win = pa_window(window);
   const bool few = (long long)c.rows * (heads / c.heads) <= 16LL * c.seqs;
 #define ANN_PW(D, F)                                                                             \

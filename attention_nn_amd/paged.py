@@ -252,12 +252,8 @@ def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window
         out = _new((S, cols * page), _F32, q.device)
     elif _weight("out", out, S, cols * page, d) is not out:
         raise ValueError("out: rows must be contiguous")
-    L = _lib.lib()
-    nws = L.ann_op_paged_weight_ws_bytes(c, H)
-    ws = _new((nws,), torch.uint8, q.device) if nws else None
-    rc = on_device(d, L.ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, _window(window),
-                   weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0),
-                   ws.data_ptr() if nws else None, nws)
+    rc = on_device(d, _lib.lib().ann_op_paged_weight, c, qp, qt, qh, H, lse.data_ptr(), scale, _window(window),
+                   weight.data_ptr(), weight.stride(0), out.data_ptr(), out.stride(0), None, 0)
     if rc:
         _lib.check(rc)
     return out

@@ -330,7 +330,8 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
  * weight.  weight and weight_out (seqs, cols * page_size) fp32, rows w_row and
  * out_row elements apart; they may be the same, or share nothing.  c->v is not
  * read.  The sums' order does not depend on what else runs: results are
- * reproducible. */
+ * reproducible.  No workspace is needed: ann_op_paged_weight_ws_bytes gives 0, and
+ * ws is not read. */
 size_t ann_op_paged_weight_ws_bytes(const ann_paged* c, int32_t heads);
 int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,
                         int32_t heads, const float* lse, float scale, int32_t window,
