@@ -1138,7 +1138,7 @@ static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
     constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>(), f = pa_few_lds<DH, 4>();
     const long long blocks = (long long)p.tiles * a.c.heads * a.sp_many.most;
     const long long more = p.few ? (long long)a.c.seqs * a.c.heads * a.sp_few.most : 0;
-    if (blocks + more > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (blocks + more >= 1LL << 24) return hipErrorInvalidConfiguration;   // 2^32 threads: a launch would be cut short
     const dim3 grid((unsigned)(blocks + more));
     const size_t lds = p.few && f > m ? f : m;
     if (p.qb == 2)

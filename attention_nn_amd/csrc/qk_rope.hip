@@ -48,8 +48,8 @@ __device__ __forceinline__ int qk_position(const QkRows& a, int b, int t) {
 
 // One wave for each row, any D that is a multiple of 4 and any alignment.
 template <typename T, bool BWD>
-__global__ __launch_bounds__(256) void k_qk_rope_any(QkRows a, long long n) {
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void k_qk_rope_any(QkRows a, long long first, long long n) {
+  const long long w = first + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (w >= n) return;
   const int lane = threadIdx.x & 63;
   const int H = a.Hq + a.Hk, D = a.D, d4 = D / 4;
@@ -141,10 +141,10 @@ struct QrWord<bf16_t> {
 };
 
 template <typename T, int D, bool BWD>
-__global__ __launch_bounds__(256) void k_qk_rope(QkRows a, int tokens) {
+__global__ __launch_bounds__(256) void k_qk_rope(QkRows a, int first, int tokens) {
   using V = QrWord<T>;
   constexpr int NV = V::NV, W = D / NV, HP = 64 / W, U = BWD ? 2 : 4;
-  const int tok = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tok = first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (tok >= tokens) return;
   const int lane = threadIdx.x & 63, l = lane % W;
   const int b = a.B == 1 ? 0 : tok / a.T, t = tok - b * a.T;
@@ -208,34 +208,42 @@ static bool qk_words(const QkRows& a, bool bwd, int size) {
          (((uintptr_t)a.qo | (uintptr_t)a.ko | (uintptr_t)a.cs | (uintptr_t)a.sn) & 15) == 0;
 }
 
+// Rows (a wave each, four a work-group) of one launch: a grid holds less than 2^32
+// threads, and one of more is cut short without an error.
+constexpr long long QK_ROWS = 1LL << 25;
+static unsigned qk_blocks(long long rows) { return (unsigned)(((rows < QK_ROWS ? rows : QK_ROWS) + 3) / 4); }
+
 hipError_t qk_norm_rope(const QkRows& a, bool bwd, int dtype, hipStream_t st) {
   const long long tokens = (long long)a.B * a.T, n = tokens * (a.Hq + a.Hk);
   if (n == 0) return hipSuccess;
-  if ((n + 3) / 4 > 0x7fffffffLL) return hipErrorInvalidValue;
   const dim3 block(256);
-  if (qk_words(a, bwd, dtype == 0 ? 4 : 2) && tokens < (1LL << 31)) {
-    const dim3 grid((unsigned)((tokens + 3) / 4));
-#define ANN_QK(TY, D)                                                                          \
-  if (bwd) hipLaunchKernelGGL((k_qk_rope<TY, D, true>), grid, block, 0, st, a, (int)tokens);  \
-  else hipLaunchKernelGGL((k_qk_rope<TY, D, false>), grid, block, 0, st, a, (int)tokens)
-    if (dtype == 0) {
-      if (a.D == 64) { ANN_QK(float, 64); } else { ANN_QK(float, 128); }
-    } else {
-      if (a.D == 64) { ANN_QK(bf16_t, 64); } else { ANN_QK(bf16_t, 128); }
-    }
+  if (qk_words(a, bwd, dtype == 0 ? 4 : 2) && tokens < (1LL << 31) - QK_ROWS) {
+    for (long long first = 0; first < tokens; first += QK_ROWS) {
+      const dim3 grid(qk_blocks(tokens - first));
+#define ANN_QK(TY, D)                                                                                        \
+  if (bwd) hipLaunchKernelGGL((k_qk_rope<TY, D, true>), grid, block, 0, st, a, (int)first, (int)tokens);   \
+  else hipLaunchKernelGGL((k_qk_rope<TY, D, false>), grid, block, 0, st, a, (int)first, (int)tokens)
+      if (dtype == 0) {
+        if (a.D == 64) { ANN_QK(float, 64); } else { ANN_QK(float, 128); }
+      } else {
+        if (a.D == 64) { ANN_QK(bf16_t, 64); } else { ANN_QK(bf16_t, 128); }
+      }
 #undef ANN_QK
+    }
     return hipGetLastError();
   }
-  const dim3 grid((unsigned)((n + 3) / 4));
-#define ANN_QK(TY)                                                                     \
-  if (bwd) hipLaunchKernelGGL((k_qk_rope_any<TY, true>), grid, block, 0, st, a, n);   \
-  else hipLaunchKernelGGL((k_qk_rope_any<TY, false>), grid, block, 0, st, a, n)
-  if (dtype == 0) {
-    ANN_QK(float);
-  } else {
-    ANN_QK(bf16_t);
-  }
+  for (long long first = 0; first < n; first += QK_ROWS) {
+    const dim3 grid(qk_blocks(n - first));
+#define ANN_QK(TY)                                                                            \
+  if (bwd) hipLaunchKernelGGL((k_qk_rope_any<TY, true>), grid, block, 0, st, a, first, n);   \
+  else hipLaunchKernelGGL((k_qk_rope_any<TY, false>), grid, block, 0, st, a, first, n)
+    if (dtype == 0) {
+      ANN_QK(float);
+    } else {
+      ANN_QK(bf16_t);
+    }
 #undef ANN_QK
+  }
   return hipGetLastError();
 }
 
@@ -253,9 +261,9 @@ hipError_t qk_norm_rope(const QkRows& a, bool bwd, int dtype, hipStream_t st) {
 template <int DH>
 __global__ __launch_bounds__(256) void k_paged_append(PagedArgs c, QkRows a,
                                                       const bf16_t* __restrict__ v, long long vt,
-                                                      long long vh) {
+                                                      long long vh, int first) {
   constexpr int W = DH / 8, HP = 64 / W, D4 = DH / 4;
-  const int n = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (n >= c.rows) return;
   const int lane = threadIdx.x & 63, l = lane % W;
   const int s = pg_sequence(c.starts, c.seqs, n);
@@ -319,13 +327,12 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedArgs c, QkRows a,
 hipError_t paged_append(const PagedArgs& c, const QkRows& a, const bf16_t* v, long long vt,
                         long long vh, hipStream_t st) {
   if (c.rows == 0 || c.seqs == 0) return hipSuccess;
-  const dim3 grid((unsigned)((c.rows + 3) / 4)), block(256);
-  if (a.D == 64)
-    hipLaunchKernelGGL(k_paged_append<64>, grid, block, 0, st, c, a, v, vt, vh);
-  else if (a.D == 128)
-    hipLaunchKernelGGL(k_paged_append<128>, grid, block, 0, st, c, a, v, vt, vh);
-  else
-    return hipErrorInvalidValue;
+  if (a.D != 64 && a.D != 128) return hipErrorInvalidValue;
+  for (long long first = 0; first < c.rows; first += QK_ROWS) {
+    const dim3 grid(qk_blocks(c.rows - first)), block(256);
+    if (a.D == 64) hipLaunchKernelGGL(k_paged_append<64>, grid, block, 0, st, c, a, v, vt, vh, (int)first);
+    else hipLaunchKernelGGL(k_paged_append<128>, grid, block, 0, st, c, a, v, vt, vh, (int)first);
+  }
   return hipGetLastError();
 }
 

@@ -78,3 +78,35 @@ def test_weights_beside_the_new_ones():
     for w, out in ((rows[:2], rows[1:]), (rows[1:], rows[:2]), (old, both[:, cap - 1:-1]), (one, was)):
         with pytest.raises(ValueError, match="overlaps|in place"):
             paged.attention_weight(q, lse, kc, table, starts, lens, w, 0.1, out=out)
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^26 and some tokens of one sequence, of which the last ones have entries: the
+    tokens around each 2^25th and the last ones are turned, stored and answered."""
+    from attention_nn_amd import kernels, paged
+    n, cap = (1 << 26) + 5, 48
+    if torch.cuda.mem_get_info()[0] < 4 * n * 128:
+        pytest.skip("not enough memory")
+    x = torch.zeros((n, 1, 64), dtype=torch.bfloat16, device="cuda")
+    at = [i for c in (4, 1 << 25, (1 << 26) - cap) for i in range(c - 4, c + 4)] + list(range(n - cap, n))
+    rows = torch.randn((len(at), 1, 64), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    x[at] = rows
+    a = torch.rand((1, 16), generator=torch.Generator().manual_seed(1)).cuda()
+    cs, sn = a.cos(), a.sin()
+    kc, vc = (torch.zeros((3, 1, 16, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table, starts, lens = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([[2, 0, 1]], [0, n], [n]))
+    q = paged.append(x, x, x, cs, sn, kc, vc, table, starts, lens)
+    want = kernels.qk_norm_rope(rows[None], rows[None], cs, sn, torch.zeros((1, len(at)), dtype=torch.int32, device="cuda"))
+    assert torch.equal(q[at], want[0][0])
+    k, v = (c[table[0].long()].transpose(1, 2).reshape(cap, 1, 64) for c in (kc, vc))
+    assert torch.equal(k, want[1][0, -cap:]) and torch.equal(v, rows[-cap:])
+    del x
+    y, lse = paged.attention(q, kc, vc, table, starts, lens, 0.1, want_lse=True, out=q.clone())
+    last = torch.tensor([0, cap], dtype=torch.int32, device="cuda")
+    few, flse = paged.attention(q[-cap:], kc, vc, table, last, last[1:], 0.1, want_lse=True)
+    assert torch.equal(lse[-cap:] > -math.inf, flse > -math.inf)
+    assert ((lse[-cap:] - flse).abs() <= 1e-5).all()
+    # either form rounds the weights to bf16 once, and the result
+    assert ((y[-cap:].float() - few.float()).abs() <= 2.0 ** -6 * v.float().abs().amax()).all()
+    none = [i for i in at if i < n - cap]
+    assert (y[none] == 0).all() and (lse[none] == -math.inf).all()

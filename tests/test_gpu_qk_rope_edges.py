@@ -85,3 +85,26 @@ def test_autograd_twice_or_captured_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="qk_norm_rope_bwd"):
         torch.autograd.grad(y, a, gq.detach())
+
+
+@pytest.mark.parametrize("D,dtype", [(4, torch.float32), (64, torch.bfloat16)])
+def test_more_rows_than_a_launch_takes(D, dtype):
+    """2^26 and some rows, of 256 threads for every four: the first and the last ones,
+    and those around each 2^25th."""
+    from attention_nn_amd import kernels as K
+    n = (1 << 26) + 5
+    if torch.cuda.mem_get_info()[0] < 4 * n * D * dtype.itemsize:
+        pytest.skip("not enough memory")
+    x = torch.zeros((n, 1, 1, D), dtype=dtype, device="cuda")
+    at = sorted({i for c in (4, 1 << 25, 1 << 26, n) for i in range(max(0, c - 4), min(n, c + 4))})
+    rows = torch.randn((len(at), 1, 1, D), generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    x[at] = rows
+    a = torch.rand((1, D // 4), generator=torch.Generator().manual_seed(1)).cuda()
+    cs, sn = a.cos(), a.sin()
+    y, _ = K.qk_norm_rope(x, x[:, :, :0], cs, sn)
+    want, _ = K.qk_norm_rope(rows, rows[:, :, :0], cs, sn)
+    assert torch.equal(y[at], want)
+    del y
+    y, _ = K.qk_norm_rope_bwd(x, x[:, :, :0], x, x[:, :, :0], cs, sn)
+    want, _ = K.qk_norm_rope_bwd(rows, rows[:, :, :0], rows, rows[:, :, :0], cs, sn)
+    assert torch.equal(y[at], want)

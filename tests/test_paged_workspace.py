@@ -37,3 +37,13 @@ def test_one_slot_a_row():
         assert n and n % (rows * 8 * slot) == 0 and n <= rows * 8 * slot * (64 + 64)
     assert _bytes(16, 8, 16, 6, 6, 128, 1024) == 16 * 6 * 5 * slot
     assert _bytes(1, 16, 2048, 12, 12, 128, 1024) == 2048 * 12 * 4 * slot
+
+
+def test_more_work_groups_than_a_launch_takes_are_refused():
+    """A mixed batch of 65,535 sequences of 512 cache heads would need 2^25 work-groups of
+    256 threads: refused, not cut short."""
+    c = _lib.AnnPaged(k=FAKE, v=FAKE, k_page=512 * 1024, k_head=1024, k_slot=64, v_page=512 * 1024, v_head=1024,
+                      v_slot=64, table=FAKE, table_row=1, starts=FAKE, lens=FAKE, pages=1 << 20, page_size=16,
+                      heads=512, head_dim=64, seqs=65535, cols=1, rows=65536)
+    rc = _lib.lib().ann_op_paged_attention(c, FAKE, 512 * 64, 64, 512, 0.1, 0, FAKE << 1, None, FAKE, 1 << 40, None)
+    assert rc not in (0, _lib.ANN_E_ARG) and "configuration" in _lib.lib().ann_last_error().decode()
