@@ -367,9 +367,10 @@ template <> struct RopePair<bf16_t> {
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_rope(const T* __restrict__ x, T* __restrict__ y,
                                               const float* __restrict__ cs,
-                                              const float* __restrict__ sn, long long nvec, int Tn,
-                                              int H, int D, int pos0, float sgn) {
-  const long long v = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                              const float* __restrict__ sn, long long first,
+                                              long long nvec, int Tn, int H, int D, int pos0,
+                                              float sgn) {
+  const long long v = first + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (v >= nvec) return;
   const int lane = threadIdx.x & 63, nrot = D / 4;
   const size_t tab = (size_t)((int)((v / H) % Tn) + pos0) * nrot;
@@ -569,6 +570,10 @@ static bool aligned16(const void* a, const void* b) {
   return (((uintptr_t)a | (uintptr_t)b) & 15) == 0;
 }
 
+// Work-groups of 256 threads in one launch: a grid of 2^32 threads or more is cut
+// short without an error.
+constexpr int GRID_256 = 1 << 23;
+
 hipError_t op_relu2(const void* x, void* y, size_t n, int dtype, hipStream_t st) {
   if (n == 0) return hipSuccess;
   const bool vec = aligned16(x, y);
@@ -588,7 +593,6 @@ hipError_t op_rope(const void* x, void* y, const float* cs, const float* sn, int
                    int D, int pos0, int inverse, int dtype, hipStream_t st) {
   const long long nvec = (long long)B * T * H;
   if (nvec == 0) return hipSuccess;
-  const dim3 grid((unsigned)((nvec + 3) / 4));
   const float sgn = inverse ? -1.f : 1.f;
   // whole 16-byte words where every word lies in one half of its vector
   const int nv = dtype == 0 ? 4 : 8;
@@ -607,15 +611,18 @@ hipError_t op_rope(const void* x, void* y, const float* cs, const float* sn, int
   // pairs as whole words when both buffers are aligned to a pair
   const uintptr_t pa = (dtype == 0 ? 8 : 4) - 1;
   const bool vec = (((uintptr_t)x | (uintptr_t)y) & pa) == 0;
-#define ANN_ROPE(TY, V)                                                                       \
-  hipLaunchKernelGGL((k_rope<TY, V>), grid, dim3(256), 0, st, (const TY*)x, (TY*)y, cs, sn, nvec, \
-                     T, H, D, pos0, sgn)
-  if (dtype == 0) {
-    if (vec) ANN_ROPE(float, true); else ANN_ROPE(float, false);
-  } else {
-    if (vec) ANN_ROPE(bf16_t, true); else ANN_ROPE(bf16_t, false);
-  }
+  for (long long first = 0; first < nvec; first += 4LL * GRID_256) {
+    const dim3 grid((unsigned)std::min<long long>((nvec - first + 3) / 4, GRID_256));
+#define ANN_ROPE(TY, V)                                                                            \
+  hipLaunchKernelGGL((k_rope<TY, V>), grid, dim3(256), 0, st, (const TY*)x, (TY*)y, cs, sn, first, \
+                     nvec, T, H, D, pos0, sgn)
+    if (dtype == 0) {
+      if (vec) ANN_ROPE(float, true); else ANN_ROPE(float, false);
+    } else {
+      if (vec) ANN_ROPE(bf16_t, true); else ANN_ROPE(bf16_t, false);
+    }
 #undef ANN_ROPE
+  }
   return hipGetLastError();
 }
 
@@ -623,7 +630,14 @@ hipError_t op_rms(const void* x, void* y, int rows, int dim, float eps, int dtyp
   if (rows == 0) return hipSuccess;
   const int nv = dtype == 0 ? 4 : 8;
   const int c = (dim + 64 * nv - 1) / (64 * nv);   // 16-byte words per lane
-  if (dim % nv == 0 && c <= 4 && aligned16(x, y)) {
+  const bool words = dim % nv == 0 && c <= 4 && aligned16(x, y);
+  const int most = words ? 4 * GRID_256 : GRID_256;   // rows of one launch
+  if (rows > most) {   // a multiple of nv of them, so the others are aligned as well
+    const size_t at = (size_t)most * dim * (16 / nv);
+    const hipError_t e = op_rms(x, y, most, dim, eps, dtype, st);
+    return e != hipSuccess ? e : op_rms((const char*)x + at, (char*)y + at, rows - most, dim, eps, dtype, st);
+  }
+  if (words) {
     const dim3 g((rows + 3) / 4);
 #define ANN_RMS_WAVE(TY, C)                                                                     \
   hipLaunchKernelGGL((k_rms_wave<TY, C>), g, dim3(256), 0, st, (const TY*)x, (TY*)y, rows, dim, eps)
