@@ -1237,6 +1237,18 @@ bool paged_overlap(const void* out, int heads, const void* x, int64_t row, int64
                  {out, 1, 0, 1, 0, (int64_t)rows * heads * dim * 2});
 }
 
+// A cache that a call writes has a place for every row: no broadcast page, head or
+// slot, and keys and values apart.
+int paged_written(const ann_paged* c) {
+  const auto one = [&](int64_t page, int64_t head, int64_t slot) {
+    return (c->pages > 1 && page == 0) || (c->heads > 1 && head == 0) || slot == 0;
+  };
+  if (one(c->k_page, c->k_head, c->k_slot) || one(c->v_page, c->v_head, c->v_slot))
+    return fail(ANN_E_ARG, "rows of the cache share memory (a stride is 0)");
+  if (c->k == c->v) return fail(ANN_E_ARG, "keys and values share memory");
+  return ANN_OK;
+}
+
 // Whether rows of fp32 weights may not be written by way of out: they share memory,
 // and are not the same rows.
 bool weights_overlap(const float* w, int64_t w_row, const float* out, int64_t out_row, int64_t seqs,
@@ -1289,6 +1301,8 @@ int ann_op_paged_append(const ann_paged* c, const ann_qk_rows* r, void* stream) 
   if (over(r->q, r->q_stride, r->Hq, true) || over(r->k, r->k_stride, r->Hk, false) ||
       over(r->v, r->v_stride, r->Hk, false))
     return fail(ANN_E_ARG, "out overlaps the queries, keys or values");
+  rc = paged_written(c);
+  if (rc) return rc;
   HIPCHK(paged_append(p, a, (const bf16_t*)r->v, r->v_stride[1], r->v_stride[2],
                       (hipStream_t)stream));
   return ANN_OK;
@@ -1367,6 +1381,8 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
     return fail(ANN_E_ARG, "weight in place with another row stride");
   if (c->cols && weights_overlap(weight, w_row, weight_out, wo_row, c->seqs, (int64_t)c->cols * c->page_size))
     return fail(ANN_E_ARG, "weight_out overlaps weight and is not the same rows");
+  rc = paged_written(c);
+  if (rc) return rc;
   HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,
                      index, new_lens, weight_out, wo_row, (hipStream_t)stream));
   return ANN_OK;

@@ -26,8 +26,9 @@ most 2^25 elements apart), and a head of it serves ``heads / kv_heads`` query he
 Tensors live on one GPU, which need not be the current device; the work goes to
 its current stream.
 
-A page that a call writes belongs to one sequence; pages that are only read may
-be shared by several (a common prefix).
+A page that a call writes belongs to one sequence, and no two of its rows share
+memory (an expanded cache can be read only); pages that are only read may be shared
+by several (a common prefix).
 
 These calls serve: autograd does not see them, and their results require no gradient.
 """

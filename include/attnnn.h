@@ -290,8 +290,9 @@ int ann_op_qk_norm_rope_bwd(const ann_qk_rows* r, void* stream);
  * lengths outside the table end at it.  Rows of queries, keys, values and
  * cache slots are 16-byte aligned (strides multiples of 8, slots at most 2^25
  * elements apart).  A head of the cache serves heads / cache heads query heads
- * behind one another.  Pages that a call writes belong to one sequence; pages
- * that are only read may be shared. */
+ * behind one another.  Pages that a call writes belong to one sequence, and its
+ * rows share no memory (no stride of 0, k is not v); pages that are only read may be
+ * shared. */
 typedef struct ann_paged {
   void* k;               /* bf16, (pages, heads, page_size, head_dim) by the strides */
   void* v;

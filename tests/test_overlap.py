@@ -104,3 +104,25 @@ def test_weights_that_overlap_in_part_are_refused():
     for lse in (FAKE, FAKE + 2048 - 4, FAKE - 92):
         assert weight(FAKE << 3, 128, FAKE, 128, lse) == _lib.ANN_E_ARG
         assert "lse" in L.ann_last_error().decode()
+
+
+def test_a_cache_that_is_written_has_rows_of_its_own():
+    """Broadcast pages, heads or slots, and one tensor for keys and values, may be read,
+    not appended to or evicted from."""
+    from attention_nn_amd import _lib
+    L = _lib.lib()
+    plain = dict(k=FAKE, v=FAKE << 1, k_page=6 * 16 * 128, k_head=16 * 128, k_slot=128, v_page=6 * 16 * 128,
+                 v_head=16 * 128, v_slot=128, table=FAKE, table_row=8, starts=FAKE, lens=FAKE, pages=64,
+                 page_size=16, heads=6, head_dim=128, seqs=4, cols=8, rows=4)
+    for kw in ({"k_page": 0}, {"k_head": 0}, {"k_slot": 0}, {"v_page": 0}, {"v_head": 0}, {"v_slot": 0}, {"v": FAKE}):
+        c = _lib.AnnPaged(**{**plain, **kw})
+        r = _lib.AnnQkRows(q=FAKE, k=FAKE, v=FAKE, q_out=FAKE, cs=FAKE, sn=FAKE, table_rows=64, B=1, T=4, Hq=6, Hk=6,
+                           D=128, dtype=1, eps=1e-6)
+        r.k, r.v = FAKE << 2, FAKE << 3
+        for s in (r.q_stride, r.k_stride, r.v_stride):
+            s[1], s[2] = 768, 128
+        assert L.ann_op_paged_append(c, r, None) == _lib.ANN_E_ARG
+        assert "share memory" in L.ann_last_error().decode()
+        assert L.ann_op_paged_evict(c, FAKE, 8, 8, FAKE, 128, 100, 10, FAKE << 2, FAKE << 3, FAKE << 4, 128,
+                                    None) == _lib.ANN_E_ARG
+        assert "share memory" in L.ann_last_error().decode()
