@@ -78,7 +78,9 @@ __device__ __forceinline__ void pa_row(const PagedArgs& c, const int32_t* __rest
 // only where a score passes it by more than 2^8 in p: p stays at most 2^8, sums in
 // fp32 far from their range, and the accumulators are seldom rescaled.  P is
 // rounded to bf16 (relative 2^-8 of each weight, as the framework's attention
-// rounds it); its sum is of the unrounded weights.
+// rounds it); its sum is of the unrounded weights.  What that leaves of each weight as a
+// second half, as few rows have it, takes the mean relative error from 0.0023 to 0.0017
+// (the result's own rounding) and 230 us of 2048 tokens on 16384 entries to 285.
 //
 // Entries outside what a tile sees are not read: a lane past an end reads the
 // nearest entry inside, masked.  What is masked for one row of a tile and seen by
@@ -315,7 +317,7 @@ __device__ __forceinline__ bf16x8_t pa_join(pa_v4i16 a, pa_v4i16 b) {
 // weights enter as two bf16 halves (2^-17 of each).  Bound by memory on long caches
 // (one token on 16 x 8192 entries of 6 heads of 128 in 5 parts: 59 us and 5 to join
 // them, 290 MB, 4.5 TB/s of a copy's 5.2), by the wait for one read after another and
-// a chunk's some 270 instructions a wave on short ones (777 entries: 11.5 us a call;
+// a chunk's some 270 instructions a wave on short ones (777 entries: 11.7 us a call;
 // 13.0 with the page ids read only behind the length, divisions by the group, every
 // chunk's addresses formed from its page id and every chunk masked).
 template <int DH, int NW>

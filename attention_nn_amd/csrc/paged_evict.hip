@@ -202,8 +202,9 @@ __global__ __launch_bounds__(EV_T) void k_evict_pick(const int32_t* lens, int co
 // first work-group takes all of them, in order: read, wait for all, write.  Entry i
 // comes from index[i] >= i, and the ones read later lie above all that are written
 // before; those before the first that moves stay untouched (16 x 4096 entries that all
-// stay: 8.7 us a call, 94 with them copied onto themselves).  Bound by memory: rows of 256 bytes from where they lie (16 sequences to
-// 4096 entries, 6 heads of 128: 84 us for 400 MB, 4.8 TB/s; stores by way of the caches
+// stay: 8.7 us a call, 94 with them copied onto themselves).  Bound by memory: rows of
+// 256 bytes from where they lie (16 sequences of 8192 to 4096 entries, 6 heads of 128: 85 us
+// for 400 MB, 4.7 TB/s, into other pages and in place alike; stores by way of the caches
 // took 37 us more, their lines being fetched before they are written).  Eight rows a
 // lane are on their way together.
 template <int DH, int NT>
