@@ -159,7 +159,9 @@ class _QkNormRope(torch.autograd.Function):
         tensor = isinstance(pos, torch.Tensor)
         ctx.save_for_backward(q, k, cs, sn, pos if tensor else None)
         ctx.pos, ctx.eps = None if tensor else pos, eps
-        return _qk_norm_rope(q, k, cs, sn, pos, eps)
+        y = _qk_norm_rope(q, k, cs, sn, pos, eps)
+        ctx.mark_non_differentiable(*(x for x, need in zip(y, ctx.needs_input_grad) if not need))
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable

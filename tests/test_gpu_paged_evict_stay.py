@@ -33,14 +33,14 @@ def test_prefixes_that_stay(lens, keep, first):
 def test_what_stays_is_not_copied():
     """Sequences that are short enough cost less than a third of those that move."""
     from attention_nn_amd import paged
-    k = torch.zeros((16 * 128 + 1, 6, 32, 128), dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros((64 * 128 + 1, 6, 32, 128), dtype=torch.bfloat16, device="cuda")
     v = k.clone()
-    table = torch.arange(16 * 128, dtype=I32, device="cuda").view(16, 128)
-    w = torch.rand((16, 4096), device="cuda")
+    table = torch.arange(64 * 128, dtype=I32, device="cuda").view(64, 128)
+    w = torch.rand((64, 4096), device="cuda")
     w[:, 0] = -1.0
 
     def us(entries, keep):
-        lens = torch.full((16,), entries, dtype=I32, device="cuda")
+        lens = torch.full((64,), entries, dtype=I32, device="cuda")
         times = []
         for _ in range(9):
             a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))

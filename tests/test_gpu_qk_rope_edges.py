@@ -71,7 +71,10 @@ def test_autograd_of_views_and_parts():
     assert (got[0] == 0).all() and torch.equal(got[1], dk)
     y = K.qk_norm_rope(a, k, cs, sn)
     got, = torch.autograd.grad(y[0], a, gq)
-    assert torch.equal(got, dq)
+    assert torch.equal(got, dq) and not y[1].requires_grad
+    y = K.qk_norm_rope(q, b, cs, sn)
+    got, = torch.autograd.grad(y[1], b, gk)
+    assert torch.equal(got, dk) and not y[0].requires_grad
 
 
 def test_autograd_twice_or_captured_is_refused(monkeypatch):
