@@ -76,6 +76,34 @@ class AnnPaged(ctypes.Structure):
         return cls.from_buffer_copy(cls._pack(*values))
 
 
+class AnnPagedTable(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("table_row", ctypes.c_int64), ("lens", ctypes.c_void_p),
+                ("refs", ctypes.c_void_p), ("table_out", ctypes.c_void_p), ("out_row", ctypes.c_int64),
+                ("refs_out", ctypes.c_void_p), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("seqs", ctypes.c_int32), ("cols", ctypes.c_int32)]
+
+    _pack = struct.Struct("Qq3QqQ4i").pack
+
+    @classmethod
+    def from_values(cls, *values):
+        return cls.from_buffer_copy(cls._pack(*values))
+
+
+class AnnLogitRows(ctypes.Structure):
+    _fields_ = ([("logits", ctypes.c_void_p), ("stride", ctypes.c_int64)]
+                + [(k, ctypes.c_void_p) for k in ("u", "temperature", "top_k", "top_p", "min_p")]
+                + [("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32),
+                   ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float),
+                   ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                   ("ids", ctypes.c_void_p), ("logprob", ctypes.c_void_p)])
+
+    _pack = struct.Struct("Qq5Qfi2f3i4x2Q").pack
+
+    @classmethod
+    def from_values(cls, *values):
+        return cls.from_buffer_copy(cls._pack(*values))
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
@@ -124,6 +152,11 @@ SIGNATURES = {
                                            _L, _P, _L, _P, _SZ, _P]),
     "ann_op_paged_evict": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _I, _P, _L, _I, _I, _P,
                                           _P, _P, _L, _P]),
+    "ann_op_paged_assign_ws_bytes": (_SZ, [ctypes.POINTER(AnnPagedTable)]),
+    "ann_op_paged_assign": (ctypes.c_int, [ctypes.POINTER(AnnPagedTable), _P, _I, _P, _P, _P, _P, _P, _P,
+                                           _SZ, _P]),
+    "ann_op_paged_release": (ctypes.c_int, [ctypes.POINTER(AnnPagedTable), _P]),
+    "ann_op_sample_logits": (ctypes.c_int, [ctypes.POINTER(AnnLogitRows), _P]),
     "ann_profile_enable": (ctypes.c_int, [_P, _I, _I]),
     "ann_profile_read": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(_I)]),
     "ann_check_device": (ctypes.c_int, [_P, _P]),

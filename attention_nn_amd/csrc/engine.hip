@@ -1264,6 +1264,49 @@ int paged_ws(const void* ws, size_t have, size_t need) {
   return ANN_OK;
 }
 
+// Checks of a block table and the pages' counts.
+int table_args(const ann_paged_table* t, TableArgs* a) {
+  if (!t) return fail(ANN_E_ARG, "table is null");
+  if (t->pages < 1 || t->seqs < 0 || t->seqs > 65535 || t->cols < 0)
+    return fail(ANN_E_ARG, "bad shape pages=%d seqs=%d cols=%d (seqs up to 65535)", t->pages, t->seqs, t->cols);
+  int sh = 4;
+  while (sh < 10 && (1 << sh) != t->page_size) ++sh;
+  if ((1 << sh) != t->page_size)
+    return fail(ANN_E_ARG, "page_size %d must be a power of two from 16 to 1024", t->page_size);
+  if (((long long)t->cols << sh) > (1LL << 30))
+    return fail(ANN_E_ARG, "a table row of %d pages of %d passes 2^30 entries", t->cols, t->page_size);
+  if (!t->refs || !t->refs_out || (t->seqs && (!t->lens || (t->cols && (!t->table || !t->table_out)))))
+    return fail(ANN_E_ARG, "null argument");
+  if (t->seqs > 1 && t->out_row < t->cols) return fail(ANN_E_ARG, "rows of table_out overlap");
+  *a = TableArgs{t->table, t->table_row, t->lens, t->refs, t->table_out, t->out_row, t->refs_out,
+                 t->pages, sh, t->seqs, t->cols};
+  return ANN_OK;
+}
+
+// An operand of a call by name; `as`: the input that an output may be, as it lies there.
+struct Named {
+  const char* name;
+  Strided x;
+  int as;
+};
+Named flat(const char* name, const void* p, long long bytes, int as = -1) {
+  return {name, {p, 1, 0, 1, 0, bytes}, as};
+}
+// Outputs share memory with no input but the one they are, and not with each other.
+int apart(const Named* in, int n_in, const Named* out, int n_out) {
+  for (int i = 0; i < n_out; ++i) {
+    const Strided& o = out[i].x;
+    for (int j = 0; j < n_in; ++j) {
+      const Strided& x = in[j].x;
+      if (out[i].as == j && o.at == x.at && (o.n <= 1 || o.row == x.row)) continue;
+      if (overlap(o, x)) return fail(ANN_E_ARG, "%s overlaps %s", out[i].name, in[j].name);
+    }
+    for (int j = 0; j < i; ++j)
+      if (overlap(o, out[j].x)) return fail(ANN_E_ARG, "%s overlaps %s", out[i].name, out[j].name);
+  }
+  return ANN_OK;
+}
+
 }  // namespace
 
 int ann_op_qk_norm_rope(const ann_qk_rows* r, void* stream) {
@@ -1385,6 +1428,88 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
   if (rc) return rc;
   HIPCHK(paged_evict(p, c->head_dim, out_table, out_row, out_cols, weight, w_row, keep, recent,
                      index, new_lens, weight_out, wo_row, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t) {
+  TableArgs a{};
+  return table_args(t, &a) ? 0 : table_assign_ws_bytes(a);
+}
+
+int ann_op_paged_assign(const ann_paged_table* t, const int32_t* new_tokens, int32_t rows, int32_t* starts,
+                        int32_t* new_lens, int32_t* seq, int32_t* pos, int64_t* slot, void* ws,
+                        size_t ws_bytes, void* stream) {
+  TableArgs a{};
+  int rc = table_args(t, &a);
+  if (rc) return rc;
+  if (rows < 0 || rows > 1 << 30) return fail(ANN_E_ARG, "rows=%d must lie in [0, 2^30]", rows);
+  if (!starts || (t->seqs && (!new_tokens || !new_lens)) || (rows && (!seq || !pos || !slot)))
+    return fail(ANN_E_ARG, "null argument");
+  const long long S = t->seqs, C = t->cols, P = t->pages;
+  const Named in[] = {{"table", {t->table, S, t->table_row * 4, 1, 0, C * 4}, -1}, flat("refs", t->refs, P * 4),
+                      flat("lens", t->lens, S * 4), flat("new", new_tokens, S * 4)};
+  const Named out[] = {{"table_out", {t->table_out, S, t->out_row * 4, 1, 0, C * 4}, 0},
+                       flat("refs_out", t->refs_out, P * 4, 1), flat("new_lens", new_lens, S * 4, 2),
+                       flat("starts", starts, (S + 1) * 4), flat("seq", seq, rows * 4LL),
+                       flat("pos", pos, rows * 4LL), flat("slot", slot, rows * 8LL)};
+  rc = apart(in, 4, out, 7);
+  if (rc) return rc;
+  a.add = new_tokens;
+  a.rows = rows;
+  a.starts = starts;
+  a.lens_out = new_lens;
+  a.seq = seq;
+  a.pos = pos;
+  a.slot = (long long*)slot;
+  rc = paged_ws(ws, ws_bytes, table_assign_ws_bytes(a));
+  if (rc) return rc;
+  HIPCHK(table_assign(a, ws, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+int ann_op_paged_release(const ann_paged_table* t, void* stream) {
+  TableArgs a{};
+  int rc = table_args(t, &a);
+  if (rc) return rc;
+  const long long S = t->seqs, C = t->cols, P = t->pages;
+  const Named in[] = {{"table", {t->table, S, t->table_row * 4, 1, 0, C * 4}, -1}, flat("refs", t->refs, P * 4),
+                      flat("lens", t->lens, S * 4)};
+  const Named out[] = {{"table_out", {t->table_out, S, t->out_row * 4, 1, 0, C * 4}, 0},
+                       flat("refs_out", t->refs_out, P * 4, 1)};
+  rc = apart(in, 3, out, 2);
+  if (rc) return rc;
+  HIPCHK(table_release(a, (hipStream_t)stream));
+  return ANN_OK;
+}
+
+// ---- tokens from logits ------------------------------------------------------------
+
+int ann_op_sample_logits(const ann_logit_rows* r, void* stream) {
+  if (!r) return fail(ANN_E_ARG, "rows are null");
+  if (r->dtype != ANN_DTYPE_F32 && r->dtype != ANN_DTYPE_BF16) return fail(ANN_E_ARG, "bad dtype");
+  if (r->rows < 0 || r->cols < 1 || r->cols > 1 << 20)
+    return fail(ANN_E_ARG, "bad shape rows=%d cols=%d (1 .. 2^20)", r->rows, r->cols);
+  if (r->rows == 0) return ANN_OK;
+  if (!r->logits || !r->u || !r->ids) return fail(ANN_E_ARG, "null argument");
+  if (!r->temperature && !(r->temperature_all >= 0.f))
+    return fail(ANN_E_ARG, "temperature=%g must not be negative", r->temperature_all);
+  if (!r->top_p && !(r->top_p_all >= 0.f)) return fail(ANN_E_ARG, "top_p=%g must not be negative", r->top_p_all);
+  if (!r->min_p && !(r->min_p_all >= 0.f)) return fail(ANN_E_ARG, "min_p=%g must not be negative", r->min_p_all);
+  if (!r->top_k && r->top_k_all < 0) return fail(ANN_E_ARG, "top_k=%d must not be negative", r->top_k_all);
+  const int size = r->dtype == ANN_DTYPE_F32 ? 4 : 2;
+  if ((uintptr_t)r->logits & (size - 1)) return fail(ANN_E_ARG, "the logits are not aligned to their type");
+  const long long n = r->rows * 4LL;
+  const Named in[] = {{"logits", {r->logits, r->rows, r->stride * size, 1, 0, (int64_t)r->cols * size}, -1},
+                      flat("u", r->u, n), flat("temperature", r->temperature, r->temperature ? n : 0),
+                      flat("top_k", r->top_k, r->top_k ? n : 0), flat("top_p", r->top_p, r->top_p ? n : 0),
+                      flat("min_p", r->min_p, r->min_p ? n : 0)};
+  const Named out[] = {flat("ids", r->ids, n), flat("logprob", r->logprob, r->logprob ? n : 0)};
+  const int rc = apart(in, 6, out, 2);
+  if (rc) return rc;
+  const LogitRows a{r->logits, r->stride, r->u, r->temperature, r->top_k, r->top_p, r->min_p,
+                    r->temperature_all, r->top_k_all, r->top_p_all, r->min_p_all, r->rows, r->cols,
+                    r->ids, r->logprob};
+  HIPCHK(sample_logits(a, r->dtype, (hipStream_t)stream));
   return ANN_OK;
 }
 

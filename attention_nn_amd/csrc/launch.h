@@ -432,4 +432,46 @@ hipError_t paged_evict(const PagedArgs& c, int Dh, const int32_t* out_table, lon
                        int32_t* index, int32_t* new_lens, float* out, long long orow,
                        hipStream_t st);
 
+// Block tables and the pages' counts (paged_table.hip): (seqs, cols) tables by row
+// stride, outputs the inputs themselves or other memory.
+struct TableArgs {
+  const int32_t* table;
+  long long trow;
+  const int32_t* lens;
+  const int32_t* refs;
+  int32_t* table_out;
+  long long orow;
+  int32_t* refs_out;
+  int pages, sh, seqs, cols;
+  // table_assign only
+  const int32_t* add;   // new tokens of each sequence
+  int rows;
+  int32_t* starts;      // seqs + 1
+  int32_t* lens_out;
+  int32_t* seq;         // of each row: its sequence, entry and place in the cache
+  int32_t* pos;
+  long long* slot;
+};
+size_t table_assign_ws_bytes(const TableArgs& t);
+hipError_t table_assign(const TableArgs& t, void* ws, hipStream_t st);
+hipError_t table_release(const TableArgs& t, hipStream_t st);
+
+// One token of each row of logits (logits.hip): settings for each row, or (null) for all.
+struct LogitRows {
+  const void* x;
+  long long stride;    // elements from row to row
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+  int rows, cols;      // cols up to 2^20
+  int32_t* ids;
+  float* logprob;      // or null
+};
+hipError_t sample_logits(const LogitRows& r, int dtype, hipStream_t st);
+
 }  // namespace ann

@@ -6,6 +6,8 @@
     rms(x)                          model.py:48-49
     qk_norm_rope(q, k, cs, sn)      rms and rope_ht of q and k in one pass
                                     (model.py:244-247); qk_norm_rope_bwd is its gradient
+    sample_logits(logits, u, ...)   sample.py:45-49 by given random numbers, with
+                                    top_p and min_p
 
 Inputs are torch tensors on the GPU (fp32 or bf16); outputs keep the input
 dtype, computed in fp32 inside the HIP kernels.  ``rope_ht`` takes the
@@ -192,6 +194,60 @@ def qk_norm_rope(q, k, cs, sn, pos=0, eps=1e-6):
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k)):
         return _QkNormRope.apply(q, k, cs, sn, pos, eps)
     return _qk_norm_rope(q, k, cs, sn, pos, eps)
+
+
+def _setting(name, value, rows, dtype, d):
+    """(address or 0, the number for all rows, what has to outlive the call)."""
+    if not isinstance(value, torch.Tensor):
+        return 0, value, None
+    if value.dtype is not dtype or tuple(value.shape) != (rows,):
+        raise ValueError(f"{name} must be a number or {dtype} of shape {(rows,)}, got {value.dtype} "
+                         f"{tuple(value.shape)}")
+    if value.get_device() != d:
+        raise ValueError(f"{name} must be on the logits' device")
+    value = value.contiguous()
+    return value.data_ptr(), 0, value
+
+
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logprob=False):
+    """One token of each row of ``logits`` (rows, vocabulary; fp32 or bf16, any row
+    stride) by the random numbers ``u`` (rows,) fp32 in [0, 1).  -> ids (rows,)
+    int32; with ``want_logprob`` also (rows,) fp32, the log of the share with which
+    each was drawn.
+
+    Each setting is a number or a GPU tensor (rows,), ``top_k`` int32, the others
+    fp32.  In this order: an entry weighs ``exp((x - max) / temperature)``; weights below
+    ``min_p`` (and below 2^-40) are dropped; with ``top_k`` in 1 .. vocabulary - 1 every
+    entry below the k-th largest is; with ``top_p`` < 1 all but the largest whose
+    weights come to ``top_p`` of what is left.  Equal entries stay or go together.  The token is the
+    first index at which the running sum of the weights left passes ``u`` of it.
+    Temperature 0 (in a tensor: not above 0) takes the lowest index of the largest
+    entry.  A NaN is never drawn; a row of -inf gives -1 and -inf.
+
+    Weights are formed in 64 bits and added exactly, so the same call gives the same tokens."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
+        raise ValueError("expected a GPU tensor")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be (rows, vocabulary), got {tuple(logits.shape)}")
+    dt, d, device = _dt(logits), logits.get_device(), logits.device
+    rows, cols = logits.shape
+    if cols > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if not isinstance(u, torch.Tensor):
+        raise ValueError("u must be a GPU tensor")
+    up, _, u = _setting("u", u, rows, torch.float32, d)
+    t, t_all, t_keep = _setting("temperature", temperature, rows, torch.float32, d)
+    k, k_all, k_keep = _setting("top_k", top_k, rows, torch.int32, d)
+    p, p_all, p_keep = _setting("top_p", top_p, rows, torch.float32, d)
+    m, m_all, m_keep = _setting("min_p", min_p, rows, torch.float32, d)
+    k_all = min(max(int(k_all), -1), (1 << 31) - 1)
+    ids = torch.empty((rows,), dtype=torch.int32, device=device)
+    logprob = torch.empty((rows,), dtype=torch.float32, device=device) if want_logprob else None
+    a = _lib.AnnLogitRows.from_values(logits.data_ptr(), logits.stride(0), up, t, k, p, m, t_all, k_all,
+                                      p_all, m_all, rows, cols, dt, ids.data_ptr(),
+                                      logprob.data_ptr() if want_logprob else 0)
+    _lib.check(on_device(d, _lib.lib().ann_op_sample_logits, a))
+    return (ids, logprob) if want_logprob else ids
 
 
 def qk_norm_rope_bwd(gq, gk, q, k, cs, sn, pos=0, eps=1e-6):

@@ -33,6 +33,8 @@ by several (a common prefix).
 These calls serve: autograd does not see them, and their results require no gradient.
 """
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
@@ -299,3 +301,105 @@ def evict(k_cache, v_cache, table, lens, weight, keep, recent=0, out_table=None)
     if rc:
         _lib.check(rc)
     return index, left, out
+
+
+class Assigned(NamedTuple):
+    """A step's tables and row maps, as ``assign`` made them."""
+    table: torch.Tensor    # (sequences, columns) int32
+    refs: torch.Tensor     # (pages,) int32
+    starts: torch.Tensor   # (sequences + 1,) int32
+    lens: torch.Tensor     # (sequences,) int32
+    seq: torch.Tensor      # (rows,) int32: the sequence of each row, -1 behind the last
+    pos: torch.Tensor      # (rows,) int32: its entry, -1 behind
+    slot: torch.Tensor     # (rows,) int64: page * page_size + place in the page, -1 behind
+
+
+def _table_args(table, lens, refs, page_size, out, refs_out):
+    """AnnPagedTable of the call, its outputs, (device, sequences), and what has to
+    outlive the call."""
+    if not isinstance(table, _Tensor) or table.get_device() < 0:
+        raise ValueError("table: expected a GPU tensor")
+    d = table.get_device()
+    _check("table", table, _I32, 2, d)
+    S, cols = table.shape
+    _check("refs", refs, _I32, 1, d)
+    device = table.device
+    if out is None:
+        if cols > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+        out = _new((S, cols), _I32, device)
+    else:
+        _check("out", out, _I32, 2, d)
+        if out.shape != (S, cols) or (cols > 1 and out.stride(1) != 1):
+            raise ValueError(f"out {tuple(out.shape)} must be {(S, cols)}, rows contiguous")
+        if cols > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+    pages = refs.shape[0]
+    if refs_out is None:
+        refs_out = _new((pages,), _I32, device)
+    else:
+        _check("refs_out", refs_out, _I32, 1, d)
+        if refs_out.shape[0] != pages or not refs_out.is_contiguous():
+            raise ValueError(f"refs_out must be contiguous, {pages} elements")
+    refs = _column("refs", refs, pages, d)
+    lens = _column("lens", lens, S, d)
+    t = _lib.AnnPagedTable.from_values(
+        table.data_ptr(), table.stride(0), lens.data_ptr(), refs.data_ptr(), out.data_ptr(), out.stride(0),
+        refs_out.data_ptr(), pages, _page_size(page_size), S, cols)
+    return t, out, refs_out, d, S, (table, lens, refs)
+
+
+def _page_size(n):
+    """As the C ABI's 32 bits hold it: what is no page size is refused there."""
+    return n if 0 <= n < 1 << 30 else 0
+
+
+def assign(table, lens, new, refs, page_size, rows, out=None, refs_out=None, lens_out=None):
+    """Pages for the next step: sequence ``s`` is to grow by ``new[s]`` tokens.
+    -> ``Assigned``: the table with a page for every new entry, the pages' counts,
+    ``starts`` and ``lens`` of the step as ``append`` and ``attention`` take them, and
+    for each of its ``rows`` rows the sequence, the entry and the slot in the cache.
+
+    ``refs`` (pages,) int32 counts the tables that name each page; a page is free
+    where that is not above 0.  A column that names no page (-1) takes one once its entries
+    are asked for, free pages in ascending order, and keeps it until ``release``: the
+    same call again finds it there.  Sequences are served in order, whole or
+    not at all: one whose entries do not fit its table row, or for which (with all
+    asked for before it) the pages or the ``rows`` do not last, gets none and keeps
+    its length.  One that needs no page needs only the rows.
+
+    ``out``, ``refs_out`` and ``lens_out`` may be ``table``, ``refs`` and ``lens``: a step in
+    place, which a captured graph replays on its own results."""
+    t, out, refs_out, d, S, keep = _table_args(table, lens, refs, page_size, out, refs_out)
+    new = _column("new", new, S, d)
+    rows = int(rows)
+    if not 0 <= rows <= 1 << 30:
+        raise ValueError(f"rows={rows} must lie in [0, 2^30]")
+    device = out.device
+    if lens_out is None:
+        lens_out = _new((S,), _I32, device)
+    else:
+        _check("lens_out", lens_out, _I32, 1, d)
+        if lens_out.shape[0] != S or not lens_out.is_contiguous():
+            raise ValueError(f"lens_out must be contiguous, {S} elements")
+    starts, seq, pos = _new((S + 1,), _I32, device), _new((rows,), _I32, device), _new((rows,), _I32, device)
+    slot = _new((rows,), torch.int64, device)
+    L = _lib.lib()
+    nws = L.ann_op_paged_assign_ws_bytes(t)
+    ws = _new((nws,), torch.uint8, device)
+    rc = on_device(d, L.ann_op_paged_assign, t, new.data_ptr(), rows, starts.data_ptr(), lens_out.data_ptr(),
+                   seq.data_ptr(), pos.data_ptr(), slot.data_ptr(), ws.data_ptr(), nws)
+    if rc:
+        _lib.check(rc)
+    return Assigned(out, refs_out, starts, lens_out, seq, pos, slot)
+
+
+def release(table, lens, refs, page_size, out=None, refs_out=None):
+    """The pages behind each sequence's first ``lens[s]`` entries (0: of a sequence
+    that ended; fewer: of one cut back) are given back.  -> (table, refs): -1 in their columns, one less
+    in their counts.  ``out`` and ``refs_out`` may be ``table`` and ``refs``."""
+    t, out, refs_out, d, _, keep = _table_args(table, lens, refs, page_size, out, refs_out)
+    rc = on_device(d, _lib.lib().ann_op_paged_release, t)
+    if rc:
+        _lib.check(rc)
+    return out, refs_out

@@ -353,6 +353,72 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
                        int32_t recent, int32_t* index, int32_t* new_lens, float* weight_out,
                        int64_t wo_row, void* stream);
 
+/* Pages given to sequences and taken back.  refs[p] counts the tables that name
+ * page p; a page is free where it is not above 0.  An id that is no page
+ * (negative, or pages and more) is none.  table (seqs, cols) names each sequence's
+ * pages, lens[s] counts its entries.  table_out and refs_out may be table (by the same
+ * rows) and refs, else share no memory with another operand.  All device arrays. */
+typedef struct ann_paged_table {
+  const int32_t* table;  /* rows table_row elements apart */
+  int64_t table_row;
+  const int32_t* lens;
+  const int32_t* refs;   /* pages */
+  int32_t* table_out;
+  int64_t out_row;
+  int32_t* refs_out;
+  int32_t pages, page_size;   /* page_size a power of two, 16 .. 1024 */
+  int32_t seqs, cols;         /* cols * page_size <= 2^30 */
+} ann_paged_table;
+
+/* A step's tokens get their pages: sequence s is to grow by new_tokens[s] (below 0: 0)
+ * entries, and needs a page for each column that these touch and that names none.
+ * Sequences are served in order, whole or not at all: s where its entries fit its table
+ * row and the rows and pages asked for by it and those before it (that fit theirs) are
+ * no more than `rows` and the free pages; one that needs no page needs only the rows.  The
+ * columns of those served take the free pages in ascending order (refs_out 1).
+ * starts (seqs + 1) and new_lens (seqs; it may be t->lens) then describe the step as ann_paged takes
+ * it, and row r of the step is entry pos[r] of sequence seq[r], slot[r] = page *
+ * page_size + place in the page; -1 behind the last row (seq, pos, slot: rows).  ws:
+ * ann_op_paged_assign_ws_bytes bytes (16-byte aligned), one for each call in flight. */
+size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t);
+int ann_op_paged_assign(const ann_paged_table* t, const int32_t* new_tokens, int32_t rows,
+                        int32_t* starts, int32_t* new_lens, int32_t* seq, int32_t* pos,
+                        int64_t* slot, void* ws, size_t ws_bytes, void* stream);
+
+/* Sequences cut to lens entries (0: ended) give their pages back: each column behind
+ * them that names a page takes one from its count, and is -1 in table_out. */
+int ann_op_paged_release(const ann_paged_table* t, void* stream);
+
+/* ---- tokens from logits -----------------------------------------------------
+ * One token of each row by given random numbers.  m is the row's largest entry; an
+ * entry x weighs w = exp((x - m) / temperature) where that is at least max(min_p,
+ * 2^-40), else 0 (entries equal to m: 1); of these the ones not below the k-th largest
+ * entry stay, where top_k is in 1 .. cols - 1; of these, where top_p < 1, the ones not
+ * below the largest t for which the entries at or above t weigh at least top_p of
+ * all.  The token is the first index at which the running sum of the weights
+ * passes u times their sum (u outside [0, 1): the nearest number inside); logprob
+ * the log of its share.  A temperature not above 0 takes the lowest index of the
+ * largest entry.  A NaN is never drawn; a row without an entry above -infinity
+ * gives -1 and -infinity.  Weights are formed in 64 bits and added exactly. */
+typedef struct ann_logit_rows {
+  const void* logits;        /* (rows, cols) in dtype, rows `stride` elements apart */
+  int64_t stride;
+  const float* u;            /* rows */
+  const float* temperature;  /* a setting for each row, or null: the one for all */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;     /* >= 0, as min_p and top_p */
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+  int32_t rows, cols;        /* cols in 1 .. 2^20 */
+  int32_t dtype;
+  int32_t* ids;              /* rows */
+  float* logprob;            /* rows, or null */
+} ann_logit_rows;
+int ann_op_sample_logits(const ann_logit_rows* r, void* stream);
+
 /* Device status of the decode steps (no reference counterpart).  The
  * cross-work-group waits of the persistent batch-1 step and of the decode
  * attention's split combine are bounded; one that gives up sets a device flag
