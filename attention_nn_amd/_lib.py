@@ -76,6 +76,17 @@ class AnnPaged(ctypes.Structure):
         return cls.from_buffer_copy(cls._pack(*values))
 
 
+class AnnPagedPrefix(ctypes.Structure):
+    _fields_ = [("groups", ctypes.c_void_p), ("table", ctypes.c_void_p), ("row", ctypes.c_int64),
+                ("lens", ctypes.c_void_p), ("count", ctypes.c_int32), ("cols", ctypes.c_int32)]
+
+    _pack = struct.Struct("2QqQ2i").pack
+
+    @classmethod
+    def from_values(cls, *values):
+        return cls.from_buffer_copy(cls._pack(*values))
+
+
 class AnnPagedTable(ctypes.Structure):
     _fields_ = [("table", ctypes.c_void_p), ("table_row", ctypes.c_int64), ("lens", ctypes.c_void_p),
                 ("refs", ctypes.c_void_p), ("table_out", ctypes.c_void_p), ("out_row", ctypes.c_int64),
@@ -147,6 +158,10 @@ SIGNATURES = {
     "ann_op_paged_attention_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I, _I]),
     "ann_op_paged_attention": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _L, _I, _F, _I, _P,
                                               _P, _P, _SZ, _P]),
+    "ann_op_paged_attention_shared_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), ctypes.POINTER(AnnPagedPrefix),
+                                                     _I, _I]),
+    "ann_op_paged_attention_shared": (ctypes.c_int, [ctypes.POINTER(AnnPaged), ctypes.POINTER(AnnPagedPrefix),
+                                                     _P, _L, _L, _I, _F, _I, _P, _P, _P, _SZ, _P]),
     "ann_op_paged_weight_ws_bytes": (_SZ, [ctypes.POINTER(AnnPaged), _I]),
     "ann_op_paged_weight": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _L, _I, _P, _F, _I, _P,
                                            _L, _P, _L, _P, _SZ, _P]),

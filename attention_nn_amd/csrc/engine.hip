@@ -1377,6 +1377,50 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
   return ANN_OK;
 }
 
+namespace {
+int prefix_args(const ann_paged* c, const ann_paged_prefix* x, SharedPrefix* a) {
+  if (!x) return fail(ANN_E_ARG, "prefix is null");
+  if (x->count < 0 || x->count > 65535 || x->cols < 0)
+    return fail(ANN_E_ARG, "bad shape count=%d cols=%d of the prefixes (count up to 65535)", x->count, x->cols);
+  if ((long long)x->cols * c->page_size > (1LL << 30))
+    return fail(ANN_E_ARG, "a prefix of %d pages of %d passes 2^30 entries", x->cols, c->page_size);
+  if (x->count && (!x->groups || !x->lens || (x->cols && !x->table))) return fail(ANN_E_ARG, "null argument");
+  *a = SharedPrefix{x->groups, x->table, x->row, x->lens, x->count, x->cols};
+  return ANN_OK;
+}
+}  // namespace
+
+size_t ann_op_paged_attention_shared_ws_bytes(const ann_paged* c, const ann_paged_prefix* x, int32_t heads,
+                                              int32_t window) {
+  PagedArgs p;
+  SharedPrefix s;
+  if (paged_args(c, true, true, &p) || prefix_args(c, x, &s) || heads < 1 || heads % c->heads) return 0;
+  return paged_attention_shared_ws_bytes(p, s, heads, c->head_dim, window);
+}
+
+int ann_op_paged_attention_shared(const ann_paged* c, const ann_paged_prefix* x, const void* q, int64_t q_row,
+                                  int64_t q_head, int32_t heads, float scale, int32_t window, void* out,
+                                  float* lse, void* ws, size_t ws_bytes, void* stream) {
+  PagedArgs p;
+  SharedPrefix s;
+  int rc = paged_args(c, true, true, &p);
+  if (rc) return rc;
+  rc = prefix_args(c, x, &s);
+  if (rc) return rc;
+  rc = paged_query(c, q, q_row, q_head, heads, scale, window);
+  if (rc) return rc;
+  if (c->rows == 0) return ANN_OK;
+  if (!out) return fail(ANN_E_ARG, "out is null");
+  if ((uintptr_t)out & 15) return fail(ANN_E_ARG, "out must be 16-byte aligned");
+  if (paged_overlap(out, heads, q, q_row, q_head, heads, c->rows, c->head_dim, true))
+    return fail(ANN_E_ARG, "out overlaps the queries");
+  rc = paged_ws(ws, ws_bytes, paged_attention_shared_ws_bytes(p, s, heads, c->head_dim, window));
+  if (rc) return rc;
+  HIPCHK(paged_attention_shared(p, s, (const bf16_t*)q, q_row, q_head, heads, c->head_dim, scale, window,
+                                (bf16_t*)out, lse, ws, (hipStream_t)stream));
+  return ANN_OK;
+}
+
 size_t ann_op_paged_weight_ws_bytes(const ann_paged*, int32_t) { return 0; }
 
 int ann_op_paged_weight(const ann_paged* c, const void* q, int64_t q_row, int64_t q_head,

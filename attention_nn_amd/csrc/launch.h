@@ -423,6 +423,19 @@ size_t paged_attention_ws_bytes(const PagedArgs& c, int heads, int Dh, int windo
 hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
                            int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
                            void* ws, hipStream_t st);
+// The same for groups of sequences that begin with the same entries, group g (sequences
+// groups[g] .. groups[g + 1] - 1) with the first lens[g] of table[g].
+struct SharedPrefix {
+  const int32_t* groups;   // ngroups + 1
+  const int32_t* table;    // (ngroups, cols), row stride trow
+  long long trow;
+  const int32_t* lens;
+  int ngroups, cols;
+};
+size_t paged_attention_shared_ws_bytes(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window);
+hipError_t paged_attention_shared(const PagedArgs& c, const SharedPrefix& x, const bf16_t* q, long long qt,
+                                  long long qh, int heads, int Dh, float scale, int window, bf16_t* out,
+                                  float* lse, void* ws, hipStream_t st);
 // out[s][j] = w[s][j] + the weight entry j receives (j < len), else w[s][j].
 hipError_t paged_weight(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads,
                         int Dh, const float* lse, float scale, int window, const float* w,

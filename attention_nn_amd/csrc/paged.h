@@ -134,6 +134,39 @@ __device__ __forceinline__ PgTile pg_tile(const int32_t* __restrict__ starts,
   }
   return {-1, 0, {0, 0}, 0};
 }
+
+// The tile-th tile of br rows of groups of sequences (groups: ngroups + 1 of them,
+// like starts), by a whole wave: seq is the group, r its rows.
+__device__ __forceinline__ PgTile pg_group_tile(const int32_t* __restrict__ groups, int ngroups,
+                                                const int32_t* __restrict__ starts, int seqs, int rows,
+                                                int g, int br, int tile) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int g0 = 0; g0 < ngroups; g0 += 64) {
+    const int i = g0 + lane;
+    int n = 0;
+    PgRange r = {0, 0};
+    if (i < ngroups) {
+      const PgRange s = pg_range(groups[i], groups[i + 1], seqs);
+      r = pg_range(starts[s.first], starts[s.first + s.n], rows);
+      n = (r.n * g + br - 1) / br;
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    const unsigned long long past = __ballot(before + sum > tile);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      return {g0 + at, (tile - before - __builtin_amdgcn_readlane(sum - n, at)) * br,
+              {__builtin_amdgcn_readlane(r.first, at), __builtin_amdgcn_readlane(r.n, at)}, 0};
+    }
+    before += __shfl(sum, 63, 64);
+  }
+  return {-1, 0, {0, 0}, 0};
+}
 #endif
 
 }  // namespace ann

@@ -184,7 +184,18 @@ struct PaArgs {
   int few;             // rows of a sequence up to which pa_few takes it
   int packed;          // slots of pa_few: 16 a (sequence, cache head), else as pa_many's, (rows, heads)
   int br;              // rows of pa_many's tiles
+  // behind a shared prefix only (below): groups of sequences and what they share
+  const int32_t* groups;   // ngroups + 1
+  const int32_t* ptable;   // (ngroups, pcols), row stride prow
+  const int32_t* plens;
+  long long prow;
+  int ngroups, pcols;
+  float* po_pre;           // parts of the prefix: (rows, heads, most, DH), and m and sum
+  float2* ml_pre;
+  PaSplit sp_pre;
 };
+// Whose sums: of tiles of many rows, of few, of a prefix.
+enum PaWho { PA_MANY, PA_FEW, PA_PRE };
 
 // One sequence's new tokens as a call sees them.
 struct PaSeq {
@@ -217,21 +228,21 @@ struct PaRow {
   int n, h;
   long long at;   // slot * most + part
 };
-template <bool FEW>
+template <int WHO>
 __device__ __forceinline__ PaRow pa_place(const PaArgs& a, const PaSeq& q, int s, int kvh, int row,
                                           int part) {
   PaRow r;
   const int tok = q.by.div(row);
   r.n = q.first + tok;
   r.h = kvh * q.G + row - tok * q.G;
-  const long long slot = FEW && a.packed ? ((long long)s * a.c.heads + kvh) * 16 + row
-                                         : (long long)r.n * a.heads + r.h;
-  r.at = slot * (FEW ? a.sp_few.most : a.sp_many.most) + part;
+  const long long slot = WHO == PA_FEW && a.packed ? ((long long)s * a.c.heads + kvh) * 16 + row
+                                                   : (long long)r.n * a.heads + r.h;
+  r.at = slot * (WHO == PA_FEW ? a.sp_few.most : WHO == PA_MANY ? a.sp_many.most : a.sp_pre.most) + part;
   return r;
 }
 
 // Final (parts == 1) or partial result of a row: 4 dims from d on.
-template <int DH, bool FEW>
+template <int DH, int WHO>
 __device__ __forceinline__ void pa_store4(const PaArgs& a, const PaRow& w, int parts, int d, float4 o,
                                           float m, float l) {
   const long long r = (long long)w.n * a.heads + w.h;
@@ -242,20 +253,19 @@ __device__ __forceinline__ void pa_store4(const PaArgs& a, const PaRow& w, int p
     if (d == 0 && a.lse)
       a.lse[r] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * PA_LN2;
   } else {
-    *(float4*)((FEW ? a.po_few : a.po_many) + w.at * DH + d) = o;
-    if (d == 0) (FEW ? a.ml_few : a.ml_many)[w.at] = make_float2(m, l);
+    *(float4*)((WHO == PA_FEW ? a.po_few : WHO == PA_MANY ? a.po_many : a.po_pre) + w.at * DH + d) = o;
+    if (d == 0) (WHO == PA_FEW ? a.ml_few : WHO == PA_MANY ? a.ml_many : a.ml_pre)[w.at] = make_float2(m, l);
   }
 }
 
-// A row formed entry by entry, over the part [a0, b0) of what it sees.
-template <int DH, bool FEW>
+// A row at entry e formed entry by entry, over the part [a0, b0) of what it sees.
+template <int DH, int WHO>
 __device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, int s,
-                                         const int32_t* table, int kvh, int row, int a0, int b0,
-                                         int part, int parts) {
+                                         const int32_t* table, int kvh, int row, int e, int a0,
+                                         int b0, int part, int parts) {
   constexpr int DL = DH / 64;
   const int lane = threadIdx.x & 63;
-  const PaRow w = pa_place<FEW>(a, q, s, kvh, row, part);
-  const int e = q.e0 + q.by.div(row);
+  const PaRow w = pa_place<WHO>(a, q, s, kvh, row, part);
   const int lo = max(a0, e < a.window ? 0 : e - a.window + 1), hi = min(b0, e + 1);
   float m, l, o[DL];
   pa_row<DH>(a.c, table, a.q + w.n * a.qt + w.h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
@@ -263,10 +273,10 @@ __device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, int s,
   float4 v;
   if constexpr (DL == 1) {
     v = make_float4(o[0], __shfl_down(o[0], 1, 64), __shfl_down(o[0], 2, 64), __shfl_down(o[0], 3, 64));
-    if (lane % 4 == 0) pa_store4<DH, FEW>(a, w, parts, lane, v, m, l);
+    if (lane % 4 == 0) pa_store4<DH, WHO>(a, w, parts, lane, v, m, l);
   } else {
     v = make_float4(o[0], o[1], __shfl_down(o[0], 1, 64), __shfl_down(o[1], 1, 64));
-    if (lane % 2 == 0) pa_store4<DH, FEW>(a, w, parts, lane * 2, v, m, l);
+    if (lane % 2 == 0) pa_store4<DH, WHO>(a, w, parts, lane * 2, v, m, l);
   }
 }
 
@@ -307,6 +317,13 @@ __device__ __forceinline__ bf16x8_t pa_join(pa_v4i16 a, pa_v4i16 b) {
   return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The entries at its begin that sequence s shares with its group, by a whole wave.
+__device__ __forceinline__ int pa_prefix(const PaArgs& a, int s) {
+  const int g = __builtin_amdgcn_readfirstlane(pg_sequence(a.groups, a.ngroups, s));
+  if (g < 0 || s >= a.groups[g + 1]) return 0;
+  return pg_len(a.plens[g], a.pcols, a.c.sh);
+}
+
 // ---- sequences of few rows ----------------------------------------------------------
 //
 // A work-group takes a part of a sequence's entries for one cache head and 16 rows
@@ -327,7 +344,7 @@ constexpr size_t pa_few_lds() {
   const size_t sums = ((size_t)NW * 16 * (DH + 4) + 2 * NW * 16 + 16) * 4;
   return ring > sums ? ring : sums;
 }
-template <int DH, int NW>
+template <int DH, int NW, bool BEHIND = false>
 __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int row0, int kvh, int part,
                                        unsigned char* smem) {
   constexpr int RB = DH * 2, TB = 32 * RB;      // bytes of an LDS row, of a chunk's values
@@ -354,8 +371,10 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int row0, int kvh
   const int nrow = min(16, q.rows - row0);
   int lo, hi;
   pa_span(q, row0, nrow, a.window, lo, hi);
+  if constexpr (BEHIND) lo = max(lo, pa_prefix(a, s));
   const PaParts pt = pa_parts(lo, hi, a.sp_few);
   if (part >= pt.n) return;
+  const int parts = BEHIND ? 2 : pt.n;   // behind a prefix never all that a row sees
   const int a0 = max(pt.begin + part * pt.per, lo), b0 = min(pt.begin + (part + 1) * pt.per, hi);
   const int kb0 = pt.begin + part * pt.per;
   const int nch = b0 > a0 ? (b0 - kb0 + 31) / 32 : 0;
@@ -552,11 +571,12 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int row0, int kvh
   for (int k = 0; k < NI; ++k) {
     const int i = tid + k * 64 * NW, r = i / (DH / 4), d = i % (DH / 4) * 4;
     if (r >= nrow || s_bad[r]) continue;
-    pa_store4<DH, true>(a, pa_place<true>(a, q, s, kvh, row0 + r, part), pt.n, d,
+    pa_store4<DH, PA_FEW>(a, pa_place<PA_FEW>(a, q, s, kvh, row0 + r, part), parts, d,
                         make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), M[k], L[k]);
   }
   for (int r = wv; r < nrow; r += NW)
-    if (s_bad[r]) pa_again<DH, true>(a, q, s, table, kvh, row0 + r, a0, b0, part, pt.n);
+    if (s_bad[r])
+      pa_again<DH, PA_FEW>(a, q, s, table, kvh, row0 + r, q.e0 + q.by.div(row0 + r), a0, b0, part, parts);
 }
 
 // Work-groups past the sequences' take the sixteens of rows behind a sequence's first:
@@ -580,6 +600,41 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a, int blocks) 
     if (row0 == 0) return;
   }
   pa_few<DH, NW>(a, s, row0, blockIdx.x % a.c.heads, blockIdx.x / a.c.heads, pa_smem);
+}
+
+// The entries of a group's tokens n0 .. n0 + n - 1 (n <= cap) to LDS, -1 for those of
+// sequences with many rows, by a whole work-group; the entries lo .. hi - 1 that any of
+// them may see (hi 0: none sees one).
+__device__ __forceinline__ void pa_entries(const PaArgs& a, int g, int n0, int n, int cap, int* entry,
+                                           int& lo, int& hi) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const PgRange seqs = pg_range(a.groups[g], a.groups[g + 1], a.c.seqs);
+  n = min(n, cap);
+  for (int i = tid; i < cap; i += blockDim.x) entry[i] = -1;
+  __syncthreads();
+  for (int i = tid; i < seqs.n; i += blockDim.x) {
+    const int s = seqs.first + i;
+    const PgRange r = pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows);
+    if (r.n * (long long)a.G > a.few) continue;
+    const int e0 = pg_len(a.c.lens[s], a.c.cols, a.c.sh) - r.n - r.first;   // + a row: its entry
+    for (int t = max(r.first, n0); t < min(r.first + r.n, n0 + n); ++t) entry[t - n0] = max(e0 + t, -1);
+  }
+  __syncthreads();
+  int most = -1, least = 0x7fffffff;
+  for (int i = lane; i < n; i += 64) {
+    const int e = entry[i];
+    most = max(most, e);
+    if (e >= 0) least = min(least, e);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    most = max(most, __shfl_xor(most, d, 64));
+    least = min(least, __shfl_xor(least, d, 64));
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+  lo = least < a.window ? 0 : least - a.window + 1;
+  hi = most + 1;
 }
 
 // ---- sequences of many rows -----------------------------------------------------------
@@ -611,45 +666,77 @@ struct PaWalk {
 };
 template <int DH, int BK>
 constexpr size_t pa_many_lds() { return (size_t)2 * (PM_AHEAD + 1) * BK * DH * 2; }
-template <int DH, int BK, int QB>
+template <int DH, int BK, int QB, bool PRE = false>
 __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int part,
-                                        unsigned char* smem) {
+                                        unsigned char* smem, int* entry = nullptr) {
+  constexpr int WHO = PRE ? PA_PRE : PA_MANY;
   constexpr int BR = 64 * QB, RB = DH * 2, TB = BK * RB;
   constexpr int LPW = TB / 1024 / 4, RPL = 1024 / RB;   // loads a wave makes of K (and of V), rows of each
   constexpr int NKS = DH / 32, NDB = DH / 16, NBLK = BK / 16, NI = BK / 32;
   constexpr int NS = PM_AHEAD + 1;   // stages of keys, and of values
 
-  const PgTile pl = pg_tile(a.c.starts, a.c.lens, a.c.seqs, a.c.rows, a.G, a.few, BR, tile);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  // s: the sequence, or (PRE) the group
+  const PgTile pl = PRE ? pg_group_tile(a.groups, a.ngroups, a.c.starts, a.c.seqs, a.c.rows, a.G, BR, tile)
+                        : pg_tile(a.c.starts, a.c.lens, a.c.seqs, a.c.rows, a.G, a.few, BR, tile);
   if (pl.seq < 0) return;
   const int s = __builtin_amdgcn_readfirstlane(pl.seq), row0 = __builtin_amdgcn_readfirstlane(pl.row0);
   const PaSeq q = pa_seq(a, pl.r, pl.len);
   const int nrow = min(BR, q.rows - row0);
+  const int tok0 = q.by.div(row0);
   int lo, hi;
-  pa_span(q, row0, nrow, a.window, lo, hi);
-  const PaParts pt = pa_parts(lo, hi, a.sp_many);
-  if (part >= pt.n) return;
-  const int kb0 = pt.begin + part * pt.per;
+  PaParts pt;
+  if constexpr (PRE) {
+    const int shared = pg_len(a.plens[s], a.pcols, a.c.sh);
+    pt = pa_parts(0, shared, a.sp_pre);
+    if (shared == 0 || part >= pt.n) return;
+    pa_entries(a, s, q.first + tok0, q.by.div(row0 + nrow - 1) - tok0 + 1, 64 * QB, entry, lo, hi);
+    if (hi == 0) return;   // none of its rows are few: the same for all waves
+    hi = min(hi, shared);
+  } else {
+    pa_span(q, row0, nrow, a.window, lo, hi);
+    pt = pa_parts(lo, hi, a.sp_many);
+    if (part >= pt.n) return;
+  }
+  const int parts = PRE ? 2 : pt.n;   // a prefix is never all that a row sees
+  int kb0 = pt.begin + part * pt.per;
   const int a0 = max(kb0, lo), b0 = min(kb0 + pt.per, hi);
+  // parts of a prefix go by its length: a window may leave nothing of one, or its end
+  if (PRE && a0 < b0) kb0 += (a0 - kb0) / BK * BK;
   const int nt = b0 > a0 ? (b0 - kb0 + BK - 1) / BK : 0;
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r16 = lane & 15, g4 = lane >> 4;
-  const int32_t* table = a.c.table + s * a.c.trow;
+  const int32_t* table = PRE ? a.ptable + s * a.prow : a.c.table + s * a.c.trow;
 
   // this wave's rows, past the last one copies of it; their entries el .. eh
   const int wr0 = row0 + wv * 16 * QB, last = q.rows - 1;
   const bool some = wr0 <= last;
-  const int el = q.e0 + q.by.div(min(wr0, last)), eh = q.e0 + q.by.div(min(wr0 + 16 * QB - 1, last));
+  int el = q.e0 + q.by.div(min(wr0, last)), eh = q.e0 + q.by.div(min(wr0 + 16 * QB - 1, last));
   bf16x8_t qf[QB][NKS];
   int e[QB];
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const int row = min(wr0 + 16 * b + r16, last), tok = q.by.div(row);
-    e[b] = q.e0 + tok;
+    if constexpr (PRE) e[b] = entry[tok - tok0];
+    else e[b] = q.e0 + tok;
     const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qf[b][ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
+  }
+  if constexpr (PRE) {
+    el = eh = e[0];
+#pragma unroll
+    for (int b = 1; b < QB; ++b) {
+      el = min(el, e[b]);
+      eh = max(eh, e[b]);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      el = min(el, __shfl_xor(el, d, 64));
+      eh = max(eh, __shfl_xor(eh, d, 64));
+    }
+    el = __builtin_amdgcn_readfirstlane(el);
+    eh = __builtin_amdgcn_readfirstlane(eh);
   }
   floatx4_t o[QB][NDB];
   float m[QB], msl[QB], lsum[QB];
@@ -737,7 +824,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
   static_assert(KG == 8 && KG == VG && PG * KG == NBLK * 4, "one value fragment beside each key fragment");
   int f0 = max(a0 - kb0, eh < a.window ? 0 : eh - a.window + 1 - kb0);
   f0 = f0 > 0 ? (f0 + BK - 1) / BK : 0;
-  const int f1 = some ? min((min(b0, el + 1) - kb0) / BK, (b0 - kb0) / BK - 1 - PM_AHEAD) : 0;
+  const int f1 = some && (!PRE || nt) ? min((min(b0, el + 1) - kb0) / BK, (b0 - kb0) / BK - 1 - PM_AHEAD) : 0;
   floatx4_t sc[2][QB][NBLK];
   auto step = [&](int t, auto stage, auto free) __attribute__((always_inline)) {
     constexpr bool FREE = decltype(free)::value;
@@ -868,7 +955,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const int row = wr0 + 16 * b + r16;
-    const PaRow w = pa_place<false>(a, q, s, kvh, min(row, last), part);
+    const PaRow w = pa_place<WHO>(a, q, s, kvh, min(row, last), part);
     float l = lsum[b];
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -881,12 +968,13 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
     if (row <= last && !((bad >> r16) & 1))
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
-        pa_store4<DH, false>(a, w, pt.n, db * 16 + g4 * 4,
+        pa_store4<DH, WHO>(a, w, parts, db * 16 + g4 * 4,
                              make_float4(o[b][db][0], o[b][db][1], o[b][db][2], o[b][db][3]), M, l);
     while (bad) {
       const int r = __builtin_ctzll(bad);
       bad &= bad - 1;
-      pa_again<DH, false>(a, q, s, table, kvh, wr0 + 16 * b + r, a0, b0, part, pt.n);
+      pa_again<DH, WHO>(a, q, s, table, kvh, wr0 + 16 * b + r, PRE ? __shfl(e[b], r, 64) : q.e0 + q.by.div(wr0 + 16 * b + r),
+                        a0, b0, part, parts);
     }
   }
 }
@@ -956,7 +1044,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PaArgs a, int each, int grou
       // heads of one token may lie in two tiles, of other numbers of parts
       np[g] = h < a.heads ? pa_parts(lo, hi, sp).n : 1;
       if (np[g] == 1) np[g] = 0;
-      const long long at = few ? pa_place<true>(a, q, s, kvh, row, 0).at : pa_place<false>(a, q, s, kvh, row, 0).at;
+      const long long at = few ? pa_place<PA_FEW>(a, q, s, kvh, row, 0).at : pa_place<PA_MANY>(a, q, s, kvh, row, 0).at;
       po[g] = (few ? a.po_few : a.po_many) + at * DH + l * 4;
       const float2* pml = (few ? a.ml_few : a.ml_many) + at;
       float f[NP];
@@ -1167,11 +1255,9 @@ static hipError_t pa_launch(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
-                           int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
-                           void* ws, hipStream_t st) {
-  if (c.rows == 0 || c.seqs == 0) return hipSuccess;
-  const PaPlan p = pa_plan(c, heads, Dh, window);
+// What a call is given, and what comes of the scale.
+static PaArgs pa_args(const PagedArgs& c, const bf16_t* q, long long qt, long long qh, int heads, float scale,
+                      int window, bf16_t* out, float* lse) {
   PaArgs a{};
   a.c = c;
   a.q = q;
@@ -1188,6 +1274,15 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.flip = scale < 0.f ? 0x80008000u : 0u;
   a.out = out;
   a.lse = lse;
+  return a;
+}
+
+hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, long long qh,
+                           int heads, int Dh, float scale, int window, bf16_t* out, float* lse,
+                           void* ws, hipStream_t st) {
+  if (c.rows == 0 || c.seqs == 0) return hipSuccess;
+  const PaPlan p = pa_plan(c, heads, Dh, window);
+  PaArgs a = pa_args(c, q, qt, qh, heads, scale, window, out, lse);
   a.sp_few = p.sp_few;
   a.sp_many = p.sp_many;
   a.few = p.few;
@@ -1200,6 +1295,247 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
   a.ml_many = a.ml_few + n.few;
   if (Dh == 64) return pa_launch<64>(a, p, st);
   if (Dh == 128) return pa_launch<128>(a, p, st);
+  return hipErrorInvalidValue;
+}
+
+// ---- behind a shared prefix -----------------------------------------------------------
+//
+// Groups of consecutive sequences begin with the same entries, group g with the first
+// plens[g] of ptable[g].  Their rows are one tile's rows (pa_many's, each row with
+// its own entry), so that a prefix is read once for 64 or 128 of them; what a
+// sequence has behind the prefix goes as in calls of few rows.  Both leave parts
+// (sums that are not divided, with their maximum), in one launch, and a second
+// joins a row's parts.  A sequence of more than 16 new tokens has tiles of its own,
+// which read what they share from the caches: it takes the whole of its table.
+constexpr int PS_TOKENS = 16;
+constexpr int PS_PRE = 48, PS_OWN = 16;   // parts of a prefix and behind it at most: 64 in all
+
+struct PsGrid {
+  int many, pre, few;           // work-groups
+  int many_full, pre_full;      // tiles that the rows fill
+  bool by_seq;                  // few: PS_TOKENS * G / 16 sixteens for each sequence, else by the rows
+};
+
+// Tile and (cache head, part) of work-group L of tiles, `full` of which go first, those of
+// one (cache head, part) together on one XCD (as in k_paged_many).
+struct PsTile {
+  int tile, w;
+};
+__device__ __forceinline__ PsTile ps_tile(int L, int full, int pairs) {
+  const int first = full * pairs;
+  if (L >= first) return {full + (L - first) / pairs, (L - first) % pairs};
+  int w = L;
+  if (first % 8 == 0) w = (L % 8) * (first / 8) + L / 8;
+  return {w % full, w / full};
+}
+
+template <int DH, int QB>
+__global__ __launch_bounds__(256, 2) void k_paged_shared(PaArgs a, PsGrid g) {
+  constexpr int BK = DH == 64 ? 64 : 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
+  const int heads = a.c.heads;
+  int L = blockIdx.x;
+  if (L < g.many) {
+    const PsTile t = ps_tile(L, g.many_full, heads * a.sp_many.most);
+    pa_many<DH, BK, QB>(a, t.tile, t.w % heads, t.w / heads, pa_smem);
+    return;
+  }
+  L -= g.many;
+  if (L < g.pre) {
+    const PsTile t = ps_tile(L, g.pre_full, heads * a.sp_pre.most);
+    pa_many<DH, BK, QB, true>(a, t.tile, t.w % heads, t.w / heads, pa_smem,
+                              (int*)(pa_smem + pa_many_lds<DH, BK>()));
+    return;
+  }
+  L -= g.pre;
+  const int kvh = L % heads, part = L / heads % a.sp_few.most, i = L / heads / a.sp_few.most;
+  int s = i, row0 = 0;
+  if (g.by_seq) {
+    s = i % a.c.seqs;
+    row0 = 16 * (i / a.c.seqs);
+  } else if (i >= a.c.seqs) {   // as in k_paged_few
+    const int at = 16 * (i - a.c.seqs + 1);
+    s = __builtin_amdgcn_readfirstlane(pg_sequence(a.c.starts, a.c.seqs, a.by.div(at)));
+    if (s < 0) return;
+    row0 = (at - pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows).first * a.G + 15) & ~15;
+    if (row0 == 0) return;
+  }
+  pa_few<DH, 4, true>(a, s, row0, kvh, part, pa_smem);
+}
+
+// The parts of each row joined: those of its prefix, then its own, in order.  A wave
+// takes a token and as many of its heads as it has W lanes of four dims for, `waves`
+// waves a token.
+template <int DH>
+__global__ __launch_bounds__(256) void k_shared_join(PaArgs a, int groups, int waves) {
+  constexpr int W = DH / 4, HPW = 64 / W, NP = 64 / W;   // NP: parts a lane weighs, 64 in all
+  const int lane = threadIdx.x & 63, l = lane % W;
+  const int wv = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = wv / waves;
+  if (n >= a.c.rows) return;
+  const int s = __builtin_amdgcn_readfirstlane(pg_sequence(a.c.starts, a.c.seqs, n));
+  if (s < 0) return;
+  const PaSeq q = pa_seq(a, s);
+  if (n - q.first >= q.n) return;
+  const bool few = q.rows <= a.few;
+  const int shared = few ? pa_prefix(a, s) : 0;
+  const int np0 = few && shared && q.e0 + n - q.first >= 0 ? pa_parts(0, shared, a.sp_pre).n : 0;
+  for (int g = wv % waves; g < groups; g += waves) {
+    const int h = g * HPW + lane / W, hc = min(h, a.heads - 1);
+    const int kvh = q.by.div(hc), row = (n - q.first) * q.G + hc - kvh * q.G;
+    const int row0 = row & ~((few ? 16 : a.br) - 1);
+    int lo, hi;
+    pa_span(q, row0, min(few ? 16 : a.br, q.rows - row0), a.window, lo, hi);
+    int np1 = pa_parts(max(lo, shared), hi, few ? a.sp_few : a.sp_many).n;
+    if ((!few && np1 == 1) || h >= a.heads) np1 = 0;   // nothing to join, or no such head
+    const int np = np1 ? np0 + np1 : 0;
+    const long long at0 = ((long long)n * a.heads + hc) * a.sp_pre.most;
+    const long long at1 = ((long long)n * a.heads + hc) * (few ? a.sp_few.most : a.sp_many.most);
+    const float* po0 = a.po_pre + at0 * DH + l * 4;
+    const float* po1 = (few ? a.po_few : a.po_many) + at1 * DH + l * 4;
+    const float2* ml1 = (few ? a.ml_few : a.ml_many) + at1;
+    float m[NP], f[NP], M = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int i = l + W * k;
+      const float2 ml = i >= np ? make_float2(-INFINITY, 0.f) : i < np0 ? a.ml_pre[at0 + i] : ml1[i - np0];
+      m[k] = ml.x;
+      f[k] = ml.y;
+      M = fmaxf(M, m[k]);
+    }
+    M = group_max<W>(M);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      m[k] = __builtin_amdgcn_exp2f(m[k] - base);
+      sum += f[k] * m[k];
+    }
+    sum = group_sum<W>(sum);
+    floatx4_t o = (floatx4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      for (int i0 = 0; i0 < W; i0 += 4) {
+        if (!__any(W * k + i0 < np)) break;
+        floatx4_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int x = max(min(W * k + i0 + i, np - 1), 0);
+          v[i] = *(const floatx4_t*)(x < np0 ? po0 + x * DH : po1 + (x - np0) * DH);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = __shfl(m[k], i0 + i, W);
+          if (W * k + i0 + i < np) o += v[i] * w;
+        }
+      }
+    if (!np) continue;
+    const long long r = (long long)n * a.heads + h;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *(uint2*)(a.out + r * DH + l * 4) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+    if (a.lse && l == 0) a.lse[r] = sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * PA_LN2;
+  }
+}
+
+struct PsPlan {
+  int qb;
+  PsGrid grid;
+  PaSplit pre, few, many;
+};
+static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
+  static const int cus = device_cus();
+  PsPlan p{};
+  const int G = heads / c.heads;
+  const long long rows = (long long)c.rows * G, pairs = (long long)c.seqs * c.heads;
+  const auto clamp = [](long long v, long long hi) { return (int)(v < 1 ? 1 : v > hi ? hi : v); };
+  // sequences of many tokens, of which a call may have none, as in other calls
+  const PaPlan whole = pa_plan(c, heads, Dh, window);
+  const bool many = c.rows > PS_TOKENS;
+  p.many = whole.many ? whole.sp_many : PaSplit{1, 1};
+  const int groups = x.ngroups < 1 ? 1 : x.ngroups < c.rows ? x.ngroups : c.rows;
+  p.qb = whole.many ? whole.qb : rows / groups > 64 ? 2 : 1;
+  const int br = 64 * p.qb;
+  p.grid.many_full = clamp(rows / br, 1 << 30);
+  p.grid.pre_full = p.grid.many_full;
+  const long long tiles = rows / br + groups, width = (long long)x.cols << c.sh;
+  // two work-groups a CU, of 128 entries at least
+  p.pre.split = clamp(2LL * cus / (tiles * c.heads), clamp((width + 127) / 128, PS_PRE));
+  const long long own = (long long)c.cols << c.sh;
+  p.few.split = pairs >= cus ? 1 : clamp(2LL * cus / pairs, clamp((own + 127) / 128, PS_OWN));
+  p.few.most = clamp((own + 4095) / 4096, PS_OWN);
+  if (p.few.most < p.few.split) p.few.most = p.few.split;
+  const long long slot = (long long)(Dh + 2) * sizeof(float) * c.rows * heads;   // a part of every row
+  p.pre.split = p.pre.most = clamp((long long)PA_WS_MAX / slot, p.pre.split);
+  p.few.most = clamp((long long)PA_WS_MAX / slot, p.few.most);
+  if (p.few.split > p.few.most) p.few.split = p.few.most;
+  const long long more = (rows - 1) / 16, each = (long long)c.seqs * (G - 1);
+  p.grid.by_seq = each < more;
+  const long long blocks[3] = {many ? (rows / br + c.rows / (PS_TOKENS + 1)) * c.heads * p.many.most : 0,
+                               x.ngroups > 0 ? tiles * c.heads * p.pre.most : 0,
+                               (c.seqs + (each < more ? each : more)) * c.heads * p.few.most};
+  if (blocks[0] + blocks[1] + blocks[2] >= 1LL << 24) return p;   // 2^32 threads: refused by its grid of none
+  p.grid.many = (int)blocks[0];
+  p.grid.pre = (int)blocks[1];
+  p.grid.few = (int)blocks[2];
+  return p;
+}
+struct PsSlots {
+  size_t pre, few, many;
+};
+static PsSlots ps_slots(const PagedArgs& c, int heads, const PsPlan& p) {
+  const size_t rows = (size_t)c.rows * heads;
+  return {p.grid.pre ? rows * p.pre.most : 0, rows * p.few.most,
+          p.grid.many && p.many.most > 1 ? rows * p.many.most : 0};
+}
+
+size_t paged_attention_shared_ws_bytes(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
+  if (c.rows == 0 || c.seqs == 0) return 0;
+  const PsSlots n = ps_slots(c, heads, ps_plan(c, x, heads, Dh, window));
+  return (n.pre + n.few + n.many) * (Dh + 2) * sizeof(float);
+}
+
+template <int DH>
+static hipError_t ps_launch(const PaArgs& a, const PsPlan& p, hipStream_t st) {
+  constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>() + 128 * sizeof(int), f = pa_few_lds<DH, 4>();
+  const size_t lds = f > m ? f : m;
+  const dim3 grid((unsigned)(p.grid.many + p.grid.pre + p.grid.few));
+  if (grid.x == 0) return hipErrorInvalidConfiguration;
+  if (p.qb == 2) hipLaunchKernelGGL((k_paged_shared<DH, 2>), grid, dim3(256), lds, st, a, p.grid);
+  else hipLaunchKernelGGL((k_paged_shared<DH, 1>), grid, dim3(256), lds, st, a, p.grid);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int groups = (a.heads * (DH / 4) + 63) / 64;
+  const int waves = (long long)a.c.rows * groups <= 4096 ? groups : 1;
+  hipLaunchKernelGGL((k_shared_join<DH>), dim3((unsigned)(((long long)a.c.rows * waves + 3) / 4)), dim3(256), 0, st,
+                     a, groups, waves);
+  return hipGetLastError();
+}
+
+hipError_t paged_attention_shared(const PagedArgs& c, const SharedPrefix& x, const bf16_t* q, long long qt,
+                                  long long qh, int heads, int Dh, float scale, int window, bf16_t* out,
+                                  float* lse, void* ws, hipStream_t st) {
+  if (c.rows == 0 || c.seqs == 0) return hipSuccess;
+  const PsPlan p = ps_plan(c, x, heads, Dh, window);
+  PaArgs a = pa_args(c, q, qt, qh, heads, scale, window, out, lse);
+  a.sp_few = p.few;
+  a.sp_many = p.many;
+  a.sp_pre = p.pre;
+  a.few = PS_TOKENS * a.G;
+  a.br = 64 * p.qb;
+  a.groups = x.groups;
+  a.ngroups = x.ngroups;
+  a.ptable = x.table;
+  a.prow = x.trow;
+  a.pcols = x.cols;
+  a.plens = x.lens;
+  const PsSlots n = ps_slots(c, heads, p);
+  a.po_pre = (float*)ws;
+  a.po_few = a.po_pre + n.pre * Dh;
+  a.po_many = a.po_few + n.few * Dh;
+  a.ml_pre = (float2*)(a.po_many + n.many * Dh);
+  a.ml_few = a.ml_pre + n.pre;
+  a.ml_many = a.ml_few + n.few;
+  if (Dh == 64) return ps_launch<64>(a, p, st);
+  if (Dh == 128) return ps_launch<128>(a, p, st);
   return hipErrorInvalidValue;
 }
 

@@ -238,6 +238,41 @@ def attention(q, k_cache, v_cache, table, starts, lens, scale, window=0, want_ls
     return (out, lse) if want_lse else out
 
 
+def attention_shared(q, k_cache, v_cache, table, starts, lens, groups, prefix_table, prefix_lens, scale,
+                     window=0, want_lse=False, out=None):
+    """``attention`` of a batch whose sequences begin with the same entries: those of
+    group ``g``, sequences ``groups[g] .. groups[g + 1] - 1``, with the first
+    ``prefix_lens[g]`` entries of ``prefix_table[g]``.  Their own tables name the same
+    pages there (or copies: of the page that a prefix ends in, say).  -> what ``attention`` gives.
+
+    ``groups`` (groups + 1,), ``prefix_table`` (groups, columns) and ``prefix_lens`` (groups,)
+    are int32 GPU tensors that the host does not look at; ``groups`` must not fall, and sequences of no
+    group share nothing.  A prefix is read once for the tokens of all its sequences with up
+    to 16 new ones; a sequence of more is on its own.  The
+    weights of a prefix's entries enter the product with the values in bf16, of the
+    others as in ``attention``."""
+    (q, qp, qt, qh), N, H, D, d, c, (S, _, _, page, _), keep = _queries(q, k_cache, v_cache, table, starts, lens)
+    _check("prefix_table", prefix_table, _I32, 2, d)
+    count, cols = prefix_table.shape
+    if cols > 1 and prefix_table.stride(1) != 1:
+        prefix_table = prefix_table.contiguous()
+    groups, prefix_lens = _column("groups", groups, count + 1, d), _column("prefix_lens", prefix_lens, count, d)
+    x = _lib.AnnPagedPrefix.from_values(groups.data_ptr(), prefix_table.data_ptr(), prefix_table.stride(0),
+                                        prefix_lens.data_ptr(), count, cols)
+    device = q.device
+    out = _new((N, H, D), _BF16, device) if out is None else _out(out, q)
+    window = _window(window)
+    L = _lib.lib()
+    nws = L.ann_op_paged_attention_shared_ws_bytes(c, x, H, window)
+    lse = _new((N, H), _F32, device) if want_lse else None
+    ws = _new((nws,), torch.uint8, device) if nws else None
+    rc = on_device(d, L.ann_op_paged_attention_shared, c, x, qp, qt, qh, H, scale, window, out.data_ptr(),
+                   lse.data_ptr() if want_lse else None, ws.data_ptr() if nws else None, nws)
+    if rc:
+        _lib.check(rc)
+    return (out, lse) if want_lse else out
+
+
 def attention_weight(q, lse, k_cache, table, starts, lens, weight, scale, window=0, out=None):
     """``weight`` (sequences, table entries) fp32 plus the attention weight that
     each entry receives from the new tokens ``q``, over all their heads; ``lse`` as

@@ -325,6 +325,26 @@ int ann_op_paged_attention(const ann_paged* c, const void* q, int64_t q_row, int
                            int32_t heads, float scale, int32_t window, void* out, float* lse,
                            void* ws, size_t ws_bytes, void* stream);
 
+/* The same where sequences begin with the same entries: groups of them, group g
+ * sequences groups[g] .. groups[g + 1] - 1 (groups never falls), share the first lens[g]
+ * entries of table[g] (count, cols; by rows `row` elements apart), which their own
+ * tables name too (or copies of them).  A prefix is read once for its group's tokens.  Sequences of no
+ * group share nothing.  ws: ann_op_paged_attention_shared_ws_bytes bytes (16-byte
+ * aligned), one for each call in flight. */
+typedef struct ann_paged_prefix {
+  const int32_t* groups;   /* count + 1 */
+  const int32_t* table;
+  int64_t row;
+  const int32_t* lens;     /* count */
+  int32_t count, cols;     /* cols * page_size <= 2^30 */
+} ann_paged_prefix;
+size_t ann_op_paged_attention_shared_ws_bytes(const ann_paged* c, const ann_paged_prefix* x,
+                                              int32_t heads, int32_t window);
+int ann_op_paged_attention_shared(const ann_paged* c, const ann_paged_prefix* x, const void* q,
+                                  int64_t q_row, int64_t q_head, int32_t heads, float scale,
+                                  int32_t window, void* out, float* lse, void* ws, size_t ws_bytes,
+                                  void* stream);
+
 /* weight_out[s][j] = weight[s][j] + sum over sequence s's new tokens that see
  * entry j and over heads of exp(scale q.k_j - lse), lse as
  * ann_op_paged_attention gives it; entries behind the sequence keep their
