@@ -11,17 +11,16 @@
 // and added as whole numbers of 2^-F, F = 62 - log2 of the entries: exact sums, in
 // any order, LDS atomics too.  2^-46 of the largest weight an entry at 50257 of them.
 //
-// A work-group has a row; its waves hold consecutive parts of it in registers (rows
-// that do not fit are read again in each pass).  Forming all weights costs a CU as much
-// time as reading the row, so entries that cannot be drawn go first: those below
-// what min_p leaves, and below the k-th largest of the threads' maxima, under
-// which the k-th largest of all does not lie.  What is left, if 4096 entries at most,
-// is listed in LDS in the order of the indices, and thresholds and draw go over the
-// list.  top_p alone has no such bound: the entries above the 896th largest
-// maximum (some 2000) are listed and serve if their weight is enough of the whole
-// row's.  Else (flat rows, many equal values, no limits) the passes go over the row.
-// Thresholds by radix selection: sums in 2048 bins of the ordered 32-bit words,
-// three rounds at most.
+// A work-group has a row, which it reads once from memory and then from the caches, a
+// pass at a time: registers for a row of 50257 would leave a CU one work-group, and their
+// number (two) hides what a pass waits for.  Weights of all entries cost a CU 8 us of
+// its 64-bit units at that length, so entries that cannot be drawn go first: those below what
+// min_p leaves, and below the k-th largest of the threads' maxima, under which
+// the k-th largest of all does not lie.  What is left, if 4096 entries at most, is
+// listed in LDS in the order of the indices, and thresholds and draw go over the
+// list; 256 entries at most by one wave without a barrier.  top_p alone has no such
+// bound: the weights of all entries, added up in bins, give one.  Else (flat rows,
+// many equal values, no limits) the passes go over the row.
 #include <math.h>
 #include "common.h"
 #include "launch.h"
@@ -31,17 +30,24 @@ namespace ann {
 constexpr int SL_NT = 1024, SL_NW = SL_NT / 64;
 constexpr int SL_BINS = 2048;
 constexpr int SL_CAP = 4096;          // entries of the list
-constexpr int SL_RANK = 896;          // threads' maxima that bound a k, or the list of a top_p
+constexpr int SL_PER = SL_CAP / SL_NT;
+constexpr int SL_WAVE = 256;          // entries of it that one wave goes over
+constexpr int SL_PAIRS = 2;           // chunks that a thread reads again for others
+constexpr int SL_RANK = 896;          // a k up to which the threads' largest entries bound it
 typedef unsigned long long sl_u64;
 
 struct SlShared {
-  sl_u64 hist[SL_BINS];
+  sl_u64 hist[SL_BINS];               // zero between two selections
   float x[SL_CAP];
   int idx[SL_CAP];
+  uint32_t top[256];                  // of the threads' largest entries, by size
   sl_u64 part[2][SL_NW];
-  float fpart[2][SL_NW];
-  sl_u64 pick[2];
-  int at;
+  uint32_t mm[3][SL_NW];
+  int some[2][SL_NW];
+  sl_u64 above[2];
+  int at[2], low, bag[2];
+  unsigned short hit[SL_NT];          // threads with an entry far up, and of each wave how many, and before it
+  int hits[SL_NW], hits_before[SL_NW];
 };
 
 // Order-preserving word of a number (no NaN, no -0).
@@ -55,78 +61,114 @@ __device__ __forceinline__ float sl_value(uint32_t k) {
 // A NaN is below every number; -0 is 0.
 __device__ __forceinline__ float sl_number(float x) { return x == x ? x + 0.f : -INFINITY; }
 
-// Sum over the work-group, and (ex) over the threads before this one.
-__device__ __forceinline__ sl_u64 sl_scan(sl_u64 v, sl_u64& ex, SlShared& sh, int which) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  sl_u64 in = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const sl_u64 u = __shfl_up(in, o, 64);
-    if (lane >= o) in += u;
-  }
-  __syncthreads();   // the part's last readers are done
-  if (lane == 63) sh.part[which][wv] = in;
-  __syncthreads();
-  sl_u64 before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < SL_NW; ++w) {
-    if (w == wv) before = all;
-    all += sh.part[which][w];
-  }
-  ex = before + in - v;
-  return all;
+// Wave reductions of the device library.
+extern "C" __device__ unsigned __ockl_wfred_max_u32(unsigned);
+extern "C" __device__ unsigned __ockl_wfred_min_u32(unsigned);
+
+// Sums over the lanes up to this one, by row shifts and broadcasts of the vector unit.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sl_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ sl_u64 sl_dpp(sl_u64 v) {
+  return (sl_u64)sl_dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | sl_dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <typename N>
+__device__ __forceinline__ N sl_wave_scan(N v) {
+  v += sl_dpp<0x111, 0xf>(v);   // shifts by 1, 2, 4, 8 within a row of 16
+  v += sl_dpp<0x112, 0xf>(v);
+  v += sl_dpp<0x114, 0xf>(v);
+  v += sl_dpp<0x118, 0xf>(v);
+  v += sl_dpp<0x142, 0xa>(v);   // lane 15 to the second row, 47 to the fourth
+  v += sl_dpp<0x143, 0xc>(v);   // lane 31 to the third and fourth
+  return v;
+}
+__device__ __forceinline__ uint32_t sl_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ sl_u64 sl_lane(sl_u64 v, int lane) {
+  return (sl_u64)sl_lane((uint32_t)(v >> 32), lane) << 32 | sl_lane((uint32_t)v, lane);
 }
 
-// The weights of a row.
+// Sum over the work-group, and (ex) over the threads before this one; one barrier.
+// Calls take turns with `part` (which), and a barrier lies between two of one turn.
+__device__ __forceinline__ sl_u64 sl_scan(sl_u64 v, sl_u64& ex, sl_u64* part) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const sl_u64 in = sl_wave_scan(v);
+  if (lane == 63) part[wv] = in;
+  __syncthreads();
+  const sl_u64 own = part[lane % SL_NW], sums = sl_wave_scan(lane < SL_NW ? own : 0);
+  ex = in - v + sl_lane(sums - own, wv);
+  return sl_lane(sums, SL_NW - 1);
+}
+
+// The weights of a row, whole numbers of 2^-F.
 struct SlWeight {
-  float m;              // the largest entry
-  float low;            // entries below have no weight (those above may have none either)
-  double md, c, least;  // m, log2(e) / T, the least weight that counts
-  double magic;         // 2^(52 - F): a sum's last F bits of fraction are the fixed-point weight
-  sl_u64 one;           // 2^F
-  __device__ __forceinline__ sl_u64 operator()(float x) const {
-    if (!(x >= low)) return 0;
-    if (x == m) return one;
-    const double y = ((double)x - md) * c;
-    if (!(y > -41.0)) return 0;
-    const double n = rint(y), f = y - n;
+  double md, c, least;  // the largest entry, log2(e) / T, the least weight that counts
+  double magic;         // 2^(52 - F): the last 52 bits of a sum with it are the other number's times 2^F
+  float low;            // entries below have no weight (those above may have none either); a NaN has none
+  double k[10], round;  // of the polynomial; 1.5 * 2^52: the last bits of a sum with it are the nearest integer
+  __device__ __forceinline__ void open(float temp, float min_p, int frac) {
+    c = fmax(1.4426950408889634 / (double)temp, 0x1p-1000);   // an infinite T: all alike
+    least = fmin(fmax((double)min_p, 0x1p-40), 1.0);
+    magic = ldexp(1.0, 52 - frac);
     // (2^f - 1) / f on [-1/2, 1/2], interpolated at the Chebyshev nodes: relative 2^-50 of 2^f
-    double q = 0x1.e5e9f548e5725p-28;
-    q = fma(q, f, 0x1.b6571de2f2351p-24);
-    q = fma(q, f, 0x1.62bfe46117445p-20);
-    q = fma(q, f, 0x1.ffcb76789860fp-17);
-    q = fma(q, f, 0x1.4309130378460p-13);
-    q = fma(q, f, 0x1.5d87fe908f88ap-10);
-    q = fma(q, f, 0x1.3b2ab6fba385fp-7);
-    q = fma(q, f, 0x1.c6b08d7044119p-5);
-    q = fma(q, f, 0x1.ebfbdff82c590p-3);
-    q = fma(q, f, 0x1.62e42fefa39f7p-1);
-    const double w = ldexp(fma(q, f, 1.0), (int)n);
-    if (!(w >= least)) return 0;
-    return (sl_u64)__double_as_longlong(w + magic) & ((one << 1) - 1);
+    const double q[10] = {0x1.e5e9f548e5725p-28, 0x1.b6571de2f2351p-24, 0x1.62bfe46117445p-20, 0x1.ffcb76789860fp-17,
+                          0x1.4309130378460p-13, 0x1.5d87fe908f88ap-10, 0x1.3b2ab6fba385fp-7,  0x1.c6b08d7044119p-5,
+                          0x1.ebfbdff82c590p-3,  0x1.62e42fefa39f7p-1};
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      k[i] = q[i];
+      if (i) asm volatile("" : "+s"(k[i]));   // scalar registers: else every use moves it to vector ones first
+      else asm volatile("" : "+v"(k[i]));     // but for one of the first product's two
+    }
+    round = 0x1.8p52;
+    asm volatile("" : "+s"(round));
+  }
+  // With reach = log2(least) / c less some: the bound `low` for a finite largest entry m.  No word
+  // from there on is so far down that 2^n leaves the range below.
+  __device__ __forceinline__ void bound(float m, double reach) {
+    md = (double)m;
+    const double at = (double)m + reach;
+    low = fmaxf((float)(at - fabs(at) * 0x1p-22), -3.4028235e38f);
+    if (!(low <= m)) low = m;
+    // a few words, by which 2^-22 passes the bound
+    for (int i = 0; i < 16 && low < m && ((double)low - md) * c < -60.0; ++i) low = sl_value(sl_key(low) + 1);
+  }
+  // Without a branch; additions and products only: the unit that converts and scales is slower.
+  __device__ __forceinline__ sl_u64 operator()(float x) const {
+    const double d = (double)x - md;
+    const double t = fma(d, c, round), n = t - round, f = fma(d, c, -n);
+    double q = k[0];
+#pragma unroll
+    for (int i = 1; i < 10; ++i) q = fma(q, f, k[i]);
+    const double p = fma(q, f, 1.0);   // in [0.7, 1.42]: times 2^n, n >= -61, by its exponent
+    const double w = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+    const sl_u64 bits = (sl_u64)__double_as_longlong(w + magic) & 0xfffffffffffffull;
+    return x >= low && w >= least ? bits : 0;
   }
 };
 
-// The row as the work-group holds it: chunk c, 16 bytes, is entries c NE - shift on;
-// group g is chunks 64 g + lane, and wave w has groups w J .. w J + J - 1.  NJ > 0: J <=
-// NJ, in registers.
+// A row as a work-group has it: chunk c, 16 bytes, is entries c NE - shift on; group g is
+// chunks 64 g + lane, and wave w has groups w J .. w J + J - 1.  NJ > 0: J <= NJ, in registers;
+// else it is read in every pass.  NaNs are as they are: no comparison takes one.
 template <typename T, int NJ>
 struct SlRow {
   static constexpr int NE = 16 / (int)sizeof(T);
   const unsigned char* base;   // 16-byte aligned
   int shift, n, chunks, J;
   int g0, lane;                // the wave's first group
-  float held[NJ ? NJ : 1][NE];
+  uint4 held[NJ ? NJ : 1];
 
   // Index of entry e of this lane's chunk of group g.
   __device__ __forceinline__ int index(int g, int e) const { return (g * 64 * NE + e - shift) + lane * NE; }
   // The first and last words may hold bytes of other rows, or before and behind the
   // tensor: within its allocation, which no aligned 16-byte word crosses the end of.
-  __device__ __forceinline__ uint4 load(int g) const {
-    return lane < chunks - g * 64 ? *(const uint4*)(base + (long long)g * 1024 + lane * 16) : make_uint4(0, 0, 0, 0);
+  // A chunk past the last one is that one.
+  __device__ __forceinline__ uint4 chunk(int c) const {
+    return *(const uint4*)(base + (uint32_t)min(c, chunks - 1) * 16u);
   }
-  // The entries of a chunk; -inf outside the row and for a NaN.
-  __device__ __forceinline__ void values(const uint4& w, int g, float* v) const {
+  __device__ __forceinline__ uint4 load(int g) const { return chunk(g * 64 + lane); }
+  __device__ __forceinline__ static void unpack(const uint4& w, float* v) {
     if constexpr (sizeof(T) == 4) {
       v[0] = __uint_as_float(w.x);
       v[1] = __uint_as_float(w.y);
@@ -135,150 +177,221 @@ struct SlRow {
     } else {
       unpack8(w, v);
     }
+  }
+  // What of a chunk lies outside the row is -inf.
+  __device__ __forceinline__ uint4 inside(const uint4& w, int g) const {
+    if (g != 0 && (g + 1) * 64 < chunks) return w;   // the same for the wave
+    const int i = index(g, 0);
+    uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int e = 0; e < NE; ++e) v[e] = sl_number(v[e]);
-    if (g == 0 || (g + 1) * 64 >= chunks) {   // the same for the wave
-      const int i = index(g, 0);
-#pragma unroll
-      for (int e = 0; e < NE; ++e) v[e] = (unsigned)(i + e) < (unsigned)n ? v[e] : -INFINITY;
-    }
+    for (int e = 0; e < NE; ++e)
+      if ((unsigned)(i + e) >= (unsigned)n) {
+        if constexpr (sizeof(T) == 4) d[e] = 0xff800000u;
+        else d[e / 2] = e % 2 ? (d[e / 2] & 0xffffu) | 0xff800000u : (d[e / 2] & 0xffff0000u) | 0xff80u;
+      }
+    return make_uint4(d[0], d[1], d[2], d[3]);
   }
   __device__ __forceinline__ void open(const T* row, int cols) {
-    const uintptr_t at = (uintptr_t)row;
-    base = (const unsigned char*)(at & ~(uintptr_t)15);
-    shift = (int)(at & 15) / (int)sizeof(T);
+    const int over = (int)((uintptr_t)row & 15);
+    base = (const unsigned char*)row - over;
+    shift = over / (int)sizeof(T);
     n = cols;
     chunks = (cols + shift + NE - 1) / NE;
     J = (chunks + SL_NT - 1) / SL_NT;
     g0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * J;
     lane = threadIdx.x & 63;
     if constexpr (NJ > 0) {
-      uint4 w[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) w[j] = j < J ? load(g0 + j) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < NJ; ++j) held[j] = load(g0 + min(j, J - 1));
+    }
+  }
+  // What open has sent for has arrived.
+  __device__ __forceinline__ void arrived() {
+    if constexpr (NJ > 0) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)   // a group past the wave's last is all outside
+        held[j] = j < J ? inside(held[j], g0 + j)
+                        : sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                                         : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+    }
+  }
+  // f(values, group) for each group of the wave.
+  template <typename F>
+  __device__ __forceinline__ void groups(F&& f) const {
+    if constexpr (NJ > 0) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        values(w[j], g0 + j, held[j]);
-        if (j >= J)
+        // a copy that the compiler knows nothing of: it would keep what it forms of all of
+        // them from one pass to the next
+        uint4 w = held[j];
+        asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
+        float v[NE];
+        unpack(w, v);
+        f(v, g0 + j);
+      }
+    } else {
+      constexpr int D = 4;   // loads at once
+#pragma unroll 1
+      for (int j0 = 0; j0 < J; j0 += D) {
+        uint4 w[D];
 #pragma unroll
-          for (int e = 0; e < NE; ++e) held[j][e] = -INFINITY;
+        for (int d = 0; d < D; ++d) w[d] = load(g0 + min(j0 + d, J - 1));
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+          if (j0 + d < J) {
+            float v[NE];
+            unpack(inside(w[d], g0 + j0 + d), v);
+            f(v, g0 + j0 + d);
+          }
       }
     }
   }
-  // f(values, group) for each chunk of the thread: a few instructions for each value, or
-  // they are not held
-  template <typename F>
-  __device__ __forceinline__ void chunks_of(F&& f) const {
-    if constexpr (NJ > 0) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) f(held[j], g0 + j);
-    } else {
-      walk(f);
-    }
-  }
+  // f(number, -) of each entry, two at a time: of long ones' temporaries
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
-    chunks_of([&](const float* v, int) {
-#pragma unroll
-      for (int e = 0; e < NE; ++e) f(v[e]);
-    });
-  }
-  // The same from memory, a chunk ahead: where f is long.  52 copies of a weight's
-  // instructions are 60 KB of code, and a row that was read is in the caches.
-  template <typename F>
-  __device__ __forceinline__ void walk(F&& f) const {
-    uint4 next = load(g0);
-#pragma unroll 1
-    for (int j = 0; j < J; ++j) {
-      const uint4 w = next;
-      if (j + 1 < J) next = load(g0 + j + 1);
-      float v[NE];
-      values(w, g0 + j, v);
-      f(v, g0 + j);
-    }
-  }
-  template <typename F>
-  __device__ __forceinline__ void heavy(F&& f) const {
-    walk([&](const float* v, int) {
+    groups([&](const float* v, int) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        f(v[e]);
-        __builtin_amdgcn_sched_barrier(0);   // one weight's temporaries at a time
+        f(v[e], 0);
+        if (e % 2) __builtin_amdgcn_sched_barrier(0);
       }
     });
   }
 };
 
-// Up to N numbers a thread.
+// Up to N entries a thread, and their weights.
 template <int N>
 struct SlFew {
   float v[N];
+  sl_u64 w[N];
   template <typename F>
-  __device__ __forceinline__ void heavy(F&& f) const {
+  __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      f(v[i]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int i = 0; i < N; ++i) f(v[i], w[i]);
   }
 };
 
-// The largest word t in [lo, hi] such that the entries with words in [t, hi] count
-// (MASS: weigh) `want` at least, lo where all of [lo, hi] does not.  MASS with
-// share >= 0: want is that share of what [lo, hi] weighs.  once: after one round, a
-// word at or below t (the lower end of its bin).
-template <bool MASS, typename S>
-__device__ __forceinline__ uint32_t sl_select(const S& src, const SlWeight& wt, uint32_t lo, uint32_t hi,
-                                              sl_u64 want, double share, bool once, SlShared& sh) {
-  const int tid = threadIdx.x;
-  sl_u64 above = 0;   // of the entries above hi
-  while (true) {
-    const uint32_t range = hi - lo;
-    const int bits = 32 - __clz((int)range);   // 0 for one word
-    const int s = bits > 11 ? bits - 11 : 0;
-    __syncthreads();
-    sh.hist[tid] = 0;
-    sh.hist[tid + SL_NT] = 0;
-    if (tid == 0) sh.at = -1;
-    __syncthreads();
-    src.heavy([&](float x) {
-      const uint32_t k = sl_key(x);
-      if (k >= lo && k <= hi) {
-        if constexpr (MASS) {
-          const sl_u64 w = wt(x);
-          if (w) atomicAdd(&sh.hist[(k - lo) >> s], w);
-        } else {
-          atomicAdd((unsigned*)&sh.hist[(k - lo) >> s], 1u);
-        }
-      }
-    });
-    __syncthreads();
-    const int b = SL_BINS - 1 - 2 * tid;
-    const sl_u64 v1 = sh.hist[b], v0 = sh.hist[b - 1];
-    sl_u64 ex;
-    const sl_u64 all = sl_scan(v1 + v0, ex, sh, 0);
-    if (MASS && share >= 0.0) {
-      want = (sl_u64)ceil(share * (double)all);
-      if (want == 0) want = 1;
-      if (want > all) want = all;
-      share = -1.0;
-    }
-    ex += above;
-    if (ex < want && want <= ex + v1) {
-      sh.at = b;
-      sh.pick[0] = ex;
-    } else if (ex + v1 < want && want <= ex + v1 + v0) {
-      sh.at = b - 1;
-      sh.pick[0] = ex + v1;
-    }
-    __syncthreads();
-    const int at = sh.at;
-    if (at < 0) return lo;
-    above = sh.pick[0];
-    lo += (uint32_t)at << s;
-    if (s == 0 || once) return lo;
-    hi = min(hi, lo + ((1u << s) - 1));
+// A threshold on its way: the largest word t of [lo, hi] such that the entries with words from t
+// on count, or weigh, `want` at least; `above` of them lie above hi.
+struct SlPart {
+  uint32_t lo, hi;
+  sl_u64 above, want;
+  int turn;          // of the shared results
+};
+
+// What a round's bins hold: the one of them in which t lies (-1: none does, there are not
+// `want`), p.above with what lies above it.  share >= 0: want is that share of all.
+template <bool MASS>
+__device__ __forceinline__ int sl_bin(SlPart& p, double share, SlShared& sh) {
+  constexpr int PER = SL_BINS / SL_NT;
+  const int tid = threadIdx.x, turn = p.turn ^= 1;
+  if (tid == 0) sh.at[turn] = -1;
+  __syncthreads();
+  sl_u64 v[PER], sum = 0, ex;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {   // from the upper end down
+    sl_u64* bin = &sh.hist[SL_BINS - 1 - PER * tid - i];
+    sum += v[i] = *bin;
+    *bin = 0;
   }
+  const sl_u64 all = sl_scan(sum, ex, sh.part[turn]);
+  if (MASS && share >= 0.0) {
+    p.want = (sl_u64)ceil(share * (double)all);
+    if (p.want == 0) p.want = 1;
+    if (p.want > all) p.want = all;
+  }
+  ex += p.above;
+  if (ex < p.want && p.want <= ex + sum) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (p.want <= ex + v[i]) {
+        sh.at[turn] = SL_BINS - 1 - PER * tid - i;
+        sh.above[turn] = ex;
+        break;
+      }
+      ex += v[i];
+    }
+  }
+  __syncthreads();
+  p.above = sh.above[turn];
+  return sh.at[turn];
+}
+// An entry's weight: formed here of a row's, at hand of a list's.
+__device__ __forceinline__ sl_u64 sl_mass(const SlWeight& wt, float x, int) { return wt(x); }
+__device__ __forceinline__ sl_u64 sl_mass(const SlWeight&, float, sl_u64 w) { return w; }
+// To a bin where `in`; the weight is formed first, by all lanes.
+template <bool MASS, typename W>
+__device__ __forceinline__ void sl_add(const SlWeight& wt, float x, W w, bool in, int bin, SlShared& sh) {
+  if constexpr (MASS) {
+    const sl_u64 mass = sl_mass(wt, x, w);
+    if (in && mass) atomicAdd(&sh.hist[bin], mass);
+  } else {
+    if (in) atomicAdd((unsigned*)&sh.hist[bin], 1u);
+  }
+}
+// One round: [lo, hi] becomes the one of up to 2048 equal parts of it that holds t; false
+// where none does.
+template <bool MASS, typename S>
+__device__ __forceinline__ bool sl_round(const S& src, const SlWeight& wt, SlPart& p, double share, SlShared& sh) {
+  const int bits = 32 - __clz((int)(p.hi - p.lo));   // 0 for one word
+  const int s = bits > 11 ? bits - 11 : 0;
+  const uint32_t lo = p.lo;
+  const float x0 = sl_value(lo), x1 = sl_value(p.hi);
+  src.each([&](float x, auto w) {
+    sl_add<MASS>(wt, x, w, x >= x0 && x <= x1, (int)((sl_key(x + 0.f) - lo) >> s), sh);   // -0 is 0
+  });
+  const int at = sl_bin<MASS>(p, share, sh);
+  if (at < 0) return false;
+  p.lo += (uint32_t)at << s;
+  p.hi = min(p.hi, p.lo + ((1u << s) - 1));
+  return true;
+}
+// The first round over a whole row, whose largest entry is p.hi's: parts of equal difference
+// instead, since half of all words are numbers below 1.  `floor`: about the least entry
+// (what lies below goes to the lowest part).
+template <bool MASS, typename S>
+__device__ __forceinline__ bool sl_first(const S& src, const SlWeight& wt, SlPart& p, double share, float floor,
+                                         SlShared& sh) {
+  const float m = sl_value(p.hi), least = fmaxf(sl_value(p.lo), floor), c = SL_BINS / (m - least);
+  if (!(c > 0.f && c < 1e30f)) return sl_round<MASS>(src, wt, p, share, sh);   // not finite, or one value
+  const uint32_t lo = p.lo;
+  const auto bin = [&](float x) { return SL_BINS - 1 - (int)fminf((m - x) * c, SL_BINS - 1.f); };   // rises with x
+  const float x0 = sl_value(lo);
+  src.each([&](float x, auto w) {
+    sl_add<MASS>(wt, x, w, x >= x0, bin(x), sh);
+  });
+  const int at = sl_bin<MASS>(p, share, sh);
+  if (at < 0) return false;
+  // the least words of that part and of the next, by 64 lanes at a time
+  const int lane = threadIdx.x & 63;
+  const auto least_in = [&](int b) {
+    uint32_t a = lo, n = p.hi - lo + 1;   // it is one of the n words from a on, or the next
+    while (n) {
+      const uint32_t step = n / 64 + 1, at = lane * step;
+      const unsigned long long in = __ballot(at < n && bin(sl_value(a + at)) >= b);
+      // the first lane that has reached the part; or all n words lie below
+      const uint32_t first = in ? (uint32_t)__builtin_ctzll(in) : (n + step - 1) / step;
+      if (first == 0) return a;
+      const uint32_t past = (first - 1) * step + 1;   // the word behind the last one below
+      a += past;
+      n = in ? step - 1 : n - past;
+    }
+    return a;
+  };
+  const uint32_t a = least_in(at), b = least_in(at + 1);
+  p.lo = a;
+  p.hi = b - 1;
+  return true;
+}
+// All rounds: the word, or lo where there are not `want`.
+template <bool MASS, typename S>
+__device__ __forceinline__ uint32_t sl_select(const S& src, const SlWeight& wt, SlPart& p, double share, SlShared& sh) {
+  const uint32_t none = p.lo;
+  while (p.lo != p.hi || share >= 0.0) {
+    if (!sl_round<MASS>(src, wt, p, share, sh)) return none;
+    share = -1.0;
+  }
+  return p.lo;
 }
 
 struct SlArgs {
@@ -287,47 +400,56 @@ struct SlArgs {
 };
 
 template <typename T, int NJ>
-__global__ __launch_bounds__(SL_NT) void k_sample_logits(SlArgs a) {
+__global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char sl_smem[];
   SlShared& sh = *(SlShared*)sl_smem;
+  constexpr int NE = SlRow<T, NJ>::NE;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = blockIdx.x, V = a.r.cols;
+  SlRow<T, NJ> row;
+  row.open((const T*)a.r.x + r * a.r.stride, V);
   float u = a.r.u[r];
   const float temp = a.r.temperature ? a.r.temperature[r] : a.r.temperature_all;
   const int k = a.r.top_k ? a.r.top_k[r] : a.r.top_k_all;
   const float top_p = a.r.top_p ? a.r.top_p[r] : a.r.top_p_all;
   const float min_p = a.r.min_p ? a.r.min_p[r] : a.r.min_p_all;
+  const bool by_k = k > 0 && k < V, by_p = top_p < 1.f;
+#pragma unroll
+  for (int b = 0; b < SL_BINS; b += SL_NT) sh.hist[b + tid] = 0;
+  if (tid < 256) sh.top[tid] = 0;
+  if (tid == 0) sh.low = 0x7fffffff;
+  if (tid < 2) sh.bag[tid] = 0;
 
   SlWeight wt;
-  wt.c = 1.4426950408889634 / (double)temp;
-  wt.least = fmin(fmax((double)min_p, 0x1p-40), 1.0);
-  wt.magic = ldexp(1.0, 52 - a.frac);
-  wt.one = 1ull << a.frac;
-  const double reach = (log2(wt.least) - 1e-3) / wt.c;   // where weights end, less some
-  SlRow<T, NJ> row;
-  row.open((const T*)a.r.x + r * a.r.stride, V);
+  wt.open(temp, min_p, a.frac);
+  const double reach = (log2(wt.least) - 1e-3) / wt.c;   // while the row is on its way
+  row.arrived();
 
-  // ---- the largest entry, and the smallest of the threads' largest
-  float mine = -INFINITY;
-  row.each([&](float x) { mine = fmaxf(mine, x); });
-  float tmin;
-  {
-    const float hi = group_max<64>(mine), lo = -group_max<64>(mine > -INFINITY ? -mine : -INFINITY);
-    if (lane == 0) {
-      sh.fpart[0][wv] = hi;
-      sh.fpart[1][wv] = lo;
-    }
-    __syncthreads();
-    wt.m = sh.fpart[0][0];
-    tmin = sh.fpart[1][0];
+  // ---- the largest entry, the least of the threads' largest, and the least of some entries
+  float most = -INFINITY, few = INFINITY;
+  row.groups([&](const float* v, int g) {
 #pragma unroll
-    for (int w = 1; w < SL_NW; ++w) {
-      wt.m = fmaxf(wt.m, sh.fpart[0][w]);
-      tmin = fminf(tmin, sh.fpart[1][w]);
+    for (int e = 0; e < NE; ++e) most = fmaxf(most, v[e]);
+    if (g == row.g0)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) few = fminf(few, v[e] > -INFINITY ? v[e] : INFINITY);
+  });
+  most += 0.f;   // 0 for -0
+  const uint32_t key = sl_key(most);
+  {
+    const uint32_t top = __ockl_wfred_max_u32(key), low = __ockl_wfred_min_u32(sl_key(few + 0.f));
+    const uint32_t least = __ockl_wfred_min_u32(most > -INFINITY ? key : 0xffffffffu);
+    if (lane == 0) {
+      sh.mm[0][wv] = top;
+      sh.mm[1][wv] = least;
+      sh.mm[2][wv] = low;
     }
   }
-  if (wt.m == -INFINITY) {   // nothing to draw
+  __syncthreads();
+  const uint32_t kmax = __ockl_wfred_max_u32(sh.mm[0][lane % SL_NW]);
+  const float m = sl_value(kmax);
+  if (m == -INFINITY) {   // nothing to draw
     if (tid == 0) {
       a.r.ids[r] = -1;
       if (a.r.logprob) a.r.logprob[r] = -INFINITY;
@@ -336,205 +458,433 @@ __global__ __launch_bounds__(SL_NT) void k_sample_logits(SlArgs a) {
   }
   if (!(temp > 0.f)) {   // the lowest index of the largest
     int at = 0x7fffffff;
-    row.chunks_of([&](const float* v, int g) {
+    if (most == m)
+      row.groups([&](const float* v, int g) {
 #pragma unroll
-      for (int e = 0; e < SlRow<T, NJ>::NE; ++e)
-        if (v[e] == wt.m) at = min(at, row.index(g, e));
-    });
-    if (tid == 0) sh.at = 0x7fffffff;
-    __syncthreads();
-    if (at != 0x7fffffff) atomicMin(&sh.at, at);
+        for (int e = 0; e < NE; ++e)
+          if (v[e] == m) at = min(at, row.index(g, e));
+      });
+    if (at != 0x7fffffff) atomicMin(&sh.low, at);
     __syncthreads();
     if (tid == 0) {
-      a.r.ids[r] = sh.at;
+      a.r.ids[r] = sh.low;
       if (a.r.logprob) a.r.logprob[r] = 0.f;
     }
     return;
   }
   u = u >= 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
 
-  // ---- a bound below which no entry counts
-  wt.md = (double)wt.m;
-  {
-    const double at = wt.md + reach;
-    const float f = (float)(at - fabs(at) * 0x1p-22);
-    wt.low = f > -3.4028235e38f ? f : -3.4028235e38f;
-    if (!(wt.low <= wt.m)) wt.low = wt.m;
-  }
-  const uint32_t kmax = sl_key(wt.m), klow = sl_key(wt.low);
-  const bool by_k = k > 0 && k < V, by_p = top_p < 1.f;
-  const double share = by_p ? fmax((double)top_p, 0.0) : 1.0;
-
-  uint32_t thr = klow;     // of the words that are kept so far
-  bool ranked = !by_k;     // thr holds the k-th largest
-  SlFew<1> top;
-  top.v[0] = mine;
-  const uint32_t tlow = max(klow, sl_key(tmin));
-  const bool bound = by_k && k <= SL_RANK && V > SL_CAP;
-  if (bound) thr = max(thr, sl_select<false>(top, wt, tlow, kmax, (sl_u64)k, -1.0, true, sh));
-
-  const auto count = [&](uint32_t from, sl_u64& before) {   // entries from a word on
+  // Entries from a word on, and those of the waves before this one.
+  int before = 0, turn = 0;
+  const auto count = [&](uint32_t from) {
     const float x0 = sl_value(from);
-    int n = 0;
-    row.each([&](float x) { n += x >= x0; });
-    return sl_scan((sl_u64)n, before, sh, 1);
-  };
-  sl_u64 before, total = 0;   // total: weight of all that min_p leaves, where known
-  sl_u64 n = count(thr, before);
-  uint32_t from = thr;        // the list's least word
-  if (n > SL_CAP && by_k) {
-    // many equal values, or many to keep: the k-th largest itself
-    thr = max(thr, sl_select<false>(row, wt, thr, kmax, (sl_u64)k, -1.0, false, sh));
-    ranked = true;
-    from = thr;
-    n = count(from, before);
-  }
-  if (n > SL_CAP && by_p && !by_k) {
-    const uint32_t cut = max(thr, sl_select<false>(top, wt, tlow, kmax, (sl_u64)SL_RANK, -1.0, true, sh));
-    const float x0 = sl_value(cut);
-    int some = 0;
-    sl_u64 all = 0, listed = 0, ex;
-    row.heavy([&](float x) {
-      const sl_u64 w = wt(x);
-      all += w;
-      if (x >= x0) {
-        ++some;
-        listed += w;
-      }
+    uint32_t some = 0;
+    row.groups([&](const float* v, int) {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) some += v[e] >= x0;
     });
-    total = sl_scan(all, ex, sh, 0);
-    const sl_u64 got = sl_scan(listed, ex, sh, 1), few = sl_scan((sl_u64)some, before, sh, 0);
-    if (few <= SL_CAP && (double)got >= share * (double)total) {
-      from = cut;
-      n = few;
+    const uint32_t all = sl_lane(sl_wave_scan(some), 63);
+    turn ^= 1;
+    if (lane == 0) sh.some[turn][wv] = (int)all;
+    __syncthreads();
+    const uint32_t own = (uint32_t)sh.some[turn][lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
+    before = (int)sl_lane(in - own, wv);
+    return (int)sl_lane(in, SL_NW - 1);
+  };
+  if (m == INFINITY) {   // the infinite entries weigh 1, all others nothing
+    const int n = count(kmax), pick = (int)((double)u * n);
+    int at = before;
+    row.groups([&](const float* v, int g) {
+      int p = at;   // behind the lower lanes' entries
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const unsigned long long in = __ballot(v[e] == m);
+        p = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, p));
+        at += __popcll(in);
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (v[e] == m && p++ == pick) {
+          a.r.ids[r] = row.index(g, e);
+          if (a.r.logprob) a.r.logprob[r] = (float)-log((double)n);
+        }
+    });
+    return;
+  }
+  const uint32_t tmin = __ockl_wfred_min_u32(sh.mm[1][lane % SL_NW]);
+  const float floor = sl_value(__ockl_wfred_min_u32(sh.mm[2][lane % SL_NW]));
+
+  // The threads' largest entries in 256 bins: k of them are at or above the lower end of the
+  // bin that the k-th lies in, so the k-th largest of all is.
+  uint32_t kth = 0;
+  if (by_k && k <= SL_RANK && V > SL_CAP && kmax > tmin) {
+    const int bits = 32 - __clz((int)(kmax - tmin)), s = bits > 8 ? bits - 8 : 0;
+    if (key >= tmin) atomicAdd(&sh.top[(key - tmin) >> s], 1u);
+    __syncthreads();
+    const uint4 c = *(const uint4*)&sh.top[252 - 4 * lane];   // from the upper end down: w, z, y, x
+    const uint32_t sum = c.x + c.y + c.z + c.w, in = sl_wave_scan(sum), want = (uint32_t)k;
+    const unsigned long long past = __ballot(in >= want);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      uint32_t n = in - sum + c.w;
+      int b = 255 - 4 * lane;
+      if (n < want) n += c.z, --b;
+      if (n < want) n += c.y, --b;
+      if (n < want) --b;
+      kth = tmin + (sl_lane((uint32_t)b, at) << s);
     }
   }
 
-  sl_u64 left, ex;       // what is kept weighs, and before this thread's
-  double target;
-  int id = -1;
-  float drawn = 0.f;
-  if (n <= SL_CAP) {
-    // ---- the list, in the order of the indices: wave, chunk, lane, entry
+  wt.bound(m, reach);
+  const double share = by_p ? fmax((double)top_p, 0.0) : 1.0;
+  uint32_t thr = max(sl_key(wt.low), kth);   // the least word that is kept so far
+  bool ranked = !by_k;                       // thr is the k-th largest, if there are as many
+  SlPart sp{thr, kmax, 0, (sl_u64)k, 0};   // its turns are not those of count
+
+  // The list of all from a word on, where few threads have an entry that far up: the chunks of
+  // those, in the order of the indices (wave, group, lane), are shared out among all and
+  // read again.  Its number, or -1 where they are too many.
+  const auto few_of = [&](uint32_t from) {
     const float x0 = sl_value(from);
-    constexpr int NE = SlRow<T, NJ>::NE;
-    int at = __builtin_amdgcn_readfirstlane((int)before);   // of lane 0: before the wave
-    row.chunks_of([&](const float* v, int g) {
-      int some = 0;
+    const unsigned long long mine = __ballot(most >= x0);
+    if (lane == 0) sh.hits[wv] = __popcll(mine);
+    __syncthreads();
+    const uint32_t own = (uint32_t)sh.hits[lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
+    const int hits = (int)sl_lane(in, SL_NW - 1), pairs = hits * row.J;
+    if (hits > SL_PAIRS * SL_NT || pairs > SL_PAIRS * SL_NT) return -1;
+    if (wv == 0 && lane < SL_NW) sh.hits_before[lane] = (int)(in - own);
+    if (most >= x0) sh.hit[sl_lane(in - own, wv) + __popcll(mine & ((1ull << lane) - 1))] = (unsigned short)tid;
+    __syncthreads();
+    float v[SL_PAIRS][NE];
+    int first[SL_PAIRS], some = 0;
+    const int per = (pairs + SL_NT - 1) / SL_NT;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) some += v[e] >= x0;
-      if (!__any(some)) return;
-      int sum = some;
+    for (int i = 0; i < SL_PAIRS; ++i) {
+      const int pair = tid * per + i;
+      const bool real = i < per && pair < pairs;
+      // of the pairs of a wave's h hits the ones with group j are h in a row
+      const int w = sh.hit[real ? pair / row.J : 0] >> 6, h = sh.hits[w], b = sh.hits_before[w];
+      const int q = (real ? pair : b * row.J) - b * row.J, j = q / h, c = (w * row.J + j) * 64 + (sh.hit[b + q - j * h] & 63);
+      first[i] = c * NE - row.shift;
+      row.unpack(row.chunk(c), v[i]);
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int w = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += w;
+      for (int e = 0; e < NE; ++e) {
+        if (!real || (unsigned)(first[i] + e) >= (unsigned)V) v[i][e] = -INFINITY;
+        some += v[i][e] >= x0;
       }
-      int p = at + sum - some;
+    }
+    sl_u64 ex;
+    sp.turn ^= 1;
+    const int n = (int)sl_scan((sl_u64)some, ex, sh.part[sp.turn]);
+    if (n > SL_CAP) return -1;
+    int p = (int)ex;
+#pragma unroll
+    for (int i = 0; i < SL_PAIRS; ++i)
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (v[i][e] >= x0) {
+          sh.x[p] = v[i][e] + 0.f;
+          sh.idx[p] = first[i] + e;
+          ++p;
+        }
+    __syncthreads();
+    return n;
+  };
+  // The entries with words of [from, to] in any order, without their indices: their number.
+  const auto bag_of = [&](uint32_t from, uint32_t to) {
+    const float x0 = sl_value(from), x1 = sl_value(to);
+    turn ^= 1;
+    if (tid == 0) sh.bag[turn ^ 1] = 0;
+    row.groups([&](const float* v, int) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) any = any || (v[e] >= x0 && v[e] <= x1);
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+          if (v[e] >= x0 && v[e] <= x1) {
+            const int p = atomicAdd(&sh.bag[turn], 1);
+            if (p < SL_CAP) sh.x[p] = v[e] + 0.f;
+          }
+      }
+    });
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(sh.bag[turn]);
+  };
+
+  uint32_t from = thr;                   // the list's least word
+  int n = few_of(from);
+  bool listed = n >= 0;
+  if (!listed) n = count(from);
+  double part = by_p ? share : -1.0;     // of the mass, while that is not known
+  if (n > SL_CAP && by_k) {
+    // many equal values, or many to keep: the k-th largest itself
+    if (sl_first<false>(row, wt, sp, -1.0, floor, sh)) thr = max(thr, sl_select<false>(row, wt, sp, -1.0, sh));
+    ranked = true;
+    from = thr;
+    n = count(from);
+  }
+  bool rest = n > SL_CAP;                // not all that is kept is listed
+  if (rest && by_p) {
+    // all weights in bins; then what is kept, or at least what one bin holds, may fit the list
+    sp = SlPart{thr, kmax, 0, 0, sp.turn};
+    sl_first<true>(row, wt, sp, share, floor, sh);
+    part = -1.0;
+    from = sp.lo;
+    n = few_of(from);
+    listed = n >= 0;
+    if (!listed) n = count(from);
+    rest = n > SL_CAP;
+    if (rest) {
+      listed = true;
+      n = 0;                             // none where one word is left
+      while (sp.lo != sp.hi && (n = bag_of(sp.lo, sp.hi)) > SL_CAP) sl_round<true>(row, wt, sp, -1.0, sh);
+      if (sp.lo == sp.hi) n = 0;
+    }
+  } else if (rest) {
+    n = 0;
+  } else {
+    sp = SlPart{thr, kmax, 0, 0, sp.turn};
+  }
+
+  // ---- the list, in the order of the indices: wave, group, lane, entry
+  if (n && !listed) {
+    const float x0 = sl_value(from);
+    int at = before;
+    const auto write = [&](const float* v, int g) {
+      unsigned long long in[NE];
+      int p = at;   // behind the lower lanes' entries
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        in[e] = __ballot(v[e] >= x0);
+        p = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], p));
+        at += __popcll(in[e]);
+      }
 #pragma unroll
       for (int e = 0; e < NE; ++e)
         if (v[e] >= x0) {
-          sh.x[p] = v[e];
+          sh.x[p] = v[e] + 0.f;
           sh.idx[p] = row.index(g, e);
           ++p;
         }
-      at += __builtin_amdgcn_readlane(sum, 63);
-    });
+    };
+    const auto some = [&](const float* v) {
+      float top = v[0];
+#pragma unroll
+      for (int e = 1; e < NE; ++e) top = fmaxf(top, v[e]);
+      return top >= x0;
+    };
+    if constexpr (NJ > 0) {   // the groups with an entry first: a branch on a vector's result waits for it
+      uint32_t hit = 0;
+      row.groups([&](const float* v, int g) { hit |= some(v) ? 1u << (g - row.g0) : 0; });
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) hit |= __shfl_xor(hit, o, 64);
+      hit = __builtin_amdgcn_readfirstlane(hit);
+      row.groups([&](const float* v, int g) {
+        if (hit >> (g - row.g0) & 1) write(v, g);
+      });
+    } else {
+      row.groups([&](const float* v, int g) {
+        if (__any(some(v))) write(v, g);
+      });
+    }
     __syncthreads();
-    const int per = ((int)n + SL_NT - 1) / SL_NT;   // of a thread, in a row
-    SlFew<SL_CAP / SL_NT> list;
+  }
+
+  sl_u64 left;           // weight of all that is kept
+  int id = -1;
+  float drawn = 0.f;
+  if (!rest && n <= SL_WAVE) {
+    // ---- one wave, thresholds by bisection
+    if (wv) return;
+    constexpr int N = SL_WAVE / 64;
+    const int per = (n + 63) / 64;   // entries of a lane, in a row
+    float x[N];
+    uint32_t keys[N];
+    sl_u64 w[N], sum = 0;
 #pragma unroll
-    for (int i = 0; i < SL_CAP / SL_NT; ++i) {
-      const int j = tid * per + i;
-      list.v[i] = i < per && j < (int)n ? sh.x[j] : -INFINITY;
+    for (int i = 0; i < N; ++i) {
+      const int j = lane * per + i;
+      const bool real = i < per && j < n;
+      x[i] = real ? sh.x[j] : -INFINITY;
+      keys[i] = real ? sl_key(x[i]) : 0;
     }
-    if (!ranked) thr = max(thr, sl_select<false>(list, wt, from, kmax, (sl_u64)k, -1.0, false, sh));
-    if (by_p) {
-      sl_u64 want = 0;
-      double part = share;
-      if (total) {   // of the whole row, as sl_select forms it
-        want = (sl_u64)ceil(share * (double)total);
-        if (want == 0) want = 1;
-        part = -1.0;
+    if (!ranked && n >= k && per == 1) {   // an entry's rank by the others, one by one
+      uint32_t rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) rank += sl_lane(keys[0], i) > keys[0];
+      thr = max(thr, __ockl_wfred_min_u32(lane < n && rank < (uint32_t)k ? keys[0] : 0xffffffffu));
+    } else if (!ranked && n >= k) {   // else all of them are among the k
+      uint32_t lo = from, hi = kmax;
+      while (lo < hi) {
+        const uint32_t mid = hi - ((hi - lo) >> 1);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(keys[i] >= mid));
+        if (c >= k) lo = mid;
+        else hi = mid - 1;
       }
-      thr = max(thr, sl_select<true>(list, wt, max(thr, from), kmax, want, part, false, sh));
+      thr = max(thr, lo);
     }
-    sl_u64 w[SL_CAP / SL_NT], sum = 0;
 #pragma unroll
-    for (int i = 0; i < SL_CAP / SL_NT; ++i) {
-      w[i] = sl_key(list.v[i]) >= thr ? wt(list.v[i]) : 0;
+    for (int i = 0; i < N; ++i) {
+      w[i] = keys[i] >= thr ? wt(x[i]) : 0;
       sum += w[i];
-      __builtin_amdgcn_sched_barrier(0);
     }
-    left = sl_scan(sum, ex, sh, 1);
-    target = (double)u * (double)left;
-    if (sum && (double)ex <= target && target < (double)(ex + sum)) {
+    if (by_p) {
+      sl_u64 want = sp.want;
+      if (part >= 0.0) {
+        want = (sl_u64)ceil(part * (double)sl_lane(sl_wave_scan(sum), 63));
+        if (want == 0) want = 1;
+      }
+      uint32_t lo = thr, hi = kmax;
+      if (per == 1) {   // what lies above an entry weighs
+        sl_u64 above = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          const sl_u64 wi = sl_lane(w[0], i);
+          above += sl_lane(keys[0], i) > keys[0] ? wi : 0;
+        }
+        lo = hi = __ockl_wfred_min_u32(w[0] && above < want ? keys[0] : 0xffffffffu);
+      }
+      while (lo < hi) {
+        const uint32_t mid = hi - ((hi - lo) >> 1);
+        sl_u64 c = 0;
 #pragma unroll
-      for (int i = 0; i < SL_CAP / SL_NT; ++i) {
-        ex += w[i];
-        if (w[i] && id < 0 && target < (double)ex) {
-          id = sh.idx[tid * per + i];
-          drawn = list.v[i];
+        for (int i = 0; i < N; ++i) c += keys[i] >= mid ? w[i] : 0;
+        if (sl_lane(sl_wave_scan(c), 63) >= want) lo = mid;
+        else hi = mid - 1;
+      }
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (keys[i] < lo) w[i] = 0;
+        sum += w[i];
+      }
+    }
+    const sl_u64 in = sl_wave_scan(sum);
+    left = sl_lane(in, 63);
+    const double target = (double)u * (double)left;
+    sl_u64 run = in - sum;
+    if (sum && (double)run <= target && target < (double)in) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        run += w[i];
+        if (w[i] && id < 0 && target < (double)run) {
+          id = sh.idx[lane * per + i];
+          drawn = x[i];
         }
       }
     }
   } else {
-    // ---- the row itself
-    if (by_p) thr = max(thr, sl_select<true>(row, wt, thr, kmax, 0, share, false, sh));
-    const float x0 = sl_value(thr);
-    sl_u64 sum = 0;
-    row.heavy([&](float x) { sum += x >= x0 ? wt(x) : 0; });
-    left = sl_scan(sum, ex, sh, 1);
-    target = (double)u * (double)left;
-    // the wave whose entries' weight holds the target walks them again, from memory
-    sl_u64 start = 0, end = 0;
+    if (n) {
+      const int per = (n + SL_NT - 1) / SL_NT;   // of a thread, in a row
+      SlFew<SL_PER> list;
 #pragma unroll
-    for (int w = 0; w < SL_NW; ++w) {
-      if (w < wv) start += sh.part[1][w];
-      if (w <= wv) end += sh.part[1][w];
-    }
-    if ((double)start <= target && target < (double)end) {
-      constexpr int NE = SlRow<T, NJ>::NE;
-#pragma unroll 1
-      for (int j = 0; j < row.J; ++j) {
-        float v[NE];
-        row.values(row.load(row.g0 + j), row.g0 + j, v);
-        sl_u64 w[NE], mass = 0;
+      for (int i = 0; i < SL_PER; ++i) {
+        const int j = tid * per + i;
+        list.v[i] = i < per && j < n ? sh.x[j] : -INFINITY;
+        list.w[i] = i < per ? wt(list.v[i]) : 0;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (!ranked) {
+        SlPart q{from, kmax, 0, (sl_u64)k, sp.turn};
+        thr = max(thr, sl_select<false>(list, wt, q, -1.0, sh));
+        sp.turn = q.turn;
+        sp.lo = max(sp.lo, thr);
+      }
+      if (by_p) thr = max(thr, sl_select<true>(list, wt, sp, part, sh));
+      if (!rest) {
+        // ---- the draw from the list
+        sl_u64 sum = 0, ex;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          w[e] = v[e] >= x0 ? wt(v[e]) : 0;
-          mass += w[e];
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < SL_PER; ++i) {
+          if (sl_key(list.v[i]) < thr) list.w[i] = 0;
+          sum += list.w[i];
         }
-        sl_u64 in = mass;
+        sp.turn ^= 1;
+        left = sl_scan(sum, ex, sh.part[sp.turn]);
+        const double target = (double)u * (double)left;
+        if (sum && (double)ex <= target && target < (double)(ex + sum)) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const sl_u64 b = __shfl_up(in, o, 64);
-          if (lane >= o) in += b;
-        }
-        const sl_u64 all = __shfl(in, 63, 64);
-        if (target < (double)(start + all)) {
-          sl_u64 run = start + in - mass;
-          if (mass && (double)run <= target && target < (double)(run + mass)) {
-#pragma unroll
-            for (int e = 0; e < NE; ++e) {
-              run += w[e];
-              if (w[e] && id < 0 && target < (double)run) {
-                id = row.index(row.g0 + j, e);
-                drawn = v[e];
-              }
+          for (int i = 0; i < SL_PER; ++i) {
+            ex += list.w[i];
+            if (list.w[i] && id < 0 && target < (double)ex) {
+              id = sh.idx[tid * per + i];
+              drawn = list.v[i];
             }
           }
-          break;
         }
-        start += all;
+      }
+    } else if (by_p) {
+      thr = max(thr, sp.lo);
+    }
+    if (rest) {
+      // ---- the draw from the row: the wave whose weight holds the target, by all waves its
+      // groups, by the wave whose groups hold it the group, lane and entry
+      const float x0 = sl_value(thr);
+      sl_u64 sum = 0;
+      row.each([&](float x, int) {
+        const sl_u64 w = wt(x);
+        sum += x >= x0 ? w : 0;
+      });
+      sl_u64 ex;
+      sp.turn ^= 1;
+      left = sl_scan(sum, ex, sh.part[sp.turn]);
+      const double target = (double)u * (double)left;
+      const sl_u64 own = sh.part[sp.turn][lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
+      const int at = __builtin_ctzll(__ballot(target < (double)in));   // target < left
+      sl_u64 start = sl_lane(in - own, at);
+      const int per = (row.J + SL_NW - 1) / SL_NW, first = at * row.J;
+      const int ga = first + min(wv * per, row.J), gb = first + min(wv * per + per, row.J);
+      float v[NE];
+      sl_u64 w[NE];
+      const auto group = [&](int g) {
+        SlRow<T, NJ>::unpack(row.inside(row.load(g), g), v);
+        sl_u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          w[e] = wt(v[e]);
+          w[e] = v[e] >= x0 ? w[e] : 0;
+          sum += w[e];
+          if (e % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        return sum;
+      };
+      sl_u64 mass = 0;
+#pragma unroll 1
+      for (int g = ga; g < gb; ++g) mass += group(g);
+      sp.turn ^= 1;
+      sl_scan(mass, ex, sh.part[sp.turn]);
+      for (int i = 0; i < wv; ++i) start += sh.part[sp.turn][i];
+      if ((double)start <= target && target < (double)(start + sh.part[sp.turn][wv])) {
+#pragma unroll 1
+        for (int g = ga; g < gb; ++g) {
+          if (gb - ga > 1) mass = group(g);
+          const sl_u64 in = sl_wave_scan(mass), all = sl_lane(in, 63);
+          if (target < (double)(start + all)) {
+            sl_u64 run = start + in - mass;
+            if (mass && (double)run <= target && target < (double)(run + mass)) {
+#pragma unroll
+              for (int e = 0; e < NE; ++e) {
+                run += w[e];
+                if (w[e] && id < 0 && target < (double)run) {
+                  id = row.index(g, e);
+                  drawn = v[e] + 0.f;
+                }
+              }
+            }
+            break;
+          }
+          start += all;
+        }
       }
     }
   }
   if (id >= 0) {   // one thread's
     a.r.ids[r] = id;
     if (a.r.logprob) {
-      const double y = drawn == wt.m ? 0.0 : ((double)drawn - wt.md) / (double)temp;
+      const double y = drawn == m ? 0.0 : ((double)drawn - wt.md) / (double)temp;
       a.r.logprob[r] = (float)(y - log((double)left * ldexp(1.0, -a.frac)));
     }
   }
@@ -551,8 +901,8 @@ hipError_t sample_logits(const LogitRows& r, int dtype, hipStream_t st) {
   SlArgs a{r, 62};
   while (a.frac > 0 && (1LL << (62 - a.frac)) < r.cols) --a.frac;
   if (a.frac > 51) a.frac = 51;
-  // chunks a thread has: with up to 15 bytes before the row
-  const int ne = dtype == 0 ? 4 : 8, J = ((r.cols + ne - 1 + ne - 1) / ne + SL_NT - 1) / SL_NT;
+  // groups a wave has, of rows that begin up to 15 bytes behind a chunk's begin
+  const int ne = dtype == 0 ? 4 : 8, J = ((r.cols + 2 * ne - 2) / ne + SL_NT - 1) / SL_NT;
   if (dtype == 0) return J <= 2 ? sl_launch<float, 2>(a, st) : J <= 13 ? sl_launch<float, 13>(a, st) : sl_launch<float, 0>(a, st);
   return J <= 1 ? sl_launch<bf16_t, 1>(a, st) : J <= 7 ? sl_launch<bf16_t, 7>(a, st) : sl_launch<bf16_t, 0>(a, st);
 }
