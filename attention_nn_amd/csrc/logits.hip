@@ -16,7 +16,7 @@
 // number (two) hides what a pass waits for.  Weights of all entries cost a CU 8 us of
 // its 64-bit units at that length, so entries that cannot be drawn go first: those below what
 // min_p leaves, and below the k-th largest of the threads' maxima, under which
-// the k-th largest of all does not lie.  What is left, if 4096 entries at most, is
+// the k-th largest of all does not lie.  What is left, if 8192 entries at most, is
 // listed in LDS in the order of the indices, and thresholds and draw go over the
 // list; 256 entries at most by one wave without a barrier.  top_p alone has no such
 // bound: the weights of all entries, added up in bins, give one.  Else (flat rows,
@@ -29,7 +29,7 @@ namespace ann {
 
 constexpr int SL_NT = 1024, SL_NW = SL_NT / 64;
 constexpr int SL_BINS = 2048;
-constexpr int SL_CAP = 4096;          // entries of the list
+constexpr int SL_CAP = 8192;          // entries of the list
 constexpr int SL_PER = SL_CAP / SL_NT;
 constexpr int SL_WAVE = 256;          // entries of it that one wave goes over
 constexpr int SL_PAIRS = 2;           // chunks that a thread reads again for others
@@ -38,8 +38,7 @@ typedef unsigned long long sl_u64;
 
 struct SlShared {
   sl_u64 hist[SL_BINS];               // zero between two selections
-  float x[SL_CAP];
-  int idx[SL_CAP];
+  float2 list[SL_CAP];                // an entry and (its bits) its index
   uint32_t top[256];                  // of the threads' largest entries, by size
   sl_u64 part[2][SL_NW];
   uint32_t mm[3][SL_NW];
@@ -246,6 +245,24 @@ struct SlRow {
       }
     }
   }
+  // f(values, group) for the groups of which in(values) holds for a lane.
+  template <typename I, typename F>
+  __device__ __forceinline__ void groups_with(I&& in, F&& f) const {
+    if constexpr (NJ > 0) {   // all asked first: a branch on a vector's result waits for it
+      uint32_t hit = 0;
+      groups([&](const float* v, int g) { hit |= in(v) ? 1u << (g - g0) : 0; });
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) hit |= __shfl_xor(hit, o, 64);
+      hit = __builtin_amdgcn_readfirstlane(hit);
+      groups([&](const float* v, int g) {
+        if (hit >> (g - g0) & 1) f(v, g);
+      });
+    } else {
+      groups([&](const float* v, int g) {
+        if (__any(in(v))) f(v, g);
+      });
+    }
+  }
   // f(number, -) of each entry, two at a time: of long ones' temporaries
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
@@ -383,11 +400,12 @@ __device__ __forceinline__ bool sl_first(const S& src, const SlWeight& wt, SlPar
   p.hi = b - 1;
   return true;
 }
-// All rounds: the word, or lo where there are not `want`.
+// All rounds: the word, or lo where there are not `want`; where words no more than `grain`
+// apart are one number, any of those.
 template <bool MASS, typename S>
-__device__ __forceinline__ uint32_t sl_select(const S& src, const SlWeight& wt, SlPart& p, double share, SlShared& sh) {
+__device__ __forceinline__ uint32_t sl_select(const S& src, const SlWeight& wt, SlPart& p, double share, uint32_t grain, SlShared& sh) {
   const uint32_t none = p.lo;
-  while (p.lo != p.hi || share >= 0.0) {
+  while (p.hi - p.lo > grain || share >= 0.0) {
     if (!sl_round<MASS>(src, wt, p, share, sh)) return none;
     share = -1.0;
   }
@@ -404,6 +422,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char sl_smem[];
   SlShared& sh = *(SlShared*)sl_smem;
   constexpr int NE = SlRow<T, NJ>::NE;
+  constexpr uint32_t GRAIN = sizeof(T) == 4 ? 0 : 0xffff;   // words of bf16 lie 2^16 apart
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = blockIdx.x, V = a.r.cols;
@@ -583,8 +602,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 #pragma unroll
       for (int e = 0; e < NE; ++e)
         if (v[i][e] >= x0) {
-          sh.x[p] = v[i][e] + 0.f;
-          sh.idx[p] = first[i] + e;
+          sh.list[p] = make_float2(v[i][e] + 0.f, __int_as_float(first[i] + e));
           ++p;
         }
     __syncthreads();
@@ -595,19 +613,29 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     const float x0 = sl_value(from), x1 = sl_value(to);
     turn ^= 1;
     if (tid == 0) sh.bag[turn ^ 1] = 0;
-    row.groups([&](const float* v, int) {
-      bool any = false;
+    // first the groups that may have one: within half the range of its middle and some more
+    const float mid = 0.5f * x0 + 0.5f * x1, reach = (x1 - x0) * 0.5000002f + (fabsf(x0) + fabsf(x1)) * 1e-6f;
+    const auto near = [&](const float* v) {
+      float d = fabsf(v[0] - mid);
 #pragma unroll
-      for (int e = 0; e < NE; ++e) any = any || (v[e] >= x0 && v[e] <= x1);
-      if (any) {
+      for (int e = 1; e < NE; ++e) d = fminf(d, fabsf(v[e] - mid));
+      return d <= reach;
+    };
+    const auto take = [&](const float* v) {
+      int some = 0;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) some += v[e] >= x0 && v[e] <= x1;
+      if (some) {
+        int p = atomicAdd(&sh.bag[turn], some);
 #pragma unroll
         for (int e = 0; e < NE; ++e)
           if (v[e] >= x0 && v[e] <= x1) {
-            const int p = atomicAdd(&sh.bag[turn], 1);
-            if (p < SL_CAP) sh.x[p] = v[e] + 0.f;
+            if (p < SL_CAP) sh.list[p].x = v[e] + 0.f;
+            ++p;
           }
       }
-    });
+    };
+    row.groups_with(near, [&](const float* v, int) { take(v); });
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(sh.bag[turn]);
   };
@@ -619,27 +647,25 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   double part = by_p ? share : -1.0;     // of the mass, while that is not known
   if (n > SL_CAP && by_k) {
     // many equal values, or many to keep: the k-th largest itself
-    if (sl_first<false>(row, wt, sp, -1.0, floor, sh)) thr = max(thr, sl_select<false>(row, wt, sp, -1.0, sh));
+    if (sl_first<false>(row, wt, sp, -1.0, floor, sh)) thr = max(thr, sl_select<false>(row, wt, sp, -1.0, GRAIN, sh));
     ranked = true;
     from = thr;
     n = count(from);
   }
   bool rest = n > SL_CAP;                // not all that is kept is listed
   if (rest && by_p) {
-    // all weights in bins; then what is kept, or at least what one bin holds, may fit the list
+    // all weights in bins; then few threads have what is kept, or what one bin holds is listed
     sp = SlPart{thr, kmax, 0, 0, sp.turn};
     sl_first<true>(row, wt, sp, share, floor, sh);
     part = -1.0;
     from = sp.lo;
     n = few_of(from);
-    listed = n >= 0;
-    if (!listed) n = count(from);
-    rest = n > SL_CAP;
+    listed = true;
+    rest = n < 0;
     if (rest) {
-      listed = true;
       n = 0;                             // none where one word is left
-      while (sp.lo != sp.hi && (n = bag_of(sp.lo, sp.hi)) > SL_CAP) sl_round<true>(row, wt, sp, -1.0, sh);
-      if (sp.lo == sp.hi) n = 0;
+      while (sp.hi - sp.lo > GRAIN && (n = bag_of(sp.lo, sp.hi)) > SL_CAP) sl_round<true>(row, wt, sp, -1.0, sh);
+      if (sp.hi - sp.lo <= GRAIN) n = 0;
     }
   } else if (rest) {
     n = 0;
@@ -663,8 +689,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 #pragma unroll
       for (int e = 0; e < NE; ++e)
         if (v[e] >= x0) {
-          sh.x[p] = v[e] + 0.f;
-          sh.idx[p] = row.index(g, e);
+          sh.list[p] = make_float2(v[e] + 0.f, __int_as_float(row.index(g, e)));
           ++p;
         }
     };
@@ -674,20 +699,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       for (int e = 1; e < NE; ++e) top = fmaxf(top, v[e]);
       return top >= x0;
     };
-    if constexpr (NJ > 0) {   // the groups with an entry first: a branch on a vector's result waits for it
-      uint32_t hit = 0;
-      row.groups([&](const float* v, int g) { hit |= some(v) ? 1u << (g - row.g0) : 0; });
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) hit |= __shfl_xor(hit, o, 64);
-      hit = __builtin_amdgcn_readfirstlane(hit);
-      row.groups([&](const float* v, int g) {
-        if (hit >> (g - row.g0) & 1) write(v, g);
-      });
-    } else {
-      row.groups([&](const float* v, int g) {
-        if (__any(some(v))) write(v, g);
-      });
-    }
+    row.groups_with(some, write);
     __syncthreads();
   }
 
@@ -706,7 +718,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     for (int i = 0; i < N; ++i) {
       const int j = lane * per + i;
       const bool real = i < per && j < n;
-      x[i] = real ? sh.x[j] : -INFINITY;
+      x[i] = real ? sh.list[j].x : -INFINITY;
       keys[i] = real ? sl_key(x[i]) : 0;
     }
     if (!ranked && n >= k && per == 1) {   // an entry's rank by the others, one by one
@@ -716,7 +728,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       thr = max(thr, __ockl_wfred_min_u32(lane < n && rank < (uint32_t)k ? keys[0] : 0xffffffffu));
     } else if (!ranked && n >= k) {   // else all of them are among the k
       uint32_t lo = from, hi = kmax;
-      while (lo < hi) {
+      while (hi - lo > GRAIN) {
         const uint32_t mid = hi - ((hi - lo) >> 1);
         int c = 0;
 #pragma unroll
@@ -747,7 +759,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
         }
         lo = hi = __ockl_wfred_min_u32(w[0] && above < want ? keys[0] : 0xffffffffu);
       }
-      while (lo < hi) {
+      while (hi - lo > GRAIN) {
         const uint32_t mid = hi - ((hi - lo) >> 1);
         sl_u64 c = 0;
 #pragma unroll
@@ -771,7 +783,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       for (int i = 0; i < N; ++i) {
         run += w[i];
         if (w[i] && id < 0 && target < (double)run) {
-          id = sh.idx[lane * per + i];
+          id = __float_as_int(sh.list[lane * per + i].y);
           drawn = x[i];
         }
       }
@@ -783,17 +795,17 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 #pragma unroll
       for (int i = 0; i < SL_PER; ++i) {
         const int j = tid * per + i;
-        list.v[i] = i < per && j < n ? sh.x[j] : -INFINITY;
+        list.v[i] = i < per && j < n ? sh.list[j].x : -INFINITY;
         list.w[i] = i < per ? wt(list.v[i]) : 0;
         __builtin_amdgcn_sched_barrier(0);
       }
       if (!ranked) {
         SlPart q{from, kmax, 0, (sl_u64)k, sp.turn};
-        thr = max(thr, sl_select<false>(list, wt, q, -1.0, sh));
+        thr = max(thr, sl_select<false>(list, wt, q, -1.0, GRAIN, sh));
         sp.turn = q.turn;
         sp.lo = max(sp.lo, thr);
       }
-      if (by_p) thr = max(thr, sl_select<true>(list, wt, sp, part, sh));
+      if (by_p) thr = max(thr, sl_select<true>(list, wt, sp, part, GRAIN, sh));
       if (!rest) {
         // ---- the draw from the list
         sl_u64 sum = 0, ex;
@@ -810,7 +822,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
           for (int i = 0; i < SL_PER; ++i) {
             ex += list.w[i];
             if (list.w[i] && id < 0 && target < (double)ex) {
-              id = sh.idx[tid * per + i];
+              id = __float_as_int(sh.list[tid * per + i].y);
               drawn = list.v[i];
             }
           }
@@ -892,6 +904,9 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 
 template <typename T, int NJ>
 static hipError_t sl_launch(const SlArgs& a, hipStream_t st) {
+  static PerDevice limit;
+  const hipError_t e = lds_limit(limit, (const void*)k_sample_logits<T, NJ>, sizeof(SlShared));
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_sample_logits<T, NJ>), dim3((unsigned)a.r.rows), dim3(SL_NT), sizeof(SlShared), st, a);
   return hipGetLastError();
 }
