@@ -230,10 +230,10 @@ struct PaRow {
 };
 template <int WHO>
 __device__ __forceinline__ PaRow pa_place(const PaArgs& a, const PaSeq& q, int s, int kvh, int row,
-                                          int part) {
+                                          int part, const int* token = nullptr, int tok0 = 0) {
   PaRow r;
   const int tok = q.by.div(row);
-  r.n = q.first + tok;
+  r.n = WHO == PA_PRE ? token[tok - tok0] : q.first + tok;
   r.h = kvh * q.G + row - tok * q.G;
   const long long slot = WHO == PA_FEW && a.packed ? ((long long)s * a.c.heads + kvh) * 16 + row
                                                    : (long long)r.n * a.heads + r.h;
@@ -260,12 +260,10 @@ __device__ __forceinline__ void pa_store4(const PaArgs& a, const PaRow& w, int p
 
 // A row at entry e formed entry by entry, over the part [a0, b0) of what it sees.
 template <int DH, int WHO>
-__device__ __forceinline__ void pa_again(const PaArgs& a, const PaSeq& q, int s,
-                                         const int32_t* table, int kvh, int row, int e, int a0,
-                                         int b0, int part, int parts) {
+__device__ __forceinline__ void pa_again(const PaArgs& a, const PaRow& w, const int32_t* table, int kvh,
+                                         int e, int a0, int b0, int parts) {
   constexpr int DL = DH / 64;
   const int lane = threadIdx.x & 63;
-  const PaRow w = pa_place<WHO>(a, q, s, kvh, row, part);
   const int lo = max(a0, e < a.window ? 0 : e - a.window + 1), hi = min(b0, e + 1);
   float m, l, o[DL];
   pa_row<DH>(a.c, table, a.q + w.n * a.qt + w.h * a.qh, kvh, lo, hi, a.ssl2, m, l, o);
@@ -576,7 +574,8 @@ __device__ __forceinline__ void pa_few(const PaArgs& a, int s, int row0, int kvh
   }
   for (int r = wv; r < nrow; r += NW)
     if (s_bad[r])
-      pa_again<DH, PA_FEW>(a, q, s, table, kvh, row0 + r, q.e0 + q.by.div(row0 + r), a0, b0, part, parts);
+      pa_again<DH, PA_FEW>(a, pa_place<PA_FEW>(a, q, s, kvh, row0 + r, part), table, kvh,
+                           q.e0 + q.by.div(row0 + r), a0, b0, parts);
 }
 
 // Work-groups past the sequences' take the sixteens of rows behind a sequence's first:
@@ -602,30 +601,47 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_few(PaArgs a, int blocks) 
   pa_few<DH, NW>(a, s, row0, blockIdx.x % a.c.heads, blockIdx.x / a.c.heads, pa_smem);
 }
 
-// The entries of a group's tokens n0 .. n0 + n - 1 (n <= cap) to LDS, -1 for those of
-// sequences with many rows, by a whole work-group; the entries lo .. hi - 1 that any of
-// them may see (hi 0: none sees one).
-__device__ __forceinline__ void pa_entries(const PaArgs& a, int g, int n0, int n, int cap, int* entry,
-                                           int& lo, int& hi) {
-  const int tid = threadIdx.x, lane = tid & 63;
+// The tokens of a group's sequences with few rows, one behind the other: of those from
+// number t0 on the call's row and the entry, to LDS (n <= 64 of them, 64 + 64 + 4 words), and
+// the entries lo .. hi - 1 that any of them may see (hi 0: none sees one), by a whole
+// work-group.  How many tokens there are.
+__device__ __forceinline__ int pa_tokens(const PaArgs& a, int g, int t0, int* lds, int& lo, int& hi) {
+  int* token = lds;
+  int* entry = lds + 64;
+  int* part = lds + 128;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const PgRange seqs = pg_range(a.groups[g], a.groups[g + 1], a.c.seqs);
-  n = min(n, cap);
-  for (int i = tid; i < cap; i += blockDim.x) entry[i] = -1;
-  __syncthreads();
-  for (int i = tid; i < seqs.n; i += blockDim.x) {
-    const int s = seqs.first + i;
-    const PgRange r = pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows);
-    if (r.n * (long long)a.G > a.few) continue;
-    const int e0 = pg_len(a.c.lens[s], a.c.cols, a.c.sh) - r.n - r.first;   // + a row: its entry
-    for (int t = max(r.first, n0); t < min(r.first + r.n, n0 + n); ++t) entry[t - n0] = max(e0 + t, -1);
+  if (tid < 64) entry[tid] = -1;
+  int all = 0;
+  for (int i0 = 0; i0 < seqs.n; i0 += 256) {
+    const int s = seqs.first + i0 + tid;
+    PgRange r = {0, 0};
+    int len = 0;
+    if (i0 + tid < seqs.n) {
+      len = a.c.lens[s];
+      r = pg_range(a.c.starts[s], a.c.starts[s + 1], a.c.rows);
+      if (r.n * (long long)a.G > a.few) r.n = 0;
+    }
+    int sum = r.n;   // of this thread's sequence and the wave's before it
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    __syncthreads();
+    if (lane == 63) part[wv] = sum;
+    __syncthreads();
+    int at = all + sum - r.n;
+    for (int w = 0; w < wv; ++w) at += part[w];
+    all += part[0] + part[1] + part[2] + part[3];
+    const int e0 = pg_len(len, a.c.cols, a.c.sh) - r.n;
+    for (int i = max(0, t0 - at); i < min(r.n, t0 + 64 - at); ++i) {
+      token[at + i - t0] = r.first + i;
+      entry[at + i - t0] = max(e0 + i, -1);
+    }
   }
   __syncthreads();
-  int most = -1, least = 0x7fffffff;
-  for (int i = lane; i < n; i += 64) {
-    const int e = entry[i];
-    most = max(most, e);
-    if (e >= 0) least = min(least, e);
-  }
+  int most = entry[lane], least = most >= 0 ? most : 0x7fffffff;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     most = max(most, __shfl_xor(most, d, 64));
@@ -635,6 +651,7 @@ __device__ __forceinline__ void pa_entries(const PaArgs& a, int g, int n0, int n
   least = __builtin_amdgcn_readfirstlane(least);
   lo = least < a.window ? 0 : least - a.window + 1;
   hi = most + 1;
+  return __builtin_amdgcn_readfirstlane(all);
 }
 
 // ---- sequences of many rows -----------------------------------------------------------
@@ -668,7 +685,8 @@ template <int DH, int BK>
 constexpr size_t pa_many_lds() { return (size_t)2 * (PM_AHEAD + 1) * BK * DH * 2; }
 template <int DH, int BK, int QB, bool PRE = false>
 __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int part,
-                                        unsigned char* smem, int* entry = nullptr) {
+                                        unsigned char* smem, int* lds = nullptr) {
+  static_assert(!PRE || QB == 1, "64 tokens");
   constexpr int WHO = PRE ? PA_PRE : PA_MANY;
   constexpr int BR = 64 * QB, RB = DH * 2, TB = BK * RB;
   constexpr int LPW = TB / 1024 / 4, RPL = 1024 / RB;   // loads a wave makes of K (and of V), rows of each
@@ -683,20 +701,23 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
                         : pg_tile(a.c.starts, a.c.lens, a.c.seqs, a.c.rows, a.G, a.few, BR, tile);
   if (pl.seq < 0) return;
   const int s = __builtin_amdgcn_readfirstlane(pl.seq), row0 = __builtin_amdgcn_readfirstlane(pl.row0);
-  const PaSeq q = pa_seq(a, pl.r, pl.len);
-  const int nrow = min(BR, q.rows - row0);
+  PaSeq q = pa_seq(a, pl.r, pl.len);
   const int tok0 = q.by.div(row0);
+  const int* token = lds;
+  const int* entry = lds + 64;
   int lo, hi;
   PaParts pt;
   if constexpr (PRE) {
     const int shared = pg_len(a.plens[s], a.pcols, a.c.sh);
     pt = pa_parts(0, shared, a.sp_pre);
     if (shared == 0 || part >= pt.n) return;
-    pa_entries(a, s, q.first + tok0, q.by.div(row0 + nrow - 1) - tok0 + 1, 64 * QB, entry, lo, hi);
-    if (hi == 0) return;   // none of its rows are few: the same for all waves
+    // rows of a group: those of its sequences with few, of which there may be fewer tiles
+    q.n = pa_tokens(a, s, tok0, lds, lo, hi);
+    q.rows = q.n * q.G;
+    if (hi == 0 || row0 >= q.rows) return;   // the same for all waves
     hi = min(hi, shared);
   } else {
-    pa_span(q, row0, nrow, a.window, lo, hi);
+    pa_span(q, row0, min(BR, q.rows - row0), a.window, lo, hi);
     pt = pa_parts(lo, hi, a.sp_many);
     if (part >= pt.n) return;
   }
@@ -719,7 +740,8 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
     const int row = min(wr0 + 16 * b + r16, last), tok = q.by.div(row);
     if constexpr (PRE) e[b] = entry[tok - tok0];
     else e[b] = q.e0 + tok;
-    const bf16_t* qr = a.q + (q.first + tok) * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
+    const int n = PRE ? token[tok - tok0] : q.first + tok;
+    const bf16_t* qr = a.q + n * a.qt + (kvh * q.G + row - tok * q.G) * a.qh + g4 * 8;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qf[b][ks] = pa_signed(qr + ks * 32, a.keep, a.flip);
   }
@@ -881,7 +903,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
       constexpr int x = decltype(xc)::value, ks = x / NBLK, i = x % NBLK;
       kf[x] = pa_rd_b128<KO + i * 16 * RB>(kadr[ks]);
     });
-    uint32_t pw[QB][NBLK][2];
+    uint32_t pw[QB][NBLK][2], pl[PRE ? QB : 1][NBLK][2];   // the weights in bf16, and (PRE) what that leaves of them
     pa_static_for<0, KG>([&](auto xc) __attribute__((always_inline)) {
       constexpr int x = decltype(xc)::value, ks = x / NBLK, i = x % NBLK, vi = x / NDB, db = x % NDB;
       pa_wait_lgkm<(x < 4 ? 3 + 2 * x : 15 - x)>(kf[x]);
@@ -902,7 +924,12 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
           const float v = __builtin_amdgcn_exp2f(s0[b][k / 4][k % 4] * a.sl2 - msl[b]);
           s0[b][k / 4][k % 4] = v;
           lsum[b] += v;
-          if (k % 2 == 1) pw[b][k / 4][(k % 4) / 2] = pack2(s0[b][k / 4][k % 4 - 1], v);
+          if (k % 2 == 1) {
+            const float u = s0[b][k / 4][k % 4 - 1];
+            const uint32_t w = pack2(u, v);
+            pw[b][k / 4][(k % 4) / 2] = w;
+            if constexpr (PRE) pl[b][k / 4][(k % 4) / 2] = pack2(u - lo_f(w), v - hi_f(w));
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -915,6 +942,10 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
       for (int b = 0; b < QB; ++b) {
         const uint32_t w4[4] = {pw[b][2 * i][0], pw[b][2 * i][1], pw[b][2 * i + 1][0], pw[b][2 * i + 1][1]};
         o[b][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *(const bf16x8_t*)w4, o[b][db], 0, 0, 0);
+        if constexpr (PRE) {
+          const uint32_t l4[4] = {pl[b][2 * i][0], pl[b][2 * i][1], pl[b][2 * i + 1][0], pl[b][2 * i + 1][1]};
+          o[b][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *(const bf16x8_t*)l4, o[b][db], 0, 0, 0);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -955,7 +986,7 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const int row = wr0 + 16 * b + r16;
-    const PaRow w = pa_place<WHO>(a, q, s, kvh, min(row, last), part);
+    const PaRow w = pa_place<WHO>(a, q, s, kvh, min(row, last), part, token, tok0);
     float l = lsum[b];
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -973,8 +1004,9 @@ __device__ __forceinline__ void pa_many(const PaArgs& a, int tile, int kvh, int 
     while (bad) {
       const int r = __builtin_ctzll(bad);
       bad &= bad - 1;
-      pa_again<DH, WHO>(a, q, s, table, kvh, wr0 + 16 * b + r, PRE ? __shfl(e[b], r, 64) : q.e0 + q.by.div(wr0 + 16 * b + r),
-                        a0, b0, part, parts);
+      const int row = wr0 + 16 * b + r;
+      pa_again<DH, WHO>(a, pa_place<WHO>(a, q, s, kvh, row, part, token, tok0), table, kvh,
+                        PRE ? __shfl(e[b], r, 64) : q.e0 + q.by.div(row), a0, b0, parts);
     }
   }
 }
@@ -1330,7 +1362,7 @@ __device__ __forceinline__ PsTile ps_tile(int L, int full, int pairs) {
 }
 
 template <int DH, int QB>
-__global__ __launch_bounds__(256, 2) void k_paged_shared(PaArgs a, PsGrid g) {
+__global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void k_paged_shared(PaArgs a, PsGrid g) {
   constexpr int BK = DH == 64 ? 64 : 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char pa_smem[];
   const int heads = a.c.heads;
@@ -1343,7 +1375,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_shared(PaArgs a, PsGrid g) {
   L -= g.many;
   if (L < g.pre) {
     const PsTile t = ps_tile(L, g.pre_full, heads * a.sp_pre.most);
-    pa_many<DH, BK, QB, true>(a, t.tile, t.w % heads, t.w / heads, pa_smem,
+    pa_many<DH, BK, 1, true>(a, t.tile, t.w % heads, t.w / heads, pa_smem,
                               (int*)(pa_smem + pa_many_lds<DH, BK>()));
     return;
   }
@@ -1437,40 +1469,66 @@ __global__ __launch_bounds__(256) void k_shared_join(PaArgs a, int groups, int w
 }
 
 struct PsPlan {
-  int qb;
+  int qb;              // row blocks of the tiles of many tokens; those of a prefix have one
   PsGrid grid;
   PaSplit pre, few, many;
 };
+// Whether reading a prefix once saves what the join and the parts cost: where that is
+// 48 MB of keys and values or more, as the tables' widths have it (us with and without:
+// 8 sequences of 6 heads of 128 behind 1000 entries, 21 MB, 13.8 and 11.8; 90 of 3 heads of 64 behind
+// 500, 34 MB, 12.6 and 9.6; 2 behind 16000, 49 MB, 24.3 and 27.6; 32 behind 2048, 195 MB, 15.7 and 28.0).
+static bool ps_worth(const PagedArgs& c, const SharedPrefix& x, int Dh) {
+  const double again = (double)(c.seqs - x.ngroups) * (double)((long long)x.cols << c.sh);
+  return x.ngroups > 0 && again * c.heads * Dh * 4 >= 48e6;
+}
 static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
   static const int cus = device_cus();
   PsPlan p{};
-  const int G = heads / c.heads;
+  const int G = heads / c.heads, step = Dh == 64 ? 64 : 32;
   const long long rows = (long long)c.rows * G, pairs = (long long)c.seqs * c.heads;
   const auto clamp = [](long long v, long long hi) { return (int)(v < 1 ? 1 : v > hi ? hi : v); };
   // sequences of many tokens, of which a call may have none, as in other calls
   const PaPlan whole = pa_plan(c, heads, Dh, window);
   const bool many = c.rows > PS_TOKENS;
   p.many = whole.many ? whole.sp_many : PaSplit{1, 1};
-  const int groups = x.ngroups < 1 ? 1 : x.ngroups < c.rows ? x.ngroups : c.rows;
-  p.qb = whole.many ? whole.qb : rows / groups > 64 ? 2 : 1;
-  const int br = 64 * p.qb;
+  // tiles of 64 rows at head dim 64, three on a CU (24 sequences, a third of one token and the others of up
+  // to 300, of 8 heads behind two prefixes of 4096: 63.5 us; 69.3 by 128 rows, two on a CU)
+  p.qb = whole.many && Dh == 128 ? whole.qb : 1;
+  const int br = 64 * p.qb, groups = x.ngroups < c.rows ? x.ngroups : c.rows;
   p.grid.many_full = clamp(rows / br, 1 << 30);
-  p.grid.pre_full = p.grid.many_full;
-  const long long tiles = rows / br + groups, width = (long long)x.cols << c.sh;
-  // two work-groups a CU, of 128 entries at least
-  p.pre.split = clamp(2LL * cus / (tiles * c.heads), clamp((width + 127) / 128, PS_PRE));
-  const long long own = (long long)c.cols << c.sh;
+  p.grid.pre_full = clamp(rows / 64, 1 << 30);
+  const long long tiles = rows / 64 + groups, width = (long long)x.cols << c.sh, own = (long long)c.cols << c.sh;
+  const long long slot = (long long)(Dh + 2) * sizeof(float) * c.rows * heads;   // a part of every row
+  // Parts of a prefix: the fewest that keep its work-groups from being the last, by a step's time
+  // (as in pa_plan), 6 us around them, what memory takes for all entries anyway, and the parts' way
+  // to memory and back.  us measured in 1, 2, 4, 8, 16, 32 parts: 64 sequences of 12 heads of 128
+  // behind 8192 entries 130 / 73 / 45 / 33 / 37 / 43; 48 of 4 tokens, 8 heads on 2, four
+  // prefixes of 3001, 54 / 35 / 26 / 24 / 28 / 36; 16, 8 heads on 2, 16384 entries 242 / 128 / 70 / 43 / 30 / 25.
+  const bool h = Dh == 64;
+  const float alone = h ? 0.5f : 0.475f, both = h ? 0.86f : 0.68f;
+  const double behind = own > width ? (double)(own - width) * c.seqs : 0.0;
+  const float memory = (float)(((double)width * groups + behind) * c.heads * Dh * 4 / 5.1e6);
+  float best = 0.f;
+  for (const int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48}) {
+    if (n > 1 && (width / n < 128 || slot * n > (long long)PA_WS_MAX)) break;
+    const int each = (int)((tiles * c.heads * n + cus - 1) / cus);
+    const float steps = (float)((width + (long long)step * n - 1) / ((long long)step * n));
+    const float walk = 6.f + steps * ((float)(each / 2) * both + (float)(each % 2) * alone);
+    const float us = (walk > memory ? walk : memory) + (float)slot * (float)n * 2.5f / 4e6f;
+    if (best == 0.f || us < best) {
+      best = us;
+      p.pre = {n, n};
+    }
+  }
   p.few.split = pairs >= cus ? 1 : clamp(2LL * cus / pairs, clamp((own + 127) / 128, PS_OWN));
   p.few.most = clamp((own + 4095) / 4096, PS_OWN);
   if (p.few.most < p.few.split) p.few.most = p.few.split;
-  const long long slot = (long long)(Dh + 2) * sizeof(float) * c.rows * heads;   // a part of every row
-  p.pre.split = p.pre.most = clamp((long long)PA_WS_MAX / slot, p.pre.split);
   p.few.most = clamp((long long)PA_WS_MAX / slot, p.few.most);
   if (p.few.split > p.few.most) p.few.split = p.few.most;
   const long long more = (rows - 1) / 16, each = (long long)c.seqs * (G - 1);
   p.grid.by_seq = each < more;
   const long long blocks[3] = {many ? (rows / br + c.rows / (PS_TOKENS + 1)) * c.heads * p.many.most : 0,
-                               x.ngroups > 0 ? tiles * c.heads * p.pre.most : 0,
+                               tiles * c.heads * p.pre.most,
                                (c.seqs + (each < more ? each : more)) * c.heads * p.few.most};
   if (blocks[0] + blocks[1] + blocks[2] >= 1LL << 24) return p;   // 2^32 threads: refused by its grid of none
   p.grid.many = (int)blocks[0];
@@ -1489,17 +1547,18 @@ static PsSlots ps_slots(const PagedArgs& c, int heads, const PsPlan& p) {
 
 size_t paged_attention_shared_ws_bytes(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
   if (c.rows == 0 || c.seqs == 0) return 0;
+  if (!ps_worth(c, x, Dh)) return paged_attention_ws_bytes(c, heads, Dh, window);
   const PsSlots n = ps_slots(c, heads, ps_plan(c, x, heads, Dh, window));
   return (n.pre + n.few + n.many) * (Dh + 2) * sizeof(float);
 }
 
 template <int DH>
 static hipError_t ps_launch(const PaArgs& a, const PsPlan& p, hipStream_t st) {
-  constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>() + 128 * sizeof(int), f = pa_few_lds<DH, 4>();
+  constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>() + 132 * sizeof(int), f = pa_few_lds<DH, 4>();
   const size_t lds = f > m ? f : m;
   const dim3 grid((unsigned)(p.grid.many + p.grid.pre + p.grid.few));
   if (grid.x == 0) return hipErrorInvalidConfiguration;
-  if (p.qb == 2) hipLaunchKernelGGL((k_paged_shared<DH, 2>), grid, dim3(256), lds, st, a, p.grid);
+  if (DH == 128 && p.qb == 2) hipLaunchKernelGGL((k_paged_shared<128, 2>), grid, dim3(256), lds, st, a, p.grid);
   else hipLaunchKernelGGL((k_paged_shared<DH, 1>), grid, dim3(256), lds, st, a, p.grid);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -1514,6 +1573,7 @@ hipError_t paged_attention_shared(const PagedArgs& c, const SharedPrefix& x, con
                                   long long qh, int heads, int Dh, float scale, int window, bf16_t* out,
                                   float* lse, void* ws, hipStream_t st) {
   if (c.rows == 0 || c.seqs == 0) return hipSuccess;
+  if (!ps_worth(c, x, Dh)) return paged_attention(c, q, qt, qh, heads, Dh, scale, window, out, lse, ws, st);
   const PsPlan p = ps_plan(c, x, heads, Dh, window);
   PaArgs a = pa_args(c, q, qt, qh, heads, scale, window, out, lse);
   a.sp_few = p.few;

@@ -70,6 +70,15 @@ class Setup:
         self.q = (q / torch.sqrt((q * q).mean(-1, keepdim=True))).to(BF)
         self.layout = layout
 
+    def widened(self):
+        """Tables of prefixes so wide that the call shares them, however short they are."""
+        again = max(1, len(self.lens) - len(self.plens)) * self.Hk * self.D * 4
+        cols = max(self.pcols, -(-48_100_000 // (again * self.page)))
+        wide = torch.full((len(self.plens), cols), -1, dtype=I32)
+        wide[:, :self.pcols] = self.ptable
+        self.ptable = wide
+        return self
+
     def cache(self, x):
         x = x.cuda()
         if self.layout == "slots":      # (pages, page, heads, dim) underneath
@@ -129,13 +138,15 @@ def _check(s, got, lse, scale, window, out=None):
     assert ((lse[:end] - rlse[:end]).abs()[~empty] <= ltol[:end][~empty]).all()
 
 
-@pytest.mark.parametrize("scale", [0.1, -1.5, 0.0])
+@pytest.mark.parametrize("wide,scale", [(True, 0.1), (True, -1.5), (True, 0.0), (False, 0.1)])
 @pytest.mark.parametrize("i", range(len(CASES)))
-def test_attention_shared(i, scale):
+def test_attention_shared(i, wide, scale):
     from attention_nn_amd import paged
     case = dict(CASES[i])
     window = case.pop("window", 0)
     s = Setup(seed=i, **case)
+    if wide:
+        s.widened()
     kc, vc, table, starts, lens, groups, pt, pl = s.dev()
     out = torch.full((s.N, s.H, s.D), 7.0, dtype=BF, device="cuda")
     got, lse = paged.attention_shared(s.q.cuda(), kc, vc, table, starts, lens, groups, pt, pl, scale, window, True, out)
@@ -173,7 +184,7 @@ def test_lengths_and_groups_outside():
     """Sequences shorter than their prefix or out of every range, prefixes past their
     table, ids that are no page: the entries that there are, and nothing past the pool."""
     from attention_nn_amd import paged
-    s = Setup([(64, _one(1, 10, 10, 10, 10)), (64, _one(2, 10, 10))], H=2, Hk=2)
+    s = Setup([(64, _one(1, 10, 10, 10, 10)), (64, _one(2, 10, 10))], H=2, Hk=2).widened()
     s.k, s.v = torch.nan_to_num(s.k, 1.0), torch.nan_to_num(s.v, 2.0, 2.0, 2.0)
     kc, vc, table, starts, lens, groups, pt, pl = s.dev()
     s.lens = [30, 64, 65, -7, 1, 3]      # inside the prefix, at its end, empty, and fewer than there are tokens
@@ -183,7 +194,11 @@ def test_lengths_and_groups_outside():
     s.lens = [10 ** 9] * 6               # the table's end
     lens = torch.tensor(s.lens, dtype=I32, device="cuda")
     s.table[s.table < 0] = 0
-    big = torch.tensor([2 ** 31 - 1, 64], dtype=I32, device="cuda")
+    got, lse = paged.attention_shared(s.q.cuda(), kc, vc, table, starts, lens, groups, pt, pl, 0.1, want_lse=True)
+    _check(s, got, lse, 0.1, 0)
+    big = torch.tensor([2 ** 31 - 1, 10 ** 6], dtype=I32, device="cuda")
+    s.lens = [64, 63, 64, 2, 64, 60]     # prefixes that pass their table and the sequences' ends
+    lens = torch.tensor(s.lens, dtype=I32, device="cuda")
     got, lse = paged.attention_shared(s.q.cuda(), kc, vc, table, starts, lens, groups, pt, big, 0.1, want_lse=True)
     _check(s, got, lse, 0.1, 0)
     for bad in ([-5, 4, 9], [0, 4, 2 ** 31 - 1], [3, 1, 0], [2 ** 31 - 1, -1, 5]):
@@ -199,7 +214,7 @@ def test_lengths_and_groups_outside():
 def test_what_is_not_finite_reaches_only_those_that_see_it(where, bad):
     """A value of one entry that some rows of a tile do not see, by their window or their length."""
     from attention_nn_amd import paged
-    s = Setup([(100, [(4, 20), (1, 3), (1, 60), (9, 9)])], H=4, Hk=2, page=32)
+    s = Setup([(100, [(4, 20), (1, 3), (1, 60), (9, 9)])], H=4, Hk=2, page=32).widened()
     window = 50
     e = 80 if where == "prefix" else 103
     for t in range(4):
@@ -220,7 +235,7 @@ def test_rows_of_equal_maximum_and_far_scores():
     """Scores that differ by far between prefix and own entries, in both directions."""
     from attention_nn_amd import paged
     for sign in (1.0, -1.0):
-        s = Setup([(70, _one(1, 9, 30))], H=2, Hk=2)
+        s = Setup([(70, _one(1, 9, 30))], H=2, Hk=2).widened()
         for t in range(2):
             s.k[s.ptable[0].long()] = (s.q[t].float().mean(0) * 0 + 0.1).to(BF)
         s.k = torch.nan_to_num(s.k, 0.0)
@@ -242,7 +257,7 @@ def test_rows_of_equal_maximum_and_far_scores():
 
 def test_strided_queries_streams_and_graph():
     from attention_nn_amd import paged
-    s = Setup([(200, _one(1, *[70] * 9)), (33, _one(1, *[70] * 5))], H=4, Hk=2, page=32)
+    s = Setup([(200, _one(1, *[70] * 9)), (33, _one(1, *[70] * 5))], H=4, Hk=2, page=32).widened()
     kc, vc, table, starts, lens, groups, pt, pl = s.dev()
     wide = torch.full((s.N, 2 * s.H + 3, s.D), math.nan, dtype=BF, device="cuda")
     q = wide[:, 1:1 + 2 * s.H:2]
@@ -253,7 +268,7 @@ def test_strided_queries_streams_and_graph():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     odd = torch.zeros(s.N * s.H * s.D + 3, dtype=BF, device="cuda")[3:].view(s.N, s.H, s.D)
     odd.copy_(s.q)
-    wpt = torch.full((2, 2 * s.pcols), -1, dtype=I32, device="cuda")[:, ::2]
+    wpt = torch.full((2, 2 * s.ptable.shape[1]), -1, dtype=I32, device="cuda")[:, ::2]
     wpt.copy_(s.ptable)
     got = paged.attention_shared(odd, kc, vc, table, starts, lens, groups, wpt, pl, 0.1)
     assert torch.equal(got, want[0])
