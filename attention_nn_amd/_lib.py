@@ -167,7 +167,7 @@ SIGNATURES = {
                                            _L, _P, _L, _P, _SZ, _P]),
     "ann_op_paged_evict": (ctypes.c_int, [ctypes.POINTER(AnnPaged), _P, _L, _I, _P, _L, _I, _I, _P,
                                           _P, _P, _L, _P]),
-    "ann_op_paged_assign_ws_bytes": (_SZ, [ctypes.POINTER(AnnPagedTable)]),
+    "ann_op_paged_assign_ws_bytes": (_SZ, [ctypes.POINTER(AnnPagedTable), _I]),
     "ann_op_paged_assign": (ctypes.c_int, [ctypes.POINTER(AnnPagedTable), _P, _I, _P, _P, _P, _P, _P, _P,
                                            _SZ, _P]),
     "ann_op_paged_release": (ctypes.c_int, [ctypes.POINTER(AnnPagedTable), _P]),

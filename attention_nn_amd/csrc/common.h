@@ -42,6 +42,31 @@ __device__ __forceinline__ void st_once(void* p, const uint4& w) {
   __builtin_nontemporal_store(__builtin_bit_cast(uint4_hw, w), (uint4_hw*)p);
 }
 
+// Sums over the lanes up to this one, in 32 or 64 bits, by row shifts and broadcasts of the
+// vector unit.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_shift(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_shift(unsigned long long v) {
+  return (unsigned long long)dpp_shift<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_shift<CTRL, ROWS>((uint32_t)v);
+}
+template <typename N>
+__device__ __forceinline__ N wave_scan(N v) {
+  v += dpp_shift<0x111, 0xf>(v);   // by 1, 2, 4, 8 within a row of 16
+  v += dpp_shift<0x112, 0xf>(v);
+  v += dpp_shift<0x114, 0xf>(v);
+  v += dpp_shift<0x118, 0xf>(v);
+  v += dpp_shift<0x142, 0xa>(v);   // lane 15 to the second row, 47 to the fourth
+  v += dpp_shift<0x143, 0xc>(v);   // lane 31 to the third and fourth
+  return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int lane) {
+  return (unsigned long long)lane_of((uint32_t)(v >> 32), lane) << 32 | lane_of((uint32_t)v, lane);
+}
+
 template <int W>
 __device__ __forceinline__ float group_sum(float v) {
   // butterfly over groups of W consecutive lanes (W a power of two <= 64)

@@ -1475,9 +1475,11 @@ int ann_op_paged_evict(const ann_paged* c, const int32_t* out_table, int64_t out
   return ANN_OK;
 }
 
-size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t) {
+size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t, int32_t rows) {
   TableArgs a{};
-  return table_args(t, &a) ? 0 : table_assign_ws_bytes(a);
+  if (table_args(t, &a) || rows < 0) return 0;
+  a.rows = rows;
+  return table_assign_ws_bytes(a);
 }
 
 int ann_op_paged_assign(const ann_paged_table* t, const int32_t* new_tokens, int32_t rows, int32_t* starts,

@@ -64,40 +64,16 @@ __device__ __forceinline__ float sl_number(float x) { return x == x ? x + 0.f : 
 extern "C" __device__ unsigned __ockl_wfred_max_u32(unsigned);
 extern "C" __device__ unsigned __ockl_wfred_min_u32(unsigned);
 
-// Sums over the lanes up to this one, by row shifts and broadcasts of the vector unit.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t sl_dpp(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ sl_u64 sl_dpp(sl_u64 v) {
-  return (sl_u64)sl_dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | sl_dpp<CTRL, ROWS>((uint32_t)v);
-}
-template <typename N>
-__device__ __forceinline__ N sl_wave_scan(N v) {
-  v += sl_dpp<0x111, 0xf>(v);   // shifts by 1, 2, 4, 8 within a row of 16
-  v += sl_dpp<0x112, 0xf>(v);
-  v += sl_dpp<0x114, 0xf>(v);
-  v += sl_dpp<0x118, 0xf>(v);
-  v += sl_dpp<0x142, 0xa>(v);   // lane 15 to the second row, 47 to the fourth
-  v += sl_dpp<0x143, 0xc>(v);   // lane 31 to the third and fourth
-  return v;
-}
-__device__ __forceinline__ uint32_t sl_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ sl_u64 sl_lane(sl_u64 v, int lane) {
-  return (sl_u64)sl_lane((uint32_t)(v >> 32), lane) << 32 | sl_lane((uint32_t)v, lane);
-}
-
 // Sum over the work-group, and (ex) over the threads before this one; one barrier.
 // Calls take turns with `part` (which), and a barrier lies between two of one turn.
 __device__ __forceinline__ sl_u64 sl_scan(sl_u64 v, sl_u64& ex, sl_u64* part) {
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const sl_u64 in = sl_wave_scan(v);
+  const sl_u64 in = wave_scan(v);
   if (lane == 63) part[wv] = in;
   __syncthreads();
-  const sl_u64 own = part[lane % SL_NW], sums = sl_wave_scan(lane < SL_NW ? own : 0);
-  ex = in - v + sl_lane(sums - own, wv);
-  return sl_lane(sums, SL_NW - 1);
+  const sl_u64 own = part[lane % SL_NW], sums = wave_scan(lane < SL_NW ? own : 0);
+  ex = in - v + lane_of(sums - own, wv);
+  return lane_of(sums, SL_NW - 1);
 }
 
 // The weights of a row, whole numbers of 2^-F.
@@ -502,13 +478,13 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) some += v[e] >= x0;
     });
-    const uint32_t all = sl_lane(sl_wave_scan(some), 63);
+    const uint32_t all = lane_of(wave_scan(some), 63);
     turn ^= 1;
     if (lane == 0) sh.some[turn][wv] = (int)all;
     __syncthreads();
-    const uint32_t own = (uint32_t)sh.some[turn][lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
-    before = (int)sl_lane(in - own, wv);
-    return (int)sl_lane(in, SL_NW - 1);
+    const uint32_t own = (uint32_t)sh.some[turn][lane % SL_NW], in = wave_scan(lane < SL_NW ? own : 0);
+    before = (int)lane_of(in - own, wv);
+    return (int)lane_of(in, SL_NW - 1);
   };
   if (m == INFINITY) {   // the infinite entries weigh 1, all others nothing
     const int n = count(kmax), pick = (int)((double)u * n);
@@ -541,7 +517,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     if (key >= tmin) atomicAdd(&sh.top[(key - tmin) >> s], 1u);
     __syncthreads();
     const uint4 c = *(const uint4*)&sh.top[252 - 4 * lane];   // from the upper end down: w, z, y, x
-    const uint32_t sum = c.x + c.y + c.z + c.w, in = sl_wave_scan(sum), want = (uint32_t)k;
+    const uint32_t sum = c.x + c.y + c.z + c.w, in = wave_scan(sum), want = (uint32_t)k;
     const unsigned long long past = __ballot(in >= want);
     if (past) {
       const int at = __builtin_ctzll(past);
@@ -550,7 +526,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       if (n < want) n += c.z, --b;
       if (n < want) n += c.y, --b;
       if (n < want) --b;
-      kth = tmin + (sl_lane((uint32_t)b, at) << s);
+      kth = tmin + (lane_of((uint32_t)b, at) << s);
     }
   }
 
@@ -568,11 +544,11 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     const unsigned long long mine = __ballot(most >= x0);
     if (lane == 0) sh.hits[wv] = __popcll(mine);
     __syncthreads();
-    const uint32_t own = (uint32_t)sh.hits[lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
-    const int hits = (int)sl_lane(in, SL_NW - 1), pairs = hits * row.J;
+    const uint32_t own = (uint32_t)sh.hits[lane % SL_NW], in = wave_scan(lane < SL_NW ? own : 0);
+    const int hits = (int)lane_of(in, SL_NW - 1), pairs = hits * row.J;
     if (hits > SL_PAIRS * SL_NT || pairs > SL_PAIRS * SL_NT) return -1;
     if (wv == 0 && lane < SL_NW) sh.hits_before[lane] = (int)(in - own);
-    if (most >= x0) sh.hit[sl_lane(in - own, wv) + __popcll(mine & ((1ull << lane) - 1))] = (unsigned short)tid;
+    if (most >= x0) sh.hit[lane_of(in - own, wv) + __popcll(mine & ((1ull << lane) - 1))] = (unsigned short)tid;
     __syncthreads();
     float v[SL_PAIRS][NE];
     int first[SL_PAIRS], some = 0;
@@ -724,7 +700,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     if (!ranked && n >= k && per == 1) {   // an entry's rank by the others, one by one
       uint32_t rank = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) rank += sl_lane(keys[0], i) > keys[0];
+      for (int i = 0; i < n; ++i) rank += lane_of(keys[0], i) > keys[0];
       thr = max(thr, __ockl_wfred_min_u32(lane < n && rank < (uint32_t)k ? keys[0] : 0xffffffffu));
     } else if (!ranked && n >= k) {   // else all of them are among the k
       uint32_t lo = from, hi = kmax;
@@ -746,7 +722,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     if (by_p) {
       sl_u64 want = sp.want;
       if (part >= 0.0) {
-        want = (sl_u64)ceil(part * (double)sl_lane(sl_wave_scan(sum), 63));
+        want = (sl_u64)ceil(part * (double)lane_of(wave_scan(sum), 63));
         if (want == 0) want = 1;
       }
       uint32_t lo = thr, hi = kmax;
@@ -754,8 +730,8 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
         sl_u64 above = 0;
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-          const sl_u64 wi = sl_lane(w[0], i);
-          above += sl_lane(keys[0], i) > keys[0] ? wi : 0;
+          const sl_u64 wi = lane_of(w[0], i);
+          above += lane_of(keys[0], i) > keys[0] ? wi : 0;
         }
         lo = hi = __ockl_wfred_min_u32(w[0] && above < want ? keys[0] : 0xffffffffu);
       }
@@ -764,7 +740,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
         sl_u64 c = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) c += keys[i] >= mid ? w[i] : 0;
-        if (sl_lane(sl_wave_scan(c), 63) >= want) lo = mid;
+        if (lane_of(wave_scan(c), 63) >= want) lo = mid;
         else hi = mid - 1;
       }
       sum = 0;
@@ -774,8 +750,8 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
         sum += w[i];
       }
     }
-    const sl_u64 in = sl_wave_scan(sum);
-    left = sl_lane(in, 63);
+    const sl_u64 in = wave_scan(sum);
+    left = lane_of(in, 63);
     const double target = (double)u * (double)left;
     sl_u64 run = in - sum;
     if (sum && (double)run <= target && target < (double)in) {
@@ -844,9 +820,9 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       sp.turn ^= 1;
       left = sl_scan(sum, ex, sh.part[sp.turn]);
       const double target = (double)u * (double)left;
-      const sl_u64 own = sh.part[sp.turn][lane % SL_NW], in = sl_wave_scan(lane < SL_NW ? own : 0);
+      const sl_u64 own = sh.part[sp.turn][lane % SL_NW], in = wave_scan(lane < SL_NW ? own : 0);
       const int at = __builtin_ctzll(__ballot(target < (double)in));   // target < left
-      sl_u64 start = sl_lane(in - own, at);
+      sl_u64 start = lane_of(in - own, at);
       const int per = (row.J + SL_NW - 1) / SL_NW, first = at * row.J;
       const int ga = first + min(wv * per, row.J), gb = first + min(wv * per + per, row.J);
       float v[NE];
@@ -873,7 +849,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 #pragma unroll 1
         for (int g = ga; g < gb; ++g) {
           if (gb - ga > 1) mass = group(g);
-          const sl_u64 in = sl_wave_scan(mass), all = sl_lane(in, 63);
+          const sl_u64 in = wave_scan(mass), all = lane_of(in, 63);
           if (target < (double)(start + all)) {
             sl_u64 run = start + in - mass;
             if (mass && (double)run <= target && target < (double)(run + mass)) {

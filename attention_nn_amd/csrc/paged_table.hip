@@ -12,7 +12,12 @@
 // each chunk of 4096; one work-group's running sums of both, which say who is served;
 // tables and row maps, a work-group for each span of 4096 entries of a sequence,
 // whose waves find 64 pages at a time among the bits of a chunk.  A call that one
-// work-group gets through in the time of a launch or two is one launch.
+// work-group gets through in their time is one launch.
+//
+// What bounds them is neither bytes nor operations but the passes that wait for each
+// other: a launch that does next to nothing takes 3.4 us, the three 16-17 us from 64
+// sequences of 64 columns to 512 of 1024 over 524288 pages (8.3 MB, 1.6 us of copying:
+// 19.5 us), and the host 21 us to send them.
 #include "common.h"
 #include "launch.h"
 
@@ -177,13 +182,14 @@ __device__ __forceinline__ int pt_bit(unsigned long long w, int k) {
 
 // The free page of rank `rank`, for the lanes with want; by a whole wave, whose
 // lowest such rank is r0.  -1 past the last one.
-__device__ __forceinline__ int pt_page(const PtArgs& a, bool want, int rank, int r0) {
+__device__ __forceinline__ int pt_page(const unsigned long long* free_, const int32_t* chunk, int chunks, int pages,
+                                       bool want, int rank, int r0) {
   const int lane = threadIdx.x & 63;
-  const int words = (int)(((long long)a.t.pages + 63) / 64);
+  const int words = (int)(((long long)pages + 63) / 64);
   int id = -1;
-  for (int c = pg_sequence(a.chunk, a.chunks, r0); c >= 0 && c < a.chunks && __any(want); ++c) {
+  for (int c = pg_sequence(chunk, chunks, r0); c >= 0 && c < chunks && __any(want); ++c) {
     const int w = c * PT_CHUNK + lane;
-    const unsigned long long m = w < words ? a.free_[w] : 0;
+    const unsigned long long m = w < words ? free_[w] : 0;
     const int pop = __popcll(m);
     int sum = pop;
 #pragma unroll
@@ -191,7 +197,7 @@ __device__ __forceinline__ int pt_page(const PtArgs& a, bool want, int rank, int
       const int v = __shfl_up(sum, o, 64);
       if (lane >= o) sum += v;
     }
-    const int total = __shfl(sum, 63, 64), k = rank - a.chunk[c];
+    const int total = __shfl(sum, 63, 64), k = rank - chunk[c];
     int at = 0;   // words that end at or before k
 #pragma unroll
     for (int h = 32; h > 0; h >>= 1)
@@ -207,9 +213,8 @@ __device__ __forceinline__ int pt_page(const PtArgs& a, bool want, int rank, int
   return id;
 }
 
-// Columns and rows of one span of a sequence, by a work-group of 256 threads at least
-// (of which 256 have a column); page: 256 ids, cnt: 4 numbers, in LDS.
-template <int NT>
+// Columns and rows of one span of a sequence, by a work-group of 256 threads; page:
+// 256 ids, cnt: 4 numbers, in LDS.
 __device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* page, int* cnt) {
   const TableArgs& t = a.t;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -222,31 +227,31 @@ __device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* p
   const int c = c0 + tid;
   int id = 0;
   bool take = false;
-  if (tid < 256 && c < c1) {
+  if (c < c1) {
     id = t.table[s * t.trow + c];
     take = c >= tc.t0 && c < tc.t1 && !pt_page_ok(id, t.pages);
   }
   if (touched) {
     const unsigned long long m = __ballot(take);
-    if (wv < 4 && lane == 0) cnt[wv] = __popcll(m);
+    if (lane == 0) cnt[wv] = __popcll(m);
     __syncthreads();
     if (m) {   // of this wave
       int r0 = a.base[s] + a.before[(long long)s * a.spans + span];
       for (int w = 0; w < wv; ++w) r0 += cnt[w];
-      const int got = pt_page(a, take, r0 + __popcll(m & ((1ull << lane) - 1)), r0);
+      const int got = pt_page(a.free_, a.chunk, a.chunks, t.pages, take, r0 + __popcll(m & ((1ull << lane) - 1)), r0);
       if (take) {
         id = got;
         if (got >= 0) t.refs_out[got] = 1;
       }
     }
-    if (tid < 256) page[tid] = id;
+    page[tid] = id;
   }
-  if (tid < 256 && c < c1 && (take || !(a.same & 1))) t.table_out[s * t.orow + c] = id;
+  if (c < c1 && (take || !(a.same & 1))) t.table_out[s * t.orow + c] = id;
   if (!touched) return;
   __syncthreads();
   const int lo = max(at, c0 << t.sh), hi = (int)min((long long)at + n, (long long)c1 << t.sh);
   const int row0 = t.starts[s] - at;
-  for (int e = lo + tid; e < hi; e += NT) {
+  for (int e = lo + tid; e < hi; e += 256) {
     const int p = page[(e >> t.sh) - c0], r = row0 + e;
     t.seq[r] = s;
     t.pos[r] = e;
@@ -294,8 +299,147 @@ __global__ __launch_bounds__(256) void k_table_fill(PtArgs a) {
   __shared__ int page[256], cnt[4];
   const long long all = (long long)a.t.seqs * a.spans;
   for (long long w = blockIdx.x; w < all; w += gridDim.x)
-    pt_fill<256>(a, (int)(w / a.spans), (int)(w % a.spans), page, cnt);
+    pt_fill(a, (int)(w / a.spans), (int)(w % a.spans), page, cnt);
   pt_behind(a.t, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+// All of it by one work-group, which reads everything at once: a wave takes up to PT_HELD
+// pieces of 64 columns, whose ids it keeps.  Its time goes with the pieces and the pages;
+// us against those of three launches (which the host needs 21 us for):
+//   4 sequences of 64 columns, 512 pages      5.6  12.0
+//   16, 1024 pages, 8192 rows                 7.2  13.1
+//   64, 4096 pages                           10.2  16.3
+//   64, 12288 pages                          16.4  16.3
+//   256 (16 pieces a wave), 12288 pages      45.9  16.4
+//   64, 49152 pages                          27.0  16.2
+//   8, 2048 pages, 16384 rows                12.4  12.2
+constexpr int PT_HELD = 4, PT_SEQS = 16 * PT_HELD, PT_PAGES = 16384, PT_ROWS = 8192;
+struct PtShared {
+  int32_t at[PT_SEQS], n[PT_SEQS], base[PT_SEQS], first[PT_SEQS];
+  int32_t need[16 * PT_HELD];             // of a piece
+  unsigned long long free_[PT_PAGES / 64];
+  int32_t chunk[PT_PAGES / 64 / PT_CHUNK + 1];
+  uint32_t part[2][2][16];
+  int rows;
+};
+// Sums of x and y over the threads before this one; tx, ty: over all.  One barrier.
+__device__ __forceinline__ void pt_sums(uint32_t& x, uint32_t& y, uint32_t& tx, uint32_t& ty, uint32_t (*part)[16]) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t ix = wave_scan(x), iy = wave_scan(y);
+  if (lane == 63) {
+    part[0][wv] = ix;
+    part[1][wv] = iy;
+  }
+  __syncthreads();
+  const uint32_t px = part[0][lane % 16], py = part[1][lane % 16];
+  const uint32_t sx = wave_scan(lane < 16 ? px : 0), sy = wave_scan(lane < 16 ? py : 0);
+  x = ix - x + lane_of(sx - px, wv);
+  y = iy - y + lane_of(sy - py, wv);
+  tx = lane_of(sx, 15);
+  ty = lane_of(sy, 15);
+}
+__global__ __launch_bounds__(1024) void k_table_one(PtArgs a) {
+  __shared__ PtShared sh;
+  const TableArgs& t = a.t;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per = (t.cols + 63) / 64, pieces = t.seqs * per, words = (t.pages + 63) / 64;
+  a.free_ = sh.free_;
+  int ids[PT_HELD];
+#pragma unroll
+  for (int i = 0; i < PT_HELD; ++i) {
+    const int q = wv + 16 * i;
+    if (q < pieces) ids[i] = t.table[(q / per) * t.trow + min(q % per * 64 + lane, t.cols - 1)];
+  }
+  if (tid < t.seqs) {
+    const int at = pg_len(t.lens[tid], t.cols, t.sh), want = max(t.add[tid], 0);
+    sh.at[tid] = at;
+    sh.n[tid] = (long long)at + want <= (long long)t.cols << t.sh ? want : -1;
+  }
+#pragma unroll 4
+  for (int w = wv; w < words; w += 16) pt_word(a, w);
+  __syncthreads();
+  // what the pieces need, and the free pages of each chunk
+#pragma unroll
+  for (int i = 0; i < PT_HELD; ++i) {
+    const int q = wv + 16 * i;
+    if (q < pieces) {
+      const int s = q / per, c = q % per * 64 + lane;
+      const PtCols tc = pt_cols(sh.at[s], sh.n[s], t.sh);
+      const unsigned long long m = __ballot(c >= tc.t0 && c < tc.t1 && !pt_page_ok(ids[i], t.pages));
+      if (lane == 0) sh.need[q] = __popcll(m);
+    }
+  }
+  for (int c = wv; c < a.chunks; c += 16) {
+    const int w = c * PT_CHUNK + lane;
+    const uint32_t n = wave_scan((uint32_t)(w < words ? __popcll(sh.free_[w]) : 0));
+    if (lane == 63) sh.chunk[c] = (int)n;
+  }
+  __syncthreads();
+  // who is served: sums of what is asked for, at most one more than there is of each, in 32
+  // bits; the chunks' free pages, 16 at most, by every wave
+  const uint32_t own = lane < a.chunks ? (uint32_t)sh.chunk[lane] : 0, upto = wave_scan(own);
+  const uint32_t free_pages = lane_of(upto, 63);
+  const int n = tid < t.seqs ? sh.n[tid] : -1;
+  int need = 0;
+  if (n > 0)
+    for (int i = 0; i < per; ++i) need += sh.need[tid * per + i];
+  uint32_t x = (uint32_t)min(need, t.pages + 1), y = (uint32_t)min(max(n, 0), t.rows + 1), tx, ty;
+  const uint32_t xi = x, yi = y;
+  pt_sums(x, y, tx, ty, sh.part[0]);   // behind its barrier the chunks' sums are read
+  const bool ok = n >= 0 && y + yi <= (uint32_t)t.rows && (need == 0 || x + xi <= free_pages);
+  x = ok ? (uint32_t)need : 0;
+  y = ok ? (uint32_t)n : 0;
+  pt_sums(x, y, tx, ty, sh.part[1]);
+  if (wv == 0 && lane < a.chunks) sh.chunk[lane] = (int)(upto - own);
+  if (tid < t.seqs) {
+    const int g = ok ? n : 0;
+    sh.n[tid] = g;
+    sh.base[tid] = (int)x;
+    sh.first[tid] = (int)y;
+    t.starts[tid] = (int)y;
+    t.lens_out[tid] = sh.at[tid] + g;
+  }
+  if (tid == 0) {
+    t.starts[t.seqs] = (int)ty;
+    sh.rows = (int)ty;
+  }
+  __syncthreads();
+  // tables and rows
+#pragma unroll
+  for (int i = 0; i < PT_HELD; ++i) {
+    const int q = wv + 16 * i;
+    if (q >= pieces) break;
+    const int s = q / per, c0 = q % per * 64, c = c0 + lane, at = sh.at[s], n = sh.n[s];
+    const PtCols tc = pt_cols(at, n, t.sh);
+    int id = ids[i];
+    const bool take = c >= tc.t0 && c < tc.t1 && !pt_page_ok(id, t.pages);
+    const unsigned long long m = __ballot(take);
+    if (m) {
+      int rank = sh.base[s];
+      for (int j = q - q % per; j < q; ++j) rank += sh.need[j];
+      const int got = pt_page(sh.free_, sh.chunk, a.chunks, t.pages, take, rank + __popcll(m & ((1ull << lane) - 1)), rank);
+      if (take) {
+        id = got;
+        if (got >= 0) t.refs_out[got] = 1;
+      }
+    }
+    if (c < t.cols && (take || !(a.same & 1))) t.table_out[s * t.orow + c] = id;
+    const int lo = max(at, c0 << t.sh), hi = (int)min((long long)at + n, (long long)(c0 + 64) << t.sh);
+    const int row0 = sh.first[s] - at;
+    for (int e0 = lo; e0 < hi; e0 += 64) {
+      const int e = e0 + lane, p = __shfl(id, (e >> t.sh) - c0, 64);
+      if (e < hi) {
+        t.seq[row0 + e] = s;
+        t.pos[row0 + e] = e;
+        t.slot[row0 + e] = pt_page_ok(p, t.pages) ? ((long long)p << t.sh) + (e & ((1 << t.sh) - 1)) : -1;
+      }
+    }
+  }
+  for (int r = sh.rows + tid; r < t.rows; r += 1024) {
+    t.seq[r] = -1;
+    t.pos[r] = -1;
+    t.slot[r] = -1;
+  }
 }
 
 // ---- pages returned ---------------------------------------------------------------
@@ -308,20 +452,64 @@ __global__ __launch_bounds__(256) void k_refs_copy(const int32_t* __restrict__ i
 
 // Columns behind a sequence's entries name no page any more; each one named counts
 // one less.  Whole-number atomics: in any order the same counts.
+__device__ __forceinline__ int pt_have(const TableArgs& t, int s) {   // columns that its entries touch
+  return (int)(((long long)pg_len(t.lens[s], t.cols, t.sh) + (1 << t.sh) - 1) >> t.sh);
+}
 __global__ __launch_bounds__(256) void k_table_release(TableArgs t, int same) {
-  const int tid = threadIdx.x;
-  const int per = (t.cols + 255) / 256;   // work-groups a sequence
-  for (long long w = blockIdx.x; w < (long long)t.seqs * per; w += gridDim.x) {
-    const int s = (int)(w / per), c = (int)(w % per) * 256 + tid;
+  const int tid = threadIdx.x, per = (t.cols + 63) / 64;   // waves a sequence
+  for (long long w = (long long)blockIdx.x * 4 + (tid >> 6); w < (long long)t.seqs * per; w += (long long)gridDim.x * 4) {
+    const int s = (int)(w / per), c = (int)(w % per) * 64 + (tid & 63);
     if (c >= t.cols) continue;
-    const int have = (int)(((long long)pg_len(t.lens[s], t.cols, t.sh) + (1 << t.sh) - 1) >> t.sh);
-    int id = t.table[s * t.trow + c];
-    if (c >= have) {
+    const int id = t.table[s * t.trow + c];
+    if (c >= pt_have(t, s)) {
       if (pt_page_ok(id, t.pages)) atomicSub(&t.refs_out[id], 1);
       if (id != -1 || !same) t.table_out[s * t.orow + c] = -1;
     } else if (!same) {
       t.table_out[s * t.orow + c] = id;
     }
+  }
+}
+// The same by one work-group, which reads everything at once and counts in LDS.  64
+// sequences of 64 columns, 12288 pages: 6.6 us, one call after another 7.1 (two launches
+// 4.2, but 10.0, which is what the host takes); 256 of them 16.3 and 16.1.
+constexpr int PT_COUNTS = 12288;
+__global__ __launch_bounds__(1024) void k_table_release_one(TableArgs t, int same) {
+  __shared__ int gone[PT_COUNTS];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per = (t.cols + 63) / 64, pieces = t.seqs * per;
+  int ids[PT_HELD], have[PT_HELD], refs[PT_COUNTS / 1024];
+#pragma unroll
+  for (int i = 0; i < PT_HELD; ++i) {
+    const int q = wv + 16 * i;
+    if (q < pieces) {
+      ids[i] = t.table[(q / per) * t.trow + min(q % per * 64 + lane, t.cols - 1)];
+      have[i] = t.lens[q / per];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PT_COUNTS / 1024; ++i) {
+    const int p = tid + 1024 * i;
+    if (p < t.pages) refs[i] = t.refs[p];
+    gone[p] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PT_HELD; ++i) {
+    const int q = wv + 16 * i;
+    if (q >= pieces) break;
+    const int c = q % per * 64 + lane;
+    if (c < t.cols) {
+      int id = ids[i];
+      const bool behind = c >= (int)(((long long)pg_len(have[i], t.cols, t.sh) + (1 << t.sh) - 1) >> t.sh);
+      if (behind && pt_page_ok(id, t.pages)) atomicAdd(&gone[id], 1);
+      if (behind ? id != -1 || !same : !same) t.table_out[(q / per) * t.orow + c] = behind ? -1 : id;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PT_COUNTS / 1024; ++i) {
+    const int p = tid + 1024 * i;
+    if (p < t.pages && (gone[p] || t.refs != t.refs_out)) t.refs_out[p] = refs[i] - gone[p];
   }
 }
 
@@ -330,7 +518,13 @@ static int pt_spans(const TableArgs& t) {
 }
 static int pt_chunks(const TableArgs& t) { return (int)(((long long)t.pages + 64 * PT_CHUNK - 1) / (64 * PT_CHUNK)); }
 
+static bool pt_held(const TableArgs& t) { return (long long)t.seqs * ((t.cols + 63) / 64) <= 16 * PT_HELD; }
+static bool pt_one(const TableArgs& t) {
+  return pt_held(t) && t.seqs <= PT_SEQS && t.pages <= PT_PAGES && t.rows <= PT_ROWS;
+}
+
 size_t table_assign_ws_bytes(const TableArgs& t) {
+  if (pt_one(t)) return 0;
   const size_t words = ((size_t)t.pages + 63) / 64;
   return words * 8 + ((size_t)pt_chunks(t) + 1 + (size_t)t.seqs * (4 + (size_t)pt_spans(t))) * 4;
 }
@@ -341,6 +535,10 @@ hipError_t table_assign(const TableArgs& t, void* ws, hipStream_t st) {
   a.same = (t.table == t.table_out) | (t.refs == t.refs_out) << 1;
   a.spans = pt_spans(t);
   a.chunks = pt_chunks(t);
+  if (pt_one(t)) {
+    hipLaunchKernelGGL(k_table_one, dim3(1), dim3(1024), 0, st, a);
+    return hipGetLastError();
+  }
   a.free_ = (unsigned long long*)ws;
   a.chunk = (int32_t*)(a.free_ + ((size_t)t.pages + 63) / 64);
   a.at = a.chunk + a.chunks + 1;
@@ -362,16 +560,20 @@ hipError_t table_assign(const TableArgs& t, void* ws, hipStream_t st) {
 }
 
 hipError_t table_release(const TableArgs& t, hipStream_t st) {
+  const int same = t.table == t.table_out;
+  if (pt_held(t) && t.pages <= PT_COUNTS) {
+    hipLaunchKernelGGL(k_table_release_one, dim3(1), dim3(1024), 0, st, t, same);
+    return hipGetLastError();
+  }
   if (t.refs != t.refs_out) {
     hipLaunchKernelGGL(k_refs_copy, dim3((unsigned)(((long long)t.pages + 255) / 256)), dim3(256), 0, st, t.refs,
                        t.refs_out, t.pages);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  const long long all = (long long)t.seqs * ((t.cols + 255) / 256);
+  const long long all = ((long long)t.seqs * ((t.cols + 63) / 64) + 3) / 4;
   if (all == 0) return hipSuccess;
-  hipLaunchKernelGGL(k_table_release, dim3((unsigned)(all > 65536 ? 65536 : all)), dim3(256), 0, st, t,
-                     t.table == t.table_out);
+  hipLaunchKernelGGL(k_table_release, dim3((unsigned)(all > 65536 ? 65536 : all)), dim3(256), 0, st, t, same);
   return hipGetLastError();
 }
 

@@ -420,10 +420,10 @@ def assign(table, lens, new, refs, page_size, rows, out=None, refs_out=None, len
     starts, seq, pos = _new((S + 1,), _I32, device), _new((rows,), _I32, device), _new((rows,), _I32, device)
     slot = _new((rows,), torch.int64, device)
     L = _lib.lib()
-    nws = L.ann_op_paged_assign_ws_bytes(t)
-    ws = _new((nws,), torch.uint8, device)
+    nws = L.ann_op_paged_assign_ws_bytes(t, rows)
+    ws = _new((nws,), torch.uint8, device) if nws else None
     rc = on_device(d, L.ann_op_paged_assign, t, new.data_ptr(), rows, starts.data_ptr(), lens_out.data_ptr(),
-                   seq.data_ptr(), pos.data_ptr(), slot.data_ptr(), ws.data_ptr(), nws)
+                   seq.data_ptr(), pos.data_ptr(), slot.data_ptr(), ws.data_ptr() if nws else None, nws)
     if rc:
         _lib.check(rc)
     return Assigned(out, refs_out, starts, lens_out, seq, pos, slot)

@@ -400,7 +400,7 @@ typedef struct ann_paged_table {
  * it, and row r of the step is entry pos[r] of sequence seq[r], slot[r] = page *
  * page_size + place in the page; -1 behind the last row (seq, pos, slot: rows).  ws:
  * ann_op_paged_assign_ws_bytes bytes (16-byte aligned), one for each call in flight. */
-size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t);
+size_t ann_op_paged_assign_ws_bytes(const ann_paged_table* t, int32_t rows);
 int ann_op_paged_assign(const ann_paged_table* t, const int32_t* new_tokens, int32_t rows,
                         int32_t* starts, int32_t* new_lens, int32_t* seq, int32_t* pos,
                         int64_t* slot, void* ws, size_t ws_bytes, void* stream);
