@@ -312,7 +312,8 @@ __global__ __launch_bounds__(256) void k_table_fill(PtArgs a) {
 //   64, 12288 pages                          16.4  16.3
 //   256 (16 pieces a wave), 12288 pages      45.9  16.4
 //   64, 49152 pages                          27.0  16.2
-//   8, 2048 pages, 16384 rows                12.4  12.2
+//   1 of 256 columns, 8192 rows by 2 waves   11.3  13.6
+// More rows than that, which one wave may have to write, are the three launches'.
 constexpr int PT_HELD = 4, PT_SEQS = 16 * PT_HELD, PT_PAGES = 16384, PT_ROWS = 8192;
 struct PtShared {
   int32_t at[PT_SEQS], n[PT_SEQS], base[PT_SEQS], first[PT_SEQS];

@@ -13,6 +13,16 @@ prompts, chunks of prompts and single decoded tokens side by side::
     w = paged.attention_weight(q, lse, k_cache, table, starts, lens, w, 0.1)
     kept, lens, w = paged.evict(k_cache, v_cache, table, lens, w, keep=4096, recent=384)
 
+``assign`` gives a step's tokens their pages and rows and ``release`` takes pages back, so
+the tables too are made without the host; ``attention_shared`` reads entries that
+sequences have in common once::
+
+    a = paged.assign(table, lens, new, refs, page_size, rows)
+    q = paged.append(q, k, v, cs, sn, k_cache, v_cache, a.table, a.starts, a.lens)
+    y = paged.attention_shared(q, k_cache, v_cache, a.table, a.starts, a.lens, groups, prefix_table, prefix_lens, 0.1)
+    ids = kernels.sample_logits(logits, u, temperature=0.8, top_p=0.95)
+    table, refs = paged.release(a.table, lens, a.refs, page_size)
+
 (model.py:244-254 for one layer; the reference recomputes the context and has
 no cache.)  ``table``, ``starts`` and ``lens`` are int32 GPU tensors that the
 host does not look at, so every call can be captured into a graph and replayed
@@ -248,9 +258,7 @@ def attention_shared(q, k_cache, v_cache, table, starts, lens, groups, prefix_ta
     ``groups`` (groups + 1,), ``prefix_table`` (groups, columns) and ``prefix_lens`` (groups,)
     are int32 GPU tensors that the host does not look at; ``groups`` must not fall, and sequences of no
     group share nothing.  A prefix is read once for the tokens of all its sequences with up
-    to 16 new ones; a sequence of more is on its own.  The
-    weights of a prefix's entries enter the product with the values in bf16, of the
-    others as in ``attention``."""
+    to 16 new ones; a sequence of more is on its own."""
     (q, qp, qt, qh), N, H, D, d, c, (S, _, _, page, _), keep = _queries(q, k_cache, v_cache, table, starts, lens)
     _check("prefix_table", prefix_table, _I32, 2, d)
     count, cols = prefix_table.shape
