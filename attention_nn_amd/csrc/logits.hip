@@ -140,7 +140,7 @@ struct SlRow {
   // tensor: within its allocation, which no aligned 16-byte word crosses the end of.
   // A chunk past the last one is that one.
   __device__ __forceinline__ uint4 chunk(int c) const {
-    return *(const uint4*)(base + (uint32_t)min(c, chunks - 1) * 16u);
+    return *(const uint4*)(base + min((uint32_t)c, (uint32_t)chunks - 1) * 16u);
   }
   __device__ __forceinline__ uint4 load(int g) const { return chunk(g * 64 + lane); }
   __device__ __forceinline__ static void unpack(const uint4& w, float* v) {
@@ -548,7 +548,10 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     const int hits = (int)lane_of(in, SL_NW - 1), pairs = hits * row.J;
     if (hits > SL_PAIRS * SL_NT || pairs > SL_PAIRS * SL_NT) return -1;
     if (wv == 0 && lane < SL_NW) sh.hits_before[lane] = (int)(in - own);
-    if (most >= x0) sh.hit[lane_of(in - own, wv) + __popcll(mine & ((1ull << lane) - 1))] = (unsigned short)tid;
+    // by all lanes: inside the branch the lane that is asked may be off, and what it holds of
+    // in - own not yet formed
+    const uint32_t place = lane_of(in - own, wv) + __popcll(mine & ((1ull << lane) - 1));
+    if (most >= x0) sh.hit[place] = (unsigned short)tid;
     __syncthreads();
     float v[SL_PAIRS][NE];
     int first[SL_PAIRS], some = 0;

@@ -180,3 +180,23 @@ def test_graph_and_other_stream():
         _check(y, v, (ids, lp), dict(temperature=0.9, top_k=40, top_p=0.95))
         eager = kernels.sample_logits(xd, ud, 0.9, 40, 0.95)
         assert torch.equal(eager, ids)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("peaks", [1, 5, 30, 90])
+@pytest.mark.parametrize("cols", [9000, 50257, 53300, 70001, 131072])
+def test_few_entries_hold_what_top_p_keeps(cols, peaks, dtype):
+    """Far more entries weigh something than a list holds, and what top_p keeps of them
+    lies with a few threads, of no particular wave or lane."""
+    from attention_nn_amd import kernels
+    g = torch.Generator().manual_seed(cols + peaks)
+    x = 0.3 * torch.randn((6, cols), generator=g)
+    for r in range(6):
+        at = torch.randperm(cols, generator=g)[:peaks]
+        if r == 4:
+            at = cols - 1 - torch.arange(peaks)     # all with the last wave
+        x[r, at] = 12.0 + torch.rand(peaks, generator=g)
+    x = x.to(dtype)
+    u = torch.rand(6, generator=g)
+    for kw in (dict(top_p=0.3), dict(top_p=0.9 if peaks > 5 else 0.5), dict(top_p=0.6, top_k=cols - 1)):
+        _check(x, u, kernels.sample_logits(x.cuda(), u.cuda(), want_logprob=True, **kw), kw)
