@@ -15,9 +15,9 @@
 // work-group gets through in their time is one launch.
 //
 // What bounds them is neither bytes nor operations but the passes that wait for each
-// other: a launch that does next to nothing takes 3.4 us, the three 16-17 us from 64
-// sequences of 64 columns to 512 of 1024 over 524288 pages (8.3 MB, 1.6 us of copying:
-// 19.5 us), and the host 21 us to send them.
+// other: a launch that does next to nothing takes 3.4 us, the three 16.4 us for 64
+// sequences of 64 columns and 19.5 for 1000 of 512 over 512008 pages (8.3 MB, 1.6 us of
+// copying), and the host 21 us to send them.
 #include "common.h"
 #include "launch.h"
 

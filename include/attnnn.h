@@ -37,7 +37,9 @@
  *                                                gradient (model.py:244-247)
  *   ann_op_paged_*                               no counterpart: attention over a cache
  *                                                (model.py:248-254) that sequences of
- *                                                any lengths share
+ *                                                any lengths share, and their tables
+ *   ann_op_sample_logits                      <- /temp, top-k and categorical of given
+ *                                                logits (sample.py:45-49), with top_p, min_p
  */
 #ifndef ATTNNN_H
 #define ATTNNN_H
