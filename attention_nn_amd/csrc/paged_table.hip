@@ -58,18 +58,29 @@ __device__ __forceinline__ void pt_need(const PtArgs& a, int s) {
   const int lane = threadIdx.x & 63, sh = t.sh;
   const int at = pg_len(t.lens[s], t.cols, sh), want = max(t.add[s], 0);
   const bool fits = (long long)at + want <= (long long)t.cols << sh;
-  const PtCols c = pt_cols(at, fits ? want : 0, sh);
+  // more than there are rows is not served, and none behind it: its pages need no count
+  const PtCols c = pt_cols(at, fits && want <= t.rows ? want : 0, sh);
   const int32_t* row = t.table + s * t.trow;
   const int spc = PT_SPAN - sh;   // log2 of a span's columns
+  constexpr int D = 8;   // reads at once (131072 tokens of one sequence, pages of 16: the call 38.3 us with one, 24.9)
   int need = 0;
   for (int c0 = c.t0; c0 < c.t1;) {
-    // 64 columns at most, not past a span's end
-    const int span = c0 >> spc, end = min(min(c0 + 64, c.t1), (span + 1) << spc);
-    if (lane == 0 && (c0 == c.t0 || (c0 & ((1 << spc) - 1)) == 0))
-      a.before[(long long)s * a.spans + span] = need;
-    const int col = c0 + lane;
-    need += __popcll(__ballot(col < end && !pt_page_ok(row[min(col, end - 1)], t.pages)));
-    c0 = end;
+    int from[D + 1];
+    bool miss[D];
+    from[0] = c0;
+#pragma unroll
+    for (int d = 0; d < D; ++d) {   // 64 columns at most, not past a span's end
+      from[d + 1] = min(min(from[d] + 64, c.t1), ((from[d] >> spc) + 1) << spc);
+      const int col = from[d] + lane;
+      miss[d] = !pt_page_ok(row[min(col, c.t1 - 1)], t.pages) && col < from[d + 1];
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (lane == 0 && from[d] < c.t1 && (from[d] == c.t0 || (from[d] & ((1 << spc) - 1)) == 0))
+        a.before[(long long)s * a.spans + (from[d] >> spc)] = need;
+      need += __popcll(__ballot(miss[d]));
+    }
+    c0 = from[D];
   }
   if (lane == 0) {
     a.at[s] = at;

@@ -169,6 +169,30 @@ def test_tables_by_size(i, traced):
     assert out[0].cpu().tolist() == wt and out[1].cpu().tolist() == wr
 
 
+@pytest.mark.parametrize("page", [16, 64, 128, 1024])
+@pytest.mark.parametrize("first", [0, 7777])
+def test_long_prompts(first, page):
+    """Many columns of one sequence: whole spans, parts of them at both ends, some
+    named already; and one that asks for more than there are rows, behind which none is served."""
+    from attention_nn_amd import paged
+    cols = 70000 // page
+    g = torch.Generator().manual_seed(page + first)
+    table = torch.full((4, cols), -1, dtype=I32)
+    pages = 2 * cols + 40
+    order = torch.randperm(pages, generator=g).to(I32)
+    table[0, :-(-first // page)] = order[:-(-first // page)]
+    held = torch.rand(cols, generator=g) < 0.3
+    table[1, held] = order[cols:2 * cols][held]
+    refs = torch.zeros(pages, dtype=I32)
+    refs[table[table >= 0].long()] = 1
+    lens = torch.tensor([first, 1, 0, 0], dtype=I32)
+    for new in ([60001, 1, 3, 1], [1, 40000, 0, 2], [5, 66000, 9, 1]):
+        rows = 60010
+        ref = R.assign(table.tolist(), lens.tolist(), new, refs.tolist(), page, rows)
+        got = paged.assign(table.cuda(), lens.cuda(), torch.tensor(new, dtype=I32).cuda(), refs.cuda(), page, rows)
+        _same(got, ref)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("k", [895, 896, 897, 4000, 8191, 8192, 8193, 20000])
 def test_draws_of_many_kept(k, dtype):
@@ -229,3 +253,58 @@ def test_two_calls_at_once():
         for a, ids in out:
             _same(a, ref)
             assert ids.tolist() == want
+
+
+def test_refused_on_the_gpu():
+    """What the Python layer refuses of GPU tensors: types, shapes, layouts."""
+    from attention_nn_amd import kernels, paged
+    i = torch.zeros((3, 4), dtype=I32, device="cuda")
+    n, r = i[:, 0].contiguous(), torch.zeros(9, dtype=I32, device="cuda")
+    assert paged.assign(i, n, n, r, 16, 2).starts.tolist() == [0] * 4
+    for args, kw in (((i.long(), n, n, r, 16, 2), {}), ((i, n[:2], n, r, 16, 2), {}), ((i, n, n.float(), r, 16, 2), {}),
+                     ((i, n, n, r, 24, 2), {}), ((i, n, n, r, 16, -1), {}), ((i[0], n, n, r, 16, 2), {}),
+                     ((i, n, n, r, 16, 2), dict(out=i[:, :2])), ((i, n, n, r, 16, 2), dict(refs_out=r[:5])),
+                     ((i, n, n, r, 16, 2), dict(refs_out=r[::2])), ((i, n, n, r, 16, 2), dict(lens_out=n[:1])),
+                     ((i, n, n.cpu(), r, 16, 2), {}), ((i, n, n, i[0, :2], 16, 2), dict(out=i)),
+                     ((i[:1].expand(3, 4), n, n, r, 16, 2), dict(out=i[:1].expand(3, 4)))):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            paged.assign(*args, **kw)
+    for args in ((i, n[:2], r, 16), (i, n, r.long(), 16), (i, n, r, 0), (i, n, r, -16)):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            paged.release(*args)
+    x, u = torch.zeros((3, 50), device="cuda"), torch.zeros(3, device="cuda")
+    for args, kw in (((x.double(), u), {}), ((x[0], u), {}), ((x, u[:2]), {}), ((x, u.double()), {}), ((x, u.cpu()), {}),
+                     ((x, u), dict(temperature=-1.0)), ((x, u), dict(temperature=u[:1])), ((x, u), dict(top_k=-2)),
+                     ((x, u), dict(top_k=u)), ((x, u), dict(top_p=float("nan"))), ((x, u), dict(min_p=-0.1)),
+                     ((x[:, :0], u), {}), ((x, None), {})):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            kernels.sample_logits(*args, **kw)
+    q = torch.zeros((3, 2, 64), dtype=BF, device="cuda")
+    c = torch.zeros((9, 2, 16, 64), dtype=BF, device="cuda")
+    st, g2, t1 = torch.arange(4, dtype=I32, device="cuda"), n[:2] * 0, i[:1]
+    ok = dict(q=q, k_cache=c, v_cache=c, table=i, starts=st, lens=n + 1, groups=g2, prefix_table=t1, prefix_lens=n[:1], scale=0.1)
+    assert paged.attention_shared(**ok).shape == q.shape
+    for kw in (dict(groups=n), dict(prefix_lens=n), dict(prefix_table=t1.long()), dict(prefix_table=t1[0]),
+               dict(groups=g2.cpu()), dict(q=q.float()), dict(q=q[:, :, :32]), dict(starts=n), dict(lens=st),
+               dict(out=q.float()), dict(out=q[:2]), dict(window=-1), dict(scale=float("inf"))):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            paged.attention_shared(**{**ok, **kw})
+
+
+@pytest.mark.parametrize("wide", [True, False])
+def test_results_in_place_of_the_queries(wide, traced):
+    """Sequences of few tokens and of many behind prefixes, and one of none."""
+    from attention_nn_amd import paged
+    from tests.test_gpu_paged_shared import Setup
+    s = Setup([(130, [(1, 5), (2, 40), (40, 60)]), (70, [(3, 9), (100, 130)]), (None, [(1, 33)])], H=4, Hk=2, D=64, page=32)
+    s = s.widened() if wide else s
+    args = s.dev()
+    q = s.q.cuda()
+    want, lse = paged.attention_shared(q.clone(), *args, 0.1, want_lse=True)
+    got = []
+    names = traced(lambda: got.append(paged.attention_shared(q.clone(), *args, 0.1)))
+    assert any("k_paged_shared" in n for n in names) == wide
+    for _ in range(3):
+        x = q.clone()
+        y, l = paged.attention_shared(x, *args, 0.1, want_lse=True, out=x)
+        assert y is x and torch.equal(y, want) and torch.equal(l, lse)
