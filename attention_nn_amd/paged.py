@@ -51,7 +51,7 @@ from . import _lib
 from ._stream import on_device
 
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
-_Tensor, _empty_strided = torch.Tensor, torch.empty_strided
+_Tensor, _empty_strided, _parts = torch.Tensor, torch.empty_strided, torch.unsafe_split_with_sizes
 _paged, _qk_rows = _lib.AnnPaged.from_values, _lib.AnnQkRows.from_values
 
 
@@ -351,7 +351,7 @@ class Assigned(NamedTuple):
     """A step's tables and row maps, as ``assign`` made them."""
     table: torch.Tensor    # (sequences, columns) int32
     refs: torch.Tensor     # (pages,) int32
-    starts: torch.Tensor   # (sequences + 1,) int32
+    starts: torch.Tensor   # (sequences + 1,) int32; these four lie behind one another in one allocation
     lens: torch.Tensor     # (sequences,) int32
     seq: torch.Tensor      # (rows,) int32: the sequence of each row, -1 behind the last
     pos: torch.Tensor      # (rows,) int32: its entry, -1 behind
@@ -420,13 +420,14 @@ def assign(table, lens, new, refs, page_size, rows, out=None, refs_out=None, len
     if not 0 <= rows <= 1 << 30:
         raise ValueError(f"rows={rows} must lie in [0, 2^30]")
     device = out.device
+    # one allocation and its parts: half the time of four
     if lens_out is None:
-        lens_out = _new((S,), _I32, device)
+        starts, lens_out, seq, pos = _parts(_new((2 * (S + rows) + 1,), _I32, device), (S + 1, S, rows, rows))
     else:
         _check("lens_out", lens_out, _I32, 1, d)
         if lens_out.shape[0] != S or not lens_out.is_contiguous():
             raise ValueError(f"lens_out must be contiguous, {S} elements")
-    starts, seq, pos = _new((S + 1,), _I32, device), _new((rows,), _I32, device), _new((rows,), _I32, device)
+        starts, seq, pos = _parts(_new((S + 2 * rows + 1,), _I32, device), (S + 1, rows, rows))
     slot = _new((rows,), torch.int64, device)
     L = _lib.lib()
     nws = L.ann_op_paged_assign_ws_bytes(t, rows)
