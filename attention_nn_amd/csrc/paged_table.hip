@@ -8,16 +8,18 @@
 // (no page needed: rows only).  The i-th needed column of those served takes the i-th
 // free page.  Whole numbers, no atomics: the same call gives the same tables.
 //
-// Three launches, each a pass: needs, and the free pages as bits with the number in
-// each chunk of 4096; one work-group's running sums of both, which say who is served;
-// tables and row maps, a work-group for each span of 4096 entries of a sequence,
-// whose waves find 64 pages at a time among the bits of a chunk.  A call that one
-// work-group gets through in their time is one launch.
+// Three passes: needs, and the free pages as bits with the number in each chunk of
+// 4096; running sums of both, which say who is served; tables and row maps, a
+// work-group for each span of 4096 entries of a sequence, whose waves find 64 pages at a
+// time among the bits of a chunk.  Up to 1024 sequences every work-group of the last
+// pass forms the sums for itself, in the time of reading them: two launches; more are
+// a work-group's between the two.  A call that one work-group gets through in their
+// time is one launch.
 //
 // What bounds them is neither bytes nor operations but the passes that wait for each
-// other: a launch that does next to nothing takes 3.4 us, the three 16.4 us for 64
-// sequences of 64 columns and 19.5 for 1000 of 512 over 512008 pages (8.3 MB, 1.6 us of
-// copying), and the host 21 us to send them.
+// other: a launch that does next to nothing takes 3.4 us, two of them 12.0 us for 48
+// sequences of 128 columns and 16384 rows (three 16.7) and 16.8 for 1000 of 512 over 512008
+// pages (19.5; 8.3 MB, 1.6 us of copying), and the host 17 us to send them (three 21).
 #include "common.h"
 #include "launch.h"
 
@@ -137,6 +139,16 @@ __device__ __forceinline__ void pt_scan(long long& x, long long& y, long long& t
   y += by;
 }
 
+// What a sequence gets: its new tokens (0: not served), the rank of its first page, its
+// first row; the free pages before each chunk; rows of all.
+struct PtGrant {
+  const int32_t* n;
+  const int32_t* base;
+  const int32_t* first;
+  const int32_t* chunk;
+  int rows;
+};
+
 // Free pages before each chunk, and who is served.
 template <int NT>
 __device__ __forceinline__ void pt_grant(const PtArgs& a, long long (*part)[2]) {
@@ -224,14 +236,89 @@ __device__ __forceinline__ int pt_page(const unsigned long long* free_, const in
   return id;
 }
 
+// Sums of x and y over the threads before this one; tx, ty: over all.  One barrier.
+template <int NW>
+__device__ __forceinline__ void pt_sums(uint32_t& x, uint32_t& y, uint32_t& tx, uint32_t& ty, uint32_t (*part)[NW]) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t ix = wave_scan(x), iy = wave_scan(y);
+  if (lane == 63) {
+    part[0][wv] = ix;
+    part[1][wv] = iy;
+  }
+  __syncthreads();
+  const uint32_t px = part[0][lane % NW], py = part[1][lane % NW];
+  const uint32_t sx = wave_scan(lane < NW ? px : 0), sy = wave_scan(lane < NW ? py : 0);
+  x = ix - x + lane_of(sx - px, wv);
+  y = iy - y + lane_of(sy - py, wv);
+  tx = lane_of(sx, NW - 1);
+  ty = lane_of(sy, NW - 1);
+}
+// The same for up to PT_SUMS sequences and as many chunks as threads, by a work-group of 256
+// for itself, to LDS: sums of what is asked for, at most one more than there is of each, in
+// 32 bits.
+constexpr int PT_SUMS = 1024;
+constexpr int PT_SUM_PAGES = 256 * 64 * PT_CHUNK, PT_SUM_ROWS = 1 << 21;
+struct PtSums {
+  int32_t n[PT_SUMS], base[PT_SUMS], first[PT_SUMS], chunk[256];
+  uint32_t part[3][2][4];
+};
+__device__ __forceinline__ int pt_sum_up(const PtArgs& a, PtSums& sh) {
+  constexpr int PER = PT_SUMS / 256;
+  const TableArgs& t = a.t;
+  const int tid = threadIdx.x, s0 = tid * PER;
+  const uint32_t own = tid < a.chunks ? (uint32_t)a.chunk[tid] : 0;
+  int n[PER];
+  uint32_t need[PER], x = 0, y = 0, tx, ty, free_pages;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = min(s0 + i, t.seqs - 1);
+    n[i] = a.n[s];
+    need[i] = (uint32_t)min(a.need[s], t.pages + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (s0 + i >= t.seqs) n[i] = -1;
+    if (n[i] < 0) need[i] = 0;
+    x += need[i];
+    y += (uint32_t)min(max(n[i], 0), t.rows + 1);
+  }
+  uint32_t c = own, none = 0;
+  pt_sums<4>(c, none, free_pages, none, sh.part[0]);
+  if (tid < a.chunks) sh.chunk[tid] = (int)c;
+  pt_sums<4>(x, y, tx, ty, sh.part[1]);
+  uint32_t px = 0, py = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    x += need[i];
+    y += (uint32_t)min(max(n[i], 0), t.rows + 1);
+    const bool ok = n[i] >= 0 && y <= (uint32_t)t.rows && (need[i] == 0 || x <= free_pages);
+    n[i] = ok ? n[i] : 0;
+    need[i] = ok ? need[i] : 0;
+    px += need[i];
+    py += (uint32_t)n[i];
+  }
+  pt_sums<4>(px, py, tx, ty, sh.part[2]);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = s0 + i;
+    sh.n[s] = n[i];
+    sh.base[s] = (int)px;
+    sh.first[s] = (int)py;
+    px += need[i];
+    py += (uint32_t)n[i];
+  }
+  __syncthreads();
+  return (int)ty;
+}
+
 // Columns and rows of one span of a sequence, by a work-group of 256 threads; page:
 // 256 ids, cnt: 4 numbers, in LDS.
-__device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* page, int* cnt) {
+__device__ __forceinline__ void pt_fill(const PtArgs& a, const PtGrant& g, int s, int span, int* page, int* cnt) {
   const TableArgs& t = a.t;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int spc = PT_SPAN - t.sh;
   const int c0 = span << spc, c1 = min(t.cols, c0 + (1 << spc));
-  const int at = a.at[s], n = a.n[s];
+  const int at = a.at[s], n = g.n[s];
   const PtCols tc = pt_cols(at, n, t.sh);
   const bool touched = max(tc.t0, c0) < min(tc.t1, c1);
   if (!touched && (a.same & 1)) return;   // the same for all threads
@@ -247,9 +334,9 @@ __device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* p
     if (lane == 0) cnt[wv] = __popcll(m);
     __syncthreads();
     if (m) {   // of this wave
-      int r0 = a.base[s] + a.before[(long long)s * a.spans + span];
+      int r0 = g.base[s] + a.before[(long long)s * a.spans + span];
       for (int w = 0; w < wv; ++w) r0 += cnt[w];
-      const int got = pt_page(a.free_, a.chunk, a.chunks, t.pages, take, r0 + __popcll(m & ((1ull << lane) - 1)), r0);
+      const int got = pt_page(a.free_, g.chunk, a.chunks, t.pages, take, r0 + __popcll(m & ((1ull << lane) - 1)), r0);
       if (take) {
         id = got;
         if (got >= 0) t.refs_out[got] = 1;
@@ -261,7 +348,7 @@ __device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* p
   if (!touched) return;
   __syncthreads();
   const int lo = max(at, c0 << t.sh), hi = (int)min((long long)at + n, (long long)c1 << t.sh);
-  const int row0 = t.starts[s] - at;
+  const int row0 = g.first[s] - at;
   for (int e = lo + tid; e < hi; e += 256) {
     const int p = page[(e >> t.sh) - c0], r = row0 + e;
     t.seq[r] = s;
@@ -272,8 +359,8 @@ __device__ __forceinline__ void pt_fill(const PtArgs& a, int s, int span, int* p
 }
 
 // Rows behind the last sequence's.
-__device__ __forceinline__ void pt_behind(const TableArgs& t, int first, int step) {
-  for (int r = t.starts[t.seqs] + first; r < t.rows; r += step) {
+__device__ __forceinline__ void pt_behind(const TableArgs& t, int rows, int first, int step) {
+  for (int r = rows + first; r < t.rows; r += step) {
     t.seq[r] = -1;
     t.pos[r] = -1;
     t.slot[r] = -1;
@@ -306,25 +393,44 @@ __global__ __launch_bounds__(1024) void k_table_grant(PtArgs a) {
   pt_grant<1024>(a, part);
 }
 
+// SUMS: who is served is summed up here (k_table_grant's work).
+template <bool SUMS>
 __global__ __launch_bounds__(256) void k_table_fill(PtArgs a) {
   __shared__ int page[256], cnt[4];
-  const long long all = (long long)a.t.seqs * a.spans;
+  const TableArgs& t = a.t;
+  const int tid = threadIdx.x;
+  PtGrant g;
+  if constexpr (SUMS) {
+    __shared__ PtSums sh;
+    g = {sh.n, sh.base, sh.first, sh.chunk, pt_sum_up(a, sh)};
+    if (blockIdx.x == 0) {
+      for (int s = tid; s < t.seqs; s += 256) {
+        t.starts[s] = sh.first[s];
+        t.lens_out[s] = a.at[s] + sh.n[s];
+      }
+      if (tid == 0) t.starts[t.seqs] = g.rows;
+    }
+  } else {
+    g = {a.n, a.base, t.starts, a.chunk, t.starts[t.seqs]};
+  }
+  const long long all = (long long)t.seqs * a.spans;
   for (long long w = blockIdx.x; w < all; w += gridDim.x)
-    pt_fill(a, (int)(w / a.spans), (int)(w % a.spans), page, cnt);
-  pt_behind(a.t, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    pt_fill(a, g, (int)(w / a.spans), (int)(w % a.spans), page, cnt);
+  pt_behind(t, g.rows, blockIdx.x * 256 + tid, gridDim.x * 256);
 }
 
 // All of it by one work-group, which reads everything at once: a wave takes up to PT_HELD
 // pieces of 64 columns, whose ids it keeps.  Its time goes with the pieces and the pages;
-// us against those of three launches (which the host needs 21 us for):
-//   4 sequences of 64 columns, 512 pages      5.6  12.0
-//   16, 1024 pages, 8192 rows                 7.2  13.1
-//   64, 4096 pages                           10.2  16.3
-//   64, 12288 pages                          16.4  16.3
-//   256 (16 pieces a wave), 12288 pages      45.9  16.4
-//   64, 49152 pages                          27.0  16.2
-//   1 of 256 columns, 8192 rows by 2 waves   11.3  13.6
-// More rows than that, which one wave may have to write, are the three launches'.
+// us on the device, and of a call among others (the host sends one launch in 13, two in 17),
+// against those of two launches:
+//   4 sequences of 64 columns, 512 pages      5.2 12.7    7.3 17.0
+//   16, 1024 pages, 8192 rows                 7.2 12.9    8.1 18.5
+//   32, 8192 pages                           10.3 12.7   10.7 16.9
+//   64, 4096 pages                           13.8 13.6   10.7 17.0
+//   64, 16384 pages                          17.5 17.2   10.9 16.9
+//   1 of 256 columns, 8192 rows by 2 waves   11.1 12.7    8.6 17.1
+// The rule is where a call stops being the shorter one (256 sequences, 16 pieces a wave:
+// 46); more rows, which one wave may have to write, go with two.
 constexpr int PT_HELD = 4, PT_SEQS = 16 * PT_HELD, PT_PAGES = 16384, PT_ROWS = 8192;
 struct PtShared {
   int32_t at[PT_SEQS], n[PT_SEQS], base[PT_SEQS], first[PT_SEQS];
@@ -334,22 +440,6 @@ struct PtShared {
   uint32_t part[2][2][16];
   int rows;
 };
-// Sums of x and y over the threads before this one; tx, ty: over all.  One barrier.
-__device__ __forceinline__ void pt_sums(uint32_t& x, uint32_t& y, uint32_t& tx, uint32_t& ty, uint32_t (*part)[16]) {
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t ix = wave_scan(x), iy = wave_scan(y);
-  if (lane == 63) {
-    part[0][wv] = ix;
-    part[1][wv] = iy;
-  }
-  __syncthreads();
-  const uint32_t px = part[0][lane % 16], py = part[1][lane % 16];
-  const uint32_t sx = wave_scan(lane < 16 ? px : 0), sy = wave_scan(lane < 16 ? py : 0);
-  x = ix - x + lane_of(sx - px, wv);
-  y = iy - y + lane_of(sy - py, wv);
-  tx = lane_of(sx, 15);
-  ty = lane_of(sy, 15);
-}
 __global__ __launch_bounds__(1024) void k_table_one(PtArgs a) {
   __shared__ PtShared sh;
   const TableArgs& t = a.t;
@@ -397,11 +487,11 @@ __global__ __launch_bounds__(1024) void k_table_one(PtArgs a) {
     for (int i = 0; i < per; ++i) need += sh.need[tid * per + i];
   uint32_t x = (uint32_t)min(need, t.pages + 1), y = (uint32_t)min(max(n, 0), t.rows + 1), tx, ty;
   const uint32_t xi = x, yi = y;
-  pt_sums(x, y, tx, ty, sh.part[0]);   // behind its barrier the chunks' sums are read
+  pt_sums<16>(x, y, tx, ty, sh.part[0]);   // behind its barrier the chunks' sums are read
   const bool ok = n >= 0 && y + yi <= (uint32_t)t.rows && (need == 0 || x + xi <= free_pages);
   x = ok ? (uint32_t)need : 0;
   y = ok ? (uint32_t)n : 0;
-  pt_sums(x, y, tx, ty, sh.part[1]);
+  pt_sums<16>(x, y, tx, ty, sh.part[1]);
   if (wv == 0 && lane < a.chunks) sh.chunk[lane] = (int)(upto - own);
   if (tid < t.seqs) {
     const int g = ok ? n : 0;
@@ -562,12 +652,17 @@ hipError_t table_assign(const TableArgs& t, void* ws, hipStream_t st) {
   hipLaunchKernelGGL(k_table_need, dim3((unsigned)(sb + a.chunks)), dim3(256), 0, st, a, sb);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+  const long long all = (long long)t.seqs * a.spans, rows = ((long long)t.rows + 255) / 256;
+  const long long most = all > rows ? all : rows;
+  const dim3 grid((unsigned)(most < 1 ? 1 : most > 65536 ? 65536 : most));
+  if (t.seqs >= 1 && t.seqs <= PT_SUMS && t.pages <= PT_SUM_PAGES && t.rows <= PT_SUM_ROWS) {
+    hipLaunchKernelGGL(k_table_fill<true>, grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(k_table_grant, dim3(1), dim3(1024), 0, st, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const long long all = (long long)t.seqs * a.spans, rows = ((long long)t.rows + 255) / 256;
-  const long long grid = all > rows ? all : rows;
-  hipLaunchKernelGGL(k_table_fill, dim3((unsigned)(grid < 1 ? 1 : grid > 65536 ? 65536 : grid)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_table_fill<false>, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -308,3 +308,28 @@ def test_results_in_place_of_the_queries(wide, traced):
         x = q.clone()
         y, l = paged.attention_shared(x, *args, 0.1, want_lse=True, out=x)
         assert y is x and torch.equal(y, want) and torch.equal(l, lse)
+
+
+@pytest.mark.parametrize("S,cols,spare,rows,runs", [
+    (1024, 2, 5, 700, "k_table_fill<true>"), (1025, 2, 5, 700, "k_table_fill<false>"),
+    (70, 3, (1 << 20) - 210, 300, "k_table_fill<true>"), (70, 3, (1 << 20) - 209, 300, "k_table_fill<false>"),
+    (70, 30, 5, 1 << 21, "k_table_fill<true>"), (70, 30, 5, (1 << 21) + 1, "k_table_fill<false>"),
+])
+@pytest.mark.parametrize("short", [False, True])
+def test_sums_by_one_and_by_all(S, cols, spare, rows, runs, short, traced):
+    """Who is served, summed up by every work-group of the last launch or by one before it;
+    with rows or pages for half of them."""
+    from attention_nn_amd import paged
+    page = 16 if rows < 1 << 20 else 1024
+    table, lens, refs, g = _pool(S, cols, page, S + spare, spare=spare)
+    if short:
+        refs[torch.rand(len(refs), generator=g) < 1 - S / 4 / len(refs)] += 3
+    new = torch.minimum(torch.randint(0, page + 3, (S,), generator=g).to(I32), cols * page - lens).to(I32)
+    ref = R.assign(table.tolist(), lens.tolist(), new.tolist(), refs.tolist(), page, rows)
+    t, l, n, r = table.cuda(), lens.cuda(), new.cuda(), refs.cuda()
+    got = []
+    names = traced(lambda: got.append(paged.assign(t, l, n, r, page, rows)))
+    assert any(runs in x for x in names), names
+    for x in got:
+        _same(x, ref)
+    _same(paged.assign(t, l, n, r, page, rows, out=t, refs_out=r, lens_out=l), ref)
