@@ -1334,11 +1334,17 @@ hipError_t paged_attention(const PagedArgs& c, const bf16_t* q, long long qt, lo
 //
 // Groups of consecutive sequences begin with the same entries, group g with the first
 // plens[g] of ptable[g].  Their rows are one tile's rows (pa_many's, each row with
-// its own entry), so that a prefix is read once for 64 or 128 of them; what a
+// its own entry), so that a prefix is read once for 64 of them; what a
 // sequence has behind the prefix goes as in calls of few rows.  Both leave parts
 // (sums that are not divided, with their maximum), in one launch, and a second
 // joins a row's parts.  A sequence of more than 16 new tokens has tiles of its own,
 // which read what they share from the caches: it takes the whole of its table.
+//
+// 64 sequences of 12 heads of 128 behind 8192 entries, some 190 of their own: 124 MB,
+// 35 us (44 with cold caches, 38 and 6 of them for the join; k_paged_few 226), bound by the
+// places of its work-groups: two on a CU, the prefix's for 25 to 35 us, 768 for 8.4 us each.
+// No faster: work-groups that take several of those in turn (48: more registers, and the
+// last ones wait), the groups' words read ahead of the lengths (44.1).
 constexpr int PS_TOKENS = 16;
 constexpr int PS_PRE = 48, PS_OWN = 16;   // parts of a prefix and behind it at most: 64 in all
 
