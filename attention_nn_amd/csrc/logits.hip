@@ -11,10 +11,9 @@
 // and added as whole numbers of 2^-F, F = 62 - log2 of the entries: exact sums, in
 // any order, LDS atomics too.  2^-46 of the largest weight an entry at 50257 of them.
 //
-// A work-group has a row, which it reads once from memory and then from the caches, a
-// pass at a time: registers for a row of 50257 would leave a CU one work-group, and their
-// number (two) hides what a pass waits for.  Weights of all entries cost a CU 8 us of
-// its 64-bit units at that length, so entries that cannot be drawn go first: those below what
+// A work-group of 16 waves has a row and a CU to itself: it holds up to 53248 fp32 or 57344
+// bf16 entries in registers; longer rows are read from the caches in every pass.  Weights of
+// 50257 entries cost a CU 11 us of its vector units, so entries that cannot be drawn go first: those below what
 // min_p leaves, and below the k-th largest of the threads' maxima, under which
 // the k-th largest of all does not lie.  What is left, if 8192 entries at most, is
 // listed in LDS in the order of the indices, and thresholds and draw go over the
