@@ -895,8 +895,9 @@ static hipError_t sl_launch(const SlArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t sample_logits(const LogitRows& r, int dtype, hipStream_t st) {
-  if (r.rows == 0) return hipSuccess;
+// Up to SL_ROWS rows: a launch holds less than 2^32 threads.
+constexpr int SL_ROWS = 1 << 21;
+static hipError_t sl_rows(const LogitRows& r, int dtype, hipStream_t st) {
   SlArgs a{r, 62};
   while (a.frac > 0 && (1LL << (62 - a.frac)) < r.cols) --a.frac;
   if (a.frac > 51) a.frac = 51;
@@ -904,6 +905,24 @@ hipError_t sample_logits(const LogitRows& r, int dtype, hipStream_t st) {
   const int ne = dtype == 0 ? 4 : 8, J = ((r.cols + 2 * ne - 2) / ne + SL_NT - 1) / SL_NT;
   if (dtype == 0) return J <= 2 ? sl_launch<float, 2>(a, st) : J <= 13 ? sl_launch<float, 13>(a, st) : sl_launch<float, 0>(a, st);
   return J <= 1 ? sl_launch<bf16_t, 1>(a, st) : J <= 7 ? sl_launch<bf16_t, 7>(a, st) : sl_launch<bf16_t, 0>(a, st);
+}
+
+hipError_t sample_logits(const LogitRows& r, int dtype, hipStream_t st) {
+  for (int r0 = 0; r0 < r.rows; r0 += min(SL_ROWS, r.rows - r0)) {
+    LogitRows p = r;
+    p.rows = min(SL_ROWS, r.rows - r0);
+    p.x = (const char*)r.x + r0 * r.stride * (dtype == 0 ? 4 : 2);
+    p.u += r0;
+    if (p.temperature) p.temperature += r0;
+    if (p.top_k) p.top_k += r0;
+    if (p.top_p) p.top_p += r0;
+    if (p.min_p) p.min_p += r0;
+    p.ids += r0;
+    if (p.logprob) p.logprob += r0;
+    const hipError_t e = sl_rows(p, dtype, st);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace ann

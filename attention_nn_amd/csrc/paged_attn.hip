@@ -1563,15 +1563,15 @@ static hipError_t ps_launch(const PaArgs& a, const PsPlan& p, hipStream_t st) {
   constexpr size_t m = pa_many_lds<DH, DH == 64 ? 64 : 32>() + 132 * sizeof(int), f = pa_few_lds<DH, 4>();
   const size_t lds = f > m ? f : m;
   const dim3 grid((unsigned)(p.grid.many + p.grid.pre + p.grid.few));
-  if (grid.x == 0) return hipErrorInvalidConfiguration;
+  const int groups = (a.heads * (DH / 4) + 63) / 64;
+  const int waves = (long long)a.c.rows * groups <= 4096 ? groups : 1;
+  const long long joins = ((long long)a.c.rows * waves + 3) / 4;
+  if (grid.x == 0 || joins >= 1LL << 24) return hipErrorInvalidConfiguration;
   if (DH == 128 && p.qb == 2) hipLaunchKernelGGL((k_paged_shared<128, 2>), grid, dim3(256), lds, st, a, p.grid);
   else hipLaunchKernelGGL((k_paged_shared<DH, 1>), grid, dim3(256), lds, st, a, p.grid);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int groups = (a.heads * (DH / 4) + 63) / 64;
-  const int waves = (long long)a.c.rows * groups <= 4096 ? groups : 1;
-  hipLaunchKernelGGL((k_shared_join<DH>), dim3((unsigned)(((long long)a.c.rows * waves + 3) / 4)), dim3(256), 0, st,
-                     a, groups, waves);
+  hipLaunchKernelGGL((k_shared_join<DH>), dim3((unsigned)joins), dim3(256), 0, st, a, groups, waves);
   return hipGetLastError();
 }
 

@@ -333,3 +333,22 @@ def test_sums_by_one_and_by_all(S, cols, spare, rows, runs, short, traced):
     for x in got:
         _same(x, ref)
     _same(paged.assign(t, l, n, r, page, rows, out=t, refs_out=r, lens_out=l), ref)
+
+
+def test_more_rows_than_a_launch_holds():
+    """Two and a little more launches, settings and results of each row its own."""
+    from attention_nn_amd import kernels
+    n = (1 << 22) + 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.rand((n, 2), generator=g, device="cuda")
+    u = torch.rand(n, generator=g, device="cuda")
+    t = (torch.rand(n, generator=g, device="cuda") < 0.5).float()
+    ids, lp = kernels.sample_logits(x, u, temperature=t, want_logprob=True)
+    p0 = torch.softmax(x.double(), 1)[:, 0]
+    drawn = (u.double() >= p0).int()
+    best = (x[:, 1] > x[:, 0]).int()
+    near = (u.double() - p0).abs() < 2.0 ** -40
+    want = torch.where(t > 0, drawn, best)
+    assert ((ids == want) | near).all()
+    share = torch.where(ids == 0, p0, 1 - p0).log()
+    assert ((lp.double() - torch.where(t > 0, share, 0.0)).abs() <= 2.0 ** -22).all()

@@ -170,6 +170,14 @@ def test_workspace_of_shared_is_bounded(heads, kv_heads, dim):
                     assert n <= 3 * max(1 << 28, one), (seqs, rows, count, entries, n)
 
 
+def test_more_work_groups_than_a_launch_takes_are_refused():
+    """2^26 rows behind a prefix would be joined by 2^24 work-groups of 256 threads."""
+    c = _paged(seqs=65535, rows=1 << 26, cols=64, table_row=64, heads=1, head_dim=64, k_page=1024, v_page=1024, k_head=1024,
+               v_head=1024, k_slot=64, v_slot=64)
+    rc = _shared(c, _prefix(cols=64, row=64), heads=1, row=64, head=64, out=FAKE << 2, ws=FAKE << 3)
+    assert rc not in (0, _lib.ANN_E_ARG) and _said("configuration")
+
+
 # ---- tokens from logits ------------------------------------------------------------
 
 
