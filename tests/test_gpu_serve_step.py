@@ -352,3 +352,51 @@ def test_more_rows_than_a_launch_holds():
     assert ((ids == want) | near).all()
     share = torch.where(ids == 0, p0, 1 - p0).log()
     assert ((lp.double() - torch.where(t > 0, share, 0.0)).abs() <= 2.0 ** -22).all()
+
+
+def test_pages_past_32_bits():
+    """Prefixes and own entries in pages whose offsets in the cache pass 2^31 elements."""
+    from attention_nn_amd import paged
+    from tests.test_gpu_paged_shared import Setup
+    s = Setup([(70, [(1, 9), (2, 50), (20, 40)]), (33, [(1, 3)])], H=4, Hk=2, D=64, page=16).widened()
+    kc, vc, table, starts, lens, groups, pt, pl = s.dev()
+    q = s.q.cuda()
+    want, lse = paged.attention_shared(q, kc, vc, table, starts, lens, groups, pt, pl, 0.1, want_lse=True)
+    pages = kc.shape[0]
+    by = (1 << 31) // (kc[0].numel() * (pages // 2))      # the upper half of them lies past
+    far = []
+    for x in (kc, vc):
+        big = torch.empty((pages * by, *x.shape[1:]), dtype=BF, device="cuda")
+        big[::by] = x
+        far.append(big)
+    assert far[0].numel() > 1 << 31
+    got, l2 = paged.attention_shared(q, *far, torch.where(table >= 0, table * by, -1), starts, lens, groups,
+                                     torch.where(pt >= 0, pt * by, -1), pl, 0.1, want_lse=True)
+    assert torch.equal(got, want) and torch.equal(l2, lse)
+
+
+def test_slots_past_32_bits():
+    from attention_nn_amd import paged
+    pages, page = (1 << 22) + 5, 1024
+    for S in (3, 1200):       # two launches, and three
+        refs = torch.ones(pages, dtype=I32, device="cuda")
+        refs[-4 * S:] = 0
+        table = torch.full((S, 4), -1, dtype=I32, device="cuda")
+        new = torch.full((S,), 1500, dtype=I32, device="cuda")
+        a = paged.assign(table, new * 0, new, refs, page, S * 1500)
+        first = pages - 4 * S
+        assert (a.table[:, :2] == first + torch.arange(2 * S, device="cuda").view(S, 2)).all() and (a.table[:, 2:] == -1).all()
+        assert torch.equal(a.slot, a.table[a.seq.long(), a.pos.long() // page].long() * page + a.pos % page)
+        assert int(a.slot.max()) > 1 << 31 and int(a.refs.sum()) == pages - 4 * S + 2 * S
+        table, refs = paged.release(a.table, new * 0 + 1024, a.refs, page)
+        assert (table[:, 0] == a.table[:, 0]).all() and (table[:, 1:] == -1).all() and int(refs.sum()) == pages - 3 * S
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_rows_past_32_bits(dtype):
+    from attention_nn_amd import kernels
+    g = torch.Generator().manual_seed(8)
+    x, u = torch.randn((4, 777), generator=g).to(dtype), torch.rand(4, generator=g)
+    far = torch.empty(3 * (1 << 30) + 777, dtype=dtype, device="cuda").as_strided((4, 777), (1 << 30, 1))
+    far.copy_(x)
+    _check(x, u, kernels.sample_logits(far, u.cuda(), top_p=0.8, want_logprob=True), dict(top_p=0.8))
