@@ -400,3 +400,21 @@ def test_rows_past_32_bits(dtype):
     far = torch.empty(3 * (1 << 30) + 777, dtype=dtype, device="cuda").as_strided((4, 777), (1 << 30, 1))
     far.copy_(x)
     _check(x, u, kernels.sample_logits(far, u.cuda(), top_p=0.8, want_logprob=True), dict(top_p=0.8))
+
+
+@pytest.mark.parametrize("dtype,groups", [(F32, n) for n in (1, 2, 3, 4, 5, 8, 9, 13, 14)] + [(BF, n) for n in (1, 2, 3, 4, 5, 7, 8)])
+def test_draws_by_the_row_s_groups(dtype, groups):
+    """Rows that fill a number of groups of 16-byte words a wave, and one entry less or more, at
+    every alignment: as many as are held in registers, and longer."""
+    from attention_nn_amd import kernels
+    words = 4 if dtype is F32 else 8
+    g = torch.Generator().manual_seed(groups)
+    for cols in (groups * 1024 * words, groups * 1024 * words - words + 1, groups * 1024 * words + 1):
+        base = torch.empty((2, cols + 8), dtype=dtype, device="cuda")
+        x = (3.0 * torch.randn((2, cols), generator=g)).to(dtype)
+        u = torch.rand(2, generator=g)
+        for off in (0, 1, words - 1):
+            v = base[:, off:off + cols]
+            v.copy_(x)
+            for kw in (dict(top_p=0.9), dict(temperature=0.5, min_p=0.01), dict(top_k=40), dict(temperature=0.0)):
+                _check(x, u, kernels.sample_logits(v, u.cuda(), want_logprob=True, **kw), kw)
