@@ -29,6 +29,7 @@
 #include <math.h>
 #include "common.h"
 #include "launch.h"
+#include "words.h"
 
 namespace ann {
 
@@ -53,17 +54,6 @@ struct SlShared {
   unsigned short hit[SL_NT];          // threads with an entry far up, and of each wave how many, and before it
   int hits[SL_NW], hits_before[SL_NW];
 };
-
-// Order-preserving word of a number (no NaN, no -0).
-__device__ __forceinline__ uint32_t sl_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float sl_value(uint32_t k) {
-  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
-}
-// A NaN is below every number; -0 is 0.
-__device__ __forceinline__ float sl_number(float x) { return x == x ? x + 0.f : -INFINITY; }
 
 // Wave reductions of the device library.
 extern "C" __device__ unsigned __ockl_wfred_max_u32(unsigned);
@@ -112,7 +102,7 @@ struct SlWeight {
     low = fmaxf((float)(at - fabs(at) * 0x1p-22), -3.4028235e38f);
     if (!(low <= m)) low = m;
     // a few words, by which 2^-22 passes the bound
-    for (int i = 0; i < 16 && low < m && ((double)low - md) * c < -60.0; ++i) low = sl_value(sl_key(low) + 1);
+    for (int i = 0; i < 16 && low < m && ((double)low - md) * c < -60.0; ++i) low = word_value(word_of(low) + 1);
   }
   // Without a branch; additions and products only: the unit that converts and scales is slower.
   __device__ __forceinline__ sl_u64 operator()(float x) const {
@@ -331,17 +321,19 @@ __device__ __forceinline__ void sl_add(const SlWeight& wt, float x, W w, bool in
 // where none does.
 template <bool MASS, typename S>
 __device__ __forceinline__ bool sl_round(const S& src, const SlWeight& wt, SlPart& p, double share, SlShared& sh) {
-  const int bits = 32 - __clz((int)(p.hi - p.lo));   // 0 for one word
-  const int s = bits > 11 ? bits - 11 : 0;
-  const uint32_t lo = p.lo;
-  const float x0 = sl_value(lo), x1 = sl_value(p.hi);
+  static_assert(SL_BINS == 2048, "parts of a range");
+  const WordRange in = {p.lo, p.hi};
+  const int s = in.shift();
   src.each([&](float x, auto w) {
-    sl_add<MASS>(wt, x, w, x >= x0 && x <= x1, (int)((sl_key(x + 0.f) - lo) >> s), sh);   // -0 is 0
+    int bin;
+    const bool inside = in.has(x, s, bin);
+    sl_add<MASS>(wt, x, w, inside, bin, sh);
   });
   const int at = sl_bin<MASS>(p, share, sh);
   if (at < 0) return false;
-  p.lo += (uint32_t)at << s;
-  p.hi = min(p.hi, p.lo + ((1u << s) - 1));
+  const WordRange to = in.part(at, s);
+  p.lo = to.lo;
+  p.hi = to.hi;
   return true;
 }
 // The first round over a whole row, whose largest entry is p.hi's: parts of equal difference
@@ -350,11 +342,11 @@ __device__ __forceinline__ bool sl_round(const S& src, const SlWeight& wt, SlPar
 template <bool MASS, typename S>
 __device__ __forceinline__ bool sl_first(const S& src, const SlWeight& wt, SlPart& p, double share, float floor,
                                          SlShared& sh) {
-  const float m = sl_value(p.hi), least = fmaxf(sl_value(p.lo), floor), c = SL_BINS / (m - least);
+  const float m = word_value(p.hi), least = fmaxf(word_value(p.lo), floor), c = SL_BINS / (m - least);
   if (!(c > 0.f && c < 1e30f)) return sl_round<MASS>(src, wt, p, share, sh);   // not finite, or one value
   const uint32_t lo = p.lo;
   const auto bin = [&](float x) { return SL_BINS - 1 - (int)fminf((m - x) * c, SL_BINS - 1.f); };   // rises with x
-  const float x0 = sl_value(lo);
+  const float x0 = word_value(lo);
   src.each([&](float x, auto w) {
     sl_add<MASS>(wt, x, w, x >= x0, bin(x), sh);
   });
@@ -366,7 +358,7 @@ __device__ __forceinline__ bool sl_first(const S& src, const SlWeight& wt, SlPar
     uint32_t a = lo, n = p.hi - lo + 1;   // it is one of the n words from a on, or the next
     while (n) {
       const uint32_t step = n / 64 + 1, at = lane * step;
-      const unsigned long long in = __ballot(at < n && bin(sl_value(a + at)) >= b);
+      const unsigned long long in = __ballot(at < n && bin(word_value(a + at)) >= b);
       // the first lane that has reached the part; or all n words lie below
       const uint32_t first = in ? (uint32_t)__builtin_ctzll(in) : (n + step - 1) / step;
       if (first == 0) return a;
@@ -436,9 +428,9 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       for (int e = 0; e < NE; ++e) few = fminf(few, v[e] > -INFINITY ? v[e] : INFINITY);
   });
   most += 0.f;   // 0 for -0
-  const uint32_t key = sl_key(most);
+  const uint32_t key = word_of(most);
   {
-    const uint32_t top = __ockl_wfred_max_u32(key), low = __ockl_wfred_min_u32(sl_key(few + 0.f));
+    const uint32_t top = __ockl_wfred_max_u32(key), low = __ockl_wfred_min_u32(word_of(few + 0.f));
     const uint32_t least = __ockl_wfred_min_u32(most > -INFINITY ? key : 0xffffffffu);
     if (lane == 0) {
       sh.mm[0][wv] = top;
@@ -448,7 +440,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   }
   __syncthreads();
   const uint32_t kmax = __ockl_wfred_max_u32(sh.mm[0][lane % SL_NW]);
-  const float m = sl_value(kmax);
+  const float m = word_value(kmax);
   if (m == -INFINITY) {   // nothing to draw
     if (tid == 0) {
       a.r.ids[r] = -1;
@@ -477,7 +469,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   // Entries from a word on, and those of the waves before this one.
   int before = 0, turn = 0;
   const auto count = [&](uint32_t from) {
-    const float x0 = sl_value(from);
+    const float x0 = word_value(from);
     uint32_t some = 0;
     row.groups([&](const float* v, int) {
 #pragma unroll
@@ -512,7 +504,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     return;
   }
   const uint32_t tmin = __ockl_wfred_min_u32(sh.mm[1][lane % SL_NW]);
-  const float floor = sl_value(__ockl_wfred_min_u32(sh.mm[2][lane % SL_NW]));
+  const float floor = word_value(__ockl_wfred_min_u32(sh.mm[2][lane % SL_NW]));
 
   // The threads' largest entries in 256 bins: k of them are at or above the lower end of the
   // bin that the k-th lies in, so the k-th largest of all is.
@@ -537,7 +529,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 
   wt.bound(m, reach);
   const double share = by_p ? fmax((double)top_p, 0.0) : 1.0;
-  uint32_t thr = max(sl_key(wt.low), kth);   // the least word that is kept so far
+  uint32_t thr = max(word_of(wt.low), kth);   // the least word that is kept so far
   bool ranked = !by_k;                       // thr is the k-th largest, if there are as many
   SlPart sp{thr, kmax, 0, (sl_u64)k, 0};   // its turns are not those of count
 
@@ -545,7 +537,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   // those, in the order of the indices (wave, group, lane), are shared out among all and
   // read again.  Its number, or -1 where they are too many.
   const auto few_of = [&](uint32_t from) {
-    const float x0 = sl_value(from);
+    const float x0 = word_value(from);
     const unsigned long long mine = __ballot(most >= x0);
     if (lane == 0) sh.hits[wv] = __popcll(mine);
     __syncthreads();
@@ -594,7 +586,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   };
   // The entries with words of [from, to] in any order, without their indices: their number.
   const auto bag_of = [&](uint32_t from, uint32_t to) {
-    const float x0 = sl_value(from), x1 = sl_value(to);
+    const float x0 = word_value(from), x1 = word_most(to);
     turn ^= 1;
     if (tid == 0) sh.bag[turn ^ 1] = 0;
     // first the groups that may have one: within half the range of its middle and some more
@@ -647,9 +639,10 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     listed = true;
     rest = n < 0;
     if (rest) {
-      n = 0;                             // none where one word is left
-      while (sp.hi - sp.lo > GRAIN && (n = bag_of(sp.lo, sp.hi)) > SL_CAP) sl_round<true>(row, wt, sp, -1.0, sh);
-      if (sp.hi - sp.lo <= GRAIN) n = 0;
+      // none where one word is left.  Every round leaves a smaller range, or none and ends this.
+      n = 0;
+      while (sp.hi - sp.lo > GRAIN && (n = bag_of(sp.lo, sp.hi)) > SL_CAP && sl_round<true>(row, wt, sp, -1.0, sh)) {}
+      if (sp.hi - sp.lo <= GRAIN || n > SL_CAP) n = 0;
     }
   } else if (rest) {
     n = 0;
@@ -659,7 +652,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
 
   // ---- the list, in the order of the indices: wave, group, lane, entry
   if (n && !listed) {
-    const float x0 = sl_value(from);
+    const float x0 = word_value(from);
     int at = before;
     const auto write = [&](const float* v, int g) {
       unsigned long long in[NE];
@@ -698,7 +691,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       const int j = lane * per + i;
       const bool real = i < per && j < n;
       x[i] = real ? sh.list[j].x : -INFINITY;
-      keys[i] = real ? sl_key(x[i]) : 0;
+      keys[i] = real ? word_of(x[i]) : 0;
     }
     if (!ranked && n >= k && per == 1) {   // an entry's rank by the others, one by one
       uint32_t rank = 0;
@@ -790,7 +783,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
         sl_u64 sum = 0, ex;
 #pragma unroll
         for (int i = 0; i < SL_PER; ++i) {
-          if (sl_key(list.v[i]) < thr) list.w[i] = 0;
+          if (word_of(list.v[i]) < thr) list.w[i] = 0;
           sum += list.w[i];
         }
         sp.turn ^= 1;
@@ -813,7 +806,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     if (rest) {
       // ---- the draw from the row: the wave whose weight holds the target, by all waves its
       // groups, by the wave whose groups hold it the group, lane and entry
-      const float x0 = sl_value(thr);
+      const float x0 = word_value(thr);
       sl_u64 sum = 0;
       row.each([&](float x, int) {
         const sl_u64 w = wt(x);
