@@ -1482,10 +1482,21 @@ struct PsPlan {
 // Whether reading a prefix once saves what the join and the parts cost: where that is
 // 48 MB of keys and values or more, as the tables' widths have it (us with and without:
 // 8 sequences of 6 heads of 128 behind 1000 entries, 21 MB, 13.8 and 11.8; 90 of 3 heads of 64 behind
-// 500, 34 MB, 12.6 and 9.6; 2 behind 16000, 49 MB, 24.3 and 27.6; 32 behind 2048, 195 MB, 15.7 and 28.0).
-static bool ps_worth(const PagedArgs& c, const SharedPrefix& x, int Dh) {
-  const double again = (double)(c.seqs - x.ngroups) * (double)((long long)x.cols << c.sh);
-  return x.ngroups > 0 && again * c.heads * Dh * 4 >= 48e6;
+// 500, 34 MB, 12.6 and 9.6; 2 behind 16000, 49 MB, 24.3 and 27.6; 32 behind 2048, 195 MB, 15.7 and 28.0;
+// where 8 heads share 2 less is gained: 8 sequences behind 8192, 59 MB, 20.3 and 17.7).
+// A window leaves of the prefix what the sequences' own entries, as many as their tables hold,
+// do not fill; then only where that comes to 160 MB, and the sequences have 16 tokens at most in the
+// mean (`attention` reads the few entries of a window in one launch; 12 heads of 128: 64 behind 8192 with
+// a window of 384, 50 MB, 24.1 and 25.1, of 1024, 297 MB, 29.5 and 36.4; 16 behind 16384, window 2048, 124
+// MB, 34.3 and 28.8, 4096, 313 MB, 33.1 and 46.0; 16 with up to 2560 own ones, 4096, 141 MB, 77.5 and
+// 50.9; 6 heads: 16 of up to 704, 4096, 156 MB, 29.0 and 26.0; 24 sequences of 100 tokens in the
+// mean on 12 heads, 2048, 277 MB by the window alone, 82.2 and 72.4).
+static bool ps_worth(const PagedArgs& c, const SharedPrefix& x, int Dh, int window) {
+  const long long width = (long long)x.cols << c.sh, whole = (long long)c.cols << c.sh;
+  const long long left = window - (whole > width ? whole - width : 0);
+  const bool all = window <= 0 || left >= width;
+  const double again = (double)(c.seqs - x.ngroups) * (double)(all ? width : left) * c.heads * Dh * 4;
+  return x.ngroups > 0 && (all ? again >= 48e6 : again >= 160e6 && c.rows <= (long long)PS_TOKENS * c.seqs);
 }
 static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
   static const int cus = device_cus();
@@ -1503,7 +1514,11 @@ static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int 
   const int br = 64 * p.qb, groups = x.ngroups < c.rows ? x.ngroups : c.rows;
   p.grid.many_full = clamp(rows / br, 1 << 30);
   p.grid.pre_full = clamp(rows / 64, 1 << 30);
-  const long long tiles = rows / 64 + groups, width = (long long)x.cols << c.sh, own = (long long)c.cols << c.sh;
+  const long long tiles = rows / 64 + groups, width = (long long)x.cols << c.sh;
+  // entries that rows of few tokens see at most: of a prefix, of their tables, and behind a prefix
+  const auto within = [&](long long n) { return window > 0 && window + PS_TOKENS < n ? (long long)window + PS_TOKENS : n; };
+  const long long seen = within(width), own = within((long long)c.cols << c.sh);
+  const long long behind = ((long long)c.cols << c.sh) > width ? within(((long long)c.cols << c.sh) - width) : 0;
   const long long slot = (long long)(Dh + 2) * sizeof(float) * c.rows * heads;   // a part of every row
   // Parts of a prefix: the fewest that keep its work-groups from being the last, by a step's time
   // (as in pa_plan), 6 us around them, what memory takes for all entries anyway, and the parts' way
@@ -1512,13 +1527,15 @@ static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int 
   // prefixes of 3001, 54 / 35 / 26 / 24 / 28 / 36; 16, 8 heads on 2, 16384 entries 242 / 128 / 70 / 43 / 30 / 25.
   const bool h = Dh == 64;
   const float alone = h ? 0.5f : 0.475f, both = h ? 0.86f : 0.68f;
-  const double behind = own > width ? (double)(own - width) * c.seqs : 0.0;
-  const float memory = (float)(((double)width * groups + behind) * c.heads * Dh * 4 / 5.1e6);
+  const float memory = (float)(((double)seen * groups + (double)behind * c.seqs) * c.heads * Dh * 4 / 5.1e6);
   float best = 0.f;
   for (const int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48}) {
     if (n > 1 && (width / n < 128 || slot * n > (long long)PA_WS_MAX)) break;
-    const int each = (int)((tiles * c.heads * n + cus - 1) / cus);
-    const float steps = (float)((width + (long long)step * n - 1) / ((long long)step * n));
+    // parts go by the prefix's length: those that a window reaches (96 sequences of 12 heads of 128 behind 4096,
+    // window 384: by the prefix's length 28.5 us, by this 19.0), and the steps of one
+    const long long reached = seen < width ? clamp(seen * n / width + 1, n) : n, part = (width + n - 1) / n;
+    const int each = (int)((tiles * c.heads * reached + cus - 1) / cus);
+    const float steps = (float)(((part < seen ? part : seen) + step - 1) / step);
     const float walk = 6.f + steps * ((float)(each / 2) * both + (float)(each % 2) * alone);
     const float us = (walk > memory ? walk : memory) + (float)slot * (float)n * 2.5f / 4e6f;
     if (best == 0.f || us < best) {
@@ -1553,7 +1570,7 @@ static PsSlots ps_slots(const PagedArgs& c, int heads, const PsPlan& p) {
 
 size_t paged_attention_shared_ws_bytes(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
   if (c.rows == 0 || c.seqs == 0) return 0;
-  if (!ps_worth(c, x, Dh)) return paged_attention_ws_bytes(c, heads, Dh, window);
+  if (!ps_worth(c, x, Dh, window)) return paged_attention_ws_bytes(c, heads, Dh, window);
   const PsSlots n = ps_slots(c, heads, ps_plan(c, x, heads, Dh, window));
   return (n.pre + n.few + n.many) * (Dh + 2) * sizeof(float);
 }
@@ -1579,7 +1596,7 @@ hipError_t paged_attention_shared(const PagedArgs& c, const SharedPrefix& x, con
                                   long long qh, int heads, int Dh, float scale, int window, bf16_t* out,
                                   float* lse, void* ws, hipStream_t st) {
   if (c.rows == 0 || c.seqs == 0) return hipSuccess;
-  if (!ps_worth(c, x, Dh)) return paged_attention(c, q, qt, qh, heads, Dh, scale, window, out, lse, ws, st);
+  if (!ps_worth(c, x, Dh, window)) return paged_attention(c, q, qt, qh, heads, Dh, scale, window, out, lse, ws, st);
   const PsPlan p = ps_plan(c, x, heads, Dh, window);
   PaArgs a = pa_args(c, q, qt, qh, heads, scale, window, out, lse);
   a.sp_few = p.few;
