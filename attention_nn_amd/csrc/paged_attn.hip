@@ -1553,25 +1553,32 @@ static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int 
   const long long blocks[3] = {many ? (rows / br + c.rows / (PS_TOKENS + 1)) * c.heads * p.many.most : 0,
                                tiles * c.heads * p.pre.most,
                                (c.seqs + (each < more ? each : more)) * c.heads * p.few.most};
-  if (blocks[0] + blocks[1] + blocks[2] >= 1LL << 24) return p;   // 2^32 threads: refused by its grid of none
+  if (blocks[0] + blocks[1] + blocks[2] >= 1LL << 24) return p;   // 2^32 threads, more than a launch takes: a grid of none
   p.grid.many = (int)blocks[0];
   p.grid.pre = (int)blocks[1];
   p.grid.few = (int)blocks[2];
   return p;
+}
+// Whether a call goes behind its prefixes, and how; else as attention does.
+static bool ps_taken(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window, PsPlan* p) {
+  if (!ps_worth(c, x, Dh, window)) return false;
+  *p = ps_plan(c, x, heads, Dh, window);
+  return p->grid.pre > 0;
 }
 struct PsSlots {
   size_t pre, few, many;
 };
 static PsSlots ps_slots(const PagedArgs& c, int heads, const PsPlan& p) {
   const size_t rows = (size_t)c.rows * heads;
-  return {p.grid.pre ? rows * p.pre.most : 0, rows * p.few.most,
+  return {rows * p.pre.most, rows * p.few.most,
           p.grid.many && p.many.most > 1 ? rows * p.many.most : 0};
 }
 
 size_t paged_attention_shared_ws_bytes(const PagedArgs& c, const SharedPrefix& x, int heads, int Dh, int window) {
   if (c.rows == 0 || c.seqs == 0) return 0;
-  if (!ps_worth(c, x, Dh, window)) return paged_attention_ws_bytes(c, heads, Dh, window);
-  const PsSlots n = ps_slots(c, heads, ps_plan(c, x, heads, Dh, window));
+  PsPlan p;
+  if (!ps_taken(c, x, heads, Dh, window, &p)) return paged_attention_ws_bytes(c, heads, Dh, window);
+  const PsSlots n = ps_slots(c, heads, p);
   return (n.pre + n.few + n.many) * (Dh + 2) * sizeof(float);
 }
 
@@ -1583,7 +1590,7 @@ static hipError_t ps_launch(const PaArgs& a, const PsPlan& p, hipStream_t st) {
   const int groups = (a.heads * (DH / 4) + 63) / 64;
   const int waves = (long long)a.c.rows * groups <= 4096 ? groups : 1;
   const long long joins = ((long long)a.c.rows * waves + 3) / 4;
-  if (grid.x == 0 || joins >= 1LL << 24) return hipErrorInvalidConfiguration;
+  if (joins >= 1LL << 24) return hipErrorInvalidConfiguration;
   if (DH == 128 && p.qb == 2) hipLaunchKernelGGL((k_paged_shared<128, 2>), grid, dim3(256), lds, st, a, p.grid);
   else hipLaunchKernelGGL((k_paged_shared<DH, 1>), grid, dim3(256), lds, st, a, p.grid);
   hipError_t e = hipGetLastError();
@@ -1596,8 +1603,8 @@ hipError_t paged_attention_shared(const PagedArgs& c, const SharedPrefix& x, con
                                   long long qh, int heads, int Dh, float scale, int window, bf16_t* out,
                                   float* lse, void* ws, hipStream_t st) {
   if (c.rows == 0 || c.seqs == 0) return hipSuccess;
-  if (!ps_worth(c, x, Dh, window)) return paged_attention(c, q, qt, qh, heads, Dh, scale, window, out, lse, ws, st);
-  const PsPlan p = ps_plan(c, x, heads, Dh, window);
+  PsPlan p;
+  if (!ps_taken(c, x, heads, Dh, window, &p)) return paged_attention(c, q, qt, qh, heads, Dh, scale, window, out, lse, ws, st);
   PaArgs a = pa_args(c, q, qt, qh, heads, scale, window, out, lse);
   a.sp_few = p.few;
   a.sp_many = p.many;

@@ -1,5 +1,6 @@
-"""Which calls behind a shared prefix go as attention does where a window leaves little of it
-to read once, by the workspace that a call asks for (paged.attention_shared)."""
+"""Which calls behind a shared prefix go as attention does, where a window leaves little of it
+to read once or a launch would not hold them, by the workspace that a call asks for
+(paged.attention_shared)."""
 
 import pytest
 
@@ -51,3 +52,12 @@ def test_much_left_is_shared(shape):
 def test_a_window_past_every_entry_is_none():
     for window in (8192 + 256, 1 << 30):
         assert _bytes(64, 64, 256, 8192, 12, 12, 128, window)[0] == _bytes(64, 64, 256, 8192, 12, 12, 128, 0)[0]
+
+
+def test_more_work_groups_than_a_launch_takes():
+    """2^21 new tokens of 128 heads would take more work-groups behind a prefix than one
+    launch has, and go as attention does."""
+    shared, alone = _bytes(1024, 1 << 21, 4096, 8192, 128, 128, 64, 0)
+    assert shared == alone
+    shared, _ = _bytes(1024, 1 << 15, 4096, 8192, 128, 128, 64, 0)
+    assert shared >= 2 * (1 << 15) * 128 * (64 + 2) * 4
