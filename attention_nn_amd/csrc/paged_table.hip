@@ -436,7 +436,7 @@ struct PtShared {
   int32_t at[PT_SEQS], n[PT_SEQS], base[PT_SEQS], first[PT_SEQS];
   int32_t need[16 * PT_HELD];             // of a piece
   unsigned long long free_[PT_PAGES / 64];
-  int32_t chunk[PT_PAGES / 64 / PT_CHUNK + 1];
+  int32_t chunk[PT_PAGES / (64 * PT_CHUNK)];
   uint32_t part[2][2][16];
   int rows;
 };
@@ -478,7 +478,8 @@ __global__ __launch_bounds__(1024) void k_table_one(PtArgs a) {
   }
   __syncthreads();
   // who is served: sums of what is asked for, at most one more than there is of each, in 32
-  // bits; the chunks' free pages, 16 at most, by every wave
+  // bits; the chunks' free pages, by every wave, a chunk a lane
+  static_assert(PT_PAGES % (64 * PT_CHUNK) == 0 && PT_PAGES / (64 * PT_CHUNK) <= 64, "chunks: 4");
   const uint32_t own = lane < a.chunks ? (uint32_t)sh.chunk[lane] : 0, upto = wave_scan(own);
   const uint32_t free_pages = lane_of(upto, 63);
   const int n = tid < t.seqs ? sh.n[tid] : -1;
