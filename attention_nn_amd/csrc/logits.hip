@@ -542,8 +542,8 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     if (lane == 0) sh.hits[wv] = __popcll(mine);
     __syncthreads();
     const uint32_t own = (uint32_t)sh.hits[lane % SL_NW], in = wave_scan(lane < SL_NW ? own : 0);
-    const int hits = (int)lane_of(in, SL_NW - 1), pairs = hits * row.J;
-    if (hits > SL_PAIRS * SL_NT || pairs > SL_PAIRS * SL_NT) return -1;
+    const int hits = (int)lane_of(in, SL_NW - 1), pairs = hits * row.J;   // a hit for each thread at most
+    if (pairs > SL_PAIRS * SL_NT) return -1;
     if (wv == 0 && lane < SL_NW) sh.hits_before[lane] = (int)(in - own);
     // by all lanes: inside the branch the lane that is asked may be off, and what it holds of
     // in - own not yet formed
