@@ -62,6 +62,17 @@ __device__ __forceinline__ N wave_scan(N v) {
   v += dpp_shift<0x143, 0xc>(v);   // lane 31 to the third and fourth
   return v;
 }
+// The largest of all lanes', and the least.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, dpp_shift<0x111, 0xf>(v));
+  v = max(v, dpp_shift<0x112, 0xf>(v));
+  v = max(v, dpp_shift<0x114, 0xf>(v));
+  v = max(v, dpp_shift<0x118, 0xf>(v));
+  v = max(v, dpp_shift<0x142, 0xa>(v));
+  v = max(v, dpp_shift<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) { return ~wave_max(~v); }
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int lane) {
   return (unsigned long long)lane_of((uint32_t)(v >> 32), lane) << 32 | lane_of((uint32_t)v, lane);

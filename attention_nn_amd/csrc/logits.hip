@@ -55,10 +55,6 @@ struct SlShared {
   int hits[SL_NW], hits_before[SL_NW];
 };
 
-// Wave reductions of the device library.
-extern "C" __device__ unsigned __ockl_wfred_max_u32(unsigned);
-extern "C" __device__ unsigned __ockl_wfred_min_u32(unsigned);
-
 // Sum over the work-group, and (ex) over the threads before this one; one barrier.
 // Calls take turns with `part` (which), and a barrier lies between two of one turn.
 __device__ __forceinline__ sl_u64 sl_scan(sl_u64 v, sl_u64& ex, sl_u64* part) {
@@ -430,8 +426,8 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
   most += 0.f;   // 0 for -0
   const uint32_t key = word_of(most);
   {
-    const uint32_t top = __ockl_wfred_max_u32(key), low = __ockl_wfred_min_u32(word_of(few + 0.f));
-    const uint32_t least = __ockl_wfred_min_u32(most > -INFINITY ? key : 0xffffffffu);
+    const uint32_t top = wave_max(key), low = wave_min(word_of(few + 0.f));
+    const uint32_t least = wave_min(most > -INFINITY ? key : 0xffffffffu);
     if (lane == 0) {
       sh.mm[0][wv] = top;
       sh.mm[1][wv] = least;
@@ -439,7 +435,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     }
   }
   __syncthreads();
-  const uint32_t kmax = __ockl_wfred_max_u32(sh.mm[0][lane % SL_NW]);
+  const uint32_t kmax = wave_max(sh.mm[0][lane % SL_NW]);
   const float m = word_value(kmax);
   if (m == -INFINITY) {   // nothing to draw
     if (tid == 0) {
@@ -503,8 +499,8 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
     });
     return;
   }
-  const uint32_t tmin = __ockl_wfred_min_u32(sh.mm[1][lane % SL_NW]);
-  const float floor = word_value(__ockl_wfred_min_u32(sh.mm[2][lane % SL_NW]));
+  const uint32_t tmin = wave_min(sh.mm[1][lane % SL_NW]);
+  const float floor = word_value(wave_min(sh.mm[2][lane % SL_NW]));
 
   // The threads' largest entries in 256 bins: k of them are at or above the lower end of the
   // bin that the k-th lies in, so the k-th largest of all is.
@@ -697,7 +693,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
       uint32_t rank = 0;
 #pragma unroll 4
       for (int i = 0; i < n; ++i) rank += lane_of(keys[0], i) > keys[0];
-      thr = max(thr, __ockl_wfred_min_u32(lane < n && rank < (uint32_t)k ? keys[0] : 0xffffffffu));
+      thr = max(thr, wave_min(lane < n && rank < (uint32_t)k ? keys[0] : 0xffffffffu));
     } else if (!ranked && n >= k) {   // else all of them are among the k
       uint32_t lo = from, hi = kmax;
       while (hi - lo > GRAIN) {
@@ -729,7 +725,7 @@ __global__ __launch_bounds__(SL_NT, 4) void k_sample_logits(SlArgs a) {
           const sl_u64 wi = lane_of(w[0], i);
           above += lane_of(keys[0], i) > keys[0] ? wi : 0;
         }
-        lo = hi = __ockl_wfred_min_u32(w[0] && above < want ? keys[0] : 0xffffffffu);
+        lo = hi = wave_min(w[0] && above < want ? keys[0] : 0xffffffffu);
       }
       while (hi - lo > GRAIN) {
         const uint32_t mid = hi - ((hi - lo) >> 1);
