@@ -21,10 +21,10 @@
 // bound: the weights of all entries, added up in bins, give one.  Else (flat rows,
 // many equal values, no limits) the passes go over the row.
 //
-// 50257 entries: one row by top_k 50 10.9 us, of them 3 to read it; 64 rows, a setting each, 43.4,
+// 50257 entries: one row by top_k 50 10.9 us, of them 3 to read it; 64 rows, a setting each, 43.0,
 // the longest by top_p alone: 14 for all weights into bins and 10 for those that stay, both bound by
 // the CU's vector instructions (33 an entry), 10 for thresholds; 512 rows of bf16 by min_p 0.02 and
-// top_p 0.9 38.6, two rounds of the CUs.  No faster: a threshold from 32-bit weights first, then
+// top_p 0.9 38.9, two rounds of the CUs.  No faster: a threshold from 32-bit weights first, then
 // one pass for all sums (42.4: 41 instructions an entry).
 #include <math.h>
 #include "common.h"

@@ -1489,7 +1489,7 @@ struct PsPlan {
 // mean (`attention` reads the few entries of a window in one launch; 12 heads of 128: 64 behind 8192 with
 // a window of 384, 50 MB, 24.1 and 25.1, of 1024, 297 MB, 29.5 and 36.4; 16 behind 16384, window 2048, 124
 // MB, 34.3 and 28.8, 4096, 313 MB, 33.1 and 46.0; 16 with up to 2560 own ones, 4096, 141 MB, 77.5 and
-// 50.9; 6 heads: 16 of up to 704, 4096, 156 MB, 29.0 and 26.0; 24 sequences of 100 tokens in the
+// 50.9; 6 heads: 16 of up to 704, 4096, 156 MB, 29.0 and 26.0; 24 sequences of 89 tokens in the
 // mean on 12 heads, 2048, 277 MB by the window alone, 82.2 and 72.4).
 static bool ps_worth(const PagedArgs& c, const SharedPrefix& x, int Dh, int window) {
   const long long width = (long long)x.cols << c.sh, whole = (long long)c.cols << c.sh;

@@ -224,7 +224,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wan
     Temperature 0 (in a tensor: not above 0) takes the lowest index of the largest
     entry.  A NaN is never drawn; a row of -inf gives -1 and -inf.
 
-    Weights are formed in 64 bits and added exactly, so the same call gives the same tokens."""
+    Weights are formed in 64 bits and added exactly, so the same call gives the same tokens.
+    Autograd does not see this call."""
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         raise ValueError("expected a GPU tensor")
     if logits.dim() != 2:

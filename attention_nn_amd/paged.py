@@ -260,7 +260,8 @@ def attention_shared(q, k_cache, v_cache, table, starts, lens, groups, prefix_ta
     group share nothing.  A prefix is read once for the tokens of all its sequences with up
     to 16 new ones; a sequence of more is on its own.  Where the tables are so narrow, or a
     window leaves so little of a prefix, that this saves too little, all goes as in
-    ``attention``.  ``out`` may be ``q``."""
+    ``attention``; else the weights enter the product with the values in two bf16 halves for
+    sequences of up to 16 new tokens, in bf16 for those of more.  ``out`` may be ``q``."""
     (q, qp, qt, qh), N, H, D, d, c, (S, _, _, page, _), keep = _queries(q, k_cache, v_cache, table, starts, lens)
     _check("prefix_table", prefix_table, _I32, 2, d)
     count, cols = prefix_table.shape
