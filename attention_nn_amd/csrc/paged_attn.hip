@@ -1516,7 +1516,10 @@ static PsPlan ps_plan(const PagedArgs& c, const SharedPrefix& x, int heads, int 
   p.grid.pre_full = clamp(rows / 64, 1 << 30);
   const long long tiles = rows / 64 + groups, width = (long long)x.cols << c.sh;
   // entries that rows of few tokens see at most: of a prefix, of their tables, and behind a prefix
-  const auto within = [&](long long n) { return window > 0 && window + PS_TOKENS < n ? (long long)window + PS_TOKENS : n; };
+  const auto within = [&](long long n) {
+    const long long most = (long long)window + PS_TOKENS;
+    return window > 0 && most < n ? most : n;
+  };
   const long long seen = within(width), own = within((long long)c.cols << c.sh);
   const long long behind = ((long long)c.cols << c.sh) > width ? within(((long long)c.cols << c.sh) - width) : 0;
   const long long slot = (long long)(Dh + 2) * sizeof(float) * c.rows * heads;   // a part of every row

@@ -50,7 +50,7 @@ def test_much_left_is_shared(shape):
 
 
 def test_a_window_past_every_entry_is_none():
-    for window in (8192 + 256, 1 << 30):
+    for window in (8192 + 256, 1 << 30, (1 << 31) - 1):
         assert _bytes(64, 64, 256, 8192, 12, 12, 128, window)[0] == _bytes(64, 64, 256, 8192, 12, 12, 128, 0)[0]
 
 
